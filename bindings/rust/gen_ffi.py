@@ -12,9 +12,9 @@ HEADER = os.path.join(HERE, "..", "..", "include", "sage_cuda.h")
 OUT = os.path.join(HERE, "src", "backend", "cuda", "ffi.rs")
 
 SCALARS = {"sage_status": "i32", "int32_t": "i32", "int64_t": "i64", "uint64_t": "u64", "uint32_t": "u32", "uint8_t": "u8",
-           "size_t": "usize", "float": "f32", "char": "c_char", "void": "c_void"}
+           "size_t": "usize", "float": "f32", "double": "f64", "char": "c_char", "void": "c_void"}
 OPAQUE = ["sage_ctx", "sage_buf", "sage_module"]
-STRUCTS = ["sage_tensor", "sage_ctx_opts", "sage_mem_stats_t", "sage_arg", "sage_window"]
+STRUCTS = ["sage_tensor", "sage_ctx_opts", "sage_mem_stats_t", "sage_arg", "sage_window", "sage_adamw_tensor", "sage_adamw_opts"]
 
 PRELUDE = '''// GENERATED by bindings/rust/gen_ffi.py from include/sage_cuda.h — do not edit by hand.
 //
@@ -38,6 +38,11 @@ pub const SAGE_ERR_UNSUPPORTED: i32 = 7;
 pub const SAGE_F32: i32 = 0;
 pub const SAGE_I32: i32 = 1;
 pub const SAGE_U32: i32 = 2;
+// storage types of the language-model operators alone
+pub const SAGE_F16: i32 = 3;
+pub const SAGE_BF16: i32 = 4;
+pub const SAGE_I8: i32 = 5;
+pub const SAGE_U8: i32 = 6;
 
 /// Tensor = buffer + Shape{extents, strides, offset} in elements (src/tensor.rs:106-110, src/shape.rs:37-43).
 #[repr(C)] #[derive(Clone, Copy)]
@@ -56,6 +61,13 @@ pub struct sage_arg { pub kind: i32, pub buf: *mut sage_buf, pub i: i64, pub f: 
 /// Every pair is ordered [w, h] like SizedExtent<2> (src/ops/conv.rs:83).
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct sage_window { pub ker: [i32; 2], pub stride: [i32; 2], pub pad: [i32; 2], pub dil: [i32; 2] }
+/// One tensor of an AdamW step; absent operands have a null `buf`.
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sage_adamw_tensor {
+    pub param: sage_tensor, pub grad: sage_tensor, pub m: sage_tensor, pub v: sage_tensor, pub m_scale: sage_tensor, pub v_scale: sage_tensor, pub copy: sage_tensor,
+}
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sage_adamw_opts { pub lr: f64, pub beta1: f64, pub beta2: f64, pub eps: f64, pub weight_decay: f64, pub grad_scale: f64, pub step: i64 }
 
 #[link(name = "sagecuda")]
 extern "C" {

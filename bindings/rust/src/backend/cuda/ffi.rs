@@ -20,6 +20,11 @@ pub const SAGE_ERR_UNSUPPORTED: i32 = 7;
 pub const SAGE_F32: i32 = 0;
 pub const SAGE_I32: i32 = 1;
 pub const SAGE_U32: i32 = 2;
+// storage types of the language-model operators alone
+pub const SAGE_F16: i32 = 3;
+pub const SAGE_BF16: i32 = 4;
+pub const SAGE_I8: i32 = 5;
+pub const SAGE_U8: i32 = 6;
 
 /// Tensor = buffer + Shape{extents, strides, offset} in elements (src/tensor.rs:106-110, src/shape.rs:37-43).
 #[repr(C)] #[derive(Clone, Copy)]
@@ -38,6 +43,13 @@ pub struct sage_arg { pub kind: i32, pub buf: *mut sage_buf, pub i: i64, pub f: 
 /// Every pair is ordered [w, h] like SizedExtent<2> (src/ops/conv.rs:83).
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct sage_window { pub ker: [i32; 2], pub stride: [i32; 2], pub pad: [i32; 2], pub dil: [i32; 2] }
+/// One tensor of an AdamW step; absent operands have a null `buf`.
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sage_adamw_tensor {
+    pub param: sage_tensor, pub grad: sage_tensor, pub m: sage_tensor, pub v: sage_tensor, pub m_scale: sage_tensor, pub v_scale: sage_tensor, pub copy: sage_tensor,
+}
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sage_adamw_opts { pub lr: f64, pub beta1: f64, pub beta2: f64, pub eps: f64, pub weight_decay: f64, pub grad_scale: f64, pub step: i64 }
 
 #[link(name = "sagecuda")]
 extern "C" {
@@ -51,8 +63,11 @@ extern "C" {
     pub fn sage_status_word(ctx: *mut sage_ctx, word: *mut u32) -> i32;
     pub fn sage_selftest_bounded_wait(ctx: *mut sage_ctx) -> i32;
     pub fn sage_ctx_stream(ctx: *mut sage_ctx) -> *mut c_void;
+    pub fn sage_ctx_use_stream(ctx: *mut sage_ctx, stream: *mut c_void) -> i32;
+    pub fn sage_ctx_use_own_stream(ctx: *mut sage_ctx) -> i32;
     pub fn sage_alloc(ctx: *mut sage_ctx, bytes: usize, buf: *mut *mut sage_buf) -> i32;
     pub fn sage_free(ctx: *mut sage_ctx, buf: *mut sage_buf) -> i32;
+    pub fn sage_buf_wrap(ctx: *mut sage_ctx, device_ptr: *mut c_void, bytes: usize, buf: *mut *mut sage_buf) -> i32;
     pub fn sage_last_oom(ctx: *mut sage_ctx, needed_bytes: *mut u64, total_bytes: *mut u64) -> i32;
     pub fn sage_mem_stats(ctx: *mut sage_ctx, stats: *mut sage_mem_stats_t) -> i32;
     pub fn sage_release_cached(ctx: *mut sage_ctx) -> i32;
@@ -84,6 +99,13 @@ extern "C" {
     pub fn sage_col2im(ctx: *mut sage_ctx, x: *const sage_tensor, w: *const sage_window, y: *const sage_tensor) -> i32;
     pub fn sage_pool2d(ctx: *mut sage_ctx, is_max: i32, x: *const sage_tensor, w: *const sage_window, y: *const sage_tensor) -> i32;
     pub fn sage_conv2d_nhwc(ctx: *mut sage_ctx, x: *const sage_tensor, filter: *const sage_tensor, w: *const sage_window, y: *const sage_tensor) -> i32;
+    pub fn sage_embedding(ctx: *mut sage_ctx, table: *const sage_tensor, ids: *const sage_tensor, scale: f32, y: *const sage_tensor) -> i32;
+    pub fn sage_embedding_grad(ctx: *mut sage_ctx, g: *const sage_tensor, ids: *const sage_tensor, scale: f32, add: i32, dtable: *const sage_tensor) -> i32;
+    pub fn sage_token_log_probs(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, log_probs: *const sage_tensor, entropy: *const sage_tensor, stats: *const sage_tensor, top_ids: *const sage_tensor, top_log_probs: *const sage_tensor) -> i32;
+    pub fn sage_token_log_probs_grad(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, stats: *const sage_tensor, entropy: *const sage_tensor, g_log_probs: *const sage_tensor, g_entropy: *const sage_tensor, dlogits: *const sage_tensor) -> i32;
+    pub fn sage_token_log_probs_and_grad(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, g_log_probs: *const sage_tensor, g_entropy: *const sage_tensor, log_probs: *const sage_tensor, entropy: *const sage_tensor, dlogits: *const sage_tensor) -> i32;
+    pub fn sage_adamw_step(ctx: *mut sage_ctx, tensors: *const sage_adamw_tensor, count: i32, opts: *const sage_adamw_opts) -> i32;
+    pub fn sage_adamw_states(ctx: *mut sage_ctx, m: *const sage_tensor, m_scale: *const sage_tensor, v: *const sage_tensor, v_scale: *const sage_tensor, m_out: *const sage_tensor, v_out: *const sage_tensor) -> i32;
     pub fn sage_ipc_export(ctx: *mut sage_ctx, buf: *mut sage_buf, handle: *mut u8, offset: *mut u64) -> i32;
     pub fn sage_ipc_open(ctx: *mut sage_ctx, handle: *const u8, peer_ptr: *mut *mut c_void) -> i32;
     pub fn sage_ipc_close(ctx: *mut sage_ctx, peer_ptr: *mut c_void) -> i32;

@@ -11,7 +11,8 @@
  * Conventions
  *  - every function returns a sage_status; 0 is success; nothing aborts or throws
  *  - sizes are in BYTES unless the name says elements; tensor offsets/strides are
- *    in ELEMENTS (4-byte elements: float / int / uint), like the reference's Shape
+ *    in ELEMENTS (4-byte elements: float / int / uint), like the reference's Shape;
+ *    the language-model operators also take elements of 2 and 1 bytes
  *  - one sage_ctx owns one device, one in-order stream and one allocator and is
  *    single-threaded, like the reference's Context + cl_queue
  *  - all launches are asynchronous on the context's stream; sage_download and
@@ -43,8 +44,9 @@ enum {
 };
 
 /* Element types the reference can actually store (all 4 bytes: src/session/device.rs:73-81,
- * src/tensor/data.rs:13-30). */
-typedef enum { SAGE_F32 = 0, SAGE_I32 = 1, SAGE_U32 = 2 } sage_dtype;
+ * src/tensor/data.rs:13-30), then the narrower ones that the language-model operators below also store: only
+ * those operators take them, every other entry point answers SAGE_ERR_INVALID. */
+typedef enum { SAGE_F32 = 0, SAGE_I32 = 1, SAGE_U32 = 2, SAGE_F16 = 3, SAGE_BF16 = 4, SAGE_I8 = 5, SAGE_U8 = 6 } sage_dtype;
 
 typedef struct sage_ctx sage_ctx;
 typedef struct sage_buf sage_buf;
@@ -110,6 +112,13 @@ sage_status sage_selftest_bounded_wait(sage_ctx *ctx);
 /* The context's CUDA stream as an opaque cudaStream_t (for event timing by the caller). */
 void *sage_ctx_stream(sage_ctx *ctx);
 
+/* For a program that shares its GPU with another runtime (no reference counterpart: the reference owns its queue): from here on
+ * the context works on `stream`, a cudaStream_t of its device that outlives its use here, behind what the context has enqueued so
+ * far; what that runtime enqueues there and what the context does are then in order.  sage_ctx_use_own_stream goes back to the
+ * context's own stream, behind what it has enqueued on the other. */
+sage_status sage_ctx_use_stream(sage_ctx *ctx, void *stream);
+sage_status sage_ctx_use_own_stream(sage_ctx *ctx);
+
 /* ------------------------------------------------------------------ memory */
 
 /* Context::alloc → Allocator::alloc → Device::alloc_buffer —
@@ -118,6 +127,10 @@ sage_status sage_alloc(sage_ctx *ctx, size_t bytes, sage_buf **buf);
 /* Drop for OpenClMemory → Pool::free — src/session/memory.rs:685-692,365-408.
  * Stream-ordered: the block may be handed to the next allocation without a sync. */
 sage_status sage_free(sage_ctx *ctx, sage_buf *buf);
+/* A buffer over device memory that the caller owns (no reference counterpart): nothing is allocated or copied, sage_free releases
+ * the handle alone.  The memory must be this context's GPU's and outlive the handle; what another stream writes there is ordered
+ * by the caller (sage_ctx_use_stream, or events). */
+sage_status sage_buf_wrap(sage_ctx *ctx, void *device_ptr, size_t bytes, sage_buf **buf);
 /* OutOfMemory{mem_needed, mem_total} of the last SAGE_ERR_OOM — memory.rs:45-54 */
 sage_status sage_last_oom(sage_ctx *ctx, uint64_t *needed_bytes, uint64_t *total_bytes);
 
@@ -253,6 +266,62 @@ sage_status sage_pool2d(sage_ctx *ctx, int32_t is_max, const sage_tensor *x, con
  * extents give it).  The reference materialises im2col(x) and calls its GEMM; here the product runs as an
  * implicit GEMM on the tensor cores when C % 32 == 0, otherwise the GEMM builds its column planes on the fly. */
 sage_status sage_conv2d_nhwc(sage_ctx *ctx, const sage_tensor *x, const sage_tensor *filter, const sage_window *w, const sage_tensor *y);
+
+/* ------------------------------------------------------------------ language models (no reference counterpart: the reference
+ * has gather / scatter, softmax_cross_entropy over a composed graph and its own Adam).
+ *
+ * Operands are views (buffer, extents, strides, offset) that must lie inside their buffers; rows ([.., D] and [.., V]) are
+ * contiguous along the last axis with any distance between rows that keeps them apart (inputs: any that is not negative), vectors
+ * may have any stride (inputs: also 0, a broadcast value).  Outputs may not share memory with an operand unless it says so.
+ * Calls with no rows return at once.  All sums are held in 32 bits in a fixed order: the same inputs give the same bits. */
+
+/* y[t, :] = scale * table[ids[t], :].  table [V, D] f32 / f16 / bf16, ids [T] i32 / u32, y [T, D] f32 or the table's type.  An id
+ * outside [0, V) stands for no token: its row is zeros. */
+sage_status sage_embedding(sage_ctx *ctx, const sage_tensor *table, const sage_tensor *ids, float scale, const sage_tensor *y);
+/* Its gradient: dtable[v, :] = scale * (sum of g[t, :] over the tokens t with ids[t] = v), rows without a token zero; with `add`
+ * the sums are added to what dtable holds.  g [T, D] f32 / f16 / bf16, dtable [V, D] f32. */
+sage_status sage_embedding_grad(sage_ctx *ctx, const sage_tensor *g, const sage_tensor *ids, float scale, int32_t add, const sage_tensor *dtable);
+
+/* Over each row x = scale * logits[r, :] (logits [R, V] f32 / f16 / bf16, scale > 0, an inverse temperature):
+ *   log_probs[r] = x[ids[r]] - log_sum_exp(x)         (ids[r] outside [0, V): no token is scored, 0)
+ *   entropy[r]   = - sum of p log p, p = softmax(x)
+ *   stats[r]     = { max of x / scale, sum of exp(x - max x) }, what the gradient reads
+ *   top_ids[r, :], top_log_probs[r, :]: the k largest logits of the row (k <= 32, k <= V), largest first, ties lowest token first
+ * entropy, stats and the pair of tops may be NULL.  -inf masks a token (log probability -inf, nothing to the entropy); a row
+ * masked throughout has log_probs -inf, entropy 0, tops -inf and no gradient.  A NaN or +inf in a row makes its log probabilities and
+ * entropy NaN; among the tops NaN counts as -inf.  Outputs are f32, top_ids i32 or u32. */
+sage_status sage_token_log_probs(sage_ctx *ctx, const sage_tensor *logits, const sage_tensor *ids, float scale, const sage_tensor *log_probs,
+                                 const sage_tensor *entropy, const sage_tensor *stats, const sage_tensor *top_ids, const sage_tensor *top_log_probs);
+/* Gradient with respect to the logits, from what sage_token_log_probs left in `stats` and `entropy`:
+ *   dlogits[r, j] = scale * (g_log_probs[r] (delta(j, ids[r]) - p_j) - g_entropy[r] p_j (log p_j + entropy[r]))
+ * Either gradient may be NULL (zero); `entropy` is needed with g_entropy.  Rows without a scored token have no part from
+ * g_log_probs.  dlogits [R, V] has the logits' type and may be the logits' own memory (same rows). */
+sage_status sage_token_log_probs_grad(sage_ctx *ctx, const sage_tensor *logits, const sage_tensor *ids, float scale, const sage_tensor *stats,
+                                      const sage_tensor *entropy, const sage_tensor *g_log_probs, const sage_tensor *g_entropy, const sage_tensor *dlogits);
+/* Both where the gradients of log_probs and entropy are known before the values are (a weighted likelihood, an entropy bonus):
+ * the logits are read once where rows fit the chip's registers. */
+sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logits, const sage_tensor *ids, float scale, const sage_tensor *g_log_probs,
+                                          const sage_tensor *g_entropy, const sage_tensor *log_probs, const sage_tensor *entropy, const sage_tensor *dlogits);
+
+/* AdamW over many tensors in one call.  For every element, g = grad * grad_scale:
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
+ * param f32, grad f32 / f16 / bf16, contiguous, of the same number of elements.  The states m, v are f32 (m_scale, v_scale
+ * unused, buf NULL), or m i8 and v u8 with f32 scales, one for each 256 elements of the tensor: |m| = m_scale code^2, sqrt(v) =
+ * v_scale code^2; zeroed codes and scales are zero states.  A second moment that is not zero does not become zero; a block in which a
+ * moment is not finite has a scale that is NaN.  `copy` (buf NULL: none) receives the updated parameters in f16 / bf16.  States of all
+ * tensors of a call have the same width.  step counts from 1. */
+typedef struct {
+    sage_tensor param, grad, m, v, m_scale, v_scale, copy;
+} sage_adamw_tensor;
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay, grad_scale;
+    int64_t step;
+} sage_adamw_opts;
+sage_status sage_adamw_step(sage_ctx *ctx, const sage_adamw_tensor *tensors, int32_t count, const sage_adamw_opts *opts);
+/* The values that 8-bit states stand for (a checkpoint, a report): m_out, v_out f32. */
+sage_status sage_adamw_states(sage_ctx *ctx, const sage_tensor *m, const sage_tensor *m_scale, const sage_tensor *v, const sage_tensor *v_scale,
+                              const sage_tensor *m_out, const sage_tensor *v_out);
 
 /* ------------------------------------------------------------------ multi-GPU (no reference counterpart:
  * the reference has no multi-device code).  Batch shards are independent; the only exchange

@@ -21,8 +21,10 @@ if not os.path.exists(_LIB_PATH):
 lib = ctypes.CDLL(_LIB_PATH)
 
 F32, I32, U32 = 0, 1, 2
-_NP = {F32: np.float32, I32: np.int32, U32: np.uint32}
-_DT = {np.dtype(np.float32): F32, np.dtype(np.int32): I32, np.dtype(np.uint32): U32}
+F16, BF16, I8, U8 = 3, 4, 5, 6  # storage types of the operators in sage_b200.language alone
+_NP = {F32: np.float32, I32: np.int32, U32: np.uint32, F16: np.float16, BF16: np.uint16, I8: np.int8, U8: np.uint8}  # bf16: its bits
+_DT = {np.dtype(np.float32): F32, np.dtype(np.int32): I32, np.dtype(np.uint32): U32, np.dtype(np.float16): F16, np.dtype(np.int8): I8, np.dtype(np.uint8): U8}
+_BY_NAME = {"float32": F32, "int32": I32, "uint32": U32, "float16": F16, "bfloat16": BF16, "int8": I8, "uint8": U8}
 MAX_DIMS = 8
 _P = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
@@ -260,6 +262,13 @@ class Context:
     def stream(self):
         return lib.sage_ctx_stream(self.h)
 
+    def use_stream(self, stream):
+        """Works on another runtime's stream (the value of a cudaStream_t) from here on, behind what was enqueued so far."""
+        self._ck(lib.sage_ctx_use_stream(self.h, _P(int(stream))))
+
+    def use_own_stream(self):
+        self._ck(lib.sage_ctx_use_own_stream(self.h))
+
     # --- raw buffers + op-level entry points (the device boundary of sage_cuda.h)
     def alloc(self, nbytes):
         b = _P()
@@ -278,19 +287,40 @@ class Context:
         self._ck(lib.sage_download(self.h, buf, ctypes.c_size_t(offset), _P(out.ctypes.data), ctypes.c_size_t(out.nbytes)))
         return out
 
-    def tensor(self, array):
-        """Uploads a numpy array into a fresh buffer and returns a DeviceTensor (contiguous)."""
+    def tensor(self, array, dtype=None):
+        """Uploads a numpy array into a fresh buffer and returns a DeviceTensor (contiguous).  Arrays of other types than the ones
+        of 4 bytes become f32 unless `dtype` asks for one (BF16 takes the bits as uint16)."""
         a = np.ascontiguousarray(array)
-        if a.dtype not in _DT:
+        if dtype is not None:
+            a = np.ascontiguousarray(a, dtype=_NP[dtype])
+        elif a.dtype not in _DT or a.dtype.itemsize != 4:
             a = a.astype(np.float32)
         buf = self.alloc(max(a.nbytes, 4))
         if a.nbytes:
             self.upload(buf, a)
-        return DeviceTensor(self, buf, _DT[a.dtype], a.shape if a.ndim else (1,))
+        return DeviceTensor(self, buf, _DT[a.dtype] if dtype is None else dtype, a.shape if a.ndim else (1,))
 
     def empty(self, shape, dtype=F32):
         n = int(np.prod(shape)) if len(shape) else 1
-        return DeviceTensor(self, self.alloc(max(n * 4, 4)), dtype, tuple(shape))
+        return DeviceTensor(self, self.alloc(max(n * np.dtype(_NP[dtype]).itemsize, 4)), dtype, tuple(shape))
+
+    def wrap(self, address, extents, dtype=F32, strides=None):
+        """A DeviceTensor over device memory that something else owns and keeps: `address` is its first element's.  No copy."""
+        extents = tuple(int(e) for e in extents)
+        t = DeviceTensor(self, None, dtype, extents, strides)
+        last = sum((e - 1) * s for e, s in zip(extents, t.strides)) if 0 not in extents else -1
+        t.buf = _P()
+        self._ck(lib.sage_buf_wrap(self.h, _P(address), ctypes.c_size_t((last + 1) * np.dtype(_NP[dtype]).itemsize), ctypes.byref(t.buf)))
+        return t
+
+    def borrow(self, t):
+        """wrap() of a device tensor of another package (a torch.Tensor: data_ptr(), shape, stride(), dtype), which is kept alive."""
+        name = str(t.dtype).split(".")[-1]
+        if name not in _BY_NAME:
+            raise SageError(1, "borrow: no element type for %s" % name)
+        d = self.wrap(t.data_ptr(), tuple(t.shape) or (1,), _BY_NAME[name], tuple(t.stride()) or (1,))
+        d.base = t
+        return d
 
 
 class DeviceTensor:
@@ -312,19 +342,27 @@ class DeviceTensor:
             t.extents[i], t.strides[i] = e, s
         return t
 
+    def ref(self):
+        """c() by reference, made once: a handle's view does not change."""
+        if getattr(self, "_ref", None) is None:
+            self._c = self.c()
+            self._ref = ctypes.byref(self._c)
+        return self._ref
+
     def view(self, extents, strides, offset=0):
         return DeviceTensor(self.ctx, self.buf, self.dtype, extents, strides, offset, owner=False)
 
     def numpy(self):
         n = lib.sage_buf_size(self.buf)
-        raw = self.ctx.download(self.buf, (n // 4,), _NP[self.dtype])
+        size = np.dtype(_NP[self.dtype]).itemsize
+        raw = self.ctx.download(self.buf, (n // size,), _NP[self.dtype])
         base = raw[self.offset:]
-        return np.ascontiguousarray(np.lib.stride_tricks.as_strided(base, shape=self.extents, strides=[s * 4 for s in self.strides]))
+        return np.ascontiguousarray(np.lib.stride_tricks.as_strided(base, shape=self.extents, strides=[s * size for s in self.strides]))
 
     def release(self):
         if self.owner and self.buf:
             self.ctx.free(self.buf)
-            self.buf = None
+            self.buf = self._ref = None
 
 
 # --------------------------------------------------------------------------- Var

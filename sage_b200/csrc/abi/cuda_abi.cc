@@ -41,6 +41,13 @@ static long long tensor_size(const sage_tensor *t) {
     return s;
 }
 
+// Elements that are not 4 bytes wide: for the operators of language_abi.cc alone.
+static bool narrow(const sage_tensor *t) { return t->dtype >= SAGE_F16 && t->dtype <= SAGE_U8; }
+template <typename... T>
+static bool narrow(const sage_tensor *t, T... more) { return narrow(t) || narrow(more...); }
+#define WIDE_OR_FAIL(what, ...) \
+    if (narrow(__VA_ARGS__)) return C.fail(SAGE_ERR_INVALID, what ": elements of 2 or 1 bytes are for the language-model operators")
+
 extern "C" {
 
 sage_status sage_device_count(int32_t *count) {
@@ -115,6 +122,16 @@ sage_status sage_selftest_bounded_wait(sage_ctx *ctx) {
     return k::bounded_wait_selftest(C);
 }
 
+sage_status sage_ctx_use_stream(sage_ctx *ctx, void *stream) {
+    CTX_OR_FAIL(ctx);
+    return C.use_stream((cudaStream_t)stream, false);
+}
+
+sage_status sage_ctx_use_own_stream(sage_ctx *ctx) {
+    CTX_OR_FAIL(ctx);
+    return C.use_stream(nullptr, true);
+}
+
 void *sage_ctx_stream(sage_ctx *ctx) { return (ctx && ctx->impl) ? (void *)ctx->impl->stream() : nullptr; }
 
 // ---------------------------------------------------------------- memory
@@ -131,6 +148,22 @@ sage_status sage_free(sage_ctx *ctx, sage_buf *buf) {
     if (!buf) return SAGE_OK;
     if (buf->block) C.allocator().free(buf->block);
     delete buf;
+    return SAGE_OK;
+}
+
+sage_status sage_buf_wrap(sage_ctx *ctx, void *device_ptr, size_t bytes, sage_buf **buf) {
+    CTX_OR_FAIL(ctx);
+    if (!buf || (!device_ptr && bytes)) return C.fail(SAGE_ERR_INVALID, "buf_wrap: no memory");
+    if (!C.dry() && bytes) {
+        cudaPointerAttributes a;
+        if (cudaPointerGetAttributes(&a, device_ptr) != cudaSuccess) {
+            cudaGetLastError();
+            return C.fail(SAGE_ERR_INVALID, "buf_wrap: not an address of this process's devices");
+        }
+        if (!(a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged) || a.device != C.device())
+            return C.fail(SAGE_ERR_INVALID, "buf_wrap: not memory of this context's device");
+    }
+    *buf = new sage_buf{nullptr, device_ptr, bytes, &C};
     return SAGE_OK;
 }
 
@@ -264,9 +297,11 @@ sage_status sage_launch(sage_ctx *ctx, sage_module *module, const char *name, co
 // ---------------------------------------------------------------- op-level entry points
 sage_status sage_map(sage_ctx *ctx, const char *expr, const sage_tensor *x, int32_t nx, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("map", y);
     if (!contiguous(y)) return C.fail(SAGE_ERR_INVALID, "map: output must be contiguous");
     std::vector<MapOperand> in(nx);
     for (int i = 0; i < nx; ++i) {
+        WIDE_OR_FAIL("map", &x[i]);
         if (x[i].ndim != y->ndim) return C.fail(SAGE_ERR_INVALID, "map: operand rank differs from the output's");
         in[i].dtype = x[i].dtype;
         in[i].ptr = tensor_ptr(&x[i]);
@@ -295,6 +330,7 @@ static void split_axes(const sage_tensor *x, const int32_t *axes, int naxes, k::
 
 sage_status sage_reduce(sage_ctx *ctx, int32_t kind, const sage_tensor *x, const int32_t *axes, int32_t naxes, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("reduce", x, y);
     if (!contiguous(y)) return C.fail(SAGE_ERR_INVALID, "reduce: output must be contiguous");
     k::Dims outer, inner;
     split_axes(x, axes, naxes, &outer, &inner);
@@ -304,6 +340,7 @@ sage_status sage_reduce(sage_ctx *ctx, int32_t kind, const sage_tensor *x, const
 
 sage_status sage_reduce_arg(sage_ctx *ctx, int32_t is_max, const sage_tensor *x, int32_t axis, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("reduce_arg", x, y);
     if (x->dtype != SAGE_F32) return C.fail(SAGE_ERR_UNSUPPORTED, "reduce_arg: only float input");
     k::Dims outer, inner;
     split_axes(x, &axis, 1, &outer, &inner);
@@ -313,12 +350,14 @@ sage_status sage_reduce_arg(sage_ctx *ctx, int32_t is_max, const sage_tensor *x,
 
 sage_status sage_softmax(sage_ctx *ctx, const sage_tensor *x, int64_t rows, int64_t inner, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("softmax", x, y);
     if (!contiguous(x) || !contiguous(y) || tensor_size(x) != rows * inner) return C.fail(SAGE_ERR_INVALID, "softmax: bad layout");
     return k::softmax_rows(C, (const float *)tensor_ptr(x), (float *)tensor_ptr(y), rows, inner);
 }
 
 sage_status sage_log_sum_exp(sage_ctx *ctx, const sage_tensor *x, int64_t rows, int64_t inner, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("log_sum_exp", x, y);
     if (!contiguous(x) || !contiguous(y) || tensor_size(x) != rows * inner || tensor_size(y) != rows)
         return C.fail(SAGE_ERR_INVALID, "log_sum_exp: bad layout");
     return k::lse_rows(C, (const float *)tensor_ptr(x), (float *)tensor_ptr(y), rows, inner);
@@ -327,6 +366,7 @@ sage_status sage_log_sum_exp(sage_ctx *ctx, const sage_tensor *x, int64_t rows, 
 sage_status sage_layer_norm(sage_ctx *ctx, const sage_tensor *x, int64_t rows, int64_t inner, const sage_tensor *gamma,
                             const sage_tensor *beta, float eps, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("layer_norm", x, gamma, beta, y);
     if (!contiguous(x) || !contiguous(y) || tensor_size(x) != rows * inner) return C.fail(SAGE_ERR_INVALID, "layer_norm: bad layout");
     const long long gs = tensor_size(gamma), bs = tensor_size(beta);
     if ((gs != 1 && gs != inner) || (bs != 1 && bs != inner)) return C.fail(SAGE_ERR_INVALID, "layer_norm: gamma/beta size");
@@ -336,6 +376,7 @@ sage_status sage_layer_norm(sage_ctx *ctx, const sage_tensor *x, int64_t rows, i
 
 sage_status sage_gather(sage_ctx *ctx, const sage_tensor *x, const sage_tensor *ind, int32_t axis, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("gather", x, ind, y);
     if (x->ndim != ind->ndim || !contiguous(y) || tensor_size(y) != tensor_size(ind)) return C.fail(SAGE_ERR_INVALID, "gather: bad shapes");
     long long xs[SAGE_MAX_DIMS];
     for (int i = 0; i < x->ndim; ++i) xs[i] = x->strides[i];
@@ -345,6 +386,7 @@ sage_status sage_gather(sage_ctx *ctx, const sage_tensor *x, const sage_tensor *
 
 sage_status sage_scatter(sage_ctx *ctx, const sage_tensor *x, const sage_tensor *ind, int32_t axis, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("scatter", x, ind, y);
     if (x->ndim != ind->ndim || x->ndim != y->ndim || !contiguous(y) || x->dtype != SAGE_F32)
         return C.fail(SAGE_ERR_INVALID, "scatter: bad shapes");
     C.note_memset();
@@ -363,6 +405,7 @@ sage_status sage_scatter(sage_ctx *ctx, const sage_tensor *x, const sage_tensor 
 
 sage_status sage_unslice(sage_ctx *ctx, const sage_tensor *x, int32_t axis, int64_t start, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("unslice", x, y);
     if (x->ndim != y->ndim || !contiguous(y)) return C.fail(SAGE_ERR_INVALID, "unslice: bad shapes");
     C.note_memset();
     if (!C.dry()) {
@@ -376,11 +419,13 @@ sage_status sage_unslice(sage_ctx *ctx, const sage_tensor *x, int32_t axis, int6
 
 sage_status sage_concat(sage_ctx *ctx, const sage_tensor *xs, int32_t nx, int32_t axis, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("concat", y);
     if (!contiguous(y)) return C.fail(SAGE_ERR_INVALID, "concat: output must be contiguous");
     long long ys[SAGE_MAX_DIMS];
     for (int i = 0; i < y->ndim; ++i) ys[i] = y->strides[i];
     long long at = 0;
     for (int q = 0; q < nx; ++q) {
+        WIDE_OR_FAIL("concat", &xs[q]);
         sage_status st = k::strided_copy(C, (const uint32_t *)tensor_ptr(&xs[q]), tensor_dims(&xs[q]),
                                          (uint32_t *)tensor_ptr(y) + at * y->strides[axis], ys);
         if (st) return st;
@@ -412,6 +457,7 @@ static k::Window to_window(const sage_window *w) {
 
 sage_status sage_im2col(sage_ctx *ctx, const sage_tensor *x, const sage_window *w, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("im2col", x, y);
     if (x->ndim != 4 || y->ndim != 6 || !contiguous(x) || !contiguous(y)) return C.fail(SAGE_ERR_INVALID, "im2col: bad layout");
     return k::im2col(C, (const float *)tensor_ptr(x), (float *)tensor_ptr(y), x->extents[0], x->extents[1], x->extents[2],
                      x->extents[3], y->extents[1], y->extents[2], to_window(w));
@@ -419,6 +465,7 @@ sage_status sage_im2col(sage_ctx *ctx, const sage_tensor *x, const sage_window *
 
 sage_status sage_col2im(sage_ctx *ctx, const sage_tensor *x, const sage_window *w, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("col2im", x, y);
     if (x->ndim != 6 || y->ndim != 4 || !contiguous(x) || !contiguous(y)) return C.fail(SAGE_ERR_INVALID, "col2im: bad layout");
     return k::col2im(C, (const float *)tensor_ptr(x), (float *)tensor_ptr(y), y->extents[0], y->extents[1], y->extents[2],
                      y->extents[3], x->extents[1], x->extents[2], to_window(w));
@@ -426,6 +473,7 @@ sage_status sage_col2im(sage_ctx *ctx, const sage_tensor *x, const sage_window *
 
 sage_status sage_pool2d(sage_ctx *ctx, int32_t is_max, const sage_tensor *x, const sage_window *w, const sage_tensor *y) {
     CTX_OR_FAIL(ctx);
+    WIDE_OR_FAIL("pool2d", x, y);
     if (x->ndim != 4 || y->ndim != 4 || !contiguous(x) || !contiguous(y)) return C.fail(SAGE_ERR_INVALID, "pool2d: bad layout");
     return k::pool2d(C, is_max != 0, (const float *)tensor_ptr(x), (float *)tensor_ptr(y), x->extents[0], x->extents[1],
                      x->extents[2], x->extents[3], y->extents[1], y->extents[2], to_window(w), k::PlaneOut());

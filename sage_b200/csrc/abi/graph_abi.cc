@@ -43,6 +43,11 @@ static sage_status guarded(F f) {
     }
 }
 
+// Variables hold elements of 4 bytes.
+static int var_dtype(int32_t dtype) {
+    if (dtype >= SAGE_F16 && dtype <= SAGE_U8) shape_fail("variables are f32, i32 or u32");
+    return dtype;
+}
 static Array arr(int32_t n, const int64_t *v) { return Array(v, v + n); }
 static std::vector<long long> axes_of(int32_t n, const int64_t *v) { return std::vector<long long>(v, v + n); }
 static sage_status ret(sage_var **out, const Var &v) {
@@ -84,7 +89,7 @@ sage_status sage_var_from_host(sage_session *s, int32_t dtype, int32_t ndim, con
         Context &C = s->impl->ctx();
         C.make_current();
         Tensor t;
-        sage_status st = Tensor::uninit(C, TensorDesc(infer_extents(arr(ndim, extents), 0), dtype), &t);
+        sage_status st = Tensor::uninit(C, TensorDesc(infer_extents(arr(ndim, extents), 0), var_dtype(dtype)), &t);
         if (st) return st;
         st = upload_into(C, &t, data, false);
         if (st) return st;
@@ -93,11 +98,11 @@ sage_status sage_var_from_host(sage_session *s, int32_t dtype, int32_t ndim, con
 }
 
 sage_status sage_var_from_host_lazy(int32_t dtype, int32_t ndim, const int64_t *extents, const void *data, sage_var **out) {
-    return guarded([&]() -> sage_status { return ret(out, Var::from_tensor(Tensor::from_host(infer_extents(arr(ndim, extents), 0), dtype, data))); });
+    return guarded([&]() -> sage_status { return ret(out, Var::from_tensor(Tensor::from_host(infer_extents(arr(ndim, extents), 0), var_dtype(dtype), data))); });
 }
 
 sage_status sage_var_empty(int32_t dtype, int32_t ndim, const int64_t *extents, sage_var **out) {
-    return guarded([&]() -> sage_status { return ret(out, Var::empty(arr(ndim, extents), dtype)); });
+    return guarded([&]() -> sage_status { return ret(out, Var::empty(arr(ndim, extents), var_dtype(dtype))); });
 }
 
 sage_status sage_var_set(sage_session *s, sage_var *v, const void *data, int32_t async) {

@@ -122,7 +122,8 @@ sage_status Context::create(int device, const sage_ctx_opts &opts, Context **out
     }
     if (cudaSetDevice(device) != cudaSuccess) return SAGE_ERR_DEVICE;
     if (cudaFree(0) != cudaSuccess) return SAGE_ERR_DEVICE;
-    if (cudaStreamCreateWithFlags(&c->stream_, cudaStreamNonBlocking) != cudaSuccess) return SAGE_ERR_DEVICE;
+    if (cudaStreamCreateWithFlags(&c->own_stream_, cudaStreamNonBlocking) != cudaSuccess) return SAGE_ERR_DEVICE;
+    c->stream_ = c->own_stream_;
     cudaDeviceGetAttribute(&c->sm_count, cudaDevAttrMultiProcessorCount, device);
     if (!cap) {
         size_t free_b = 0, total_b = 0;
@@ -133,6 +134,26 @@ sage_status Context::create(int device, const sage_ctx_opts &opts, Context **out
     if (cudaMalloc(&c->status_word_dev, 4096) != cudaSuccess) return SAGE_ERR_DEVICE;
     cudaMemsetAsync(c->status_word_dev, 0, 4096, c->stream_);
     *out = c.release();
+    return SAGE_OK;
+}
+
+sage_status Context::use_stream(cudaStream_t s, bool own) {
+    if (dry()) return SAGE_OK;
+    if (own) s = own_stream_;
+    if (s == stream_) return SAGE_OK;
+    cudaEvent_t ev = (cudaEvent_t)handover_event_;
+    sage_status st;
+    if (!ev) {
+        st = check_cuda(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming), "use_stream: event");
+        if (st) return st;
+        handover_event_ = ev;
+    }
+    // The pool hands blocks on in the order of launches, so the new stream waits for all that the old one holds.
+    st = check_cuda(cudaEventRecord(ev, stream_), "use_stream: record");
+    if (st) return st;
+    st = check_cuda(cudaStreamWaitEvent(s, ev, 0), "use_stream: wait");
+    if (st) return st;
+    stream_ = s;
     return SAGE_OK;
 }
 
@@ -154,7 +175,8 @@ Context::~Context() {
         gemm_trace_block = nullptr;
         alloc_.reset();
         if (status_word_dev) cudaFree(status_word_dev);
-        cudaStreamDestroy(stream_);
+        if (handover_event_) cudaEventDestroy((cudaEvent_t)handover_event_);
+        cudaStreamDestroy(own_stream_);
     }
 }
 

@@ -118,6 +118,8 @@ public:
     void make_current() const;
     bool dry() const { return device_ < 0; }
     cudaStream_t stream() const { return stream_; }
+    // Works on `s` from here on (null handles are streams too: `own` asks for the context's own one), behind what has been enqueued.
+    sage_status use_stream(cudaStream_t s, bool own);
     const sage_ctx_opts &opts() const { return opts_; }
     Allocator &allocator() { return *alloc_; }
     // Tensors keep the allocator alive past the context, so a handle dropped late still returns
@@ -202,7 +204,8 @@ public:
 private:
     Context() {}
     int device_ = -1;
-    cudaStream_t stream_ = nullptr;
+    cudaStream_t stream_ = nullptr, own_stream_ = nullptr;
+    void *handover_event_ = nullptr;  // cudaEvent_t of use_stream
     sage_ctx_opts opts_{};
     std::shared_ptr<Allocator> alloc_;
     std::string last_error_;
