@@ -15,79 +15,338 @@ namespace k {
 
 namespace {
 
-constexpr int kThreads = 256;
+// ------------------------------------------------------------------------------------------ elements
+// 16 bytes of a row as they lie in memory.  `kFill` stands for elements outside the row: -inf, which adds nothing.
+template <class T>
+struct Bits;
+template <>
+struct Bits<float> {
+    static constexpr int N = 4;
+    static constexpr unsigned kFill = 0xff800000u;
+    __device__ static unsigned element(const void *p) { return *(const unsigned *)p; }
+    __device__ static void put(uint4 &v, int j, unsigned e) { (&v.x)[j] = e; }
+    __device__ static float largest(const uint4 &v) { return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))); }
+    __device__ static void unpack(const uint4 &v, float *x) {
+        x[0] = __uint_as_float(v.x);
+        x[1] = __uint_as_float(v.y);
+        x[2] = __uint_as_float(v.z);
+        x[3] = __uint_as_float(v.w);
+    }
+};
+template <class T, class T2>
+struct Bits16 {
+    static constexpr int N = 8;
+    __device__ static unsigned element(const void *p) { return *(const unsigned short *)p; }
+    __device__ static void put(uint4 &v, int j, unsigned e) {
+        unsigned &w = (&v.x)[j / 2];
+        w = j % 2 ? (w & 0xffffu) | e << 16 : (w & 0xffff0000u) | e;
+    }
+    __device__ static T2 pair(unsigned w) { return *reinterpret_cast<T2 *>(&w); }
+    __device__ static float largest(const uint4 &v) {  // two at a time; NaN loses
+        const T2 h = __hmax2(__hmax2(pair(v.x), pair(v.y)), __hmax2(pair(v.z), pair(v.w)));
+        return fmaxf(widen(h.x), widen(h.y));
+    }
+    __device__ static void unpack(const uint4 &v, float *x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T2 h = pair((&v.x)[i]);
+            x[2 * i] = widen(h.x);
+            x[2 * i + 1] = widen(h.y);
+        }
+    }
+};
+template <>
+struct Bits<__half> : Bits16<__half, __half2> {
+    static constexpr unsigned kFill = 0xfc00fc00u;
+};
+template <>
+struct Bits<__nv_bfloat16> : Bits16<__nv_bfloat16, __nv_bfloat162> {
+    static constexpr unsigned kFill = 0xff80ff80u;
+};
 
-// Larger for larger logits and, among equals, for lower tokens; no two tokens of a row have the same.  NaN counts as -inf.
-__device__ __forceinline__ unsigned long long rank_key(float x, unsigned token) {
+// A row cut into 16-byte vectors at addresses that are multiples of 16: vector i holds elements i * N - head onwards, and those of
+// [first, full) lie wholly in the row.  The others are read element by element, so nothing outside the row is touched.
+template <class T>
+struct RowVectors {
+    static constexpr int N = Bits<T>::N;
+    const char *origin;  // of vector 0; in front of the row when head > 0
+    int head, first, full, count, cols;
+    __device__ RowVectors(const void *row, long long cols_) {
+        head = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+        origin = (const char *)row - head * sizeof(T);
+        cols = (int)cols_;
+        first = head ? 1 : 0;
+        full = (int)((head + cols_) / N);
+        count = (int)((head + cols_ + N - 1) / N);
+    }
+    __device__ __forceinline__ bool whole(int i) const { return i >= first && i < full; }
+    __device__ __forceinline__ long long element(int i) const { return (long long)i * N - head; }
+    template <bool READ_ONLY>
+    __device__ __forceinline__ uint4 load(int i) const {
+        const uint4 *p = reinterpret_cast<const uint4 *>(origin) + i;
+        if (whole(i)) {
+            uint4 v;
+            if (READ_ONLY) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+            else asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+            return v;
+        }
+        return load_edge(i);
+    }
+    __device__ __noinline__ uint4 load_edge(int i) const {
+        uint4 v = nothing();
+        const long long e = element(i);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (e + j >= 0 && e + j < cols) Bits<T>::put(v, j, Bits<T>::element(origin + 16ll * i + j * (int)sizeof(T)));
+        return v;
+    }
+    __device__ __forceinline__ static uint4 nothing() { return make_uint4(Bits<T>::kFill, Bits<T>::kFill, Bits<T>::kFill, Bits<T>::kFill); }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; below 2^-126 zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ------------------------------------------------------------------------------------------ sums of a part of a row
+// The part's largest logit m, s = sum exp(c (x - m)) and w = sum (x - m) exp(c (x - m)); with m = -inf both are relative to 0.
+// c2 = c log2(e).  Differences are taken before they are scaled, so that a large m costs nothing.
+struct Sums {
+    float m = -INFINITY, s = 0.f, w = 0.f;
+};
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+// Makes the sums relative to `m`.  A factor of zero takes all with it (a part of masks of the type's lowest value), NaN stays in s.
+__device__ __forceinline__ void move_to(Sums &a, float m, float c2) {
+    const float d = a.m - base_of(m), f = exp2_fast(d * c2);
+    a.w = f > 0.f ? f * (a.w + d * a.s) : 0.f;
+    a.s *= f;
+    a.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c2) {
+    const float m = fmaxf(a.m, b.m);
+    move_to(a, m, c2);
+    move_to(b, m, c2);
+    a.s += b.s;
+    a.w += b.w;
+    return a;
+}
+template <class T, int U>
+__device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float c2) {
+    float m = Bits<T>::largest(v[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) m = fmaxf(m, Bits<T>::largest(v[u]));
+    if (m > a.m) move_to(a, m, c2);
+    const float base = base_of(a.m);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float x[Bits<T>::N];
+        Bits<T>::unpack(v[u], x);
+#pragma unroll
+        for (int j = 0; j < Bits<T>::N; ++j) {
+            const float d = x[j] - base, e = exp2_fast(d * c2);
+            a.s += e;
+            a.w = fmaf(e, fmaxf(d, -FLT_MAX), a.w);  // masked: 0 times a number
+        }
+    }
+}
+__device__ __forceinline__ Sums warp_join(Sums a, float c2, int width = 32) {
+    for (int o = width / 2; o; o >>= 1) {
+        Sums b;
+        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+        b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
+        a = join(a, b, c2);
+    }
+    return a;
+}
+// Of all threads, in every thread.  `shared`: one for each warp.
+template <int THREADS>
+__device__ __forceinline__ Sums block_join(Sums a, float c2, Sums *shared) {
+    a = warp_join(a, c2);
+    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = a;
+    __syncthreads();
+    constexpr int W = THREADS / 32;
+    return warp_join(shared[threadIdx.x % W], c2, W);  // lanes that hold the same values join to the same result
+}
+
+// ------------------------------------------------------------------------------------------ clusters: CTAs that share a row
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// The address in CTA `rank`'s shared memory of what lies at `p` in this one's.
+__device__ __forceinline__ unsigned peer_shared(const void *p, unsigned rank) {
+    unsigned a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void peer_store(unsigned a, float x) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(x) : "memory"); }
+__device__ __forceinline__ void peer_store(unsigned a, unsigned long long x) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(x) : "memory"); }
+
+// ------------------------------------------------------------------------------------------ alternatives
+// Larger for larger logits and, among equals, for lower tokens; no two tokens of a row have the same, and none has 0.  NaN counts as -inf.
+__device__ __forceinline__ unsigned rank_bits(float x) {
     x = x != x ? -INFINITY : x + 0.f;  // -0 and 0 are equal
     const unsigned b = __float_as_uint(x);
-    return (unsigned long long)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xffffffffu - token);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ unsigned long long rank_key(float x, unsigned token) { return (unsigned long long)rank_bits(x) << 32 | (0xffffffffu - token); }
 __device__ __forceinline__ float rank_logit(unsigned long long key) {
     const unsigned b = (unsigned)(key >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
-template <class V, class F>
-__device__ V block_combine(V v, F f, V *shared) {
-    for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = v;
+// The warp's largest keys, sorted over its lanes; `least` is the k-th, what a key has to pass.
+struct TopList {
+    unsigned long long key = 0, least = 0;
+    __device__ __forceinline__ void offer(unsigned long long x, bool want, int k) {
+        unsigned todo = __ballot_sync(0xffffffffu, want && x > least);
+        while (todo) {
+            const unsigned long long y = __shfl_sync(0xffffffffu, x, __ffs(todo) - 1);
+            todo &= todo - 1;
+            if (y <= least) continue;
+            const unsigned lane = threadIdx.x % 32, at = __popc(__ballot_sync(0xffffffffu, key > y));
+            const unsigned long long before = __shfl_up_sync(0xffffffffu, key, 1);
+            key = lane < at ? key : lane == at ? y : before;
+            least = __shfl_sync(0xffffffffu, key, k - 1);
+        }
+    }
+};
+
+template <int THREADS>
+struct TopShared {
+    unsigned short chosen[THREADS];
+    int count;
+    unsigned long long lists[THREADS / 32][kMaxTop];
+};
+
+// The k largest of the block's vectors [begin, end), in warp 0's list.  Each thread knows the largest of the vectors it has summed
+// (begin + its number + multiples of THREADS).  The k-th largest of those maxima bounds the k-th largest element from below, and only
+// threads whose maximum reaches it hold candidates: about k of them, whose vectors are read again (from L2).  The bound is taken to
+// 16 bits of the order, which ties and nearness make a little lower.  Where many threads reach it (masks that leave less than k tokens,
+// equal logits), everything is read again in order.
+template <class T, int THREADS>
+__device__ TopList block_top(const RowVectors<T> &row, int begin, int end, float thread_max, int k, TopShared<THREADS> &sh) {
+    constexpr int N = Bits<T>::N, W = THREADS / 32;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const unsigned mine = begin + (int)threadIdx.x < end ? rank_bits(thread_max) >> 16 : 0;
+    unsigned bound = 0;
+    for (int bit = 15; bit >= 0; --bit) {
+        const unsigned t = bound | 1u << bit;
+        if (__syncthreads_count(mine >= t) >= k) bound = t;
+    }
+    if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    v = shared[0];
-    for (int i = 1; i < kThreads / 32; ++i) v = f(v, shared[i]);
+    if (mine >= bound) sh.chosen[atomicAdd(&sh.count, 1)] = (unsigned short)threadIdx.x;  // in any order: keys decide
     __syncthreads();
-    return v;
+    const int sets = sh.count;
+    const bool all = sets > THREADS / 4;
+    TopList list;
+    for (int q = warp; q < (all ? W : sets); q += W) {
+        // all: the warp's 32 vectors of every THREADS; else the vectors of one thread, one for each lane
+        const int from = all ? begin + warp * 32 + lane : begin + sh.chosen[q] + lane * THREADS, step = all ? THREADS : 32 * THREADS;
+        for (int base = from - (all ? lane : lane * THREADS), i = from; base < end; base += step, i += step) {
+            const bool some = i < end;
+            const uint4 v = some ? row.template load<true>(i) : RowVectors<T>::nothing();
+            float x[N];
+            Bits<T>::unpack(v, x);
+            const long long e = row.element(i);
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < N; ++j) any |= rank_bits(x[j]) >> 16 >= bound;
+            if (!__any_sync(0xffffffffu, any && some)) continue;
+#pragma unroll 1
+            for (int j = 0; j < N; ++j) {
+                float y = x[0];
+#pragma unroll
+                for (int l = 1; l < N; ++l) y = j == l ? x[l] : y;
+                const bool in = some && e + j >= 0 && e + j < row.cols && rank_bits(y) >> 16 >= bound;
+                list.offer(rank_key(y, (unsigned)(e + j)), in, k);
+            }
+        }
+    }
+    if (lane < kMaxTop) sh.lists[warp][lane] = lane < k ? list.key : 0;
+    __syncthreads();
+    if (warp == 0)
+        for (int w = 1; w < W; ++w) list.offer(sh.lists[w][lane], true, k);
+    return list;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) log_probs_kernel(const LogProbs a) {
+// ------------------------------------------------------------------------------------------ values
+constexpr int kMaxCluster = 8;
+
+// A cluster of `parts` CTAs for each row; each reads a part of it once.
+template <class T, int THREADS, bool TOP>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(const LogProbs a, const int parts) {
+    constexpr int U = 4;
+    __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
+    __shared__ unsigned long long part_lists[TOP ? kMaxCluster : 1][kMaxTop];
+    __shared__ TopShared<TOP ? THREADS : 32> top;
     grid_dependency_sync();
-    __shared__ float fs[kThreads / 32];
-    __shared__ unsigned long long ks[kThreads / 32];
-    const long long r = blockIdx.x, vocab = a.logits.cols;
+    if (parts > 1) cluster_arrive();
+    const long long r = blockIdx.x / (unsigned)parts;
+    const unsigned rank = parts > 1 ? cluster_rank() : 0;
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
-    float m = -INFINITY;
-    for (long long j = threadIdx.x; j < vocab; j += kThreads) m = fmaxf(m, widen(x[j]));
-    m = block_combine(m, [](float p, float q) { return fmaxf(p, q); }, fs);
-    const float base = m == -INFINITY ? 0.f : m;
-    float s = 0.f, sd = 0.f;
-    for (long long j = threadIdx.x; j < vocab; j += kThreads) {
-        const float d = (widen(x[j]) - base) * a.scale, e = expf(d);
-        s += e;
-        sd += e * fmaxf(d, -FLT_MAX);
-    }
-    s = block_combine(s, [](float p, float q) { return p + q; }, fs);
-    sd = block_combine(sd, [](float p, float q) { return p + q; }, fs);
-    const bool none = s == 0.f;
-    const float ln_s = logf(s);
-    if (threadIdx.x == 0) {
+    const RowVectors<T> row(x, a.logits.cols);
+    const int each = (row.count + parts - 1) / parts, begin = (int)rank * each, end = min(begin + each, row.count);
+    const float c2 = a.scale * 1.4426950408889634f;
+    float own = 0.f;
+    bool scored = false;
+    if (rank == 0 && threadIdx.x == 0) {
         const int id = ((const int *)a.ids.ptr)[r * a.ids.stride];
-        float lp = 0.f;
-        if (id >= 0 && id < vocab) lp = none ? -INFINITY : (widen(x[id]) - base) * a.scale - ln_s;
-        ((float *)a.log_probs.ptr)[r * a.log_probs.stride] = lp;
-        if (a.entropy.ptr) ((float *)a.entropy.ptr)[r * a.entropy.stride] = none ? 0.f : ln_s - sd / s;
+        scored = id >= 0 && id < a.logits.cols;
+        if (scored) own = widen(x[id]);
+    }
+    Sums mine;
+    for (int i = begin + (int)threadIdx.x; i < end; i += THREADS * U) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = i + u * THREADS < end ? row.template load<true>(i + u * THREADS) : RowVectors<T>::nothing();
+        add_vectors<T, U>(mine, v, c2);
+    }
+    const float thread_max = mine.m;
+    Sums all = block_join<THREADS>(mine, c2, sums);
+    TopList list;
+    if constexpr (TOP) list = block_top<T, THREADS>(row, begin, end, thread_max, a.top, top);
+    const int lane = threadIdx.x % 32;
+    if (parts > 1) {  // everything to the first CTA, which has started by now
+        cluster_wait();
+        if (threadIdx.x == 0) {
+            const unsigned to = peer_shared(&part_sums[rank], 0);
+            peer_store(to, all.m);
+            peer_store(to + 4, all.s);
+            peer_store(to + 8, all.w);
+        }
+        if (TOP && threadIdx.x < 32) peer_store(peer_shared(&part_lists[TOP ? rank : 0][lane], 0), lane < a.top ? list.key : 0ull);
+        cluster_arrive();
+        cluster_wait();
+        if (rank) return;
+        all = warp_join(lane % kMaxCluster < parts ? part_sums[lane % kMaxCluster] : Sums(), c2, kMaxCluster);
+        if (TOP && threadIdx.x < 32)
+            for (int p = 1; p < parts; ++p) list.offer(part_lists[TOP ? p : 0][lane], true, a.top);
+    }
+    const float base = base_of(all.m), ln_s = logf(all.s);
+    const bool none = all.s == 0.f;
+    if (threadIdx.x == 0) {
+        ((float *)a.log_probs.ptr)[r * a.log_probs.stride] = !scored ? 0.f : none ? -INFINITY : (own - base) * a.scale - ln_s;
+        if (a.entropy.ptr) ((float *)a.entropy.ptr)[r * a.entropy.stride] = none ? 0.f : ln_s - a.scale * (all.w / all.s);
         if (a.stats.ptr) {
-            ((float *)a.stats.ptr)[r * a.stats.pitch] = m;
-            ((float *)a.stats.ptr)[r * a.stats.pitch + 1] = s;
+            ((float *)a.stats.ptr)[r * a.stats.pitch] = all.m;
+            ((float *)a.stats.ptr)[r * a.stats.pitch + 1] = all.s;
         }
     }
-    unsigned long long below = ~0ull;
-    for (int i = 0; i < a.top; ++i) {
-        unsigned long long best = 0;
-        for (long long j = threadIdx.x; j < vocab; j += kThreads) {
-            const unsigned long long key = rank_key(widen(x[j]), (unsigned)j);
-            if (key < below && key > best) best = key;
-        }
-        below = block_combine(best, [](unsigned long long p, unsigned long long q) { return p > q ? p : q; }, ks);
-        if (threadIdx.x == 0) {
-            ((int *)a.top_ids.ptr)[r * a.top_ids.pitch + i] = (int)(0xffffffffu - (unsigned)below);
-            ((float *)a.top_log_probs.ptr)[r * a.top_log_probs.pitch + i] = none ? -INFINITY : (rank_logit(below) - base) * a.scale - ln_s;
-        }
+    if (TOP && (int)threadIdx.x < a.top) {
+        ((int *)a.top_ids.ptr)[r * a.top_ids.pitch + lane] = (int)(0xffffffffu - (unsigned)list.key);
+        ((float *)a.top_log_probs.ptr)[r * a.top_log_probs.pitch + lane] = none ? -INFINITY : (rank_logit(list.key) - base) * a.scale - ln_s;
     }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) log_probs_grad_kernel(const LogProbsGrad a) {
+__global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad a) {
     grid_dependency_sync();
     const long long r = blockIdx.x, vocab = a.logits.cols;
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
@@ -98,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) log_probs_grad_kernel(const LogProbs
     const float ge = a.g_entropy.ptr ? ((const float *)a.g_entropy.ptr)[r * a.g_entropy.stride] : 0.f;
     const float h = a.g_entropy.ptr ? ((const float *)a.entropy.ptr)[r * a.entropy.stride] : 0.f;
     const float ln_s = logf(s);
-    for (long long j = threadIdx.x; j < vocab; j += kThreads) {
+    for (long long j = threadIdx.x; j < vocab; j += 256) {
         float v = 0.f;
         if (s != 0.f) {
             const float d = (widen(x[j]) - m) * a.scale, p = expf(d) / s;
@@ -108,6 +367,21 @@ __global__ void __launch_bounds__(kThreads) log_probs_grad_kernel(const LogProbs
     }
 }
 
+// How many CTAs share a row: the fewest steps of a grid of `slots` resident CTAs, each step the part's bytes and a fixed cost that
+// measures like 24 KB of them (joining, the cluster's barriers).
+int parts_of_rows(long long rows, long long bytes, long long slots) {
+    int best = 1;
+    double least = 0;
+    for (int c = 1; c <= kMaxCluster; c *= 2) {
+        const double cost = (double)((rows * c + slots - 1) / slots) * ((double)bytes / c + 24576.0);
+        if (c == 1 || cost < least) {
+            best = c;
+            least = cost;
+        }
+    }
+    return rows * best > 0x7fffffffll ? 1 : best;
+}
+
 }  // namespace
 
 sage_status token_log_probs(Context &ctx, const LogProbs &a) {
@@ -115,7 +389,15 @@ sage_status token_log_probs(Context &ctx, const LogProbs &a) {
     ctx.note_launch("token_log_probs");
     if (ctx.dry()) return SAGE_OK;
     return with_type(a.logits.dtype, [&](auto t) {
-        return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), log_probs_kernel<decltype(t)>, dim3((unsigned)a.logits.rows), dim3(kThreads), 0, a), "token_log_probs");
+        typedef decltype(t) T;
+        const long long bytes = a.logits.cols * (long long)sizeof(T);
+        auto launch = [&](auto kernel, int threads) {
+            const int parts = threads == 128 ? 1 : parts_of_rows(a.logits.rows, bytes, ctx.sm_count * 2ll);
+            return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, parts), "token_log_probs");
+        };
+        // Short rows: four warps for each, or most threads of a large block would have nothing to read.
+        if (bytes <= 16384) return a.top ? launch(log_probs_kernel<T, 128, true>, 128) : launch(log_probs_kernel<T, 128, false>, 128);
+        return a.top ? launch(log_probs_kernel<T, 512, true>, 512) : launch(log_probs_kernel<T, 512, false>, 512);
     });
 }
 
@@ -124,7 +406,7 @@ sage_status token_log_probs_grad(Context &ctx, const LogProbsGrad &a) {
     ctx.note_launch("token_log_probs_grad");
     if (ctx.dry()) return SAGE_OK;
     return with_type(a.logits.dtype, [&](auto t) {
-        return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), log_probs_grad_kernel<decltype(t)>, dim3((unsigned)a.logits.rows), dim3(kThreads), 0, a), "token_log_probs_grad");
+        return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), log_probs_grad_kernel<decltype(t)>, dim3((unsigned)a.logits.rows), dim3(256), 0, a), "token_log_probs_grad");
     });
 }
 
