@@ -81,16 +81,33 @@ struct RowVectors {
     }
     __device__ __forceinline__ bool whole(int i) const { return i >= first && i < full; }
     __device__ __forceinline__ long long element(int i) const { return (long long)i * N - head; }
+    // Of a vector that lies wholly in the row.
     template <bool READ_ONLY>
-    __device__ __forceinline__ uint4 load(int i) const {
+    __device__ __forceinline__ uint4 load_whole(int i) const {
         const uint4 *p = reinterpret_cast<const uint4 *>(origin) + i;
-        if (whole(i)) {
-            uint4 v;
-            if (READ_ONLY) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-            else asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-            return v;
+        uint4 v;
+        if (READ_ONLY) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+        else asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+        return v;
+    }
+    __device__ __forceinline__ uint4 load(int i) const { return whole(i) ? load_whole<true>(i) : load_edge(i); }
+    // Vectors i, i + STEP ...: those of [0, end).
+    template <int U, int STEP, bool READ_ONLY>
+    __device__ __forceinline__ void load_all(uint4 (&v)[U], int i, int end) const {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u] = nothing();
+            if (i + u * STEP < end && whole(i + u * STEP)) v[u] = load_whole<READ_ONLY>(i + u * STEP);
         }
-        return load_edge(i);
+        // the row's first and last vector, where they reach beyond it
+#pragma unroll 1
+        for (int at = 0; at < count; at += max(count - 1, 1)) {
+            if (whole(at) || at < i || at >= end || at > i + (U - 1) * STEP || (at - i) % STEP) continue;
+            const uint4 e = load_edge(at);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u * STEP == at) v[u] = e;
+        }
     }
     __device__ __noinline__ uint4 load_edge(int i) const {
         uint4 v = nothing();
@@ -251,7 +268,7 @@ __device__ TopList block_top(const RowVectors<T> &row, int begin, int end, float
         const int from = all ? begin + warp * 32 + lane : begin + sh.chosen[q] + lane * THREADS, step = all ? THREADS : 32 * THREADS;
         for (int base = from - (all ? lane : lane * THREADS), i = from; base < end; base += step, i += step) {
             const bool some = i < end;
-            const uint4 v = some ? row.template load<true>(i) : RowVectors<T>::nothing();
+            const uint4 v = some ? row.load(i) : RowVectors<T>::nothing();
             float x[N];
             Bits<T>::unpack(v, x);
             const long long e = row.element(i);
@@ -304,8 +321,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     Sums mine;
     for (int i = begin + (int)threadIdx.x; i < end; i += THREADS * U) {
         uint4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = i + u * THREADS < end ? row.template load<true>(i + u * THREADS) : RowVectors<T>::nothing();
+        row.template load_all<U, THREADS, true>(v, i, end);
         add_vectors<T, U>(mine, v, c2);
     }
     const float thread_max = mine.m;
@@ -345,26 +361,146 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     }
 }
 
+// ------------------------------------------------------------------------------------------ gradient
+// With e = exp(c (x - m)), p = e / S and K = H - ln S:
+//   dx_j = c gl (delta - p_j) - c ge p_j (c (x_j - m) + K) = e (slope (x_j - m) + level) + c gl delta.
+struct GradRow {
+    float base, c2, slope, level, at_id;
+    int id;
+    __device__ GradRow(float m, float s, float scale, float gl, float ge, float entropy, int id_) {
+        base = s != s ? s : base_of(m);  // a row with a NaN or +inf: every gradient is NaN
+        c2 = scale * 1.4426950408889634f;
+        id = id_;
+        if (s == 0.f) gl = ge = 0.f;  // masked throughout
+        const float share = s == 0.f ? 0.f : scale / s;
+        slope = -share * (ge * scale);
+        level = -share * (ge != 0.f ? gl + ge * (entropy - logf(s)) : gl);
+        at_id = scale * gl;
+    }
+    // The gradients at one vector's logits, in the logits' type.
+    template <class T>
+    __device__ __forceinline__ uint4 gradient(const uint4 &v, long long element) const {
+        constexpr int N = Bits<T>::N;
+        float x[N], g[N];
+        Bits<T>::unpack(v, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float d = x[j] - base, e = exp2_fast(d * c2);
+            g[j] = e == 0.f ? 0.f : e * fmaf(slope, d, level);  // masked: d is not a number's worth
+        }
+        const long long at = id - element;
+        if (at >= 0 && at < N) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j == at) g[j] += at_id;
+        }
+        Pack<T> out;
+#pragma unroll
+        for (int j = 0; j < N; ++j) out.v[j] = narrowed<T>(g[j]);
+        return *reinterpret_cast<const uint4 *>(out.v);
+    }
+};
+
+// Vector i of a row of results: `same` says that the result lies on the same 16-byte grid as the logits, where one store writes it.
 template <class T>
-__global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad a) {
+__device__ __noinline__ void store_elements(T *dx, long long e, int cols, uint4 g) {
+    Pack<T> out;
+    *reinterpret_cast<uint4 *>(out.v) = g;
+#pragma unroll
+    for (int j = 0; j < Pack<T>::N; ++j)
+        if (e + j >= 0 && e + j < cols) dx[e + j] = out.v[j];
+}
+template <class T>
+__device__ __forceinline__ void store_vector(const RowVectors<T> &row, T *dx, bool same, int i, const uint4 &g) {
+    const long long e = row.element(i);
+    if (same && row.whole(i)) {
+        asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(dx + e), "r"(g.x), "r"(g.y), "r"(g.z), "r"(g.w) : "memory");
+        return;
+    }
+    store_elements(dx, e, row.cols, g);
+}
+template <class T>
+__device__ __forceinline__ bool same_grid(const T *x, const T *dx) { return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0; }
+
+__device__ __forceinline__ float at_row(const VectorArg &v, long long r) { return v.ptr ? ((const float *)v.ptr)[r * v.stride] : 0.f; }
+__device__ __forceinline__ int token_of(const LogProbsGrad &a, long long r) {
+    const int id = ((const int *)a.ids.ptr)[r * a.ids.stride];
+    return id >= 0 && id < a.logits.cols ? id : -1;
+}
+
+// From the forward pass's sums: `pieces` blocks for a row, kGradVectors vectors each.  Bound by memory: a read and a write.
+constexpr int kGradVectors = 1024;
+template <class T>
+__global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad a, const unsigned pieces) {
+    constexpr int U = kGradVectors / 256;
     grid_dependency_sync();
-    const long long r = blockIdx.x, vocab = a.logits.cols;
+    const long long r = blockIdx.x / pieces;
+    const int piece = blockIdx.x - (unsigned)r * pieces;
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
     T *dx = (T *)a.dlogits.ptr + r * a.dlogits.pitch;
-    const float m = ((const float *)a.stats.ptr)[r * a.stats.pitch], s = ((const float *)a.stats.ptr)[r * a.stats.pitch + 1];
-    const int id = ((const int *)a.ids.ptr)[r * a.ids.stride];
-    const float gl = a.g_log_probs.ptr && id >= 0 && id < vocab ? ((const float *)a.g_log_probs.ptr)[r * a.g_log_probs.stride] : 0.f;
-    const float ge = a.g_entropy.ptr ? ((const float *)a.g_entropy.ptr)[r * a.g_entropy.stride] : 0.f;
-    const float h = a.g_entropy.ptr ? ((const float *)a.entropy.ptr)[r * a.entropy.stride] : 0.f;
-    const float ln_s = logf(s);
-    for (long long j = threadIdx.x; j < vocab; j += 256) {
-        float v = 0.f;
-        if (s != 0.f) {
-            const float d = (widen(x[j]) - m) * a.scale, p = expf(d) / s;
-            v = (j == id ? gl : 0.f) - gl * p - ge * p * (fmaxf(d, -FLT_MAX) - ln_s + h);
+    const RowVectors<T> row(x, a.logits.cols);
+    const int i = piece * kGradVectors + threadIdx.x;
+    uint4 v[U];
+    row.template load_all<U, 256, false>(v, i, row.count);  // plain loads: the results may be written over the logits
+    const float *stats = (const float *)a.stats.ptr + r * a.stats.pitch;
+    const int id = token_of(a, r);
+    const GradRow g(stats[0], stats[1], a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), at_row(a.entropy, r), id);
+    const bool same = same_grid(x, dx);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (i + u * 256 < row.count) store_vector(row, dx, same, i + u * 256, g.template gradient<T>(v[u], row.element(i + u * 256)));
+}
+
+// Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
+// gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.
+template <class T, int THREADS, int NV>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int parts) {
+    __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
+    grid_dependency_sync();
+    if (parts > 1) cluster_arrive();
+    const long long r = blockIdx.x / (unsigned)parts;
+    const unsigned rank = parts > 1 ? cluster_rank() : 0;
+    const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
+    T *dx = (T *)a.dlogits.ptr + r * a.dlogits.pitch;
+    const RowVectors<T> row(x, a.logits.cols);
+    const int each = (row.count + parts - 1) / parts, begin = (int)rank * each, end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
+    const float c2 = a.scale * 1.4426950408889634f;
+    uint4 v[NV];
+    row.template load_all<NV, THREADS, false>(v, i, end);
+    const int id = token_of(a, r);
+    const float own = id >= 0 ? widen(x[id]) : 0.f, gl = id >= 0 ? at_row(a.g_log_probs, r) : 0.f, ge = at_row(a.g_entropy, r);
+    Sums all;
+    add_vectors<T, NV>(all, v, c2);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) asm volatile("" : "+r"(v[u].x), "+r"(v[u].y), "+r"(v[u].z), "+r"(v[u].w));  // as loaded: unpacked twice rather than kept unpacked
+    all = block_join<THREADS>(all, c2, sums);
+    if (parts > 1) {
+        cluster_wait();
+        if ((int)threadIdx.x < parts) {
+            const unsigned to = peer_shared(&part_sums[rank], threadIdx.x);
+            peer_store(to, all.m);
+            peer_store(to + 4, all.s);
+            peer_store(to + 8, all.w);
         }
-        dx[j] = narrowed<T>(v * a.scale);
+        cluster_arrive();  // after the token's own logit has been read: from here on results may take the logits' place
+        cluster_wait();
+        const int p = threadIdx.x % kMaxCluster;
+        all = warp_join(p < parts ? part_sums[p] : Sums(), c2, kMaxCluster);
+    } else {
+        __syncthreads();
     }
+    const float base = base_of(all.m), ln_s = logf(all.s);
+    const bool none = all.s == 0.f;
+    const float h = none ? 0.f : ln_s - a.scale * (all.w / all.s);
+    if (rank == 0 && threadIdx.x == 0) {
+        ((float *)log_probs.ptr)[r * log_probs.stride] = id < 0 ? 0.f : none ? -INFINITY : (own - base) * a.scale - ln_s;
+        if (entropy.ptr) ((float *)entropy.ptr)[r * entropy.stride] = h;
+    }
+    const GradRow g(all.m, all.s, a.scale, gl, ge, h, id);
+    const bool same = same_grid(x, dx);
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+        if (i + u * THREADS < end) store_vector(row, dx, same, i + u * THREADS, g.template gradient<T>(v[u], row.element(i + u * THREADS)));
 }
 
 // How many CTAs share a row: the fewest steps of a grid of `slots` resident CTAs, each step the part's bytes and a fixed cost that
@@ -406,12 +542,46 @@ sage_status token_log_probs_grad(Context &ctx, const LogProbsGrad &a) {
     ctx.note_launch("token_log_probs_grad");
     if (ctx.dry()) return SAGE_OK;
     return with_type(a.logits.dtype, [&](auto t) {
-        return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), log_probs_grad_kernel<decltype(t)>, dim3((unsigned)a.logits.rows), dim3(256), 0, a), "token_log_probs_grad");
+        typedef decltype(t) T;
+        const long long n = Bits<T>::N, pieces = ((a.logits.cols + 2 * n - 2) / n + kGradVectors - 1) / kGradVectors;  // the most vectors that a row can touch
+        const long long most = 0x7fffffffll / pieces;  // rows of one launch
+        for (long long at = 0; at < a.logits.rows; at += most) {
+            LogProbsGrad b = a;
+            b.logits.rows = a.logits.rows - at < most ? a.logits.rows - at : most;
+            b.logits.ptr = (T *)a.logits.ptr + at * a.logits.pitch;
+            b.dlogits.ptr = (T *)a.dlogits.ptr + at * a.dlogits.pitch;
+            b.stats.ptr = (float *)a.stats.ptr + at * a.stats.pitch;
+            for (auto *v : {&b.ids, &b.entropy, &b.g_log_probs, &b.g_entropy})
+                if (v->ptr) v->ptr = (float *)v->ptr + at * v->stride;
+            sage_status st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), log_probs_grad_kernel<T>, dim3((unsigned)(b.logits.rows * pieces)), dim3(256), 0, b, (unsigned)pieces),
+                                            "token_log_probs_grad");
+            if (st) return st;
+        }
+        return (sage_status)SAGE_OK;
     });
 }
 
 sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const VectorArg &log_probs, const VectorArg &entropy) {
     if (!a.logits.rows) return SAGE_OK;
+    constexpr int NV = 8;
+    const long long vectors = (a.logits.cols * (a.logits.dtype == SAGE_F32 ? 4 : 2) + 15) / 16 + 1;  // the most that a row can touch
+    const bool small = vectors <= 128 * NV;
+    int parts = 1;
+    while (!small && vectors > (long long)parts * 512 * NV) parts *= 2;
+    // Rows that fit the registers of a cluster, in as many parts as keep all SMs busy.
+    if (parts <= kMaxCluster && a.logits.rows * kMaxCluster <= 0x7fffffffll) {
+        ctx.note_launch("token_log_probs_and_grad");
+        if (ctx.dry()) return SAGE_OK;
+        if (!small)
+            while (parts < kMaxCluster && a.logits.rows * parts < ctx.sm_count * 2ll) parts *= 2;
+        return with_type(a.logits.dtype, [&](auto t) {
+            typedef decltype(t) T;
+            const dim3 grid((unsigned)(a.logits.rows * parts));
+            return ctx.check_cuda(small ? launch_dependent(ctx.pdl, ctx.stream(), log_probs_and_grad_kernel<T, 128, NV>, grid, dim3(128), 0, a, log_probs, entropy, 1)
+                                        : launch_dependent(ctx.pdl, ctx.stream(), parts, log_probs_and_grad_kernel<T, 512, NV>, grid, dim3(512), 0, a, log_probs, entropy, parts),
+                                  "token_log_probs_and_grad");
+        });
+    }
     Block *scratch = ctx.allocator().alloc((size_t)a.logits.rows * 12);
     if (!scratch) return ctx.fail(SAGE_ERR_OOM, "token_log_probs_and_grad: out of memory");
     LogProbs f;
