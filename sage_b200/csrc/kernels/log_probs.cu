@@ -26,13 +26,14 @@ struct Bits<float> {
     __device__ static unsigned element(const void *p) { return *(const unsigned *)p; }
     __device__ static void put(uint4 &v, int j, unsigned e) { (&v.x)[j] = e; }
     __device__ static float largest(const uint4 &v) { return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))); }
-    __device__ static void unpack(const uint4 &v, float *x) {
-        x[0] = __uint_as_float(v.x);
-        x[1] = __uint_as_float(v.y);
-        x[2] = __uint_as_float(v.z);
-        x[3] = __uint_as_float(v.w);
+    __device__ static void unpack(const uint4 &v, float2 *x) {
+        x[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+        x[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
     }
+    __device__ static uint4 packed(const float2 *x) { return make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y)); }
 };
+__device__ __forceinline__ __half2 narrowed_pair(__half2 *, float2 x) { return __float22half2_rn(x); }
+__device__ __forceinline__ __nv_bfloat162 narrowed_pair(__nv_bfloat162 *, float2 x) { return __float22bfloat162_rn(x); }
 template <class T, class T2>
 struct Bits16 {
     static constexpr int N = 8;
@@ -46,13 +47,21 @@ struct Bits16 {
         const T2 h = __hmax2(__hmax2(pair(v.x), pair(v.y)), __hmax2(pair(v.z), pair(v.w)));
         return fmaxf(widen(h.x), widen(h.y));
     }
-    __device__ static void unpack(const uint4 &v, float *x) {
+    __device__ static void unpack(const uint4 &v, float2 *x) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const T2 h = pair((&v.x)[i]);
-            x[2 * i] = widen(h.x);
-            x[2 * i + 1] = widen(h.y);
+            x[i] = make_float2(widen(h.x), widen(h.y));
         }
+    }
+    __device__ static uint4 packed(const float2 *x) {
+        uint4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T2 h = narrowed_pair((T2 *)nullptr, x[i]);
+            (&v.x)[i] = *reinterpret_cast<const unsigned *>(&h);
+        }
+        return v;
     }
 };
 template <>
@@ -126,27 +135,49 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; below 2^-126 ze
     return y;
 }
 
+// Two f32 operations in one instruction, each rounded by itself.
+__device__ __forceinline__ unsigned long long bits_of(float2 x) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x.x), "f"(x.y));
+    return r;
+}
+__device__ __forceinline__ float2 pair_of(unsigned long long r) {
+    float2 x;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x.x), "=f"(x.y) : "l"(r));
+    return x;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // ------------------------------------------------------------------------------------------ sums of a part of a row
-// The part's largest logit m, s = sum exp(c (x - m)) and w = sum (x - m) exp(c (x - m)); with m = -inf both are relative to 0.
-// c2 = c log2(e).  Differences are taken before they are scaled, so that a large m costs nothing.
+// The part's largest logit m, s = sum of 2^t and w = sum of t 2^t with t = c2 (x - m), c2 = c log2(e); with m = -inf both are relative
+// to 0.  Differences are taken before they are scaled, so that a large m costs nothing.  Below 2^-200 a term is zero, and t is held at
+// kLeast in w: a masked logit adds 0 times a number.
+constexpr float kLeast = -200.f, kLn2 = 0.69314718055994531f;
 struct Sums {
     float m = -INFINITY, s = 0.f, w = 0.f;
 };
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 // Makes the sums relative to `m`.  A factor of zero takes all with it (a part of masks of the type's lowest value), NaN stays in s.
 __device__ __forceinline__ void move_to(Sums &a, float m, float c2) {
-    const float d = a.m - base_of(m), f = exp2_fast(d * c2);
-    a.w = f > 0.f ? f * (a.w + d * a.s) : 0.f;
+    const float t = (a.m - base_of(m)) * c2, f = exp2_fast(t);
+    a.w = f > 0.f ? f * (a.w + t * a.s) : 0.f;
     a.s *= f;
     a.m = m;
-}
-__device__ __forceinline__ Sums join(Sums a, Sums b, float c2) {
-    const float m = fmaxf(a.m, b.m);
-    move_to(a, m, c2);
-    move_to(b, m, c2);
-    a.s += b.s;
-    a.w += b.w;
-    return a;
 }
 template <class T, int U>
 __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float c2) {
@@ -154,37 +185,41 @@ __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float 
 #pragma unroll
     for (int u = 1; u < U; ++u) m = fmaxf(m, Bits<T>::largest(v[u]));
     if (m > a.m) move_to(a, m, c2);
-    const float base = base_of(a.m);
+    const float2 base = both(-base_of(a.m)), factor = both(c2);
+    float2 s = make_float2(a.s, 0.f), w = make_float2(a.w, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        float x[Bits<T>::N];
+        float2 x[Bits<T>::N / 2];
         Bits<T>::unpack(v[u], x);
 #pragma unroll
-        for (int j = 0; j < Bits<T>::N; ++j) {
-            const float d = x[j] - base, e = exp2_fast(d * c2);
-            a.s += e;
-            a.w = fmaf(e, fmaxf(d, -FLT_MAX), a.w);  // masked: 0 times a number
+        for (int j = 0; j < Bits<T>::N / 2; ++j) {
+            const float2 t = mul2(add2(x[j], base), factor), e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+            s = add2(s, e);
+            w = fma2(e, make_float2(fmaxf(t.x, kLeast), fmaxf(t.y, kLeast)), w);
         }
     }
+    a.s = s.x + s.y;
+    a.w = w.x + w.y;
 }
-__device__ __forceinline__ Sums warp_join(Sums a, float c2, int width = 32) {
-    for (int o = width / 2; o; o >>= 1) {
-        Sums b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        b.w = __shfl_xor_sync(0xffffffffu, a.w, o);
-        a = join(a, b, c2);
+// Of the warp's lanes, in all of them: the largest m first, then sums relative to it.
+__device__ __forceinline__ Sums warp_join(Sums a, float c2) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(a.m));
+    move_to(a, m, c2);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
     }
     return a;
 }
-// Of all threads, in every thread.  `shared`: one for each warp.
+// Of all threads, in warp 0.  `shared`: one for each warp.
 template <int THREADS>
 __device__ __forceinline__ Sums block_join(Sums a, float c2, Sums *shared) {
     a = warp_join(a, c2);
     if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = a;
     __syncthreads();
-    constexpr int W = THREADS / 32;
-    return warp_join(shared[threadIdx.x % W], c2, W);  // lanes that hold the same values join to the same result
+    return threadIdx.x < 32 ? warp_join((int)threadIdx.x < THREADS / 32 ? shared[threadIdx.x] : Sums(), c2) : a;
 }
 
 // ------------------------------------------------------------------------------------------ clusters: CTAs that share a row
@@ -194,6 +229,7 @@ __device__ __forceinline__ unsigned cluster_rank() {
     return r;
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }  // of a thread with nothing to show
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // The address in CTA `rank`'s shared memory of what lies at `p` in this one's.
 __device__ __forceinline__ unsigned peer_shared(const void *p, unsigned rank) {
@@ -269,18 +305,18 @@ __device__ TopList block_top(const RowVectors<T> &row, int begin, int end, float
         for (int base = from - (all ? lane : lane * THREADS), i = from; base < end; base += step, i += step) {
             const bool some = i < end;
             const uint4 v = some ? row.load(i) : RowVectors<T>::nothing();
-            float x[N];
+            float2 x[N / 2];
             Bits<T>::unpack(v, x);
             const long long e = row.element(i);
             bool any = false;
 #pragma unroll
-            for (int j = 0; j < N; ++j) any |= rank_bits(x[j]) >> 16 >= bound;
+            for (int j = 0; j < N; ++j) any |= rank_bits(j % 2 ? x[j / 2].y : x[j / 2].x) >> 16 >= bound;
             if (!__any_sync(0xffffffffu, any && some)) continue;
 #pragma unroll 1
             for (int j = 0; j < N; ++j) {
-                float y = x[0];
+                float y = x[0].x;
 #pragma unroll
-                for (int l = 1; l < N; ++l) y = j == l ? x[l] : y;
+                for (int l = 1; l < N; ++l) y = j == l ? (l % 2 ? x[l / 2].y : x[l / 2].x) : y;
                 const bool in = some && e + j >= 0 && e + j < row.cols && rank_bits(y) >> 16 >= bound;
                 list.offer(rank_key(y, (unsigned)(e + j)), in, k);
             }
@@ -304,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     __shared__ unsigned long long part_lists[TOP ? kMaxCluster : 1][kMaxTop];
     __shared__ TopShared<TOP ? THREADS : 32> top;
     grid_dependency_sync();
-    if (parts > 1) cluster_arrive();
+    if (parts > 1) cluster_arrive_relaxed();
     const long long r = blockIdx.x / (unsigned)parts;
     const unsigned rank = parts > 1 ? cluster_rank() : 0;
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
@@ -329,7 +365,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     TopList list;
     if constexpr (TOP) list = block_top<T, THREADS>(row, begin, end, thread_max, a.top, top);
     const int lane = threadIdx.x % 32;
-    if (parts > 1) {  // everything to the first CTA, which has started by now
+    if (parts > 1) {  // everything to the first CTA, which has started when the wait ends
         cluster_wait();
         if (threadIdx.x == 0) {
             const unsigned to = peer_shared(&part_sums[rank], 0);
@@ -338,18 +374,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
             peer_store(to + 8, all.w);
         }
         if (TOP && threadIdx.x < 32) peer_store(peer_shared(&part_lists[TOP ? rank : 0][lane], 0), lane < a.top ? list.key : 0ull);
-        cluster_arrive();
+        if (threadIdx.x < 32) cluster_arrive();
+        else cluster_arrive_relaxed();
         cluster_wait();
-        if (rank) return;
-        all = warp_join(lane % kMaxCluster < parts ? part_sums[lane % kMaxCluster] : Sums(), c2, kMaxCluster);
-        if (TOP && threadIdx.x < 32)
+        if (rank || threadIdx.x >= 32) return;
+        all = warp_join(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
+        if (TOP)
             for (int p = 1; p < parts; ++p) list.offer(part_lists[TOP ? p : 0][lane], true, a.top);
     }
+    if (threadIdx.x >= 32) return;
     const float base = base_of(all.m), ln_s = logf(all.s);
     const bool none = all.s == 0.f;
     if (threadIdx.x == 0) {
         ((float *)a.log_probs.ptr)[r * a.log_probs.stride] = !scored ? 0.f : none ? -INFINITY : (own - base) * a.scale - ln_s;
-        if (a.entropy.ptr) ((float *)a.entropy.ptr)[r * a.entropy.stride] = none ? 0.f : ln_s - a.scale * (all.w / all.s);
+        if (a.entropy.ptr) ((float *)a.entropy.ptr)[r * a.entropy.stride] = none ? 0.f : ln_s - kLn2 * (all.w / all.s);
         if (a.stats.ptr) {
             ((float *)a.stats.ptr)[r * a.stats.pitch] = all.m;
             ((float *)a.stats.ptr)[r * a.stats.pitch + 1] = all.s;
@@ -362,42 +400,41 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
 }
 
 // ------------------------------------------------------------------------------------------ gradient
-// With e = exp(c (x - m)), p = e / S and K = H - ln S:
-//   dx_j = c gl (delta - p_j) - c ge p_j (c (x_j - m) + K) = e (slope (x_j - m) + level) + c gl delta.
+// With t = c2 (x - m), e = 2^t, p = e / S and K = H - ln S:
+//   dx_j = c gl (delta - p_j) - c ge p_j (ln2 t_j + K) = e (slope t_j + level) + c gl delta.
 struct GradRow {
     float base, c2, slope, level, at_id;
     int id;
-    __device__ GradRow(float m, float s, float scale, float gl, float ge, float entropy, int id_) {
-        base = s != s ? s : base_of(m);  // a row with a NaN or +inf: every gradient is NaN
+    __device__ void set(float m, float s, float scale, float gl, float ge, float entropy, int id_) {
+        base = base_of(m);
         c2 = scale * 1.4426950408889634f;
         id = id_;
         if (s == 0.f) gl = ge = 0.f;  // masked throughout
         const float share = s == 0.f ? 0.f : scale / s;
-        slope = -share * (ge * scale);
-        level = -share * (ge != 0.f ? gl + ge * (entropy - logf(s)) : gl);
+        slope = -share * (ge * kLn2);
+        level = -share * (ge != 0.f ? gl + ge * (entropy - logf(s)) : gl);  // NaN where s is: so is every gradient
         at_id = scale * gl;
     }
     // The gradients at one vector's logits, in the logits' type.
     template <class T>
-    __device__ __forceinline__ uint4 gradient(const uint4 &v, long long element) const {
+    __device__ __forceinline__ uint4 gradient(const uint4 &v, int element) const {
         constexpr int N = Bits<T>::N;
-        float x[N], g[N];
+        const float2 b = both(-base), f = both(c2), k = both(slope), l = both(level);
+        float2 x[N / 2];
         Bits<T>::unpack(v, x);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float d = x[j] - base, e = exp2_fast(d * c2);
-            g[j] = e == 0.f ? 0.f : e * fmaf(slope, d, level);  // masked: d is not a number's worth
+        for (int j = 0; j < N / 2; ++j) {
+            float2 t = mul2(add2(x[j], b), f);
+            t = make_float2(fmaxf(t.x, kLeast), fmaxf(t.y, kLeast));  // masked: 0 times a number
+            x[j] = mul2(make_float2(exp2_fast(t.x), exp2_fast(t.y)), fma2(k, t, l));
         }
-        const long long at = id - element;
-        if (at >= 0 && at < N) {
+        const unsigned at = (unsigned)(id - element);
+        if (at < (unsigned)N) {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (j == at) g[j] += at_id;
+                if (j == (int)at) (j % 2 ? x[j / 2].y : x[j / 2].x) += at_id;
         }
-        Pack<T> out;
-#pragma unroll
-        for (int j = 0; j < N; ++j) out.v[j] = narrowed<T>(g[j]);
-        return *reinterpret_cast<const uint4 *>(out.v);
+        return Bits<T>::packed(x);
     }
 };
 
@@ -444,11 +481,12 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
     row.template load_all<U, 256, false>(v, i, row.count);  // plain loads: the results may be written over the logits
     const float *stats = (const float *)a.stats.ptr + r * a.stats.pitch;
     const int id = token_of(a, r);
-    const GradRow g(stats[0], stats[1], a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), at_row(a.entropy, r), id);
+    GradRow g;
+    g.set(stats[0], stats[1], a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), at_row(a.entropy, r), id);
     const bool same = same_grid(x, dx);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        if (i + u * 256 < row.count) store_vector(row, dx, same, i + u * 256, g.template gradient<T>(v[u], row.element(i + u * 256)));
+        if (i + u * 256 < row.count) store_vector(row, dx, same, i + u * 256, g.template gradient<T>(v[u], (int)row.element(i + u * 256)));
 }
 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
@@ -456,8 +494,9 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
 template <class T, int THREADS, int NV>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int parts) {
     __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
+    __shared__ GradRow constants;
     grid_dependency_sync();
-    if (parts > 1) cluster_arrive();
+    if (parts > 1) cluster_arrive_relaxed();
     const long long r = blockIdx.x / (unsigned)parts;
     const unsigned rank = parts > 1 ? cluster_rank() : 0;
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
@@ -467,13 +506,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
     const float c2 = a.scale * 1.4426950408889634f;
     uint4 v[NV];
     row.template load_all<NV, THREADS, false>(v, i, end);
-    const int id = token_of(a, r);
-    const float own = id >= 0 ? widen(x[id]) : 0.f, gl = id >= 0 ? at_row(a.g_log_probs, r) : 0.f, ge = at_row(a.g_entropy, r);
     Sums all;
     add_vectors<T, NV>(all, v, c2);
 #pragma unroll
     for (int u = 0; u < NV; ++u) asm volatile("" : "+r"(v[u].x), "+r"(v[u].y), "+r"(v[u].z), "+r"(v[u].w));  // as loaded: unpacked twice rather than kept unpacked
     all = block_join<THREADS>(all, c2, sums);
+    const int id = token_of(a, r);
+    float own = 0.f;
+    if (threadIdx.x == 0 && rank == 0 && id >= 0) own = widen(x[id]);
     if (parts > 1) {
         cluster_wait();
         if ((int)threadIdx.x < parts) {
@@ -482,25 +522,31 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
             peer_store(to + 4, all.s);
             peer_store(to + 8, all.w);
         }
-        cluster_arrive();  // after the token's own logit has been read: from here on results may take the logits' place
+        // Behind the token's own logit too: from here on results may take the logits' place.
+        if (threadIdx.x < 32) cluster_arrive();
+        else cluster_arrive_relaxed();
         cluster_wait();
-        const int p = threadIdx.x % kMaxCluster;
-        all = warp_join(p < parts ? part_sums[p] : Sums(), c2, kMaxCluster);
-    } else {
-        __syncthreads();
     }
-    const float base = base_of(all.m), ln_s = logf(all.s);
-    const bool none = all.s == 0.f;
-    const float h = none ? 0.f : ln_s - a.scale * (all.w / all.s);
-    if (rank == 0 && threadIdx.x == 0) {
-        ((float *)log_probs.ptr)[r * log_probs.stride] = id < 0 ? 0.f : none ? -INFINITY : (own - base) * a.scale - ln_s;
-        if (entropy.ptr) ((float *)entropy.ptr)[r * entropy.stride] = h;
+    if (threadIdx.x < 32) {  // the row's constants once; a thread's other work is 64 elements
+        const int lane = threadIdx.x;
+        if (parts > 1) all = warp_join(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
+        if (lane == 0) {
+            const float ln_s = logf(all.s);
+            const bool none = all.s == 0.f;
+            const float h = none ? 0.f : ln_s - kLn2 * (all.w / all.s);
+            constants.set(all.m, all.s, a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), h, id);
+            if (rank == 0) {
+                ((float *)log_probs.ptr)[r * log_probs.stride] = id < 0 ? 0.f : none ? -INFINITY : (own - base_of(all.m)) * a.scale - ln_s;
+                if (entropy.ptr) ((float *)entropy.ptr)[r * entropy.stride] = h;
+            }
+        }
     }
-    const GradRow g(all.m, all.s, a.scale, gl, ge, h, id);
+    __syncthreads();
+    const GradRow g = constants;
     const bool same = same_grid(x, dx);
 #pragma unroll
     for (int u = 0; u < NV; ++u)
-        if (i + u * THREADS < end) store_vector(row, dx, same, i + u * THREADS, g.template gradient<T>(v[u], row.element(i + u * THREADS)));
+        if (i + u * THREADS < end) store_vector(row, dx, same, i + u * THREADS, g.template gradient<T>(v[u], (int)row.element(i + u * THREADS)));
 }
 
 // How many CTAs share a row: the fewest steps of a grid of `slots` resident CTAs, each step the part's bytes and a fixed cost that
