@@ -34,6 +34,11 @@ struct Bits<float> {
 };
 __device__ __forceinline__ __half2 narrowed_pair(__half2 *, float2 x) { return __float22half2_rn(x); }
 __device__ __forceinline__ __nv_bfloat162 narrowed_pair(__nv_bfloat162 *, float2 x) { return __float22bfloat162_rn(x); }
+__device__ __forceinline__ float2 widened_pair(__half2 x) { return __half22float2(x); }
+__device__ __forceinline__ float2 widened_pair(__nv_bfloat162 x) {  // an f32's upper half
+    const unsigned w = *reinterpret_cast<const unsigned *>(&x);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 template <class T, class T2>
 struct Bits16 {
     static constexpr int N = 8;
@@ -49,10 +54,7 @@ struct Bits16 {
     }
     __device__ static void unpack(const uint4 &v, float2 *x) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const T2 h = pair((&v.x)[i]);
-            x[i] = make_float2(widen(h.x), widen(h.y));
-        }
+        for (int i = 0; i < 4; ++i) x[i] = widened_pair(pair((&v.x)[i]));
     }
     __device__ static uint4 packed(const float2 *x) {
         uint4 v;
@@ -89,28 +91,22 @@ struct RowVectors {
         count = (int)((head + cols_ + N - 1) / N);
     }
     __device__ __forceinline__ bool whole(int i) const { return i >= first && i < full; }
-    __device__ __forceinline__ long long element(int i) const { return (long long)i * N - head; }
-    // Of a vector that lies wholly in the row.
-    template <bool READ_ONLY>
-    __device__ __forceinline__ uint4 load_whole(int i) const {
-        const uint4 *p = reinterpret_cast<const uint4 *>(origin) + i;
-        uint4 v;
-        if (READ_ONLY) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-        else asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-        return v;
-    }
-    __device__ __forceinline__ uint4 load(int i) const { return whole(i) ? load_whole<true>(i) : load_edge(i); }
-    // Vectors i, i + STEP ...: those of [0, end).
-    template <int U, int STEP, bool READ_ONLY>
+    __device__ __forceinline__ bool ragged() const { return first != 0 || full != count; }
+    __device__ __forceinline__ int element(int i) const { return i * N - head; }
+    __device__ __forceinline__ uint4 load(int i) const { return whole(i) ? __ldcg(reinterpret_cast<const uint4 *>(origin) + i) : load_edge(i); }
+    // Vectors i, i + STEP ...: those in front of `end`.
+    template <int U, int STEP>
     __device__ __forceinline__ void load_all(uint4 (&v)[U], int i, int end) const {
+        const uint4 *p = reinterpret_cast<const uint4 *>(origin) + i;
+        const int stop = min(end, full);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             v[u] = nothing();
-            if (i + u * STEP < end && whole(i + u * STEP)) v[u] = load_whole<READ_ONLY>(i + u * STEP);
+            if (i + u * STEP < stop && (u > 0 || i >= first)) v[u] = __ldcg(p + u * STEP);
         }
-        // the row's first and last vector, where they reach beyond it
+        if (!ragged()) return;
 #pragma unroll 1
-        for (int at = 0; at < count; at += max(count - 1, 1)) {
+        for (int at = 0; at < count; at += max(count - 1, 1)) {  // the row's first and last vector, where they reach beyond it
             if (whole(at) || at < i || at >= end || at > i + (U - 1) * STEP || (at - i) % STEP) continue;
             const uint4 e = load_edge(at);
 #pragma unroll
@@ -120,10 +116,10 @@ struct RowVectors {
     }
     __device__ __noinline__ uint4 load_edge(int i) const {
         uint4 v = nothing();
-        const long long e = element(i);
+        const int e = element(i);
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (e + j >= 0 && e + j < cols) Bits<T>::put(v, j, Bits<T>::element(origin + 16ll * i + j * (int)sizeof(T)));
+            if (e + j >= 0 && (unsigned)(e + j) < (unsigned)cols) Bits<T>::put(v, j, Bits<T>::element(origin + 16ll * i + j * (int)sizeof(T)));
         return v;
     }
     __device__ __forceinline__ static uint4 nothing() { return make_uint4(Bits<T>::kFill, Bits<T>::kFill, Bits<T>::kFill, Bits<T>::kFill); }
@@ -307,7 +303,7 @@ __device__ TopList block_top(const RowVectors<T> &row, int begin, int end, float
             const uint4 v = some ? row.load(i) : RowVectors<T>::nothing();
             float2 x[N / 2];
             Bits<T>::unpack(v, x);
-            const long long e = row.element(i);
+            const int e = row.element(i);
             bool any = false;
 #pragma unroll
             for (int j = 0; j < N; ++j) any |= rank_bits(j % 2 ? x[j / 2].y : x[j / 2].x) >> 16 >= bound;
@@ -317,7 +313,7 @@ __device__ TopList block_top(const RowVectors<T> &row, int begin, int end, float
                 float y = x[0].x;
 #pragma unroll
                 for (int l = 1; l < N; ++l) y = j == l ? (l % 2 ? x[l / 2].y : x[l / 2].x) : y;
-                const bool in = some && e + j >= 0 && e + j < row.cols && rank_bits(y) >> 16 >= bound;
+                const bool in = some && (unsigned)(e + j) < (unsigned)row.cols && rank_bits(y) >> 16 >= bound;
                 list.offer(rank_key(y, (unsigned)(e + j)), in, k);
             }
         }
@@ -332,20 +328,21 @@ __device__ TopList block_top(const RowVectors<T> &row, int begin, int end, float
 // ------------------------------------------------------------------------------------------ values
 constexpr int kMaxCluster = 8;
 
-// A cluster of `parts` CTAs for each row; each reads a part of it once.
+// A cluster of 2^shift CTAs for each row; each reads a part of it once.
 template <class T, int THREADS, bool TOP>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(const LogProbs a, const int parts) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(const LogProbs a, const int shift) {
     constexpr int U = 4;
     __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
     __shared__ unsigned long long part_lists[TOP ? kMaxCluster : 1][kMaxTop];
     __shared__ TopShared<TOP ? THREADS : 32> top;
     grid_dependency_sync();
+    const int parts = 1 << shift;
     if (parts > 1) cluster_arrive_relaxed();
-    const long long r = blockIdx.x / (unsigned)parts;
+    const long long r = blockIdx.x >> shift;
     const unsigned rank = parts > 1 ? cluster_rank() : 0;
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
     const RowVectors<T> row(x, a.logits.cols);
-    const int each = (row.count + parts - 1) / parts, begin = (int)rank * each, end = min(begin + each, row.count);
+    const int each = (row.count + parts - 1) >> shift, begin = (int)rank * each, end = min(begin + each, row.count);
     const float c2 = a.scale * 1.4426950408889634f;
     float own = 0.f;
     bool scored = false;
@@ -357,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     Sums mine;
     for (int i = begin + (int)threadIdx.x; i < end; i += THREADS * U) {
         uint4 v[U];
-        row.template load_all<U, THREADS, true>(v, i, end);
+        row.template load_all<U, THREADS>(v, i, end);
         add_vectors<T, U>(mine, v, c2);
     }
     const float thread_max = mine.m;
@@ -417,7 +414,7 @@ struct GradRow {
     }
     // The gradients at one vector's logits, in the logits' type.
     template <class T>
-    __device__ __forceinline__ uint4 gradient(const uint4 &v, int element) const {
+    __device__ __forceinline__ uint4 gradient(const uint4 &v, int element) const {  // `element`: the vector's first
         constexpr int N = Bits<T>::N;
         const float2 b = both(-base), f = both(c2), k = both(slope), l = both(level);
         float2 x[N / 2];
@@ -438,23 +435,27 @@ struct GradRow {
     }
 };
 
-// Vector i of a row of results: `same` says that the result lies on the same 16-byte grid as the logits, where one store writes it.
 template <class T>
-__device__ __noinline__ void store_elements(T *dx, long long e, int cols, uint4 g) {
+__device__ __noinline__ void store_elements(T *dx, int e, int cols, uint4 g) {
     Pack<T> out;
     *reinterpret_cast<uint4 *>(out.v) = g;
 #pragma unroll
     for (int j = 0; j < Pack<T>::N; ++j)
-        if (e + j >= 0 && e + j < cols) dx[e + j] = out.v[j];
+        if ((unsigned)(e + j) < (unsigned)cols) dx[e + j] = out.v[j];
 }
-template <class T>
-__device__ __forceinline__ void store_vector(const RowVectors<T> &row, T *dx, bool same, int i, const uint4 &g) {
-    const long long e = row.element(i);
-    if (same && row.whole(i)) {
-        asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(dx + e), "r"(g.x), "r"(g.y), "r"(g.z), "r"(g.w) : "memory");
-        return;
+// Gradients at the vectors that load_all loaded.  `same` says that the results lie on the same 16-byte grid as the logits, where one
+// store writes a vector.
+template <class T, int U, int STEP>
+__device__ __forceinline__ void store_all(const RowVectors<T> &row, const GradRow &g, T *dx, bool same, const uint4 (&v)[U], int i, int end) {
+    uint4 *p = reinterpret_cast<uint4 *>(dx + row.element(0)) + i;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (i + u * STEP >= end) return;
+        const int e = row.element(i + u * STEP);
+        const uint4 out = g.gradient<T>(v[u], e);
+        if (same && i + u * STEP < row.full && (u > 0 || i >= row.first)) p[u * STEP] = out;
+        else store_elements(dx, e, row.cols, out);
     }
-    store_elements(dx, e, row.cols, g);
 }
 template <class T>
 __device__ __forceinline__ bool same_grid(const T *x, const T *dx) { return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0; }
@@ -478,34 +479,33 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
     const RowVectors<T> row(x, a.logits.cols);
     const int i = piece * kGradVectors + threadIdx.x;
     uint4 v[U];
-    row.template load_all<U, 256, false>(v, i, row.count);  // plain loads: the results may be written over the logits
+    row.template load_all<U, 256>(v, i, row.count);
     const float *stats = (const float *)a.stats.ptr + r * a.stats.pitch;
     const int id = token_of(a, r);
     GradRow g;
     g.set(stats[0], stats[1], a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), at_row(a.entropy, r), id);
     const bool same = same_grid(x, dx);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (i + u * 256 < row.count) store_vector(row, dx, same, i + u * 256, g.template gradient<T>(v[u], (int)row.element(i + u * 256)));
+    store_all<T, U, 256>(row, g, dx, same, v, i, row.count);
 }
 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
 // gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.
 template <class T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int parts) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int shift) {
     __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
     __shared__ GradRow constants;
     grid_dependency_sync();
+    const int parts = 1 << shift;
     if (parts > 1) cluster_arrive_relaxed();
-    const long long r = blockIdx.x / (unsigned)parts;
+    const long long r = blockIdx.x >> shift;
     const unsigned rank = parts > 1 ? cluster_rank() : 0;
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
     T *dx = (T *)a.dlogits.ptr + r * a.dlogits.pitch;
     const RowVectors<T> row(x, a.logits.cols);
-    const int each = (row.count + parts - 1) / parts, begin = (int)rank * each, end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
+    const int each = (row.count + parts - 1) >> shift, begin = (int)rank * each, end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
     const float c2 = a.scale * 1.4426950408889634f;
     uint4 v[NV];
-    row.template load_all<NV, THREADS, false>(v, i, end);
+    row.template load_all<NV, THREADS>(v, i, end);
     Sums all;
     add_vectors<T, NV>(all, v, c2);
 #pragma unroll
@@ -544,10 +544,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
     __syncthreads();
     const GradRow g = constants;
     const bool same = same_grid(x, dx);
-#pragma unroll
-    for (int u = 0; u < NV; ++u)
-        if (i + u * THREADS < end) store_vector(row, dx, same, i + u * THREADS, g.template gradient<T>(v[u], (int)row.element(i + u * THREADS)));
+    store_all<T, NV, THREADS>(row, g, dx, same, v, i, end);
 }
+
+int log2_of(int power) { return __builtin_ctz((unsigned)power); }
 
 // How many CTAs share a row: the fewest steps of a grid of `slots` resident CTAs, each step the part's bytes and a fixed cost that
 // measures like 24 KB of them (joining, the cluster's barriers).
@@ -575,7 +575,7 @@ sage_status token_log_probs(Context &ctx, const LogProbs &a) {
         const long long bytes = a.logits.cols * (long long)sizeof(T);
         auto launch = [&](auto kernel, int threads) {
             const int parts = threads == 128 ? 1 : parts_of_rows(a.logits.rows, bytes, ctx.sm_count * 2ll);
-            return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, parts), "token_log_probs");
+            return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log2_of(parts)), "token_log_probs");
         };
         // Short rows: four warps for each, or most threads of a large block would have nothing to read.
         if (bytes <= 16384) return a.top ? launch(log_probs_kernel<T, 128, true>, 128) : launch(log_probs_kernel<T, 128, false>, 128);
@@ -623,8 +623,8 @@ sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const 
         return with_type(a.logits.dtype, [&](auto t) {
             typedef decltype(t) T;
             const dim3 grid((unsigned)(a.logits.rows * parts));
-            return ctx.check_cuda(small ? launch_dependent(ctx.pdl, ctx.stream(), log_probs_and_grad_kernel<T, 128, NV>, grid, dim3(128), 0, a, log_probs, entropy, 1)
-                                        : launch_dependent(ctx.pdl, ctx.stream(), parts, log_probs_and_grad_kernel<T, 512, NV>, grid, dim3(512), 0, a, log_probs, entropy, parts),
+            return ctx.check_cuda(small ? launch_dependent(ctx.pdl, ctx.stream(), log_probs_and_grad_kernel<T, 128, NV>, grid, dim3(128), 0, a, log_probs, entropy, 0)
+                                        : launch_dependent(ctx.pdl, ctx.stream(), parts, log_probs_and_grad_kernel<T, 512, NV>, grid, dim3(512), 0, a, log_probs, entropy, log2_of(parts)),
                                   "token_log_probs_and_grad");
         });
     }
