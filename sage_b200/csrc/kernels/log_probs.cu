@@ -175,8 +175,9 @@ __device__ __forceinline__ void move_to(Sums &a, float m, float c2) {
     a.s *= f;
     a.m = m;
 }
+// `used`: how many of the vectors the block's threads have; the others are empty in all of them.
 template <class T, int U>
-__device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float c2) {
+__device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float c2, int used = U) {
     float m = Bits<T>::largest(v[0]);
 #pragma unroll
     for (int u = 1; u < U; ++u) m = fmaxf(m, Bits<T>::largest(v[u]));
@@ -185,6 +186,7 @@ __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float 
     float2 s = make_float2(a.s, 0.f), w = make_float2(a.w, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+        if (u >= used) break;
         float2 x[Bits<T>::N / 2];
         Bits<T>::unpack(v[u], x);
 #pragma unroll
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
     uint4 v[NV];
     row.template load_all<NV, THREADS>(v, i, end);
     Sums all;
-    add_vectors<T, NV>(all, v, c2);
+    add_vectors<T, NV>(all, v, c2, (end - begin + THREADS - 1) / THREADS);
 #pragma unroll
     for (int u = 0; u < NV; ++u) asm volatile("" : "+r"(v[u].x), "+r"(v[u].y), "+r"(v[u].z), "+r"(v[u].w));  // as loaded: unpacked twice rather than kept unpacked
     all = block_join<THREADS>(all, c2, sums);
@@ -545,6 +547,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
     const GradRow g = constants;
     const bool same = same_grid(x, dx);
     store_all<T, NV, THREADS>(row, g, dx, same, v, i, end);
+}
+
+// The most 16-byte vectors that a row touches.
+long long most_vectors(const RowsArg &x) {
+    const long long size = x.dtype == SAGE_F32 ? 4 : 2, n = 16 / size;
+    const bool fixed = x.rows <= 1 || x.pitch * size % 16 == 0;  // every row starts at the same place of a vector
+    const long long head = fixed ? (long long)(reinterpret_cast<uintptr_t>(x.ptr) % 16) / size : n - 1;
+    return (head + x.cols + n - 1) / n;
 }
 
 int log2_of(int power) { return __builtin_ctz((unsigned)power); }
@@ -589,7 +599,7 @@ sage_status token_log_probs_grad(Context &ctx, const LogProbsGrad &a) {
     if (ctx.dry()) return SAGE_OK;
     return with_type(a.logits.dtype, [&](auto t) {
         typedef decltype(t) T;
-        const long long n = Bits<T>::N, pieces = ((a.logits.cols + 2 * n - 2) / n + kGradVectors - 1) / kGradVectors;  // the most vectors that a row can touch
+        const long long pieces = (most_vectors(a.logits) + kGradVectors - 1) / kGradVectors;
         const long long most = 0x7fffffffll / pieces;  // rows of one launch
         for (long long at = 0; at < a.logits.rows; at += most) {
             LogProbsGrad b = a;
@@ -610,7 +620,7 @@ sage_status token_log_probs_grad(Context &ctx, const LogProbsGrad &a) {
 sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const VectorArg &log_probs, const VectorArg &entropy) {
     if (!a.logits.rows) return SAGE_OK;
     constexpr int NV = 8;
-    const long long vectors = (a.logits.cols * (a.logits.dtype == SAGE_F32 ? 4 : 2) + 15) / 16 + 1;  // the most that a row can touch
+    const long long vectors = most_vectors(a.logits);
     const bool small = vectors <= 128 * NV;
     int parts = 1;
     while (!small && vectors > (long long)parts * 512 * NV) parts *= 2;
