@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
 // gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.
 template <class T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int shift) {
+__global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int shift) {
     __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
     __shared__ GradRow constants;
     grid_dependency_sync();
@@ -513,9 +513,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
 #pragma unroll
     for (int u = 0; u < NV; ++u) asm volatile("" : "+r"(v[u].x), "+r"(v[u].y), "+r"(v[u].z), "+r"(v[u].w));  // as loaded: unpacked twice rather than kept unpacked
     all = block_join<THREADS>(all, c2, sums);
-    const int id = token_of(a, r);
+    int id = -1;
     float own = 0.f;
-    if (threadIdx.x == 0 && rank == 0 && id >= 0) own = widen(x[id]);
+    if (threadIdx.x == 0) {
+        id = token_of(a, r);
+        if (rank == 0 && id >= 0) own = widen(x[id]);
+    }
     if (parts > 1) {
         cluster_wait();
         if ((int)threadIdx.x < parts) {
@@ -621,21 +624,24 @@ sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const 
     if (!a.logits.rows) return SAGE_OK;
     constexpr int NV = 8;
     const long long vectors = most_vectors(a.logits);
-    const bool small = vectors <= 128 * NV;
+    // Blocks of 256 threads where eight of them hold a row, four on an SM: their loads, sums and stores interleave better than those of
+    // two blocks of 512 (8192 x 131072 bf16: 896 and 992 us; 16 vectors a thread 918 at best).
+    const int threads = vectors <= 128 * NV ? 128 : vectors <= kMaxCluster * 256 * NV ? 256 : 512;
     int parts = 1;
-    while (!small && vectors > (long long)parts * 512 * NV) parts *= 2;
+    while (vectors > (long long)parts * threads * NV) parts *= 2;
     // Rows that fit the registers of a cluster, in as many parts as keep all SMs busy.
     if (parts <= kMaxCluster && a.logits.rows * kMaxCluster <= 0x7fffffffll) {
         ctx.note_launch("token_log_probs_and_grad");
         if (ctx.dry()) return SAGE_OK;
-        if (!small)
-            while (parts < kMaxCluster && a.logits.rows * parts < ctx.sm_count * 2ll) parts *= 2;
+        if (threads > 128)
+            while (parts < kMaxCluster && a.logits.rows * parts * threads < ctx.sm_count * 1024ll) parts *= 2;
         return with_type(a.logits.dtype, [&](auto t) {
             typedef decltype(t) T;
-            const dim3 grid((unsigned)(a.logits.rows * parts));
-            return ctx.check_cuda(small ? launch_dependent(ctx.pdl, ctx.stream(), log_probs_and_grad_kernel<T, 128, NV>, grid, dim3(128), 0, a, log_probs, entropy, 0)
-                                        : launch_dependent(ctx.pdl, ctx.stream(), parts, log_probs_and_grad_kernel<T, 512, NV>, grid, dim3(512), 0, a, log_probs, entropy, log2_of(parts)),
-                                  "token_log_probs_and_grad");
+            auto launch = [&](auto kernel) {
+                return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log_probs, entropy, log2_of(parts)),
+                                      "token_log_probs_and_grad");
+            };
+            return threads == 128 ? launch(log_probs_and_grad_kernel<T, 128, NV>) : threads == 256 ? launch(log_probs_and_grad_kernel<T, 256, NV>) : launch(log_probs_and_grad_kernel<T, 512, NV>);
         });
     }
     Block *scratch = ctx.allocator().alloc((size_t)a.logits.rows * 12);
