@@ -64,57 +64,53 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T *__restrict__ ta
 // Tokens are sorted by table row (those of a row in their order), then rows are summed in pieces of a fixed length of that order, so
 // that a frequent token's thousands of rows are spread like any others.  Two launches, no sums by atomics: the same bits every time.
 
-// Sorting.  Each block owns `range` table rows and reads all ids: its warps, each over a contiguous share of the tokens, count its
-// rows' tokens, the counts become places (in front of them all tokens of lower rows), and a second pass puts the tokens there.  148
-// times the ids out of L2 instead of a radix sort's passes through memory and launches: 65 521 ids take 8 us of the 52 of a gradient of
-// width 1000, 4096 ids 3 us.
-constexpr int kSortWarps = 16;
-__global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const int *__restrict__ ids, long long ids_stride, int tokens, int vocab, int range, int *__restrict__ row_start,
+// Sorting.  Each of 2^bits blocks owns the table rows whose numbers end in its own (frequent tokens have low numbers: neighbours go to
+// different blocks) and reads all ids: its warps, each over a contiguous share of the tokens, count its rows' tokens, the counts become
+// places (in front of them all tokens of the blocks before), and a second pass puts the tokens there.  A hundred times the ids out of L2
+// instead of a radix sort's passes through memory and launches.
+constexpr int kSortWarps = 32, kSortRows = 1536;  // rows of a block at most: their counts fill shared memory
+__global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const int *__restrict__ ids, long long ids_stride, int tokens, int vocab, int bits, int2 *__restrict__ spans, int *__restrict__ total,
                                                                          int *__restrict__ order, int *__restrict__ sorted, unsigned *__restrict__ arrived, int counters) {
-    extern __shared__ int places[];  // [warp][row of the range]
+    extern __shared__ int places[];  // [warp][row of the block]
     __shared__ int warp_sums[kSortWarps], below_all;
     constexpr int U = 8;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int v0 = blockIdx.x * range, rows = min(range, vocab - v0);
-    for (int i = threadIdx.x; i < kSortWarps * range; i += kSortWarps * 32) places[i] = 0;
+    const unsigned own = blockIdx.x, ending = (1u << bits) - 1;
+    const int rows = (int)(((unsigned)vocab - own + ending) >> bits);
+    for (int i = threadIdx.x; i < kSortWarps * rows; i += kSortWarps * 32) places[i] = 0;
     grid_dependency_sync();
     for (int i = blockIdx.x * (kSortWarps * 32) + threadIdx.x; i < counters; i += gridDim.x * (kSortWarps * 32)) arrived[i] = 0;
     __syncthreads();
-    const int share = ((tokens + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, begin = min((long long)warp * share, (long long)tokens), end = min(begin + (long long)share, (long long)tokens);
-    int *mine = places + warp * range, below = 0;
+    const int share = ((tokens + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, begin = (int)min((long long)warp * share, (long long)tokens), end = (int)min(begin + (long long)share, (long long)tokens);
+    int *mine = places + warp * rows, below = 0;
     for (int t0 = begin; t0 < end; t0 += 32 * U) {
         int id[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) id[u] = t0 + u * 32 + lane < end ? ids[(t0 + u * 32 + lane) * ids_stride] : -1;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            below += (unsigned)id[u] < (unsigned)v0;
-            const bool in = (unsigned)id[u] - (unsigned)v0 < (unsigned)rows && id[u] >= 0;
-            const unsigned all = __ballot_sync(0xffffffffu, in);
-            if (!all) continue;
-            if (in) {
-                const unsigned same = __match_any_sync(all, id[u]);
-                if (lane == __ffs(same) - 1) mine[id[u] - v0] += __popc(same);
-            }
-            __syncwarp();
+            const bool some = (unsigned)id[u] < (unsigned)vocab;
+            below += some && (id[u] & ending) < own;
+            if (some && (id[u] & ending) == own) atomicAdd(mine + (id[u] >> bits), 1);  // a count: any order
         }
     }
     for (int o = 16; o; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
     if (lane == 0) warp_sums[warp] = below;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int s = 0;
-        for (int w = 0; w < kSortWarps; ++w) s += warp_sums[w];
-        below_all = s;
+    if (warp == 0) {
+        int s = warp_sums[lane];
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) below_all = s;
     }
     __syncthreads();
     int next = below_all;  // place of the next row's first token
     for (int r0 = 0; r0 < rows; r0 += kSortWarps * 32) {
         const int r = r0 + threadIdx.x;
-        int total = 0;
+        int count = 0;
         if (r < rows)
-            for (int w = 0; w < kSortWarps; ++w) total += places[w * range + r];
-        int sum = total;
+#pragma unroll 8
+            for (int w = 0; w < kSortWarps; ++w) count += places[w * rows + r];
+        int sum = count;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int left = __shfl_up_sync(0xffffffffu, sum, o);
@@ -122,41 +118,50 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const i
         }
         if (lane == 31) warp_sums[warp] = sum;
         __syncthreads();
-        int at = next + sum - total, chunk = 0;
-        for (int w = 0; w < kSortWarps; ++w) {
-            if (w < warp) at += warp_sums[w];
-            chunk += warp_sums[w];
+        int ahead = lane < warp ? warp_sums[lane] : 0, all = warp_sums[lane];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+            all += __shfl_xor_sync(0xffffffffu, all, o);
         }
-        next += chunk;
+        int at = next + ahead + sum - count;
+        next += all;
         if (r < rows) {
-            row_start[v0 + r] = at;
+            spans[((long long)r << bits) + own] = make_int2(at, at + count);
+#pragma unroll 8
             for (int w = 0; w < kSortWarps; ++w) {
-                const int c = places[w * range + r];
-                places[w * range + r] = at;
+                const int c = places[w * rows + r];
+                places[w * rows + r] = at;
                 at += c;
             }
         }
         __syncthreads();
     }
-    if (v0 + rows == vocab && threadIdx.x == 0) row_start[vocab] = next;
+    if (own == ending && threadIdx.x == 0) *total = next;
     for (int t0 = begin; t0 < end; t0 += 32 * U) {
-        int id[U];
+        int id[U], from[U];
+        unsigned same[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) id[u] = t0 + u * 32 + lane < end ? ids[(t0 + u * 32 + lane) * ids_stride] : -1;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool in = (unsigned)id[u] - (unsigned)v0 < (unsigned)rows && id[u] >= 0;
+            const bool in = (unsigned)id[u] < (unsigned)vocab && (id[u] & ending) == own;
             const unsigned all = __ballot_sync(0xffffffffu, in);
-            if (!all) continue;
+            same[u] = 0;
+            __syncwarp();  // places of u - 1 are taken
             if (in) {
-                const unsigned same = __match_any_sync(all, id[u]);
-                const int at = mine[id[u] - v0], place = at + __popc(same & ((1u << lane) - 1));
+                same[u] = __match_any_sync(all, id[u]);
+                if (lane == __ffs(same[u]) - 1) from[u] = atomicAdd(mine + (id[u] >> bits), __popc(same[u]));  // one lane for each row: in the order of u
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = __shfl_sync(0xffffffffu, from[u], same[u] ? __ffs(same[u]) - 1 : lane);
+            if (same[u]) {
+                const int place = at + __popc(same[u] & ((1u << lane) - 1));
                 order[place] = t0 + u * 32 + lane;
                 sorted[place] = id[u];
-                __syncwarp(all);
-                if (lane == __ffs(same) - 1) mine[id[u] - v0] = at + __popc(same);
             }
-            __syncwarp();
         }
     }
 }
@@ -174,7 +179,8 @@ struct EmbeddingGrad {
     long long ld;
     int dim, vocab, slices, chunks, add;
     float scale;
-    const int *row_start, *order, *sorted;
+    const int2 *spans;  // a row's places in the order
+    const int *total, *order, *sorted;
     float *partial;
     unsigned *arrived;
 };
@@ -210,9 +216,11 @@ __global__ void __launch_bounds__(kSumTokens) embedding_grad_kernel(const __grid
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if ((int)blockIdx.x >= a.chunks * a.slices) {  // rows without a token
         const long long v0 = (long long)(blockIdx.x - a.chunks * a.slices) * kZeroRows, v1 = min(v0 + kZeroRows, (long long)a.vocab);
-        for (long long v = v0 + warp; v < v1; v += kSumWarps) {
-            if (a.row_start[v] != a.row_start[v + 1]) continue;
-            float *row = a.dtable + v * a.ld;
+        const long long first = v0 + warp * (kZeroRows / kSumWarps);  // the warp's rows, looked up at once
+        int2 span = make_int2(0, 1);
+        if (lane < kZeroRows / kSumWarps && first + lane < v1) span = a.spans[first + lane];
+        for (unsigned todo = __ballot_sync(0xffffffffu, span.x == span.y); todo; todo &= todo - 1) {
+            float *row = a.dtable + (first + __ffs(todo) - 1) * a.ld;
             if (WIDE)
                 for (int c = lane * 4; c < a.dim; c += 128) *reinterpret_cast<float4 *>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
             else
@@ -220,7 +228,7 @@ __global__ void __launch_bounds__(kSumTokens) embedding_grad_kernel(const __grid
         }
         return;
     }
-    const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices, total = a.row_start[a.vocab];
+    const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices, total = *a.total;
     if (chunk * kSumTokens >= total) return;
     const C cols(slice, a.dim);
     auto output = [&](int v, const float (&x)[N]) {
@@ -229,18 +237,18 @@ __global__ void __launch_bounds__(kSumTokens) embedding_grad_kernel(const __grid
             if (cols.first >= a.dim) return;
 #pragma unroll
             for (int q = 0; q < N; q += 4) {
-                float4 *p = reinterpret_cast<float4 *>(row + cols.first + q);
-                float4 o = a.add ? *p : make_float4(0.f, 0.f, 0.f, 0.f);
-                o.x += x[q] * a.scale;
-                o.y += x[q + 1] * a.scale;
-                o.z += x[q + 2] * a.scale;
-                o.w += x[q + 3] * a.scale;
-                *p = o;
+                const float4 o = make_float4(x[q] * a.scale, x[q + 1] * a.scale, x[q + 2] * a.scale, x[q + 3] * a.scale);
+                // One addition to each element in all, made in L2: reading the row first would stop the warp at the end of every row.
+                if (a.add) asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(row + cols.first + q), "f"(o.x), "f"(o.y), "f"(o.z), "f"(o.w) : "memory");
+                else *reinterpret_cast<float4 *>(row + cols.first + q) = o;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (cols.has(j)) row[cols.column(j)] = (a.add ? row[cols.column(j)] : 0.f) + x[j] * a.scale;
+                if (cols.has(j)) {
+                    if (a.add) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(row + cols.column(j)), "f"(x[j] * a.scale) : "memory");
+                    else row[cols.column(j)] = x[j] * a.scale;
+                }
         }
     };
     auto keep = [&](float *to, const float (&x)[N]) {
@@ -355,7 +363,8 @@ __global__ void __launch_bounds__(kSumTokens) embedding_grad_kernel(const __grid
             for (int k = 0; k < 2; ++k) {
                 last[k] = 0;
                 if (spans[k] < 0) continue;
-                const int c0 = a.row_start[spans[k]] / kSumTokens, c1 = (a.row_start[spans[k] + 1] - 1) / kSumTokens;
+                const int2 at = a.spans[spans[k]];
+                const int c0 = at.x / kSumTokens, c1 = (at.y - 1) / kSumTokens;
                 last[k] = atomicAdd(a.arrived + (long long)c0 * a.slices + slice, 1u) == (unsigned)(c1 - c0);
             }
             __threadfence();
@@ -364,7 +373,7 @@ __global__ void __launch_bounds__(kSumTokens) embedding_grad_kernel(const __grid
     __syncthreads();
     for (int k = 0; k < 2; ++k) {
         if (!last[k]) continue;  // the same for the whole block
-        const int v = spans[k], c0 = a.row_start[v] / kSumTokens, pieces = (a.row_start[v + 1] - 1) / kSumTokens - c0 + 1;
+        const int v = spans[k], c0 = a.spans[v].x / kSumTokens, pieces = (a.spans[v].y - 1) / kSumTokens - c0 + 1;
         float sum[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) sum[j] = 0.f;
@@ -427,12 +436,13 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     const long long zero_blocks = add ? 0 : (vocab + kZeroRows - 1) / kZeroRows;
     if (chunks * slices + zero_blocks > 0x7fffffffll || chunks * kSumTokens > 0x7fff0000ll) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many rows");
     const auto rounded = [](long long words) { return (words + 63) / 64 * 64; };
-    const long long starts = rounded(vocab + 1), places = rounded(tokens), counters = rounded(chunks * slices);
+    const long long starts = rounded(2 * vocab + 1), places = rounded(tokens), counters = rounded(chunks * slices);
     Block *scratch = ctx.allocator().alloc((size_t)(starts + 2 * places + counters + 2 * chunks * slices * 32 * n) * 4);
     if (!scratch) return ctx.fail(SAGE_ERR_OOM, "embedding_grad: out of memory");
     EmbeddingGrad a;
     int *words = (int *)scratch->ptr;
-    a.row_start = words;
+    a.spans = (const int2 *)words;
+    a.total = words + 2 * vocab;
     a.order = words + starts;
     a.sorted = a.order + places;
     a.arrived = (unsigned *)(words + starts + 2 * places);
@@ -448,19 +458,17 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     a.add = add;
     a.scale = scale;
     const bool wide = dim % n == 0 && on_16(g.ptr, g.pitch, 16 / n) && on_16(dtable.ptr, dtable.pitch, 4);
-    // One block for each SM where shared memory holds the counts of that many rows.
-    const int most = 2048;
-    long long range = (vocab + ctx.sm_count - 1) / ctx.sm_count;
-    range = range < 32 ? 32 : range > most ? most : range;
-    const size_t smem = (size_t)range * kSortWarps * 4;
+    int bits = 0;  // about one block for each SM; more where shared memory does not hold the counts of that many rows
+    while ((2ll << bits) <= vocab && ((2 << bits) <= ctx.sm_count || ((vocab - 1) >> bits) + 1 > kSortRows)) ++bits;
+    const size_t smem = (size_t)(((vocab - 1) >> bits) + 1) * kSortWarps * 4;
     sage_status st = SAGE_OK;
     ctx.note_launch("embedding_sort");
     ctx.note_launch("embedding_grad");
     if (!ctx.dry()) {
-        st = ctx.check_cuda(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most * kSortWarps * 4), "embedding_sort");
+        st = ctx.check_cuda(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortRows * kSortWarps * 4), "embedding_sort");
         if (!st)
-            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), embedding_sort_kernel, dim3((unsigned)((vocab + range - 1) / range)), dim3(kSortWarps * 32), smem, (const int *)ids.ptr, ids.stride,
-                                                 (int)tokens, (int)vocab, (int)range, (int *)a.row_start, (int *)a.order, (int *)a.sorted, a.arrived, (int)counters),
+            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), embedding_sort_kernel, dim3(1u << bits), dim3(kSortWarps * 32), smem, (const int *)ids.ptr, ids.stride,
+                                                 (int)tokens, (int)vocab, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted, a.arrived, (int)counters),
                                 "embedding_sort");
         if (!st)
             st = with_type(g.dtype, [&](auto t) {
