@@ -64,52 +64,94 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T *__restrict__ ta
 // Tokens are sorted by table row (those of a row in their order), then rows are summed in pieces of a fixed length of that order, so
 // that a frequent token's thousands of rows are spread like any others.  Two launches, no sums by atomics: the same bits every time.
 
+constexpr int kZeroRows = 64;  // of a block that writes zeros
+// Zeros into the rows of the table, 16 bytes at a time where they lie on such boundaries.
+struct Zeros {
+    float *dtable;
+    long long ld;
+    int dim, wide;
+    // The block's rows from `first` on; with `spans` those that no token reaches.
+    __device__ __forceinline__ void rows(long long first, int vocab, const int2 *spans) const {
+        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32, each = (kZeroRows + warps - 1) / warps;
+        first += warp * each;  // the warp's rows, looked up 32 at once
+        const long long end = min(first + each, (long long)vocab);
+        for (long long v0 = first; v0 < end; v0 += 32) {
+            bool empty = v0 + lane < end;
+            if (empty && spans) {
+                const int2 span = spans[v0 + lane];
+                empty = span.x == span.y;
+            }
+            for (unsigned todo = __ballot_sync(0xffffffffu, empty); todo; todo &= todo - 1) {
+                float *row = dtable + (v0 + __ffs(todo) - 1) * ld;
+                if (wide)
+                    for (int c = lane * 4; c < dim; c += 128) *reinterpret_cast<float4 *>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+                else
+                    for (int c = lane; c < dim; c += 32) row[c] = 0.f;
+            }
+        }
+    }
+};
+
 // Sorting.  Each of 2^bits blocks owns the table rows whose numbers end in its own (frequent tokens have low numbers: neighbours go to
 // different blocks) and reads all ids: its warps, each over a contiguous share of the tokens, count its rows' tokens, the counts become
 // places (in front of them all tokens of the blocks before), and a second pass puts the tokens there.  A hundred times the ids out of L2
 // instead of a radix sort's passes through memory and launches.
-constexpr int kSortWarps = 32, kSortRows = 1536;  // rows of a block at most: their counts fill shared memory
+constexpr int kSortWarps = 32, kSortRows = 1024, kSortList = 256;  // rows of a block and own tokens of a warp that shared memory holds
 __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const int *__restrict__ ids, long long ids_stride, int tokens, int vocab, int bits, int2 *__restrict__ spans, int *__restrict__ total,
-                                                                         int *__restrict__ order, int *__restrict__ sorted, unsigned *__restrict__ arrived, int counters) {
-    extern __shared__ int places[];  // [warp][row of the block]
+                                                                         int *__restrict__ order, int *__restrict__ sorted, unsigned *__restrict__ arrived, int counters, const Zeros zeros) {
+    if (blockIdx.x >> bits) {  // blocks behind the sorting ones: all of the table is zero until the sums are written
+        grid_dependency_sync();
+        zeros.rows((long long)(blockIdx.x - (1u << bits)) * kZeroRows, vocab, nullptr);
+        return;
+    }
+    extern __shared__ int2 lists[];  // [warp][kSortList] {token, id}, then [warp][row of the block] counts, later places
+    int *places = reinterpret_cast<int *>(lists + blockDim.x / 32 * kSortList);
     __shared__ int warp_sums[kSortWarps], below_all;
     constexpr int U = 8;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
     const unsigned own = blockIdx.x, ending = (1u << bits) - 1;
     const int rows = (int)(((unsigned)vocab - own + ending) >> bits);
-    for (int i = threadIdx.x; i < kSortWarps * rows; i += kSortWarps * 32) places[i] = 0;
+    for (int i = threadIdx.x; i < warps * rows; i += blockDim.x) places[i] = 0;
     grid_dependency_sync();
-    for (int i = blockIdx.x * (kSortWarps * 32) + threadIdx.x; i < counters; i += gridDim.x * (kSortWarps * 32)) arrived[i] = 0;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < counters; i += (ending + 1) * blockDim.x) arrived[i] = 0;
     __syncthreads();
-    const int share = ((tokens + kSortWarps - 1) / kSortWarps + 31) / 32 * 32, begin = (int)min((long long)warp * share, (long long)tokens), end = (int)min(begin + (long long)share, (long long)tokens);
-    int *mine = places + warp * rows, below = 0;
+    const int share = ((tokens + warps - 1) / warps + 31) / 32 * 32, begin = (int)min((long long)warp * share, (long long)tokens), end = (int)min(begin + (long long)share, (long long)tokens);
+    int2 *list = lists + warp * kSortList;
+    int *mine = places + warp * rows, below = 0, found = 0;
     for (int t0 = begin; t0 < end; t0 += 32 * U) {
         int id[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) id[u] = t0 + u * 32 + lane < end ? ids[(t0 + u * 32 + lane) * ids_stride] : -1;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool some = (unsigned)id[u] < (unsigned)vocab;
-            below += some && (id[u] & ending) < own;
-            if (some && (id[u] & ending) == own) atomicAdd(mine + (id[u] >> bits), 1);  // a count: any order
+            const unsigned block = (unsigned)id[u] < (unsigned)vocab ? (unsigned)id[u] & ending : ~0u;
+            below += block < own;
+            const unsigned all = __ballot_sync(0xffffffffu, block == own);
+            if (!all) continue;
+            if (block == own) {
+                atomicAdd(mine + (id[u] >> bits), 1);  // a count: any order
+                const int at = found + __popc(all & ((1u << lane) - 1));
+                if (at < kSortList) list[at] = make_int2(t0 + u * 32 + lane, id[u]);
+            }
+            found += __popc(all);
         }
     }
     for (int o = 16; o; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
     if (lane == 0) warp_sums[warp] = below;
     __syncthreads();
     if (warp == 0) {
-        int s = warp_sums[lane];
+        int s = lane < warps ? warp_sums[lane] : 0;
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) below_all = s;
     }
     __syncthreads();
     int next = below_all;  // place of the next row's first token
-    for (int r0 = 0; r0 < rows; r0 += kSortWarps * 32) {
+    for (int r0 = 0; r0 < rows; r0 += blockDim.x) {
         const int r = r0 + threadIdx.x;
         int count = 0;
         if (r < rows)
 #pragma unroll 8
-            for (int w = 0; w < kSortWarps; ++w) count += places[w * rows + r];
+            for (int w = 0; w < warps; ++w) count += places[w * rows + r];
         int sum = count;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -118,7 +160,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const i
         }
         if (lane == 31) warp_sums[warp] = sum;
         __syncthreads();
-        int ahead = lane < warp ? warp_sums[lane] : 0, all = warp_sums[lane];
+        int all = lane < warps ? warp_sums[lane] : 0, ahead = lane < warp ? all : 0;
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
@@ -128,277 +170,213 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const i
         next += all;
         if (r < rows) {
             spans[((long long)r << bits) + own] = make_int2(at, at + count);
+            if (count)
 #pragma unroll 8
-            for (int w = 0; w < kSortWarps; ++w) {
-                const int c = places[w * rows + r];
-                places[w * rows + r] = at;
-                at += c;
-            }
+                for (int w = 0; w < warps; ++w) {
+                    const int c = places[w * rows + r];
+                    places[w * rows + r] = at;
+                    at += c;
+                }
         }
         __syncthreads();
     }
     if (own == ending && threadIdx.x == 0) *total = next;
-    for (int t0 = begin; t0 < end; t0 += 32 * U) {
-        int id[U], from[U];
-        unsigned same[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) id[u] = t0 + u * 32 + lane < end ? ids[(t0 + u * 32 + lane) * ids_stride] : -1;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = (unsigned)id[u] < (unsigned)vocab && (id[u] & ending) == own;
-            const unsigned all = __ballot_sync(0xffffffffu, in);
-            same[u] = 0;
-            __syncwarp();  // places of u - 1 are taken
-            if (in) {
-                same[u] = __match_any_sync(all, id[u]);
-                if (lane == __ffs(same[u]) - 1) from[u] = atomicAdd(mine + (id[u] >> bits), __popc(same[u]));  // one lane for each row: in the order of u
-            }
+    // 32 tokens of the warp's own at a time, from its list, or from all of its share where the list was too short
+    auto put = [&](int t, int id, bool in) {
+        const unsigned all = __ballot_sync(0xffffffffu, in);
+        if (!all) return;
+        __syncwarp();
+        unsigned same = 1u << lane;
+        int from = 0;
+        if (in) {
+            same = __match_any_sync(all, id);
+            if (lane == __ffs(same) - 1) from = atomicAdd(mine + (id >> bits), __popc(same));  // one lane for each row
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = __shfl_sync(0xffffffffu, from[u], same[u] ? __ffs(same[u]) - 1 : lane);
-            if (same[u]) {
-                const int place = at + __popc(same[u] & ((1u << lane) - 1));
-                order[place] = t0 + u * 32 + lane;
-                sorted[place] = id[u];
-            }
+        const int at = __shfl_sync(0xffffffffu, from, __ffs(same) - 1) + __popc(same & ((1u << lane) - 1));
+        if (in) {
+            order[at] = t;
+            sorted[at] = id;
+        }
+    };
+    if (found <= kSortList) {
+        __syncwarp();
+        for (int i = 0; i < found; i += 32) {
+            const bool in = i + lane < found;
+            const int2 t = in ? list[i + lane] : make_int2(0, 0);
+            put(t.x, t.y, in);
+        }
+    } else {
+        for (int t0 = begin; t0 < end; t0 += 32) {
+            const int t = t0 + lane, id = t < end ? ids[t * ids_stride] : -1;
+            put(t, id, (unsigned)id < (unsigned)vocab && ((unsigned)id & ending) == own);
         }
     }
 }
 
-// Summing.  A block takes 256 tokens of the sorted order, 32 to a warp, and 32 lanes' columns; the rows of g that end in a warp's 32 go
-// straight to the table, the others are joined over the warps in shared memory, and what goes on beyond the block's 256 is left in
-// `partial` (slot 2 c: of a row that began before block c, 2 c + 1: of one that goes on behind it); the last block of such a row to
-// arrive adds the pieces up, in their order.  Further blocks write the rows that no token reaches.
-// Bound by memory: g once, the table once.
-constexpr int kSumWarps = 8, kSumTokens = 32 * kSumWarps, kZeroRows = 64;
+// Summing.  A block takes `length` tokens of the sorted order and four columns for each of its threads, and adds the rows of g up one
+// after the other; a row of the table that ends is written, what goes on beyond the block's tokens is left in `partial` (slot 2 c: of a
+// row that began before block c, 2 c + 1: of one that goes on behind it), and the last block of such a row to arrive adds the pieces up,
+// in their order.  Further blocks write the rows that no token reaches.
+// Bound by memory: g once, the table once.  Each thread copies its own columns of the next tokens into shared memory asynchronously (no
+// barriers, and no registers that wait for them): kAhead rows of the block in flight, six blocks of 256
+// threads on an SM.
 struct EmbeddingGrad {
     const void *g;
     long long ldg;
-    float *dtable;
-    long long ld;
-    int dim, vocab, slices, chunks, add;
+    Zeros table;
+    int vocab, tokens, slices, chunks, length, add;
     float scale;
     const int2 *spans;  // a row's places in the order
     const int *total, *order, *sorted;
     float *partial;
     unsigned *arrived;
 };
+constexpr int kMaxLength = 256, kAhead = 8;
 
-template <class T, bool WIDE>
-struct Columns {  // a lane's columns of a slice: N in a row, or N that lie 32 apart
-    static constexpr int N = 16 / (int)sizeof(T);
+template <class T>
+struct alignas(4 * sizeof(T)) Four {
+    T v[4];
+};
+// The thread's columns: four in a row, or (rows that do not lie on such boundaries) four that lie blockDim.x apart.
+template <bool WIDE>
+struct Columns {
     int first, dim;
-    __device__ Columns(int slice, int dim_) : first(slice * 32 * N + (threadIdx.x % 32) * (WIDE ? N : 1)), dim(dim_) {}
-    __device__ __forceinline__ int column(int j) const { return first + (WIDE ? j : 32 * j); }
+    __device__ Columns(int slice, int dim_) : first(slice * blockDim.x * 4 + threadIdx.x * (WIDE ? 4 : 1)), dim(dim_) {}
+    __device__ __forceinline__ int column(int j) const { return first + (WIDE ? j : j * (int)blockDim.x); }
     __device__ __forceinline__ bool has(int j) const { return column(j) < dim; }
-    __device__ __forceinline__ Pack<T> load(const T *row) const {
-        Pack<T> v;
-        if (WIDE) {
-            if (first < dim) v = *reinterpret_cast<const Pack<T> *>(row + first);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (has(j)) v.v[j] = row[column(j)];
-        }
-        return v;
-    }
 };
 
 template <class T, bool WIDE>
-__global__ void __launch_bounds__(kSumTokens) embedding_grad_kernel(const __grid_constant__ EmbeddingGrad a) {
-    typedef Columns<T, WIDE> C;
-    constexpr int N = C::N, U = 8;
-    __shared__ float head[kSumWarps][32 * N], tail[kSumWarps][32 * N];
-    __shared__ int head_row[kSumWarps], tail_row[kSumWarps], head_ends[kSumWarps];  // rows: -1 = none
-    __shared__ int spans[2], last[2];  // rows that go on beyond the block (-1 = none): began before it, or in it
+__global__ void __launch_bounds__(256) embedding_grad_kernel(const __grid_constant__ EmbeddingGrad a) {
+    extern __shared__ char ahead[];  // WIDE: [kAhead][thread] of Four<T>
+    __shared__ int rows[kMaxLength + 2], tokens[kMaxLength], last[2];
     grid_dependency_sync();
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if ((int)blockIdx.x >= a.chunks * a.slices) {  // rows without a token
-        const long long v0 = (long long)(blockIdx.x - a.chunks * a.slices) * kZeroRows, v1 = min(v0 + kZeroRows, (long long)a.vocab);
-        const long long first = v0 + warp * (kZeroRows / kSumWarps);  // the warp's rows, looked up at once
-        int2 span = make_int2(0, 1);
-        if (lane < kZeroRows / kSumWarps && first + lane < v1) span = a.spans[first + lane];
-        for (unsigned todo = __ballot_sync(0xffffffffu, span.x == span.y); todo; todo &= todo - 1) {
-            float *row = a.dtable + (first + __ffs(todo) - 1) * a.ld;
-            if (WIDE)
-                for (int c = lane * 4; c < a.dim; c += 128) *reinterpret_cast<float4 *>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-            else
-                for (int c = lane; c < a.dim; c += 32) row[c] = 0.f;
-        }
+    if ((int)blockIdx.x >= a.chunks * a.slices) {
+        a.table.rows((long long)(blockIdx.x - a.chunks * a.slices) * kZeroRows, a.vocab, a.spans);
         return;
     }
-    const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices, total = *a.total;
-    if (chunk * kSumTokens >= total) return;
-    const C cols(slice, a.dim);
-    auto output = [&](int v, const float (&x)[N]) {
-        float *row = a.dtable + v * a.ld;
+    const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices, from = chunk * a.length, total = *a.total;
+    for (int i = threadIdx.x; i < a.length + 2; i += blockDim.x) {  // rows[i + 1]: of the i-th token, and of those in front and behind; -1 = none
+        const int place = from + i - 1;
+        const bool there = place >= 0 && place < total;
+        rows[i] = there ? a.sorted[place] : -1;
+        if (i > 0 && i <= a.length) tokens[i - 1] = there ? a.order[place] : 0;
+    }
+    if (from >= total) return;  // the whole block
+    const int n = min(a.length, total - from);
+    __syncthreads();
+    const Columns<WIDE> cols(slice, a.table.dim);
+    const T *g = (const T *)a.g + cols.first;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    auto output = [&](int v) {
+        float *row = a.table.dtable + v * a.table.ld;
+        // Added: one addition to each element in all, made in L2; reading the row first would stop the thread at the end of every row.
         if (WIDE) {
-            if (cols.first >= a.dim) return;
-#pragma unroll
-            for (int q = 0; q < N; q += 4) {
-                const float4 o = make_float4(x[q] * a.scale, x[q + 1] * a.scale, x[q + 2] * a.scale, x[q + 3] * a.scale);
-                // One addition to each element in all, made in L2: reading the row first would stop the warp at the end of every row.
-                if (a.add) asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(row + cols.first + q), "f"(o.x), "f"(o.y), "f"(o.z), "f"(o.w) : "memory");
-                else *reinterpret_cast<float4 *>(row + cols.first + q) = o;
-            }
+            if (cols.first >= cols.dim) return;
+            const float4 o = make_float4(sum[0] * a.scale, sum[1] * a.scale, sum[2] * a.scale, sum[3] * a.scale);
+            if (a.add) asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(row + cols.first), "f"(o.x), "f"(o.y), "f"(o.z), "f"(o.w) : "memory");
+            else *reinterpret_cast<float4 *>(row + cols.first) = o;
         } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (cols.has(j)) {
-                    if (a.add) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(row + cols.column(j)), "f"(x[j] * a.scale) : "memory");
-                    else row[cols.column(j)] = x[j] * a.scale;
-                }
+            for (int j = 0; j < 4; ++j) {
+                if (!cols.has(j)) continue;
+                if (a.add) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(row + cols.column(j)), "f"(sum[j] * a.scale) : "memory");
+                else row[cols.column(j)] = sum[j] * a.scale;
+            }
         }
     };
-    auto keep = [&](float *to, const float (&x)[N]) {
+    const long long stride = (long long)a.slices * blockDim.x * 4;  // of the partial sums: [slot][slice][column][thread]
+    float *partial = a.partial + (long long)slice * blockDim.x * 4 + threadIdx.x;
+    auto leave = [&](int slot) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) to[j * 32 + lane] = x[j];
+        for (int j = 0; j < 4; ++j) __stcg(partial + slot * stride + j * blockDim.x, sum[j]);
     };
-
-    // the warp's 32 places
-    const int from = chunk * kSumTokens + warp * 32, n = min(32, total - from);
-    int first_row = -1, tail_kept = -1, ends = 0;
-    if (n > 0) {
-        const int row = lane < n ? a.sorted[from + lane] : -1, token = lane < n ? a.order[from + lane] : 0;
-        const int before = from > 0 ? a.sorted[from - 1] : -1, after = from + n < total ? a.sorted[from + n] : -1;
-        const int left = __shfl_up_sync(0xffffffffu, row, 1);
-        const unsigned starts = __ballot_sync(0xffffffffu, lane < n && row != (lane ? left : before));
-        float sum[N];
+    const bool before = rows[0] == rows[1];  // the first row began in front
+    bool first = true;                       // ... and goes on
+    auto ended = [&](int i) {                // the row of tokens [.., i)
+        if (first && before) leave(2 * chunk);
+        else output(rows[i]);
+        first = false;
+        sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+    };
+    if (WIDE) {
+        Four<T> *mine = reinterpret_cast<Four<T> *>(ahead) + threadIdx.x;
+        const bool some = cols.first < cols.dim;
+        auto fetch = [&](int i) {
+            if (some && i < n)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((unsigned)__cvta_generic_to_shared(mine + i % kAhead * blockDim.x)), "l"(g + tokens[i] * a.ldg), "n"((int)sizeof(Four<T>)) : "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] = 0.f;
-        bool began_before = !(starts & 1);
+        for (int i = 0; i < kAhead; ++i) fetch(i);
+        for (int i = 0; i < n; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+            if (i && rows[i + 1] != rows[i]) ended(i);
+            const Four<T> v = mine[i % kAhead * blockDim.x];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += widen(v.v[j]);
+            asm volatile("" ::"f"(sum[0]), "f"(sum[1]), "f"(sum[2]), "f"(sum[3]) : "memory");  // read before the place is taken again
+            fetch(i + kAhead);
+        }
+    } else {
+        constexpr int U = 8;
         for (int i0 = 0; i0 < n; i0 += U) {
-            Pack<T> v[U];
+            T v[U][4];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int t = __shfl_sync(0xffffffffu, token, (i0 + u) & 31);
-                if (i0 + u < n) v[u] = cols.load((const T *)a.g + t * a.ldg);
-            }
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i0 + u < n && cols.has(j)) v[u][j] = g[tokens[i0 + u] * a.ldg + j * (int)blockDim.x];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int i = i0 + u;
                 if (i >= n) break;
-                if (i && starts >> i & 1) {  // the row so far is complete
-                    const int done = __shfl_sync(0xffffffffu, row, i - 1);
-                    if (began_before) {
-                        first_row = done;
-                        ends = 1;
-                        keep(head[warp], sum);
-                    } else {
-                        output(done, sum);
-                    }
-                    began_before = false;
+                if (i && rows[i + 1] != rows[i]) ended(i);
 #pragma unroll
-                    for (int j = 0; j < N; ++j) sum[j] = 0.f;
-                }
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum[j] += widen(v[u].v[j]);
+                for (int j = 0; j < 4; ++j) sum[j] += widen(v[u][j]);
             }
         }
-        const int done = __shfl_sync(0xffffffffu, row, n - 1);
-        if (began_before) {
-            first_row = done;
-            ends = done != after;
-            keep(head[warp], sum);
-        } else if (done == after) {
-            tail_kept = done;
-            keep(tail[warp], sum);
-        } else {
-            output(done, sum);
-        }
     }
-    if (lane == 0) {
-        head_row[warp] = first_row;
-        head_ends[warp] = ends;
-        tail_row[warp] = tail_kept;
+    int spans_before = before ? rows[1] : -1, spans_after = -1;
+    if (rows[n + 1] != rows[n] && !(first && before)) {
+        output(rows[n]);
+    } else if (first && before) {
+        leave(2 * chunk);
+    } else {
+        leave(2 * chunk + 1);
+        spans_after = rows[n];
     }
+    if (spans_before < 0 && spans_after < 0) return;  // the whole block
+    __threadfence();
     __syncthreads();
-
-    // over the warps
-    const long long stride = (long long)a.slices * 32 * N;  // of the partial sums, padded to whole slices
-    float *partial = a.partial + slice * 32 * N + lane;
-    if (warp == 0) {
-        float sum[N];
-        int open = -1, spans_before = -1, spans_after = -1;
-        bool began_before = false;
-        auto leave = [&](int slot) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) __stcg(partial + slot * stride + j * 32, sum[j]);
-        };
-        for (int w = 0; w < kSumWarps; ++w) {
-            if (head_row[w] >= 0) {
-                if (w == 0) began_before = true;
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum[j] = (w ? sum[j] : 0.f) + head[w][j * 32 + lane];
-                open = head_row[w];
-                if (head_ends[w]) {
-                    if (began_before) {
-                        spans_before = open;
-                        leave(2 * chunk);
-                    } else {
-                        output(open, sum);
-                    }
-                    open = -1;
-                    began_before = false;
-                }
-            }
-            if (tail_row[w] >= 0) {
-                open = tail_row[w];
-                began_before = false;
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum[j] = tail[w][j * 32 + lane];
-            }
-        }
-        if (open >= 0) {
-            leave(2 * chunk + (began_before ? 0 : 1));
-            (began_before ? spans_before : spans_after) = open;
+    if (threadIdx.x < 2) {
+        const int v = threadIdx.x ? spans_after : spans_before;
+        last[threadIdx.x] = 0;
+        if (v >= 0) {
+            const int2 at = a.spans[v];
+            const int c0 = at.x / a.length, c1 = (at.y - 1) / a.length;
+            last[threadIdx.x] = atomicAdd(a.arrived + (long long)c0 * a.slices + slice, 1u) == (unsigned)(c1 - c0);
         }
         __threadfence();
-        __syncwarp();
-        if (lane == 0) {
-            spans[0] = spans_before;
-            spans[1] = spans_after;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                last[k] = 0;
-                if (spans[k] < 0) continue;
-                const int2 at = a.spans[spans[k]];
-                const int c0 = at.x / kSumTokens, c1 = (at.y - 1) / kSumTokens;
-                last[k] = atomicAdd(a.arrived + (long long)c0 * a.slices + slice, 1u) == (unsigned)(c1 - c0);
-            }
-            __threadfence();
-        }
     }
     __syncthreads();
+#pragma unroll 1
     for (int k = 0; k < 2; ++k) {
-        if (!last[k]) continue;  // the same for the whole block
-        const int v = spans[k], c0 = a.spans[v].x / kSumTokens, pieces = (a.spans[v].y - 1) / kSumTokens - c0 + 1;
-        float sum[N];
+        if (!last[k]) continue;
+        const int v = k ? spans_after : spans_before, c0 = a.spans[v].x / a.length, pieces = (a.spans[v].y - 1) / a.length - c0 + 1;
+        sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+#pragma unroll 8
+        for (int p = 0; p < pieces; ++p)
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] = 0.f;
-        const int p1 = (int)((long long)pieces * (warp + 1) / kSumWarps);
-#pragma unroll 4
-        for (int p = (int)((long long)pieces * warp / kSumWarps); p < p1; ++p) {
-            const float *from_piece = partial + (2 * (long long)(c0 + p) + (p == 0)) * stride;
-#pragma unroll
-            for (int j = 0; j < N; ++j) sum[j] += __ldcg(from_piece + j * 32);
-        }
-        keep(head[warp], sum);
-        __syncthreads();
-        if (warp == 0) {
-            for (int w = 1; w < kSumWarps; ++w)
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum[j] += head[w][j * 32 + lane];
-            output(v, sum);
-        }
-        __syncthreads();
+            for (int j = 0; j < 4; ++j) sum[j] += __ldcg(partial + (2 * (long long)(c0 + p) + (p == 0)) * stride + j * blockDim.x);
+        output(v);
     }
 }
 
 }  // namespace
 
-bool on_16(const void *p, long long pitch, size_t size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && pitch * (long long)size % 16 == 0; }
+// Do all rows start at a multiple of `boundary` bytes?
+bool on_boundary(const void *p, long long pitch, size_t size, size_t boundary) { return reinterpret_cast<uintptr_t>(p) % boundary == 0 && (size_t)pitch * size % boundary == 0; }
 
 sage_status embedding(Context &ctx, const RowsArg &table, const VectorArg &ids, float scale, const RowsArg &y) {
     if (!y.rows || !y.cols) return SAGE_OK;
@@ -411,7 +389,7 @@ sage_status embedding(Context &ctx, const RowsArg &table, const VectorArg &ids, 
             if constexpr (sizeof(Y) < sizeof(T)) return ctx.fail(SAGE_ERR_INVALID, "embedding: y is narrower than the table");
             else {
                 constexpr int V = 16 / (int)sizeof(T);
-                const bool wide = y.cols % V == 0 && on_16(table.ptr, table.pitch, sizeof(T)) && on_16(y.ptr, y.pitch, sizeof(Y));
+                const bool wide = y.cols % V == 0 && on_boundary(table.ptr, table.pitch, sizeof(T), 16) && on_boundary(y.ptr, y.pitch, sizeof(Y), 16);
                 const unsigned per_row = (unsigned)(wide ? y.cols / V : y.cols);
                 const long long each = 256 * kLookups;
                 long long most = (0x7fffffffll * each) / per_row;  // rows of one launch
@@ -432,12 +410,21 @@ sage_status embedding(Context &ctx, const RowsArg &table, const VectorArg &ids, 
 sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids, float scale, bool add, const RowsArg &dtable) {
     const long long vocab = dtable.rows, dim = dtable.cols, tokens = g.rows;
     if (!vocab || !dim || (add && !tokens)) return SAGE_OK;
-    const long long n = g.dtype == SAGE_F32 ? 4 : 8, slices = (dim + 32 * n - 1) / (32 * n), chunks = (tokens + kSumTokens - 1) / kSumTokens;
-    const long long zero_blocks = add ? 0 : (vocab + kZeroRows - 1) / kZeroRows;
-    if (chunks * slices + zero_blocks > 0x7fffffffll || chunks * kSumTokens > 0x7fff0000ll) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many rows");
+    if (tokens > 0x7fff0000ll) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many tokens");
+    const size_t size = g.dtype == SAGE_F32 ? 4 : 2;
+    const bool wide = dim % 4 == 0 && on_boundary(g.ptr, g.pitch, size, 4 * size) && on_boundary(dtable.ptr, dtable.pitch, 4, 16);
+    // Four columns a thread, up to 256 threads; so many tokens a block that four blocks an SM take all of them in one go.
+    const long long threads = dim >= 1024 ? 256 : ((dim + 3) / 4 + 31) / 32 * 32, slices = (dim + 4 * threads - 1) / (4 * threads);
+    long long length = (tokens * slices + ctx.sm_count * 4 - 1) / (ctx.sm_count * 4);
+    length = length < 16 ? 16 : length > kMaxLength ? kMaxLength : (length + 7) / 8 * 8;
+    const long long chunks = (tokens + length - 1) / length, zero_blocks = add ? 0 : (vocab + kZeroRows - 1) / kZeroRows;
+    // Where few rows are reached, all of the table is cleared beside the sorting, which keeps the memory idle; where many are, only the others,
+    // beside the sums (4096 tokens into 30522 rows of 768: 27 and 43 us; 65 521 into 50 021 of 1000: 141 and 133 us).
+    const bool clear_first = tokens * 4 <= vocab;
+    if (chunks * slices + zero_blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many rows");
     const auto rounded = [](long long words) { return (words + 63) / 64 * 64; };
     const long long starts = rounded(2 * vocab + 1), places = rounded(tokens), counters = rounded(chunks * slices);
-    Block *scratch = ctx.allocator().alloc((size_t)(starts + 2 * places + counters + 2 * chunks * slices * 32 * n) * 4);
+    Block *scratch = ctx.allocator().alloc((size_t)(starts + 2 * places + counters + 2 * chunks * slices * threads * 4) * 4);
     if (!scratch) return ctx.fail(SAGE_ERR_OOM, "embedding_grad: out of memory");
     EmbeddingGrad a;
     int *words = (int *)scratch->ptr;
@@ -449,32 +436,33 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     a.partial = (float *)(a.arrived + counters);
     a.g = g.ptr;
     a.ldg = g.pitch;
-    a.dtable = (float *)dtable.ptr;
-    a.ld = dtable.pitch;
-    a.dim = (int)dim;
+    a.table = Zeros{(float *)dtable.ptr, dtable.pitch, (int)dim, (int)(dim % 4 == 0 && on_boundary(dtable.ptr, dtable.pitch, 4, 16))};
     a.vocab = (int)vocab;
+    a.tokens = (int)tokens;
     a.slices = (int)slices;
     a.chunks = (int)chunks;
+    a.length = (int)length;
     a.add = add;
     a.scale = scale;
-    const bool wide = dim % n == 0 && on_16(g.ptr, g.pitch, 16 / n) && on_16(dtable.ptr, dtable.pitch, 4);
-    int bits = 0;  // about one block for each SM; more where shared memory does not hold the counts of that many rows
+    int bits = 0;  // about one sorting block for each SM; more where shared memory does not hold the counts of that many rows
     while ((2ll << bits) <= vocab && ((2 << bits) <= ctx.sm_count || ((vocab - 1) >> bits) + 1 > kSortRows)) ++bits;
-    const size_t smem = (size_t)(((vocab - 1) >> bits) + 1) * kSortWarps * 4;
+    const int warps = tokens <= 8192 ? 8 : kSortWarps;  // few ids: the counts of a warp cost more than its share of the ids
+    const size_t smem = (size_t)((((vocab - 1) >> bits) + 1) + 2 * kSortList) * warps * 4;
     sage_status st = SAGE_OK;
     ctx.note_launch("embedding_sort");
     ctx.note_launch("embedding_grad");
     if (!ctx.dry()) {
-        st = ctx.check_cuda(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortRows * kSortWarps * 4), "embedding_sort");
+        st = ctx.check_cuda(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortRows + 2 * kSortList) * kSortWarps * 4), "embedding_sort");
         if (!st)
-            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), embedding_sort_kernel, dim3(1u << bits), dim3(kSortWarps * 32), smem, (const int *)ids.ptr, ids.stride,
-                                                 (int)tokens, (int)vocab, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted, a.arrived, (int)counters),
+            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), embedding_sort_kernel, dim3((1u << bits) + (unsigned)(clear_first ? zero_blocks : 0)), dim3(warps * 32), smem, (const int *)ids.ptr,
+                                                 ids.stride, (int)tokens, (int)vocab, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted, a.arrived, (int)counters, a.table),
                                 "embedding_sort");
         if (!st)
             st = with_type(g.dtype, [&](auto t) {
                 typedef decltype(t) T;
-                return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? embedding_grad_kernel<T, true> : embedding_grad_kernel<T, false>, dim3((unsigned)(chunks * slices + zero_blocks)),
-                                                       dim3(kSumTokens), 0, a),
+                const size_t smem_ahead = wide ? kAhead * threads * sizeof(Four<T>) : 0;  // 32 KB at most
+                return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? embedding_grad_kernel<T, true> : embedding_grad_kernel<T, false>,
+                                                       dim3((unsigned)(chunks * slices + (clear_first ? 0 : zero_blocks))), dim3((unsigned)threads), smem_ahead, a),
                                       "embedding_grad");
             });
     }
