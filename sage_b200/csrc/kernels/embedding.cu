@@ -64,20 +64,20 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T *__restrict__ ta
 // Tokens are sorted by table row (those of a row in their order), then rows are summed in pieces of a fixed length of that order, so
 // that a frequent token's thousands of rows are spread like any others.  Two launches, no sums by atomics: the same bits every time.
 
-constexpr int kZeroRows = 64;  // of a block that writes zeros
+constexpr int kZeroRows = 8;  // of a block that writes zeros: about one to a warp (94 MB with 64 rows a block 30 us, with 6 to 12 18 us)
 // Zeros into the rows of the table, 16 bytes at a time where they lie on such boundaries.
 struct Zeros {
     float *dtable;
     long long ld;
     int dim, wide;
-    // The block's rows from `first` on; with `spans` those that no token reaches.
+    // Those of the block's rows from `first` on that no token reaches.
     __device__ __forceinline__ void rows(long long first, int vocab, const int2 *spans) const {
         const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32, each = (kZeroRows + warps - 1) / warps;
+        const long long end = min(first + kZeroRows, (long long)vocab);
         first += warp * each;  // the warp's rows, looked up 32 at once
-        const long long end = min(first + each, (long long)vocab);
-        for (long long v0 = first; v0 < end; v0 += 32) {
-            bool empty = v0 + lane < end;
-            if (empty && spans) {
+        for (long long v0 = first; v0 < min(first + each, end); v0 += 32) {
+            bool empty = v0 + lane < min(first + each, end);
+            if (empty) {
                 const int2 span = spans[v0 + lane];
                 empty = span.x == span.y;
             }
@@ -98,12 +98,7 @@ struct Zeros {
 // instead of a radix sort's passes through memory and launches.
 constexpr int kSortWarps = 32, kSortRows = 1024, kSortList = 256;  // rows of a block and own tokens of a warp that shared memory holds
 __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const int *__restrict__ ids, long long ids_stride, int tokens, int vocab, int bits, int2 *__restrict__ spans, int *__restrict__ total,
-                                                                         int *__restrict__ order, int *__restrict__ sorted, unsigned *__restrict__ arrived, int counters, const Zeros zeros) {
-    if (blockIdx.x >> bits) {  // blocks behind the sorting ones: all of the table is zero until the sums are written
-        grid_dependency_sync();
-        zeros.rows((long long)(blockIdx.x - (1u << bits)) * kZeroRows, vocab, nullptr);
-        return;
-    }
+                                                                         int *__restrict__ order, int *__restrict__ sorted, unsigned *__restrict__ arrived, int counters) {
     extern __shared__ int2 lists[];  // [warp][kSortList] {token, id}, then [warp][row of the block] counts, later places
     int *places = reinterpret_cast<int *>(lists + blockDim.x / 32 * kSortList);
     __shared__ int warp_sums[kSortWarps], below_all;
@@ -113,7 +108,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const i
     const int rows = (int)(((unsigned)vocab - own + ending) >> bits);
     for (int i = threadIdx.x; i < warps * rows; i += blockDim.x) places[i] = 0;
     grid_dependency_sync();
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < counters; i += (ending + 1) * blockDim.x) arrived[i] = 0;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < counters; i += gridDim.x * blockDim.x) arrived[i] = 0;
     __syncthreads();
     const int share = ((tokens + warps - 1) / warps + 31) / 32 * 32, begin = (int)min((long long)warp * share, (long long)tokens), end = (int)min(begin + (long long)share, (long long)tokens);
     int2 *list = lists + warp * kSortList;
@@ -249,22 +244,25 @@ struct Columns {
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(256) embedding_grad_kernel(const __grid_constant__ EmbeddingGrad a) {
     extern __shared__ char ahead[];  // WIDE: [kAhead][thread] of Four<T>
-    __shared__ int rows[kMaxLength + 2], tokens[kMaxLength], last[2];
+    __shared__ int rows[kMaxLength + 2], tokens[kMaxLength], last[2], first_piece[2];
     grid_dependency_sync();
     if ((int)blockIdx.x >= a.chunks * a.slices) {
         a.table.rows((long long)(blockIdx.x - a.chunks * a.slices) * kZeroRows, a.vocab, a.spans);
         return;
     }
-    const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices, from = chunk * a.length, total = *a.total;
+    const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices, from = chunk * a.length;
+    const int total = *a.total;  // not waited for before what it decides about has been asked for
     for (int i = threadIdx.x; i < a.length + 2; i += blockDim.x) {  // rows[i + 1]: of the i-th token, and of those in front and behind; -1 = none
-        const int place = from + i - 1;
-        const bool there = place >= 0 && place < total;
-        rows[i] = there ? a.sorted[place] : -1;
-        if (i > 0 && i <= a.length) tokens[i - 1] = there ? a.order[place] : 0;
+        const int place = from + i - 1, inside = min(max(place, 0), a.tokens - 1);
+        const int row = a.sorted[inside], token = a.order[inside];  // behind the last place: not used
+        rows[i] = place >= 0 && place < total ? row : -1;
+        if (i > 0 && i <= a.length) tokens[i - 1] = place < total ? token : 0;
     }
     if (from >= total) return;  // the whole block
     const int n = min(a.length, total - from);
     __syncthreads();
+    int2 span = make_int2(0, 1);  // of the block's first and last row, for their first two threads, which may need them at the end
+    if (threadIdx.x < 2) span = a.spans[rows[threadIdx.x ? n : 1]];
     const Columns<WIDE> cols(slice, a.table.dim);
     const T *g = (const T *)a.g + cols.first;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -353,9 +351,9 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const __grid_consta
         const int v = threadIdx.x ? spans_after : spans_before;
         last[threadIdx.x] = 0;
         if (v >= 0) {
-            const int2 at = a.spans[v];
-            const int c0 = at.x / a.length, c1 = (at.y - 1) / a.length;
-            last[threadIdx.x] = atomicAdd(a.arrived + (long long)c0 * a.slices + slice, 1u) == (unsigned)(c1 - c0);
+            const int c0 = span.x / a.length, c1 = (span.y - 1) / a.length;
+            last[threadIdx.x] = atomicAdd(a.arrived + (long long)c0 * a.slices + slice, 1u) == (unsigned)(c1 - c0) ? c1 - c0 + 1 : 0;
+            first_piece[threadIdx.x] = c0;
         }
         __threadfence();
     }
@@ -363,7 +361,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const __grid_consta
 #pragma unroll 1
     for (int k = 0; k < 2; ++k) {
         if (!last[k]) continue;
-        const int v = k ? spans_after : spans_before, c0 = a.spans[v].x / a.length, pieces = (a.spans[v].y - 1) / a.length - c0 + 1;
+        const int v = k ? spans_after : spans_before, c0 = first_piece[k], pieces = last[k];
         sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
 #pragma unroll 8
         for (int p = 0; p < pieces; ++p)
@@ -418,9 +416,6 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     long long length = (tokens * slices + ctx.sm_count * 4 - 1) / (ctx.sm_count * 4);
     length = length < 16 ? 16 : length > kMaxLength ? kMaxLength : (length + 7) / 8 * 8;
     const long long chunks = (tokens + length - 1) / length, zero_blocks = add ? 0 : (vocab + kZeroRows - 1) / kZeroRows;
-    // Where few rows are reached, all of the table is cleared beside the sorting, which keeps the memory idle; where many are, only the others,
-    // beside the sums (4096 tokens into 30522 rows of 768: 27 and 43 us; 65 521 into 50 021 of 1000: 141 and 133 us).
-    const bool clear_first = tokens * 4 <= vocab;
     if (chunks * slices + zero_blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many rows");
     const auto rounded = [](long long words) { return (words + 63) / 64 * 64; };
     const long long starts = rounded(2 * vocab + 1), places = rounded(tokens), counters = rounded(chunks * slices);
@@ -454,15 +449,15 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     if (!ctx.dry()) {
         st = ctx.check_cuda(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortRows + 2 * kSortList) * kSortWarps * 4), "embedding_sort");
         if (!st)
-            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), embedding_sort_kernel, dim3((1u << bits) + (unsigned)(clear_first ? zero_blocks : 0)), dim3(warps * 32), smem, (const int *)ids.ptr,
-                                                 ids.stride, (int)tokens, (int)vocab, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted, a.arrived, (int)counters, a.table),
+            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), embedding_sort_kernel, dim3(1u << bits), dim3(warps * 32), smem, (const int *)ids.ptr,
+                                                 ids.stride, (int)tokens, (int)vocab, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted, a.arrived, (int)counters),
                                 "embedding_sort");
         if (!st)
             st = with_type(g.dtype, [&](auto t) {
                 typedef decltype(t) T;
                 const size_t smem_ahead = wide ? kAhead * threads * sizeof(Four<T>) : 0;  // 32 KB at most
                 return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? embedding_grad_kernel<T, true> : embedding_grad_kernel<T, false>,
-                                                       dim3((unsigned)(chunks * slices + (clear_first ? 0 : zero_blocks))), dim3((unsigned)threads), smem_ahead, a),
+                                                       dim3((unsigned)(chunks * slices + zero_blocks)), dim3((unsigned)threads), smem_ahead, a),
                                       "embedding_grad");
             });
     }
