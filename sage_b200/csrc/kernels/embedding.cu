@@ -97,12 +97,13 @@ struct Zeros {
 // places (in front of them all tokens of the blocks before), and a second pass puts the tokens there.  A hundred times the ids out of L2
 // instead of a radix sort's passes through memory and launches.
 constexpr int kSortWarps = 32, kSortRows = 1024, kSortList = 256;  // rows of a block and own tokens of a warp that shared memory holds
+template <bool QUADS>
 __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const int *__restrict__ ids, long long ids_stride, int tokens, int vocab, int bits, int2 *__restrict__ spans, int *__restrict__ total,
                                                                          int *__restrict__ order, int *__restrict__ sorted, unsigned *__restrict__ arrived, int counters) {
     extern __shared__ int2 lists[];  // [warp][kSortList] {token, id}, then [warp][row of the block] counts, later places
     int *places = reinterpret_cast<int *>(lists + blockDim.x / 32 * kSortList);
     __shared__ int warp_sums[kSortWarps], below_all;
-    constexpr int U = 8;
+    constexpr int U = 4;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
     const unsigned own = blockIdx.x, ending = (1u << bits) - 1;
     const int rows = (int)(((unsigned)vocab - own + ending) >> bits);
@@ -110,25 +111,41 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const i
     grid_dependency_sync();
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < counters; i += gridDim.x * blockDim.x) arrived[i] = 0;
     __syncthreads();
-    const int share = ((tokens + warps - 1) / warps + 31) / 32 * 32, begin = (int)min((long long)warp * share, (long long)tokens), end = (int)min(begin + (long long)share, (long long)tokens);
+    const int share = ((tokens + warps - 1) / warps + 127) / 128 * 128, begin = (int)min((long long)warp * share, (long long)tokens), end = (int)min(begin + (long long)share, (long long)tokens);
     int2 *list = lists + warp * kSortList;
     int *mine = places + warp * rows, below = 0, found = 0;
-    for (int t0 = begin; t0 < end; t0 += 32 * U) {
-        int id[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) id[u] = t0 + u * 32 + lane < end ? ids[(t0 + u * 32 + lane) * ids_stride] : -1;
+    // Four tokens to a lane: tokens of a row come in the order of 128, then of the four, then of the lanes.
+    for (int t0 = begin; t0 < end; t0 += 128 * U) {
+        int id[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const unsigned block = (unsigned)id[u] < (unsigned)vocab ? (unsigned)id[u] & ending : ~0u;
-            below += block < own;
-            const unsigned all = __ballot_sync(0xffffffffu, block == own);
-            if (!all) continue;
-            if (block == own) {
-                atomicAdd(mine + (id[u] >> bits), 1);  // a count: any order
-                const int at = found + __popc(all & ((1u << lane) - 1));
-                if (at < kSortList) list[at] = make_int2(t0 + u * 32 + lane, id[u]);
+            const int t = t0 + u * 128 + lane * 4;
+            if (QUADS && t + 3 < end) {
+                const int4 q = *reinterpret_cast<const int4 *>(ids + t);
+                id[u][0] = q.x;
+                id[u][1] = q.y;
+                id[u][2] = q.z;
+                id[u][3] = q.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) id[u][j] = t + j < end ? ids[(t + j) * ids_stride] : -1;
             }
-            found += __popc(all);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool some = (unsigned)id[u][j] < (unsigned)vocab, in = some && ((unsigned)id[u][j] & ending) == own;
+                if (some && ((unsigned)id[u][j] & ending) < own) ++below;
+                const unsigned all = __ballot_sync(0xffffffffu, in);
+                if (!all) continue;
+                if (in) {
+                    atomicAdd(mine + (id[u][j] >> bits), 1);  // a count: any order
+                    const int at = found + __popc(all & ((1u << lane) - 1));
+                    if (at < kSortList) list[at] = make_int2(t0 + u * 128 + lane * 4 + j, id[u][j]);
+                }
+                found += __popc(all);
+            }
         }
     }
     for (int o = 16; o; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
@@ -447,9 +464,10 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     ctx.note_launch("embedding_sort");
     ctx.note_launch("embedding_grad");
     if (!ctx.dry()) {
-        st = ctx.check_cuda(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortRows + 2 * kSortList) * kSortWarps * 4), "embedding_sort");
+        const auto sort = ids.stride == 1 && reinterpret_cast<uintptr_t>(ids.ptr) % 16 == 0 ? embedding_sort_kernel<true> : embedding_sort_kernel<false>;
+        st = ctx.check_cuda(cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortRows + 2 * kSortList) * kSortWarps * 4), "embedding_sort");
         if (!st)
-            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), embedding_sort_kernel, dim3(1u << bits), dim3(warps * 32), smem, (const int *)ids.ptr,
+            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), sort, dim3(1u << bits), dim3(warps * 32), smem, (const int *)ids.ptr,
                                                  ids.stride, (int)tokens, (int)vocab, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted, a.arrived, (int)counters),
                                 "embedding_sort");
         if (!st)
