@@ -61,8 +61,8 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T *__restrict__ ta
 }
 
 // ------------------------------------------------------------------------------------------ gradient
-// Tokens are sorted by table row (those of a row in their order), then rows are summed in pieces of a fixed length of that order, so
-// that a frequent token's thousands of rows are spread like any others.  Two launches, no sums by atomics: the same bits every time.
+// Tokens are sorted by table row (those of a row in a fixed order), then rows are summed in pieces of a fixed length of that order, so
+// that a frequent token's thousands of rows are spread like any others.  Two or three launches, no sums by atomics: the same bits every time.
 
 constexpr int kZeroRows = 8;  // of a block that writes zeros: about one to a warp (94 MB with 64 rows a block 30 us, with 6 to 12 18 us)
 // Zeros into the rows of the table, 16 bytes at a time where they lie on such boundaries.
@@ -93,61 +93,173 @@ struct Zeros {
 };
 
 // Sorting.  Each of 2^bits blocks owns the table rows whose numbers end in its own (frequent tokens have low numbers: neighbours go to
-// different blocks) and reads all ids: its warps, each over a contiguous share of the tokens, count its rows' tokens, the counts become
-// places (in front of them all tokens of the blocks before), and a second pass puts the tokens there.  A hundred times the ids out of L2
-// instead of a radix sort's passes through memory and launches.
+// different blocks).  Its warps, each over a share of the tokens, count its rows' tokens, the counts become places (in front of them
+// all tokens of the blocks before), and a second pass puts the tokens there.  Up to kDealFrom tokens every block reads all ids for that: one
+// launch, but 128 times the ids out of L2 (65 521 of them: 15 us more than 4096).  Above, a launch in front deals the ids out, 1024 to a
+// block, so that a sorting block finds its tokens of them together.
 constexpr int kSortWarps = 32, kSortRows = 1024, kSortList = 256;  // rows of a block and own tokens of a warp that shared memory holds
-template <bool QUADS>
-__global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const int *__restrict__ ids, long long ids_stride, int tokens, int vocab, int bits, int2 *__restrict__ spans, int *__restrict__ total,
-                                                                         int *__restrict__ order, int *__restrict__ sorted, unsigned *__restrict__ arrived, int counters) {
+constexpr int kDealFrom = 16384, kDealTokens = 1024, kDealThreads = 256, kDealBits = 9;
+
+// Block s orders ids [1024 s, 1024 (s + 1)) by their sorting block: dealt[1024 s + starts[s][b]] onwards {token, id} of sorting block b.
+__global__ void __launch_bounds__(kDealThreads) embedding_deal_kernel(const int *__restrict__ ids, long long ids_stride, int tokens, int vocab, int bits, int2 *__restrict__ dealt, int *__restrict__ starts) {
+    constexpr int W = kDealThreads / 32, U = kDealTokens / kDealThreads, PER = (1 << kDealBits) / kDealThreads;
+    __shared__ int counts[W << kDealBits], warp_sums[W];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, blocks = 1 << bits;
+    for (int i = threadIdx.x; i < W * blocks; i += kDealThreads) counts[i] = 0;
+    grid_dependency_sync();
+    int id[U], rank[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int t = blockIdx.x * kDealTokens + warp * (32 * U) + u * 32 + lane;
+        id[u] = t < tokens ? ids[t * ids_stride] : -1;
+        if ((unsigned)id[u] >= (unsigned)vocab) id[u] = -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int to = id[u] & (blocks - 1);
+        const unsigned some = __ballot_sync(0xffffffffu, id[u] >= 0);
+        unsigned same = 1u << lane;
+        int from = 0;
+        __syncwarp();
+        if (id[u] >= 0) {
+            same = __match_any_sync(some, to);
+            if (lane == __ffs(same) - 1) from = atomicAdd(counts + warp * blocks + to, __popc(same));  // one lane for each sorting block
+        }
+        rank[u] = __shfl_sync(0xffffffffu, from, __ffs(same) - 1) + __popc(same & ((1u << lane) - 1));
+    }
+    __syncthreads();
+    // counts -> places: sorting blocks one after the other, in each the warps; a thread has PER sorting blocks in a row
+    int count[PER], sum = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int b = threadIdx.x * PER + k;
+        count[k] = 0;
+        if (b < blocks)
+            for (int w = 0; w < W; ++w) count[k] += counts[w * blocks + b];
+        sum += count[k];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int left = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += left;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    int at = upto - sum;
+    for (int w = 0; w < warp; ++w) at += warp_sums[w];
+    int *start = starts + (long long)blockIdx.x * (blocks + 1);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int b = threadIdx.x * PER + k;
+        if (b >= blocks) break;
+        start[b] = at;
+        if (b == blocks - 1) start[blocks] = at + count[k];
+        for (int w = 0; w < W; ++w) {
+            const int c = counts[w * blocks + b];
+            counts[w * blocks + b] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (id[u] >= 0)
+            dealt[(long long)blockIdx.x * kDealTokens + counts[warp * blocks + (id[u] & (blocks - 1))] + rank[u]] = make_int2(blockIdx.x * kDealTokens + warp * (32 * U) + u * 32 + lane, id[u]);
+}
+
+// Where a sorting block's tokens come from.
+enum Source { kStrided, kQuads, kDealt };
+struct Ids {
+    const int *ids;
+    long long stride;
+    const int2 *dealt;
+    const int *starts;
+    int tokens, vocab;
+};
+
+template <Source FROM>
+__global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const Ids in_all, int bits, int2 *__restrict__ spans, int *__restrict__ total, int *__restrict__ order, int *__restrict__ sorted,
+                                                                         unsigned *__restrict__ arrived, int counters) {
     extern __shared__ int2 lists[];  // [warp][kSortList] {token, id}, then [warp][row of the block] counts, later places
     int *places = reinterpret_cast<int *>(lists + blockDim.x / 32 * kSortList);
     __shared__ int warp_sums[kSortWarps], below_all;
-    constexpr int U = 4;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32, tokens = in_all.tokens, vocab = in_all.vocab;
     const unsigned own = blockIdx.x, ending = (1u << bits) - 1;
     const int rows = (int)(((unsigned)vocab - own + ending) >> bits);
     for (int i = threadIdx.x; i < warps * rows; i += blockDim.x) places[i] = 0;
     grid_dependency_sync();
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < counters; i += gridDim.x * blockDim.x) arrived[i] = 0;
     __syncthreads();
-    const int share = ((tokens + warps - 1) / warps + 127) / 128 * 128, begin = (int)min((long long)warp * share, (long long)tokens), end = (int)min(begin + (long long)share, (long long)tokens);
     int2 *list = lists + warp * kSortList;
     int *mine = places + warp * rows, below = 0, found = 0;
-    // Four tokens to a lane: tokens of a row come in the order of 128, then of the four, then of the lanes.
-    for (int t0 = begin; t0 < end; t0 += 128 * U) {
-        int id[U][4];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int t = t0 + u * 128 + lane * 4;
-            if (QUADS && t + 3 < end) {
-                const int4 q = *reinterpret_cast<const int4 *>(ids + t);
-                id[u][0] = q.x;
-                id[u][1] = q.y;
-                id[u][2] = q.z;
-                id[u][3] = q.w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) id[u][j] = t + j < end ? ids[(t + j) * ids_stride] : -1;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool some = (unsigned)id[u][j] < (unsigned)vocab, in = some && ((unsigned)id[u][j] & ending) == own;
-                if (some && ((unsigned)id[u][j] & ending) < own) ++below;
-                const unsigned all = __ballot_sync(0xffffffffu, in);
-                if (!all) continue;
-                if (in) {
-                    atomicAdd(mine + (id[u][j] >> bits), 1);  // a count: any order
-                    const int at = found + __popc(all & ((1u << lane) - 1));
-                    if (at < kSortList) list[at] = make_int2(t0 + u * 128 + lane * 4 + j, id[u][j]);
+    // The warp's share, 32 tokens at a time: f(token, id, is it the block's own).  In an order that depends on nothing but their number.
+    auto each = [&](auto f) {
+        if constexpr (FROM == kDealt) {
+            const int sources = (tokens + kDealTokens - 1) / kDealTokens, share = (sources + warps - 1) / warps;
+            int lanes = 32;  // that share a source
+            while (lanes > 1 && 32 / lanes < share) lanes /= 2;
+            for (int s0 = warp * share; s0 < min((warp + 1) * share, sources); s0 += 32 / lanes) {
+                const int s = s0 + lane / lanes;
+                int from = 0, to = 0;
+                if (s < min((warp + 1) * share, sources)) {
+                    const int *start = in_all.starts + (long long)s * (ending + 2) + own;
+                    from = start[0];
+                    to = start[1];
                 }
-                found += __popc(all);
+                const int2 *p = in_all.dealt + (long long)s * kDealTokens;
+                constexpr int U = 4;
+                for (int i = from + lane % lanes; __any_sync(0xffffffffu, i < to); i += U * lanes) {
+                    int2 t[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) t[u] = i + u * lanes < to ? p[i + u * lanes] : make_int2(0, -1);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) f(t[u].x, t[u].y, t[u].y >= 0);
+                }
+            }
+        } else {
+            constexpr int U = 4;
+            const int share = ((tokens + warps - 1) / warps + 127) / 128 * 128, begin = (int)min((long long)warp * share, (long long)tokens), end = (int)min(begin + (long long)share, (long long)tokens);
+            for (int t0 = begin; t0 < end; t0 += 128 * U) {  // four tokens to a lane
+                int id[U][4];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int t = t0 + u * 128 + lane * 4;
+                    if (FROM == kQuads && t + 3 < end) {
+                        const int4 q = *reinterpret_cast<const int4 *>(in_all.ids + t);
+                        id[u][0] = q.x;
+                        id[u][1] = q.y;
+                        id[u][2] = q.z;
+                        id[u][3] = q.w;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) id[u][j] = t + j < end ? in_all.ids[(t + j) * in_all.stride] : -1;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool some = (unsigned)id[u][j] < (unsigned)vocab;
+                        if (some && ((unsigned)id[u][j] & ending) < own) ++below;
+                        f(t0 + u * 128 + lane * 4 + j, id[u][j], some && ((unsigned)id[u][j] & ending) == own);
+                    }
             }
         }
-    }
+    };
+    each([&](int t, int id, bool in) {
+        const unsigned all = __ballot_sync(0xffffffffu, in);
+        if (!all) return;
+        if (in) {
+            atomicAdd(mine + (id >> bits), 1);  // a count: any order
+            const int at = found + __popc(all & ((1u << lane) - 1));
+            if (at < kSortList) list[at] = make_int2(t, id);
+        }
+        found += __popc(all);
+    });
+    if constexpr (FROM == kDealt)  // a source's first place for this block: as many of its tokens are of the blocks before
+        for (int s = threadIdx.x; s < (tokens + kDealTokens - 1) / kDealTokens; s += blockDim.x) below += in_all.starts[(long long)s * (ending + 2) + own];
     for (int o = 16; o; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
     if (lane == 0) warp_sums[warp] = below;
     __syncthreads();
@@ -218,10 +330,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const i
             put(t.x, t.y, in);
         }
     } else {
-        for (int t0 = begin; t0 < end; t0 += 32) {
-            const int t = t0 + lane, id = t < end ? ids[t * ids_stride] : -1;
-            put(t, id, (unsigned)id < (unsigned)vocab && ((unsigned)id & ending) == own);
-        }
+        each(put);
     }
 }
 
@@ -460,15 +569,33 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     while ((2ll << bits) <= vocab && ((2 << bits) <= ctx.sm_count || ((vocab - 1) >> bits) + 1 > kSortRows)) ++bits;
     const int warps = tokens <= 8192 ? 8 : kSortWarps;  // few ids: the counts of a warp cost more than its share of the ids
     const size_t smem = (size_t)((((vocab - 1) >> bits) + 1) + 2 * kSortList) * warps * 4;
+    const bool deal = tokens > kDealFrom && bits <= kDealBits;
+    Ids source = {(const int *)ids.ptr, ids.stride, nullptr, nullptr, (int)tokens, (int)vocab};
+    Block *dealt = nullptr;
+    const long long sources = (tokens + kDealTokens - 1) / kDealTokens;
     sage_status st = SAGE_OK;
+    if (deal) {
+        dealt = ctx.allocator().alloc((size_t)(sources * kDealTokens * 8 + sources * ((1ll << bits) + 1) * 4));
+        if (!dealt) {
+            ctx.allocator().free(scratch);
+            return ctx.fail(SAGE_ERR_OOM, "embedding_grad: out of memory");
+        }
+        source.dealt = (const int2 *)dealt->ptr;
+        source.starts = (const int *)(source.dealt + sources * kDealTokens);
+        ctx.note_launch("embedding_deal");
+        if (!ctx.dry())
+            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), embedding_deal_kernel, dim3((unsigned)sources), dim3(kDealThreads), 0, source.ids, source.stride, source.tokens, source.vocab, bits,
+                                                 (int2 *)source.dealt, (int *)source.starts),
+                                "embedding_deal");
+    }
     ctx.note_launch("embedding_sort");
     ctx.note_launch("embedding_grad");
-    if (!ctx.dry()) {
-        const auto sort = ids.stride == 1 && reinterpret_cast<uintptr_t>(ids.ptr) % 16 == 0 ? embedding_sort_kernel<true> : embedding_sort_kernel<false>;
+    if (!ctx.dry() && !st) {
+        const auto sort = deal ? embedding_sort_kernel<kDealt> : ids.stride == 1 && reinterpret_cast<uintptr_t>(ids.ptr) % 16 == 0 ? embedding_sort_kernel<kQuads> : embedding_sort_kernel<kStrided>;
         st = ctx.check_cuda(cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortRows + 2 * kSortList) * kSortWarps * 4), "embedding_sort");
         if (!st)
-            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), sort, dim3(1u << bits), dim3(warps * 32), smem, (const int *)ids.ptr,
-                                                 ids.stride, (int)tokens, (int)vocab, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted, a.arrived, (int)counters),
+            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), sort, dim3(1u << bits), dim3(warps * 32), smem, source, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted,
+                                                 a.arrived, (int)counters),
                                 "embedding_sort");
         if (!st)
             st = with_type(g.dtype, [&](auto t) {
@@ -479,6 +606,7 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
                                       "embedding_grad");
             });
     }
+    if (dealt) ctx.allocator().free(dealt);
     ctx.allocator().free(scratch);
     return st;
 }
