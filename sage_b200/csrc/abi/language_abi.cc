@@ -231,7 +231,7 @@ sage_status sage_adamw_step(sage_ctx *ctx, const sage_adamw_tensor *tensors, int
             s.p = (float *)c.flat(&t.param, "param", -1, &s.n);
             if (!is_real(t.grad.dtype)) c.refuse("grad", "is not f32, f16 or bf16");
             s.g = c.flat(&t.grad, "grad", s.n);
-            s.g_dtype = t.grad.dtype;
+            s.g_dtype = (short)t.grad.dtype;
             if (t.m.dtype != (states8 ? SAGE_I8 : SAGE_F32) || t.v.dtype != (states8 ? SAGE_U8 : SAGE_F32)) c.refuse("m or v", "is not of the first tensor's kind: f32 both, or i8 and u8");
             s.m = c.flat(&t.m, "m", s.n);
             s.v = c.flat(&t.v, "v", s.n);
@@ -244,7 +244,7 @@ sage_status sage_adamw_step(sage_ctx *ctx, const sage_adamw_tensor *tensors, int
             if (t.copy.buf) {
                 if (t.copy.dtype != SAGE_F16 && t.copy.dtype != SAGE_BF16) c.refuse("copy", "is not f16 or bf16");
                 s.copy = c.flat(&t.copy, "copy", s.n);
-                s.copy_dtype = t.copy.dtype;
+                s.copy_dtype = (short)t.copy.dtype;
             }
             if (s.n) slots.push_back(s);
         }

@@ -3,7 +3,11 @@
 // 8 bits: blocks of 256 elements of a tensor share a scale, and codes follow a square law, |m| = a code^2 with a = max |m| / 127^2 and
 // sqrt(v) = b code^2 with b = max sqrt(v) / 255^2: a step of 1.6 % (0.8 %) at the block's largest and 16 129 (65 025) between the
 // largest and the smallest, where even steps would lose all below a 127th.  The root of v is stored because it is what divides.
-// Every operation on the moments is rounded by itself, so that codes do not depend on how a compiler contracts them.
+// Codes and scales are those of the moments as f32 rounds them operation by operation, whatever shortcuts find them: the fast square
+// root decides a code unless its result lies so near the middle of two codes that it could err, where the exact one does.
+//
+// A warp takes a block of 256 elements at a time, eight to a lane.  Bound by memory: 28 bytes an element with f32 states and gradients,
+// 16 with 8-bit states and f32 gradients.
 #include <cuda_runtime.h>
 
 #include "language.h"
@@ -15,132 +19,234 @@ namespace k {
 
 namespace {
 
-constexpr int kSlots = 400;  // 30 KB of kernel parameters
+template <int SLOTS>
 struct Batch {
-    AdamWSlot slot[kSlots];
-    unsigned first[kSlots + 1];  // prefix sums of the slots' blocks of 256 elements
+    AdamWSlot slot[SLOTS];
+    unsigned first[SLOTS + 1];  // prefix sums of the slots' blocks of 256 elements
     int count;
 };
+constexpr int kSlots = 400, kFewSlots = 40;  // 32 KB of kernel parameters, 3 KB
 
-__device__ __forceinline__ float load_as_float(const void *p, int dtype, long long i) {
-    if (dtype == SAGE_F16) return widen(((const __half *)p)[i]);
-    if (dtype == SAGE_BF16) return widen(((const __nv_bfloat16 *)p)[i]);
-    return ((const float *)p)[i];
+__device__ __forceinline__ float fast_root(float x) {  // 2^-22 off at most, of subnormal numbers 0
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float largest(float a, float b) {  // NaN wins
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float warp_largest(float x) {
+    float y;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-// A value's moments after one more gradient; `root` is sqrt(v).
-__device__ __forceinline__ void moments(const AdamWRule &k, float g, float *m, float *v, float *root) {
-    g = __fmul_rn(g, k.grad_scale);
-    *m = __fadd_rn(__fmul_rn(*m, k.beta1), __fmul_rn(g, k.one_minus_beta1));
-    *v = __fadd_rn(__fmul_rn(*v, k.beta2), __fmul_rn(__fmul_rn(g, g), k.one_minus_beta2));
-    *root = __fsqrt_rn(*v);
-}
-__device__ __forceinline__ float updated(const AdamWRule &k, float p, float m, float root) {
-    return p * k.keep - m * k.step_size / (root * k.root_factor + k.eps);
-}
-
-// Largest of non-negative values by their bits: NaN is above infinity, and both above every number.
-__device__ __forceinline__ unsigned warp_largest(unsigned v) {
-    for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-// The factor of a block's codes and its stored scale, from the block's largest.  Below 2^-100 a block is zero.
+// The factor of a block's codes and its stored scale, from the block's largest (not negative).  Below 2^-100 a block is zero.
 template <int TOP>
-__device__ __forceinline__ float block_scale(unsigned largest, float *factor) {
-    const float x = __uint_as_float(largest);
+__device__ __forceinline__ float block_scale(float x, float *factor) {
     *factor = 0.f;
-    if (largest >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
+    if (!(x < INFINITY)) return __uint_as_float(0x7fffffffu);
     if (x < 7.888609052210118e-31f) return 0.f;
     *factor = __fmul_rn(__frcp_rn(x), (float)(TOP * TOP));
     return __fmul_rn(x, 1.f / (TOP * TOP));
 }
+// round(sqrt(t)) for 0 <= t <= 65025 (1 + 2^-20), `off` an approximate root of it: within 1e-4, so another code only where that is the
+// distance to the middle of two.
+__device__ __forceinline__ bool near_middle(float off, float *code) {
+    const float n = __fadd_rn(__fadd_rn(off, 12582912.f), -12582912.f);  // to the nearest whole number
+    *code = n;
+    return fabsf(fabsf(off - n) - 0.5f) < 2e-4f;
+}
 
-template <bool STATES8>
-__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Batch b, const AdamWRule k) {
-    grid_dependency_sync();
-    const unsigned total = b.first[b.count], lane = threadIdx.x % 32;
-    for (unsigned block = blockIdx.x * 8 + threadIdx.x / 32; block < total; block += gridDim.x * 8) {
-        int lo = 0, hi = b.count - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (b.first[mid] <= block) lo = mid;
-            else hi = mid - 1;
-        }
-        const AdamWSlot &s = b.slot[lo];
-        const long long at = (long long)(block - b.first[lo]) * kAdamWBlock;
-        float m[8], v[8], root[8], g[8];
-        unsigned m_top = 0, v_top = 0;
-        const float ms = STATES8 ? s.m_scale[at / kAdamWBlock] : 0.f, vs = STATES8 ? s.v_scale[at / kAdamWBlock] : 0.f;
+struct Element {
+    float p, g, m, v, root;
+};
+__device__ __forceinline__ void update(const AdamWRule &k, Element &e) {
+    const float g = __fmul_rn(e.g, k.grad_scale);
+    e.m = __fadd_rn(__fmul_rn(e.m, k.beta1), __fmul_rn(g, k.one_minus_beta1));
+    e.v = __fadd_rn(__fmul_rn(e.v, k.beta2), __fmul_rn(__fmul_rn(g, g), k.one_minus_beta2));
+    e.root = fast_root(e.v);
+    e.p = e.p * k.keep - __fdividef(e.m * k.step_size, e.root * k.root_factor + k.eps);
+}
+
+// Where the eight elements of a lane lie in the block: two times four in a row, or (blocks that end early, tensors off 16-byte
+// boundaries) 32 apart.
+template <bool WIDE>
+__device__ __forceinline__ int place(int i) {
+    const int lane = threadIdx.x % 32;
+    return WIDE ? i / 4 * 128 + lane * 4 + i % 4 : i * 32 + lane;
+}
+// Elements of type T at `p`, the start of the block; those of [0, n) where not WIDE.
+template <bool WIDE, class T, class F>
+__device__ __forceinline__ void load8(const T *p, int n, F put) {
+    if (WIDE) {
+        struct alignas(4 * sizeof(T)) Four {
+            T v[4];
+        };
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const long long j = at + i * 32 + lane;
-            m[i] = v[i] = root[i] = g[i] = 0.f;
-            if (j >= s.n) continue;
-            if (STATES8) {
-                const int c = ((const signed char *)s.m)[j], d = ((const unsigned char *)s.v)[j];
-                m[i] = __fmul_rn(ms, (float)(c * abs(c)));
-                const float q = __fmul_rn(vs, (float)(d * d));
-                v[i] = __fmul_rn(q, q);
-            } else {
-                m[i] = ((const float *)s.m)[j];
-                v[i] = ((const float *)s.v)[j];
-            }
-            moments(k, load_as_float(s.g, s.g_dtype, j), &m[i], &v[i], &root[i]);
-            const float p = updated(k, s.p[j], m[i], root[i]);
-            s.p[j] = p;
-            if (s.copy) {
-                if (s.copy_dtype == SAGE_F16) ((__half *)s.copy)[j] = narrowed<__half>(p);
-                else ((__nv_bfloat16 *)s.copy)[j] = narrowed<__nv_bfloat16>(p);
-            }
-            if (!STATES8) {
-                ((float *)s.m)[j] = m[i];
-                ((float *)s.v)[j] = v[i];
-            }
-            m_top = max(m_top, __float_as_uint(fabsf(m[i])));
-            v_top = max(v_top, __float_as_uint(fabsf(root[i])));
-        }
-        if (!STATES8) continue;
-        float mf, vf;
-        const float new_ms = block_scale<127>(warp_largest(m_top), &mf), new_vs = block_scale<255>(warp_largest(v_top), &vf);
-        if (lane == 0) {
-            s.m_scale[at / kAdamWBlock] = new_ms;
-            s.v_scale[at / kAdamWBlock] = new_vs;
-        }
+        for (int h = 0; h < 2; ++h) {
+            const Four q = *reinterpret_cast<const Four *>(p + place<true>(4 * h));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const long long j = at + i * 32 + lane;
-            if (j >= s.n) continue;
-            int c = mf > 0.f ? min(127, __float2int_rn(__fsqrt_rn(__fmul_rn(fabsf(m[i]), mf)))) : 0;
-            int d = vf > 0.f ? min(255, __float2int_rn(__fsqrt_rn(__fmul_rn(root[i], vf)))) : 0;
-            if (vf > 0.f && root[i] > 0.f) d = max(d, 1);
-            ((signed char *)s.m)[j] = (signed char)(m[i] < 0.f ? -c : c);
-            ((unsigned char *)s.v)[j] = (unsigned char)d;
+            for (int j = 0; j < 4; ++j) put(4 * h + j, q.v[j]);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) put(i, place<false>(i) < n ? p[place<false>(i)] : T(0.f));
+    }
+}
+template <bool WIDE, class T, class F>
+__device__ __forceinline__ void store8(T *p, int n, F get) {
+    if (WIDE) {
+        struct alignas(4 * sizeof(T)) Four {
+            T v[4];
+        };
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Four q;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q.v[j] = get(4 * h + j);
+            *reinterpret_cast<Four *>(p + place<true>(4 * h)) = q;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (place<false>(i) < n) p[place<false>(i)] = get(i);
     }
 }
 
+template <bool STATES8, bool WIDE>
+__device__ __forceinline__ void block_update(const AdamWSlot &s, const AdamWRule &k, long long block) {
+    const long long at = block * kAdamWBlock;
+    const int n = WIDE ? kAdamWBlock : (int)min(s.n - at, (long long)kAdamWBlock);
+    Element e[8];
+    if (s.g_dtype == SAGE_F32) load8<WIDE>((const float *)s.g + at, n, [&](int i, float x) { e[i].g = x; });
+    else if (s.g_dtype == SAGE_BF16) load8<WIDE>((const __nv_bfloat16 *)s.g + at, n, [&](int i, __nv_bfloat16 x) { e[i].g = widen(x); });
+    else load8<WIDE>((const __half *)s.g + at, n, [&](int i, __half x) { e[i].g = widen(x); });
+    load8<WIDE>(s.p + at, n, [&](int i, float x) { e[i].p = x; });
+    if (STATES8) {
+        const float ms = s.m_scale[block], vs = s.v_scale[block];
+        load8<WIDE>((const signed char *)s.m + at, n, [&](int i, signed char c) {
+            const float f = (float)c;
+            e[i].m = __fmul_rn(ms, f * fabsf(f));
+        });
+        load8<WIDE>((const unsigned char *)s.v + at, n, [&](int i, unsigned char c) {
+            const float f = (float)c, q = __fmul_rn(vs, f * f);
+            e[i].v = __fmul_rn(q, q);
+        });
+    } else {
+        load8<WIDE>((const float *)s.m + at, n, [&](int i, float x) { e[i].m = x; });
+        load8<WIDE>((const float *)s.v + at, n, [&](int i, float x) { e[i].v = x; });
+    }
+    if (STATES8 && !WIDE) {  // a scale that is NaN makes zeros behind the end NaN too
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (place<false>(i) >= n) e[i].m = e[i].v = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) update(k, e[i]);
+    store8<WIDE>(s.p + at, n, [&](int i) { return e[i].p; });
+    if (s.copy) {
+        if (s.copy_dtype == SAGE_BF16) store8<WIDE>((__nv_bfloat16 *)s.copy + at, n, [&](int i) { return narrowed<__nv_bfloat16>(e[i].p); });
+        else store8<WIDE>((__half *)s.copy + at, n, [&](int i) { return narrowed<__half>(e[i].p); });
+    }
+    if (!STATES8) {
+        store8<WIDE>((float *)s.m + at, n, [&](int i) { return e[i].m; });
+        store8<WIDE>((float *)s.v + at, n, [&](int i) { return e[i].v; });
+        return;
+    }
+    float m_top = 0.f, v_top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        m_top = largest(m_top, fabsf(e[i].m));
+        v_top = largest(v_top, e[i].v);
+    }
+    float mf, vf;
+    const float ms = block_scale<127>(warp_largest(m_top), &mf), vs = block_scale<255>(__fsqrt_rn(warp_largest(v_top)), &vf);
+    if (threadIdx.x % 32 == 0) {
+        s.m_scale[block] = ms;
+        s.v_scale[block] = vs;
+    }
+    store8<WIDE>((signed char *)s.m + at, n, [&](int i) {
+        const float t = __fmul_rn(fabsf(e[i].m), mf);
+        float c;
+        if (near_middle(fast_root(t), &c)) c = rintf(__fsqrt_rn(t));
+        return mf > 0.f ? (signed char)__float2int_rn(copysignf(c, e[i].m)) : (signed char)0;
+    });
+    store8<WIDE>((unsigned char *)s.v + at, n, [&](int i) {
+        float c;
+        const bool tiny = __float_as_uint(e[i].v) - 1u < 0x7fffffu;  // subnormal: the fast root of it is 0
+        if (near_middle(fast_root(__fmul_rn(e[i].root, vf)), &c) || tiny) c = rintf(__fsqrt_rn(__fmul_rn(__fsqrt_rn(e[i].v), vf)));
+        if (e[i].v > 0.f) c = fmaxf(c, 1.f);
+        return vf > 0.f ? (unsigned char)__float2int_rn(c) : (unsigned char)0;
+    });
+}
+
+template <bool STATES8, int SLOTS>
+__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Batch<SLOTS> b, const AdamWRule k) {
+    grid_dependency_sync();
+    const unsigned total = b.first[b.count];
+    int at = 0;  // the slot that holds the block; found from the last one on
+    for (unsigned block = blockIdx.x * 8 + threadIdx.x / 32; block < total; block += gridDim.x * 8) {
+        if (b.first[at + 1] <= block) {
+            int lo = at + 1, hi = b.count - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (b.first[mid] <= block) lo = mid;
+                else hi = mid - 1;
+            }
+            at = lo;
+        }
+        const AdamWSlot &s = b.slot[at];
+        const long long mine = block - b.first[at];
+        if (s.wide && (mine + 1) * kAdamWBlock <= s.n) block_update<STATES8, true>(s, k, mine);
+        else block_update<STATES8, false>(s, k, mine);
+    }
+}
+
+// Values of codes: four to a thread where `wide`, else one.
+template <bool WIDE>
 __global__ void __launch_bounds__(256) adamw_states_kernel(const signed char *m, const float *m_scale, const unsigned char *v, const float *v_scale, long long n, float *m_out, float *v_out) {
     grid_dependency_sync();
-    for (long long j = (long long)blockIdx.x * 256 + threadIdx.x; j < n; j += (long long)gridDim.x * 256) {
-        const int c = m[j], d = v[j];
-        m_out[j] = __fmul_rn(m_scale[j / kAdamWBlock], (float)(c * abs(c)));
-        const float q = __fmul_rn(v_scale[j / kAdamWBlock], (float)(d * d));
-        v_out[j] = __fmul_rn(q, q);
+    constexpr int N = WIDE ? 4 : 1;
+    struct alignas(N) Codes {
+        signed char c[N];
+    };
+    struct alignas(4 * N) Values {
+        float x[N];
+    };
+    const long long step = (long long)gridDim.x * 256 * N;
+    for (long long j = ((long long)blockIdx.x * 256 + threadIdx.x) * N; j + N <= n; j += step) {
+        const Codes c = *reinterpret_cast<const Codes *>(m + j), d = *reinterpret_cast<const Codes *>(v + j);
+        const float ms = m_scale[j / kAdamWBlock], vs = v_scale[j / kAdamWBlock];
+        Values a, b;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float f = (float)c.c[i], h = (float)(unsigned char)d.c[i], q = __fmul_rn(vs, h * h);
+            a.x[i] = __fmul_rn(ms, f * fabsf(f));
+            b.x[i] = __fmul_rn(q, q);
+        }
+        *reinterpret_cast<Values *>(m_out + j) = a;
+        *reinterpret_cast<Values *>(v_out + j) = b;
     }
 }
 
 }  // namespace
 
-sage_status adamw_step(Context &ctx, const AdamWSlot *slots, int count, bool states8, const AdamWRule &rule) {
-    for (int at = 0; at < count; at += kSlots) {
-        static thread_local Batch b;
-        b.count = count - at < kSlots ? count - at : kSlots;
+template <int SLOTS>
+static sage_status step_batches(Context &ctx, const AdamWSlot *slots, int count, bool states8, const AdamWRule &rule) {
+    for (int at = 0; at < count; at += SLOTS) {
+        static thread_local Batch<SLOTS> b;
+        b.count = count - at < SLOTS ? count - at : SLOTS;
         unsigned blocks = 0;
         for (int i = 0; i < b.count; ++i) {
-            b.slot[i] = slots[at + i];
+            AdamWSlot &s = b.slot[i] = slots[at + i];
+            const auto on = [](const void *p, size_t boundary) { return reinterpret_cast<uintptr_t>(p) % boundary == 0; };
+            s.wide = on(s.p, 16) && on(s.g, s.g_dtype == SAGE_F32 ? 16 : 8) && on(s.m, states8 ? 4 : 16) && on(s.v, states8 ? 4 : 16) && on(s.copy, 8);
             b.first[i] = blocks;
-            const long long c = (b.slot[i].n + kAdamWBlock - 1) / kAdamWBlock;
-            if (c + blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "adamw_step: too many elements in one call");
+            const long long c = (s.n + kAdamWBlock - 1) / kAdamWBlock;
+            if (c + blocks > 0x7fff0000ll) return ctx.fail(SAGE_ERR_INVALID, "adamw_step: too many elements in one call");
             blocks += (unsigned)c;
         }
         b.first[b.count] = blocks;
@@ -148,21 +254,27 @@ sage_status adamw_step(Context &ctx, const AdamWSlot *slots, int count, bool sta
         ctx.note_launch("adamw_step");
         if (ctx.dry()) continue;
         const unsigned most = (unsigned)ctx.sm_count * 8, grid = (blocks + 7) / 8 < most ? (blocks + 7) / 8 : most;
-        sage_status st = ctx.check_cuda(states8 ? launch_dependent(ctx.pdl, ctx.stream(), adamw_kernel<true>, dim3(grid), dim3(256), 0, b, rule)
-                                                : launch_dependent(ctx.pdl, ctx.stream(), adamw_kernel<false>, dim3(grid), dim3(256), 0, b, rule),
-                                        "adamw_step");
+        sage_status st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), states8 ? adamw_kernel<true, SLOTS> : adamw_kernel<false, SLOTS>, dim3(grid), dim3(256), 0, b, rule), "adamw_step");
         if (st) return st;
     }
     return SAGE_OK;
 }
 
+sage_status adamw_step(Context &ctx, const AdamWSlot *slots, int count, bool states8, const AdamWRule &rule) {
+    // Parameters of a launch are copied with it: a short list where it holds all tensors.
+    return count <= kFewSlots ? step_batches<kFewSlots>(ctx, slots, count, states8, rule) : step_batches<kSlots>(ctx, slots, count, states8, rule);
+}
+
 sage_status adamw_states(Context &ctx, const void *m, const float *m_scale, const void *v, const float *v_scale, long long n, float *m_out, float *v_out) {
     if (!n) return SAGE_OK;
+    const uintptr_t codes = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v), values = reinterpret_cast<uintptr_t>(m_out) | reinterpret_cast<uintptr_t>(v_out);
+    const bool wide = n % 4 == 0 && codes % 4 == 0 && values % 16 == 0;
     ctx.note_launch("adamw_states");
     if (ctx.dry()) return SAGE_OK;
-    const long long blocks = (n + 255) / 256;
-    const dim3 grid((unsigned)(blocks < ctx.sm_count * 32ll ? blocks : ctx.sm_count * 32ll));
-    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), adamw_states_kernel, grid, dim3(256), 0, (const signed char *)m, m_scale, (const unsigned char *)v, v_scale, n, m_out, v_out), "adamw_states");
+    const long long each = wide ? 1024 : 256, blocks = (n + each - 1) / each, most = ctx.sm_count * 32ll;
+    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? adamw_states_kernel<true> : adamw_states_kernel<false>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0,
+                                           (const signed char *)m, m_scale, (const unsigned char *)v, v_scale, n, m_out, v_out),
+                          "adamw_states");
 }
 
 }  // namespace k

@@ -54,7 +54,8 @@ struct AdamWSlot {
     float *m_scale = nullptr, *v_scale = nullptr;
     void *copy = nullptr;
     long long n = 0;
-    int g_dtype = SAGE_F32, copy_dtype = SAGE_F32;
+    short g_dtype = SAGE_F32, copy_dtype = SAGE_F32;
+    int wide = 0;  // filled in by the launcher: whole blocks lie on vector boundaries
 };
 struct AdamWRule {
     float beta1, one_minus_beta1, beta2, one_minus_beta2;
