@@ -310,7 +310,7 @@ sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logi
  * unused, buf NULL), or m i8 and v u8 with f32 scales, one for each 256 elements of the tensor: |m| = m_scale code^2, sqrt(v) =
  * v_scale code^2; zeroed codes and scales are zero states.  A second moment that is not zero does not become zero; a block in which a
  * moment is not finite has a scale that is NaN.  `copy` (buf NULL: none) receives the updated parameters in f16 / bf16.  States of all
- * tensors of a call have the same width.  step counts from 1. */
+ * tensors of a call have the same width.  step counts from 1; eps is 1e-15 at least. */
 typedef struct {
     sage_tensor param, grad, m, v, m_scale, v_scale, copy;
 } sage_adamw_tensor;

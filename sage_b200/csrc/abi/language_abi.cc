@@ -210,7 +210,7 @@ sage_status sage_adamw_step(sage_ctx *ctx, const sage_adamw_tensor *tensors, int
         if (count < 0 || (count && !tensors)) c.refuse("tensors", "is missing");
         if (o->step < 1) c.refuse("step", "is less than 1");
         if (!(o->beta1 >= 0.0 && o->beta1 < 1.0) || !(o->beta2 >= 0.0 && o->beta2 < 1.0)) c.refuse("beta1 or beta2", "is not in [0, 1)");
-        if (!(o->eps >= 0.0)) c.refuse("eps", "is negative");
+        if (!(o->eps >= 1e-15)) c.refuse("eps", "is less than 1e-15");
         k::AdamWRule rule;
         rule.beta1 = (float)o->beta1;
         rule.one_minus_beta1 = (float)(1.0 - o->beta1);

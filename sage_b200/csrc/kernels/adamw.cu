@@ -52,24 +52,35 @@ __device__ __forceinline__ float block_scale(float x, float *factor) {
     *factor = __fmul_rn(__frcp_rn(x), (float)(TOP * TOP));
     return __fmul_rn(x, 1.f / (TOP * TOP));
 }
-// round(sqrt(t)) for 0 <= t <= 65025 (1 + 2^-20), `off` an approximate root of it: within 1e-4, so another code only where that is the
-// distance to the middle of two.
-__device__ __forceinline__ bool near_middle(float off, float *code) {
-    const float n = __fadd_rn(__fadd_rn(off, 12582912.f), -12582912.f);  // to the nearest whole number
-    *code = n;
-    return fabsf(fabsf(off - n) - 0.5f) < 2e-4f;
+// Codes of eight elements: the nearest whole numbers to the roots of t (with `sign`'s sign), from approximate roots.  1.5 2^23 added leaves the
+// whole number in the low bits.  `off` is the furthest that a root lies from its code: where that is within the approximation's error of
+// one half, another code might be nearer, and the caller takes the exact root.
+constexpr float kMagic = 12582912.f;
+__device__ __forceinline__ unsigned rounded(float root, float *off) {
+    const float n = __fadd_rn(root, kMagic);
+    *off = fmaxf(*off, fabsf(__fadd_rn(root, -__fadd_rn(n, -kMagic))));
+    return __float_as_uint(n);
 }
+__device__ __forceinline__ unsigned low_bytes(const unsigned *n) { return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410); }
 
-struct Element {
-    float p, g, m, v, root;
+// The moments of eight elements after one more gradient, rounded operation by operation; the parameters, with approximate roots and
+// quotients (2^-21).
+struct Elements {
+    float2 p[4], g[4], m[4], v[4], root[4];
 };
-__device__ __forceinline__ void update(const AdamWRule &k, Element &e) {
-    const float g = __fmul_rn(e.g, k.grad_scale);
-    e.m = __fadd_rn(__fmul_rn(e.m, k.beta1), __fmul_rn(g, k.one_minus_beta1));
-    e.v = __fadd_rn(__fmul_rn(e.v, k.beta2), __fmul_rn(__fmul_rn(g, g), k.one_minus_beta2));
-    e.root = fast_root(e.v);
-    e.p = e.p * k.keep - __fdividef(e.m * k.step_size, e.root * k.root_factor + k.eps);
+__device__ __forceinline__ void update(const AdamWRule &k, Elements &e) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 g = mul2(e.g[i], both(k.grad_scale));
+        const float2 zero = both(k.minus_zero);  // products rounded before they are added
+        e.m[i] = add2(fma2(e.m[i], both(k.beta1), zero), fma2(g, both(k.one_minus_beta1), zero));
+        e.v[i] = add2(fma2(e.v[i], both(k.beta2), zero), fma2(mul2(g, g), both(k.one_minus_beta2), zero));
+        e.root[i] = make_float2(fast_root(e.v[i].x), fast_root(e.v[i].y));
+        const float2 below = fma2(e.root[i], both(k.root_factor), both(k.eps)), step = mul2(e.m[i], both(-k.step_size));
+        e.p[i] = fma2(e.p[i], both(k.keep), make_float2(__fdividef(step.x, below.x), __fdividef(step.y, below.y)));
+    }
 }
+__device__ __forceinline__ float &at(float2 *x, int i) { return i % 2 ? x[i / 2].y : x[i / 2].x; }
 
 // Where the eight elements of a lane lie in the block: two times four in a row, or (blocks that end early, tensors off 16-byte
 // boundaries) 32 apart.
@@ -118,69 +129,105 @@ __device__ __forceinline__ void store8(T *p, int n, F get) {
 
 template <bool STATES8, bool WIDE>
 __device__ __forceinline__ void block_update(const AdamWSlot &s, const AdamWRule &k, long long block) {
-    const long long at = block * kAdamWBlock;
-    const int n = WIDE ? kAdamWBlock : (int)min(s.n - at, (long long)kAdamWBlock);
-    Element e[8];
-    if (s.g_dtype == SAGE_F32) load8<WIDE>((const float *)s.g + at, n, [&](int i, float x) { e[i].g = x; });
-    else if (s.g_dtype == SAGE_BF16) load8<WIDE>((const __nv_bfloat16 *)s.g + at, n, [&](int i, __nv_bfloat16 x) { e[i].g = widen(x); });
-    else load8<WIDE>((const __half *)s.g + at, n, [&](int i, __half x) { e[i].g = widen(x); });
-    load8<WIDE>(s.p + at, n, [&](int i, float x) { e[i].p = x; });
+    const long long from = block * kAdamWBlock;
+    const int n = WIDE ? kAdamWBlock : (int)min(s.n - from, (long long)kAdamWBlock);
+    Elements e;
+    if (s.g_dtype == SAGE_F32) load8<WIDE>((const float *)s.g + from, n, [&](int i, float x) { at(e.g, i) = x; });
+    else if (s.g_dtype == SAGE_BF16) load8<WIDE>((const __nv_bfloat16 *)s.g + from, n, [&](int i, __nv_bfloat16 x) { at(e.g, i) = widen(x); });
+    else load8<WIDE>((const __half *)s.g + from, n, [&](int i, __half x) { at(e.g, i) = widen(x); });
+    load8<WIDE>(s.p + from, n, [&](int i, float x) { at(e.p, i) = x; });
     if (STATES8) {
         const float ms = s.m_scale[block], vs = s.v_scale[block];
-        load8<WIDE>((const signed char *)s.m + at, n, [&](int i, signed char c) {
+        load8<WIDE>((const signed char *)s.m + from, n, [&](int i, signed char c) {
             const float f = (float)c;
-            e[i].m = __fmul_rn(ms, f * fabsf(f));
+            at(e.m, i) = __fmul_rn(ms, f * fabsf(f));
         });
-        load8<WIDE>((const unsigned char *)s.v + at, n, [&](int i, unsigned char c) {
-            const float f = (float)c, q = __fmul_rn(vs, f * f);
-            e[i].v = __fmul_rn(q, q);
-        });
+        load8<WIDE>((const unsigned char *)s.v + from, n, [&](int i, unsigned char c) { at(e.v, i) = (float)c; });
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 q = mul2(mul2(e.v[i], e.v[i]), both(vs));
+            e.v[i] = mul2(q, q);
+        }
+        if (!WIDE) {  // a scale that is NaN makes zeros behind the end NaN too
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (place<false>(i) >= n) at(e.m, i) = at(e.v, i) = 0.f;
+        }
     } else {
-        load8<WIDE>((const float *)s.m + at, n, [&](int i, float x) { e[i].m = x; });
-        load8<WIDE>((const float *)s.v + at, n, [&](int i, float x) { e[i].v = x; });
+        load8<WIDE>((const float *)s.m + from, n, [&](int i, float x) { at(e.m, i) = x; });
+        load8<WIDE>((const float *)s.v + from, n, [&](int i, float x) { at(e.v, i) = x; });
     }
-    if (STATES8 && !WIDE) {  // a scale that is NaN makes zeros behind the end NaN too
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (place<false>(i) >= n) e[i].m = e[i].v = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) update(k, e[i]);
-    store8<WIDE>(s.p + at, n, [&](int i) { return e[i].p; });
+    update(k, e);
+    store8<WIDE>(s.p + from, n, [&](int i) { return at(e.p, i); });
     if (s.copy) {
-        if (s.copy_dtype == SAGE_BF16) store8<WIDE>((__nv_bfloat16 *)s.copy + at, n, [&](int i) { return narrowed<__nv_bfloat16>(e[i].p); });
-        else store8<WIDE>((__half *)s.copy + at, n, [&](int i) { return narrowed<__half>(e[i].p); });
+        if (s.copy_dtype == SAGE_BF16) store8<WIDE>((__nv_bfloat16 *)s.copy + from, n, [&](int i) { return narrowed<__nv_bfloat16>(at(e.p, i)); });
+        else store8<WIDE>((__half *)s.copy + from, n, [&](int i) { return narrowed<__half>(at(e.p, i)); });
     }
     if (!STATES8) {
-        store8<WIDE>((float *)s.m + at, n, [&](int i) { return e[i].m; });
-        store8<WIDE>((float *)s.v + at, n, [&](int i) { return e[i].v; });
+        store8<WIDE>((float *)s.m + from, n, [&](int i) { return at(e.m, i); });
+        store8<WIDE>((float *)s.v + from, n, [&](int i) { return at(e.v, i); });
         return;
     }
     float m_top = 0.f, v_top = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        m_top = largest(m_top, fabsf(e[i].m));
-        v_top = largest(v_top, e[i].v);
+        m_top = largest(m_top, fabsf(at(e.m, i)));
+        v_top = largest(v_top, at(e.v, i));
     }
+    m_top = warp_largest(m_top);
+    v_top = __fsqrt_rn(warp_largest(v_top));
     float mf, vf;
-    const float ms = block_scale<127>(warp_largest(m_top), &mf), vs = block_scale<255>(__fsqrt_rn(warp_largest(v_top)), &vf);
+    const float ms = block_scale<127>(m_top, &mf), vs = block_scale<255>(v_top, &vf);
     if (threadIdx.x % 32 == 0) {
         s.m_scale[block] = ms;
         s.v_scale[block] = vs;
     }
-    store8<WIDE>((signed char *)s.m + at, n, [&](int i) {
-        const float t = __fmul_rn(fabsf(e[i].m), mf);
-        float c;
-        if (near_middle(fast_root(t), &c)) c = rintf(__fsqrt_rn(t));
-        return mf > 0.f ? (signed char)__float2int_rn(copysignf(c, e[i].m)) : (signed char)0;
-    });
-    store8<WIDE>((unsigned char *)s.v + at, n, [&](int i) {
-        float c;
-        const bool tiny = __float_as_uint(e[i].v) - 1u < 0x7fffffu;  // subnormal: the fast root of it is 0
-        if (near_middle(fast_root(__fmul_rn(e[i].root, vf)), &c) || tiny) c = rintf(__fsqrt_rn(__fmul_rn(__fsqrt_rn(e[i].v), vf)));
-        if (e[i].v > 0.f) c = fmaxf(c, 1.f);
-        return vf > 0.f ? (unsigned char)__float2int_rn(c) : (unsigned char)0;
-    });
+    unsigned m[8], v[8];
+    float m_off = 0.f, v_off = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        m[i] = rounded(copysignf(fast_root(__fmul_rn(fabsf(at(e.m, i)), mf)), at(e.m, i)), &m_off);
+        // one at least for what is not zero
+        v[i] = rounded(fmaxf(fast_root(__fmul_rn(at(e.root, i), vf)), at(e.v, i) > 0.f ? 0.75f : 0.f), &v_off);
+    }
+    // Two fast roots of up to 255 err by 2^-13 at most, one of up to 127 by 2^-15.  Where all of a block's v lie below 2^-80, subnormal ones count, which
+    // the fast root takes for zero.
+    if (m_off > 0.5f - 0x1p-14f || v_off > 0.5f - 0x1.8p-13f || v_top < 0x1p-40f) {
+        float none = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            float x = at(e.m, 0), y = at(e.v, 0);
+#pragma unroll
+            for (int j = 1; j < 8; ++j)
+                if (j == i) {
+                    x = at(e.m, j);
+                    y = at(e.v, j);
+                }
+            const unsigned c = rounded(copysignf(__fsqrt_rn(__fmul_rn(fabsf(x), mf)), x), &none), d = rounded(fmaxf(__fsqrt_rn(__fmul_rn(__fsqrt_rn(y), vf)), y > 0.f ? 0.75f : 0.f), &none);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j == i) {
+                    m[j] = c;
+                    v[j] = d;
+                }
+        }
+    }
+    unsigned mw[2], vw[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // no codes in blocks that are zero or not finite
+        mw[h] = mf > 0.f ? low_bytes(m + 4 * h) : 0;
+        vw[h] = vf > 0.f ? low_bytes(v + 4 * h) : 0;
+    }
+    if (WIDE) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            *reinterpret_cast<unsigned *>((unsigned char *)s.m + from + place<true>(4 * h)) = mw[h];
+            *reinterpret_cast<unsigned *>((unsigned char *)s.v + from + place<true>(4 * h)) = vw[h];
+        }
+    } else {
+        store8<false>((unsigned char *)s.m + from, n, [&](int i) { return (unsigned char)(mw[i / 4] >> (8 * (i % 4))); });
+        store8<false>((unsigned char *)s.v + from, n, [&](int i) { return (unsigned char)(vw[i / 4] >> (8 * (i % 4))); });
+    }
 }
 
 template <bool STATES8, int SLOTS>

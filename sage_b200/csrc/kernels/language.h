@@ -63,6 +63,7 @@ struct AdamWRule {
     float step_size;    // lr / (1 - beta1^t)
     float root_factor;  // 1 / sqrt(1 - beta2^t)
     float eps, grad_scale;
+    float minus_zero = -0.f;
 };
 sage_status adamw_step(Context &ctx, const AdamWSlot *slots, int count, bool states8, const AdamWRule &rule);
 sage_status adamw_states(Context &ctx, const void *m, const float *m_scale, const void *v, const float *v_scale, long long n, float *m_out, float *v_out);

@@ -131,34 +131,6 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 ulp; below 2^-126 ze
     return y;
 }
 
-// Two f32 operations in one instruction, each rounded by itself.
-__device__ __forceinline__ unsigned long long bits_of(float2 x) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x.x), "f"(x.y));
-    return r;
-}
-__device__ __forceinline__ float2 pair_of(unsigned long long r) {
-    float2 x;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x.x), "=f"(x.y) : "l"(r));
-    return x;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
-    return pair_of(r);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
-    return pair_of(r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
-    return pair_of(r);
-}
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-
 // ------------------------------------------------------------------------------------------ sums of a part of a row
 // The part's largest logit m, s = sum of 2^t and w = sum of t 2^t with t = c2 (x - m), c2 = c log2(e); with m = -inf both are relative
 // to 0.  Differences are taken before they are scaled, so that a large m costs nothing.  Below 2^-200 a term is zero, and t is held at
