@@ -24,6 +24,8 @@ F32, I32, U32 = 0, 1, 2
 F16, BF16, I8, U8 = 3, 4, 5, 6  # storage types of the operators in sage_b200.language alone
 _NP = {F32: np.float32, I32: np.int32, U32: np.uint32, F16: np.float16, BF16: np.uint16, I8: np.int8, U8: np.uint8}  # bf16: its bits
 _DT = {np.dtype(np.float32): F32, np.dtype(np.int32): I32, np.dtype(np.uint32): U32, np.dtype(np.float16): F16, np.dtype(np.int8): I8, np.dtype(np.uint8): U8}
+_SIZE = {k: np.dtype(v).itemsize for k, v in _NP.items()}
+_BORROWED = {}  # another package's element types -> ours, as they are met
 _BY_NAME = {"float32": F32, "int32": I32, "uint32": U32, "float16": F16, "bfloat16": BF16, "int8": I8, "uint8": U8}
 MAX_DIMS = 8
 _P = ctypes.c_void_p
@@ -66,6 +68,8 @@ lib.sage_graph_last_error.restype = ctypes.c_char_p
 lib.sage_ctx_stream.restype = _P
 lib.sage_buf_ptr.restype = _P
 lib.sage_buf_size.restype = ctypes.c_size_t
+_buf_wrap = lib["sage_buf_wrap"]  # of its own, for its argument types
+_buf_wrap.argtypes = [_P, _P, ctypes.c_size_t, ctypes.POINTER(_P)]
 
 
 def _arr64(v):
@@ -306,20 +310,29 @@ class Context:
 
     def wrap(self, address, extents, dtype=F32, strides=None):
         """A DeviceTensor over device memory that something else owns and keeps: `address` is its first element's.  No copy."""
-        extents = tuple(int(e) for e in extents)
         t = DeviceTensor(self, None, dtype, extents, strides)
-        last = sum((e - 1) * s for e, s in zip(extents, t.strides)) if 0 not in extents else -1
+        last = 0
+        for e, s in zip(t.extents, t.strides):
+            last += (e - 1) * s
         t.buf = _P()
-        self._ck(lib.sage_buf_wrap(self.h, _P(address), ctypes.c_size_t((last + 1) * np.dtype(_NP[dtype]).itemsize), ctypes.byref(t.buf)))
+        self._ck(_buf_wrap(self.h, address, (last + 1) * _SIZE[dtype] if 0 not in t.extents else 0, t.buf))
         return t
 
     def borrow(self, t):
         """wrap() of a device tensor of another package (a torch.Tensor: data_ptr(), shape, stride(), dtype), which is kept alive."""
-        name = str(t.dtype).split(".")[-1]
-        if name not in _BY_NAME:
-            raise SageError(1, "borrow: no element type for %s" % name)
-        d = self.wrap(t.data_ptr(), tuple(t.shape) or (1,), _BY_NAME[name], tuple(t.stride()) or (1,))
-        d.base = t
+        dtype = _BORROWED.get(t.dtype)
+        if dtype is None:
+            dtype = _BY_NAME.get(str(t.dtype).split(".")[-1])
+            if dtype is None:
+                raise SageError(1, "borrow: no element type for %s" % t.dtype)
+            _BORROWED[t.dtype] = dtype
+        extents, strides = tuple(t.shape) or (1,), t.stride() or (1,)
+        n = 1 + sum([(e - 1) * s for e, s in zip(extents, strides)]) if 0 not in extents else 0
+        buf = _P()
+        if _buf_wrap(self.h, t.data_ptr(), n * _SIZE[dtype], buf):
+            self._ck(1)
+        d = DeviceTensor.__new__(DeviceTensor)  # programs borrow hundreds of tensors at a time
+        d.__dict__ = {"ctx": self, "buf": buf, "dtype": dtype, "extents": extents, "strides": strides, "offset": 0, "owner": True, "base": t}
         return d
 
 
@@ -327,19 +340,19 @@ class DeviceTensor:
     """A buffer + Shape, the reference's Tensor (src/tensor.rs:106-110), for op-level C-ABI calls."""
 
     def __init__(self, ctx, buf, dtype, extents, strides=None, offset=0, owner=True):
-        self.ctx, self.buf, self.dtype, self.extents, self.offset, self.owner = ctx, buf, dtype, tuple(int(e) for e in extents), offset, owner
+        self.ctx, self.buf, self.dtype, self.extents, self.offset, self.owner = ctx, buf, dtype, tuple(map(int, extents)), offset, owner
         if strides is None:
             strides, p = [], 1
             for e in reversed(self.extents):
                 strides.insert(0, p)
                 p *= e
-        self.strides = tuple(int(s) for s in strides)
+        self.strides = tuple(map(int, strides))
 
     def c(self):
         t = CTensor()
         t.buf, t.dtype, t.ndim, t.offset = self.buf, self.dtype, len(self.extents), self.offset
-        for i, (e, s) in enumerate(zip(self.extents, self.strides)):
-            t.extents[i], t.strides[i] = e, s
+        n = t.ndim
+        t.extents[:n], t.strides[:n] = self.extents, self.strides
         return t
 
     def ref(self):

@@ -44,8 +44,11 @@ def token_log_probs_and_grad(logits, ids, g_log_probs, g_entropy, log_probs, ent
     logits.ctx._ck(lib.sage_token_log_probs_and_grad(logits.ctx.h, logits.ref(), ids.ref(), _F(scale), _ref(g_log_probs), _ref(g_entropy), log_probs.ref(), _ref(entropy), dlogits.ref()))
 
 
+_OPERANDS = ("param", "grad", "m", "v", "m_scale", "v_scale", "copy")
+
+
 class _AdamWTensor(ctypes.Structure):
-    _fields_ = [(n, CTensor) for n in ("param", "grad", "m", "v", "m_scale", "v_scale", "copy")]
+    _fields_ = [(n, CTensor) for n in _OPERANDS]
 
 
 class _AdamWOpts(ctypes.Structure):
@@ -65,7 +68,7 @@ class AdamWTensors:
         self.ctx, self.tensors = ctx, list(tensors)  # keeps the operands alive
         self.array = (_AdamWTensor * max(len(self.tensors), 1))()
         for slot, operands in zip(self.array, self.tensors):
-            for (name, _), t in zip(_AdamWTensor._fields_, operands):
+            for name, t in zip(_OPERANDS, operands):
                 if t is not None:
                     setattr(slot, name, t.c())
 
