@@ -240,39 +240,68 @@ struct TopList {
     }
 };
 
+constexpr int kCandidates = 256;
 template <int THREADS>
 struct TopShared {
     unsigned short chosen[THREADS];
-    int count;
-    unsigned long long lists[THREADS / 32][kMaxTop];
+    int sets, found;
+    unsigned long long candidates[kCandidates], best[kMaxTop], lists[THREADS / 32][kMaxTop];
 };
 
-// The k largest of the block's vectors [begin, end), in warp 0's list.  Each thread knows the largest of the vectors it has summed
+// best[0 .. k) = the k largest of `keys` (0 = none), sorted: a key's place is how many are above it.  best is 0 before; the block calls this
+// together and waits before it reads.
+__device__ __forceinline__ void sort_by_rank(const unsigned long long *keys, int n, int k, unsigned long long *best) {
+    for (int t = threadIdx.x; t < n; t += blockDim.x) {
+        const unsigned long long key = keys[t];
+        int above = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) above += keys[j] > key;
+        if (key && above < k) best[above] = key;
+    }
+}
+
+// The k largest of the block's vectors [begin, end), sorted, in sh.best.  Each thread knows the largest of the vectors it has summed
 // (begin + its number + multiples of THREADS).  The k-th largest of those maxima bounds the k-th largest element from below, and only
-// threads whose maximum reaches it hold candidates: about k of them, whose vectors are read again (from L2).  The bound is taken to
-// 16 bits of the order, which ties and nearness make a little lower.  Where many threads reach it (masks that leave less than k tokens,
-// equal logits), everything is read again in order.
+// threads whose maximum reaches it hold candidates: about k of them, whose vectors are read again (from L2) and whose candidates are
+// ranked.  The bound is taken to 16 bits of the order, which ties and nearness make a little lower; where that lets many threads in (masks
+// that leave less than k tokens, equal logits), to all bits, the token's among them.  Where there are more candidates than the list holds
+// all the same (thousands of open tokens in a few threads, the others masked), everything is read again in order, into sorted lists.
 template <class T, int THREADS>
-__device__ TopList block_top(const RowVectors<T> &row, int begin, int end, float thread_max, int k, TopShared<THREADS> &sh) {
+__device__ void block_top(const RowVectors<T> &row, int begin, int end, float thread_max, int k, TopShared<THREADS> &sh) {
     constexpr int N = Bits<T>::N, W = THREADS / 32;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const unsigned mine = begin + (int)threadIdx.x < end ? rank_bits(thread_max) >> 16 : 0;
-    unsigned bound = 0;
-    for (int bit = 15; bit >= 0; --bit) {
-        const unsigned t = bound | 1u << bit;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, own = begin + (int)threadIdx.x;
+    unsigned long long mine = own < end ? (unsigned long long)rank_bits(thread_max) << 32 : 0, bound = 0;
+    for (int bit = 63; bit >= 48; --bit) {
+        const unsigned long long t = bound | 1ull << bit;
         if (__syncthreads_count(mine >= t) >= k) bound = t;
     }
-    if (threadIdx.x == 0) sh.count = 0;
+    if (__syncthreads_count(mine >= bound) > THREADS / 4) {
+        const unsigned top = rank_bits(thread_max);
+        int token = -1;  // the first of the thread's largest
+        for (int i = own; i < end && token < 0; i += THREADS) {
+            float2 x[N / 2];
+            Bits<T>::unpack(row.load(i), x);
+#pragma unroll
+            for (int j = N - 1; j >= 0; --j)
+                if (rank_bits(j % 2 ? x[j / 2].y : x[j / 2].x) == top && (unsigned)(row.element(i) + j) < (unsigned)row.cols) token = row.element(i) + j;
+        }
+        mine = token >= 0 ? (unsigned long long)top << 32 | (0xffffffffu - (unsigned)token) : 0;
+        const int token_bits = 32 - __clz(row.cols);  // the bits above them are set in every key
+        for (int bit = 47; bit >= 0; --bit) {
+            const unsigned long long t = bound | 1ull << bit;
+            if ((bit < 32 && bit >= token_bits) || __syncthreads_count(mine >= t) >= k) bound = t;
+        }
+        if (__syncthreads_count(mine >= bound) < k) bound = 0;  // fewer than k threads have anything
+    }
+    if (threadIdx.x == 0) sh.sets = sh.found = 0;
+    if (threadIdx.x < kMaxTop) sh.best[threadIdx.x] = 0;
     __syncthreads();
-    if (mine >= bound) sh.chosen[atomicAdd(&sh.count, 1)] = (unsigned short)threadIdx.x;  // in any order: keys decide
+    if (mine >= bound) sh.chosen[atomicAdd(&sh.sets, 1)] = (unsigned short)threadIdx.x;  // in any order: keys decide
     __syncthreads();
-    const int sets = sh.count;
-    const bool all = sets > THREADS / 4;
-    TopList list;
-    for (int q = warp; q < (all ? W : sets); q += W) {
-        // all: the warp's 32 vectors of every THREADS; else the vectors of one thread, one for each lane
-        const int from = all ? begin + warp * 32 + lane : begin + sh.chosen[q] + lane * THREADS, step = all ? THREADS : 32 * THREADS;
-        for (int base = from - (all ? lane : lane * THREADS), i = from; base < end; base += step, i += step) {
+    const int sets = sh.sets;
+    // Vectors first, first + step ... in front of `end`, a vector to a lane; f(key, is it one)
+    auto each = [&](int first, int lane_step, int step, auto f) {
+        for (int base = first, i = first + lane * lane_step; base < end; base += step, i += step) {
             const bool some = i < end;
             const uint4 v = some ? row.load(i) : RowVectors<T>::nothing();
             float2 x[N / 2];
@@ -280,23 +309,37 @@ __device__ TopList block_top(const RowVectors<T> &row, int begin, int end, float
             const int e = row.element(i);
             bool any = false;
 #pragma unroll
-            for (int j = 0; j < N; ++j) any |= rank_bits(j % 2 ? x[j / 2].y : x[j / 2].x) >> 16 >= bound;
+            for (int j = 0; j < N; ++j) any |= rank_bits(j % 2 ? x[j / 2].y : x[j / 2].x) >= (unsigned)(bound >> 32);
             if (!__any_sync(0xffffffffu, any && some)) continue;
-#pragma unroll 1
-            for (int j = 0; j < N; ++j) {
-                float y = x[0].x;
 #pragma unroll
-                for (int l = 1; l < N; ++l) y = j == l ? (l % 2 ? x[l / 2].y : x[l / 2].x) : y;
-                const bool in = some && (unsigned)(e + j) < (unsigned)row.cols && rank_bits(y) >> 16 >= bound;
-                list.offer(rank_key(y, (unsigned)(e + j)), in, k);
+            for (int j = 0; j < N; ++j) {
+                const unsigned long long key = rank_key(j % 2 ? x[j / 2].y : x[j / 2].x, (unsigned)(e + j));
+                f(key, some && (unsigned)(e + j) < (unsigned)row.cols && key >= bound);
             }
         }
-    }
-    if (lane < kMaxTop) sh.lists[warp][lane] = lane < k ? list.key : 0;
+    };
+    const bool few = sets <= THREADS / 4;
+    if (few)
+        for (int q = warp; q < sets; q += W)
+            each(begin + sh.chosen[q], THREADS, 32 * THREADS, [&](unsigned long long key, bool in) {
+                if (!in) return;
+                const int at = atomicAdd(&sh.found, 1);
+                if (at < kCandidates) sh.candidates[at] = key;
+            });
     __syncthreads();
-    if (warp == 0)
-        for (int w = 1; w < W; ++w) list.offer(sh.lists[w][lane], true, k);
-    return list;
+    if (few && sh.found <= kCandidates) {
+        sort_by_rank(sh.candidates, sh.found, k, sh.best);
+    } else {
+        TopList list;
+        each(begin + warp * 32, 1, THREADS, [&](unsigned long long key, bool in) { list.offer(key, in, k); });
+        sh.lists[warp][lane] = lane < k ? list.key : 0;
+        __syncthreads();
+        if (warp == 0) {
+            for (int w = 1; w < W; ++w) list.offer(sh.lists[w][lane], true, k);
+            sh.best[lane] = lane < k ? list.key : 0;
+        }
+    }
+    __syncthreads();
 }
 
 // ------------------------------------------------------------------------------------------ values
@@ -307,7 +350,7 @@ template <class T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(const LogProbs a, const int shift) {
     constexpr int U = 4;
     __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
-    __shared__ unsigned long long part_lists[TOP ? kMaxCluster : 1][kMaxTop];
+    __shared__ unsigned long long part_lists[TOP ? kMaxCluster * kMaxTop : 1];
     __shared__ TopShared<TOP ? THREADS : 32> top;
     grid_dependency_sync();
     const int parts = 1 << shift;
@@ -333,8 +376,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     }
     const float thread_max = mine.m;
     Sums all = block_join<THREADS>(mine, c2, sums);
-    TopList list;
-    if constexpr (TOP) list = block_top<T, THREADS>(row, begin, end, thread_max, a.top, top);
+    if constexpr (TOP) block_top<T, THREADS>(row, begin, end, thread_max, a.top, top);
     const int lane = threadIdx.x % 32;
     if (parts > 1) {  // everything to the first CTA, which has started when the wait ends
         cluster_wait();
@@ -344,14 +386,18 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
             peer_store(to + 4, all.s);
             peer_store(to + 8, all.w);
         }
-        if (TOP && threadIdx.x < 32) peer_store(peer_shared(&part_lists[TOP ? rank : 0][lane], 0), lane < a.top ? list.key : 0ull);
+        if (TOP && (int)threadIdx.x < a.top) peer_store(peer_shared(&part_lists[rank * a.top + threadIdx.x], 0), top.best[threadIdx.x]);
         if (threadIdx.x < 32) cluster_arrive();
         else cluster_arrive_relaxed();
         cluster_wait();
-        if (rank || threadIdx.x >= 32) return;
-        all = warp_join(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
-        if (TOP)
-            for (int p = 1; p < parts; ++p) list.offer(part_lists[TOP ? p : 0][lane], true, a.top);
+        if (rank) return;
+        if constexpr (TOP) {
+            if (threadIdx.x < kMaxTop) top.best[threadIdx.x] = 0;
+            __syncthreads();
+            sort_by_rank(part_lists, parts * a.top, a.top, top.best);
+            __syncthreads();
+        }
+        if (threadIdx.x < 32) all = warp_join(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
     }
     if (threadIdx.x >= 32) return;
     const float base = base_of(all.m), ln_s = logf(all.s);
@@ -365,8 +411,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
         }
     }
     if (TOP && (int)threadIdx.x < a.top) {
-        ((int *)a.top_ids.ptr)[r * a.top_ids.pitch + lane] = (int)(0xffffffffu - (unsigned)list.key);
-        ((float *)a.top_log_probs.ptr)[r * a.top_log_probs.pitch + lane] = none ? -INFINITY : (rank_logit(list.key) - base) * a.scale - ln_s;
+        const unsigned long long key = top.best[lane];
+        ((int *)a.top_ids.ptr)[r * a.top_ids.pitch + lane] = (int)(0xffffffffu - (unsigned)key);
+        ((float *)a.top_log_probs.ptr)[r * a.top_log_probs.pitch + lane] = none ? -INFINITY : (rank_logit(key) - base) * a.scale - ln_s;
     }
 }
 
@@ -535,12 +582,13 @@ long long most_vectors(const RowsArg &x) {
 int log2_of(int power) { return __builtin_ctz((unsigned)power); }
 
 // How many CTAs share a row: the fewest steps of a grid of `slots` resident CTAs, each step the part's bytes and a fixed cost that
-// measures like 24 KB of them (joining, the cluster's barriers).
-int parts_of_rows(long long rows, long long bytes, long long slots) {
+// measures like 24 KB of them (joining, the cluster's barriers), 128 KB with alternatives (candidates found and ranked).
+constexpr double kFixed = 24576, kFixedTop = 131072;
+int parts_of_rows(long long rows, long long bytes, long long slots, double fixed) {
     int best = 1;
     double least = 0;
     for (int c = 1; c <= kMaxCluster; c *= 2) {
-        const double cost = (double)((rows * c + slots - 1) / slots) * ((double)bytes / c + 24576.0);
+        const double cost = (double)((rows * c + slots - 1) / slots) * ((double)bytes / c + fixed);
         if (c == 1 || cost < least) {
             best = c;
             least = cost;
@@ -559,7 +607,7 @@ sage_status token_log_probs(Context &ctx, const LogProbs &a) {
         typedef decltype(t) T;
         const long long bytes = a.logits.cols * (long long)sizeof(T);
         auto launch = [&](auto kernel, int threads) {
-            const int parts = threads == 128 ? 1 : parts_of_rows(a.logits.rows, bytes, ctx.sm_count * 2ll);
+            const int parts = threads == 128 ? 1 : parts_of_rows(a.logits.rows, bytes, ctx.sm_count * 2ll, a.top ? kFixedTop : kFixed);
             return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log2_of(parts)), "token_log_probs");
         };
         // Short rows: four warps for each, or most threads of a large block would have nothing to read.
