@@ -581,9 +581,18 @@ long long most_vectors(const RowsArg &x) {
 
 int log2_of(int power) { return __builtin_ctz((unsigned)power); }
 
+// The block's size: small blocks, of which more run on an SM, interleave reading and joining better, as long as there are rows for them (8192 x
+// 50021 f32: 259, 269 and 283 us with 128, 256 and 512 threads; 16384 x 8000: 85, 103 and 148); with few rows the largest, a cluster of eight of
+// which reads a row fastest (64 x 131072 bf16 with 20 alternatives: 15.5 us with 256 threads, 12.1 with 512).  Alternatives are found
+// by few threads, which have more to read again in long rows of small blocks (3000 x 131072 bf16 with 20: 234 us with 128 threads, 191 with 256).
+int threads_of_rows(long long rows, long long bytes, bool top, int sms) {
+    if (bytes <= 16384 || (rows >= 16ll * sms && (!top || bytes <= 65536))) return 128;
+    return rows * kMaxCluster < 4ll * sms ? 512 : 256;
+}
+
 // How many CTAs share a row: the fewest steps of a grid of `slots` resident CTAs, each step the part's bytes and a fixed cost that
 // measures like 24 KB of them (joining, the cluster's barriers), 128 KB with alternatives (candidates found and ranked).
-constexpr double kFixed = 24576, kFixedTop = 131072;
+constexpr double kFixed = 24576, kFixedTop = 131072;  // of a block of 512 threads
 int parts_of_rows(long long rows, long long bytes, long long slots, double fixed) {
     int best = 1;
     double least = 0;
@@ -606,13 +615,14 @@ sage_status token_log_probs(Context &ctx, const LogProbs &a) {
     return with_type(a.logits.dtype, [&](auto t) {
         typedef decltype(t) T;
         const long long bytes = a.logits.cols * (long long)sizeof(T);
-        auto launch = [&](auto kernel, int threads) {
-            const int parts = threads == 128 ? 1 : parts_of_rows(a.logits.rows, bytes, ctx.sm_count * 2ll, a.top ? kFixedTop : kFixed);
+        const int threads = threads_of_rows(a.logits.rows, bytes, a.top > 0, ctx.sm_count);
+        const int parts = threads == 128 ? 1 : parts_of_rows(a.logits.rows, bytes, ctx.sm_count * 1024ll / threads, (a.top ? kFixedTop : kFixed) * threads / 512);
+        auto launch = [&](auto kernel) {
             return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log2_of(parts)), "token_log_probs");
         };
-        // Short rows: four warps for each, or most threads of a large block would have nothing to read.
-        if (bytes <= 16384) return a.top ? launch(log_probs_kernel<T, 128, true>, 128) : launch(log_probs_kernel<T, 128, false>, 128);
-        return a.top ? launch(log_probs_kernel<T, 512, true>, 512) : launch(log_probs_kernel<T, 512, false>, 512);
+        if (threads == 128) return a.top ? launch(log_probs_kernel<T, 128, true>) : launch(log_probs_kernel<T, 128, false>);
+        if (threads == 256) return a.top ? launch(log_probs_kernel<T, 256, true>) : launch(log_probs_kernel<T, 256, false>);
+        return a.top ? launch(log_probs_kernel<T, 512, true>) : launch(log_probs_kernel<T, 512, false>);
     });
 }
 
