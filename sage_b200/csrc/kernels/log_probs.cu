@@ -99,6 +99,11 @@ struct RowVectors {
     __device__ __forceinline__ void load_all(uint4 (&v)[U], int i, int end) const {
         const uint4 *p = reinterpret_cast<const uint4 *>(origin) + i;
         const int stop = min(end, full);
+        if (i >= first && i + (U - 1) * STEP < stop) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = __ldcg(p + u * STEP);
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             v[u] = nothing();
@@ -433,9 +438,9 @@ struct GradRow {
         level = -share * (ge != 0.f ? gl + ge * (entropy - logf(s)) : gl);  // NaN where s is: so is every gradient
         at_id = scale * gl;
     }
-    // The gradients at one vector's logits, in the logits' type.
+    // The gradients at one vector's logits, in the logits' type; `own`: the token's place in the vector, if it is there.
     template <class T>
-    __device__ __forceinline__ uint4 gradient(const uint4 &v, int element) const {  // `element`: the vector's first
+    __device__ __forceinline__ uint4 gradient(const uint4 &v, bool has_own, int own) const {
         constexpr int N = Bits<T>::N;
         const float2 b = both(-base), f = both(c2), k = both(slope), l = both(level);
         float2 x[N / 2];
@@ -446,11 +451,10 @@ struct GradRow {
             t = make_float2(fmaxf(t.x, kLeast), fmaxf(t.y, kLeast));  // masked: 0 times a number
             x[j] = mul2(make_float2(exp2_fast(t.x), exp2_fast(t.y)), fma2(k, t, l));
         }
-        const unsigned at = (unsigned)(id - element);
-        if (at < (unsigned)N) {
+        if (has_own) {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (j == (int)at) (j % 2 ? x[j / 2].y : x[j / 2].x) += at_id;
+                if (j == own) (j % 2 ? x[j / 2].y : x[j / 2].x) += at_id;
         }
         return Bits<T>::packed(x);
     }
@@ -469,13 +473,19 @@ __device__ __noinline__ void store_elements(T *dx, int e, int cols, uint4 g) {
 template <class T, int U, int STEP>
 __device__ __forceinline__ void store_all(const RowVectors<T> &row, const GradRow &g, T *dx, bool same, const uint4 (&v)[U], int i, int end) {
     uint4 *p = reinterpret_cast<uint4 *>(dx + row.element(0)) + i;
+    constexpr int N = Bits<T>::N;
+    const int from_own = g.id >= 0 ? (g.id + row.head) / N - i : -1, own = (g.id + row.head) % N;  // in vectors
+    if (same && i >= row.first && i + (U - 1) * STEP < min(end, row.full)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) p[u * STEP] = g.gradient<T>(v[u], from_own == u * STEP, own);
+        return;
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         if (i + u * STEP >= end) return;
-        const int e = row.element(i + u * STEP);
-        const uint4 out = g.gradient<T>(v[u], e);
-        if (same && i + u * STEP < row.full && (u > 0 || i >= row.first)) p[u * STEP] = out;
-        else store_elements(dx, e, row.cols, out);
+        const uint4 out = g.gradient<T>(v[u], from_own == u * STEP, own);
+        if (same && row.whole(i + u * STEP)) p[u * STEP] = out;
+        else store_elements(dx, row.element(i + u * STEP), row.cols, out);
     }
 }
 template <class T>
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
 // gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.
 template <class T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int shift) {
+__global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int shift, const bool full_parts) {
     __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
     __shared__ GradRow constants;
     grid_dependency_sync();
@@ -523,7 +533,7 @@ __global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREA
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
     T *dx = (T *)a.dlogits.ptr + r * a.dlogits.pitch;
     const RowVectors<T> row(x, a.logits.cols);
-    const int each = (row.count + parts - 1) >> shift, begin = (int)rank * each, end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
+    const int each = full_parts ? THREADS * NV : (row.count + parts - 1) >> shift, begin = min((int)rank * each, row.count), end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
     const float c2 = a.scale * 1.4426950408889634f;
     uint4 v[NV];
     row.template load_all<NV, THREADS>(v, i, end);
@@ -663,12 +673,17 @@ sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const 
     if (parts <= kMaxCluster && a.logits.rows * kMaxCluster <= 0x7fffffffll) {
         ctx.note_launch("token_log_probs_and_grad");
         if (ctx.dry()) return SAGE_OK;
+        // The fewest parts: all but the last as long as registers hold, whose threads need not look where their vectors end.
+        bool full_parts = true;
         if (threads > 128)
-            while (parts < kMaxCluster && a.logits.rows * parts * threads < ctx.sm_count * 1024ll) parts *= 2;
+            while (parts < kMaxCluster && a.logits.rows * parts * threads < ctx.sm_count * 1024ll) {
+                parts *= 2;
+                full_parts = false;
+            }
         return with_type(a.logits.dtype, [&](auto t) {
             typedef decltype(t) T;
             auto launch = [&](auto kernel) {
-                return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log_probs, entropy, log2_of(parts)),
+                return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log_probs, entropy, log2_of(parts), full_parts),
                                       "token_log_probs_and_grad");
             };
             return threads == 128 ? launch(log_probs_and_grad_kernel<T, 128, NV>) : threads == 256 ? launch(log_probs_and_grad_kernel<T, 256, NV>) : launch(log_probs_and_grad_kernel<T, 512, NV>);
