@@ -4,6 +4,7 @@
 //   log p_j = c (x_j - m) - ln S,   H = ln S - sum c (x_j - m) exp(c (x_j - m)) / S.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 
 #include "language.h"
@@ -201,6 +202,11 @@ __device__ __forceinline__ Sums block_join(Sums a, float c2, Sums *shared) {
 __device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ unsigned cluster_number() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
     return r;
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -522,18 +528,17 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
 // gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.
 template <class T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int shift, const bool full_parts) {
+__global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int parts, const int each) {
     __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
     __shared__ GradRow constants;
     grid_dependency_sync();
-    const int parts = 1 << shift;
     if (parts > 1) cluster_arrive_relaxed();
-    const long long r = blockIdx.x >> shift;
+    const long long r = cluster_number();
     const unsigned rank = parts > 1 ? cluster_rank() : 0;
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
     T *dx = (T *)a.dlogits.ptr + r * a.dlogits.pitch;
     const RowVectors<T> row(x, a.logits.cols);
-    const int each = full_parts ? THREADS * NV : (row.count + parts - 1) >> shift, begin = min((int)rank * each, row.count), end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
+    const int begin = min((int)rank * each, row.count), end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
     const float c2 = a.scale * 1.4426950408889634f;
     uint4 v[NV];
     row.template load_all<NV, THREADS>(v, i, end);
@@ -664,26 +669,25 @@ sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const 
     if (!a.logits.rows) return SAGE_OK;
     constexpr int NV = 8;
     const long long vectors = most_vectors(a.logits);
-    // Blocks of 256 threads where eight of them hold a row, four on an SM: their loads, sums and stores interleave better than those of
-    // two blocks of 512 (8192 x 131072 bf16: 896 and 992 us; 16 vectors a thread 918 at best).
-    const int threads = vectors <= 128 * NV ? 128 : vectors <= kMaxCluster * 256 * NV ? 256 : 512;
-    int parts = 1;
-    while (vectors > (long long)parts * threads * NV) parts *= 2;
-    // Rows that fit the registers of a cluster, in as many parts as keep all SMs busy.
+    // The smallest blocks eight of which hold a row: more of them run on an SM, and loads, sums and stores of different ones interleave (8192
+    // x 131072 bf16: 852 us with 256 threads, 992 with 512; 8192 x 50021: 387, 484 and 540 with 128, 256 and 512).
+    const int threads = vectors <= kMaxCluster * 128 * NV ? 128 : vectors <= kMaxCluster * 256 * NV ? 256 : 512;
+    int parts = (int)std::min((vectors + threads * NV - 1) / (threads * NV), kMaxCluster + 1ll);
+    // Rows that fit the registers of a cluster.
     if (parts <= kMaxCluster && a.logits.rows * kMaxCluster <= 0x7fffffffll) {
         ctx.note_launch("token_log_probs_and_grad");
         if (ctx.dry()) return SAGE_OK;
-        // The fewest parts: all but the last as long as registers hold, whose threads need not look where their vectors end.
-        bool full_parts = true;
-        if (threads > 128)
-            while (parts < kMaxCluster && a.logits.rows * parts * threads < ctx.sm_count * 1024ll) {
-                parts *= 2;
-                full_parts = false;
-            }
+        // Parts as large as registers hold, whose threads need not look where their vectors end; smaller ones where SMs would be idle.
+        int each = threads * NV;
+        if (a.logits.rows * parts * threads < ctx.sm_count * 1024ll) {
+            parts = (int)std::min<long long>(kMaxCluster, std::max<long long>(parts, ctx.sm_count * 1024ll / (a.logits.rows * threads)));
+            parts = (int)std::min<long long>(parts, (vectors + threads - 1) / threads);
+            each = (int)((vectors + parts - 1) / parts);
+        }
         return with_type(a.logits.dtype, [&](auto t) {
             typedef decltype(t) T;
             auto launch = [&](auto kernel) {
-                return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log_probs, entropy, log2_of(parts), full_parts),
+                return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log_probs, entropy, parts, each),
                                       "token_log_probs_and_grad");
             };
             return threads == 128 ? launch(log_probs_and_grad_kernel<T, 128, NV>) : threads == 256 ? launch(log_probs_and_grad_kernel<T, 256, NV>) : launch(log_probs_and_grad_kernel<T, 512, NV>);
