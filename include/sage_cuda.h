@@ -273,7 +273,8 @@ sage_status sage_conv2d_nhwc(sage_ctx *ctx, const sage_tensor *x, const sage_ten
  * Operands are views (buffer, extents, strides, offset) that must lie inside their buffers; rows ([.., D] and [.., V]) are
  * contiguous along the last axis with any distance between rows that keeps them apart (inputs: any that is not negative), vectors
  * may have any stride (inputs: also 0, a broadcast value).  Outputs may not share memory with an operand unless it says so.
- * Calls with no rows return at once.  All sums are held in 32 bits in a fixed order: the same inputs give the same bits. */
+ * Calls with no rows return at once.  All sums are held in 32 bits in a fixed order: the same inputs, as far from 16-byte boundaries,
+ * give the same bits. */
 
 /* y[t, :] = scale * table[ids[t], :].  table [V, D] f32 / f16 / bf16, ids [T] i32 / u32, y [T, D] f32 or the table's type.  An id
  * outside [0, V) stands for no token: its row is zeros. */

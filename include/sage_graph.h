@@ -121,6 +121,14 @@ sage_status sage_op_softmax_cross_entropy(const sage_var *x, const sage_var *lab
 sage_status sage_op_layer_norm(const sage_var *x, int32_t naxes, const int64_t *axes, const sage_var *gamma,
                                const sage_var *beta, float eps, sage_var **out);                                  /* :84-100 */
 
+/* ---- language models (no reference counterpart; the kernels and their rules are sage_cuda.h's).
+ * embedding: scale * table[ids], extents of ids + [width], gradient by sorted tokens.  token_log_probs: f32 [rows, 4] over logits
+ * [rows, tokens] and one id for each row: column 0 the token's log probability under softmax(scale * logits), column 1 the row's
+ * entropy, both differentiable, then what the gradient reads.  top_tokens: u32 [rows, k], the k <= 32 largest. */
+sage_status sage_op_embedding(const sage_var *table, const sage_var *ids, float scale, sage_var **out);
+sage_status sage_op_token_log_probs(const sage_var *logits, const sage_var *ids, float scale, sage_var **out);
+sage_status sage_op_top_tokens(const sage_var *logits, int64_t k, sage_var **out);
+
 /* ---- random tensors, src/ops/rand.rs:21-140.  The reference takes two 32-bit seeds from the thread's generator at
  * every evaluation; here the caller gives them, so results can be reproduced.  uniform: [0, 1]; normal: Box-Muller. */
 sage_status sage_op_uniform(int32_t ndim, const int64_t *extents, uint32_t seed_x, uint32_t seed_y, sage_var **out);
@@ -135,6 +143,9 @@ sage_status sage_op_accuracy(const sage_var *logits, const sage_var *labels, sag
 typedef struct sage_optimizer sage_optimizer;
 sage_status sage_sgd_create(float lr, sage_optimizer **out);
 sage_status sage_adam_create(float lr, sage_optimizer **out);
+/* AdamW (no reference counterpart; the rule is sage_adamw_step's): states in 32 or 8 bits, kept by parameter, zero before the first
+ * update, which is step 1. */
+sage_status sage_adamw_create(double lr, double beta1, double beta2, double eps, double weight_decay, int32_t state_bits, sage_optimizer **out);
 /* The private fields of the reference's structs (optim.rs:14-26, 97-110); Sgd's momentum stays 0 (with
  * any other value the reference's update panics, optim.rs:68-69, and this one returns SAGE_ERR_UNSUPPORTED). */
 sage_status sage_optimizer_set_weight_decay(sage_optimizer *o, float weight_decay);

@@ -625,6 +625,22 @@ def grad_param(y, model):
     return dict(zip(params, grad(y, params)))
 
 
+def embedding(table, ids, scale=1.0):
+    """scale * table[ids]: a row of the table for each token id (zeros for ids outside it), with a gradient by sorted tokens."""
+    return _mk(lib.sage_op_embedding, table.h, ids.h, ctypes.c_float(scale))
+
+
+def token_log_probs(logits, ids, scale=1.0):
+    """(log probabilities of ids [rows] under softmax(scale * logits [rows, tokens]), the rows' entropies), both [rows]."""
+    y = _mk(lib.sage_op_token_log_probs, logits.h, ids.h, ctypes.c_float(scale))
+    return squeeze(slice_(y, 1, 0, 1), 1), squeeze(slice_(y, 1, 1, 2), 1)
+
+
+def top_tokens(logits, k):
+    """The k <= 32 largest of each row, largest first and ties lowest token first: u32 [rows, k]."""
+    return _mk(lib.sage_op_top_tokens, logits.h, ctypes.c_int64(k))
+
+
 def uniform(extents, seed_x, seed_y):
     """ops::rand::uniform (src/ops/rand.rs:21-28, 50-90) with explicit seeds: values in [0, 1]."""
     return _mk(lib.sage_op_uniform, len(extents), _arr64(extents), ctypes.c_uint32(seed_x), ctypes.c_uint32(seed_y))
@@ -682,6 +698,16 @@ class Adam(Optimizer):
     def __init__(self, lr):
         h = _P()
         _gck(lib.sage_adam_create(ctypes.c_float(lr), ctypes.byref(h)))
+        super().__init__(h)
+
+
+class AdamW(Optimizer):
+    """Adam with decoupled weight decay, the bias corrections of step 1 onwards, and states in 32 or 8 bits (1 byte each and a
+    scale for 256 elements; sage_b200.language says how)."""
+
+    def __init__(self, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, state_bits=32):
+        h, d = _P(), ctypes.c_double
+        _gck(lib.sage_adamw_create(d(lr), d(beta1), d(beta2), d(eps), d(weight_decay), int(state_bits), ctypes.byref(h)))
         super().__init__(h)
 
 

@@ -310,6 +310,10 @@ sage_status sage_op_layer_norm(const sage_var *x, int32_t naxes, const int64_t *
     OP(ops::layer_norm(x->v, axes_of(naxes, axes), gamma->v, beta->v, eps));
 }
 
+sage_status sage_op_embedding(const sage_var *table, const sage_var *ids, float scale, sage_var **out) { OP(ops::embedding(table->v, ids->v, scale)); }
+sage_status sage_op_token_log_probs(const sage_var *logits, const sage_var *ids, float scale, sage_var **out) { OP(ops::token_log_probs(logits->v, ids->v, scale)); }
+sage_status sage_op_top_tokens(const sage_var *logits, int64_t k, sage_var **out) { OP(ops::top_tokens(logits->v, k)); }
+
 sage_status sage_op_uniform(int32_t ndim, const int64_t *extents, uint32_t seed_x, uint32_t seed_y, sage_var **out) {
     OP(ops::uniform(arr(ndim, extents), seed_x, seed_y));
 }
@@ -370,9 +374,17 @@ sage_status sage_adam_create(float lr, sage_optimizer **out) {
     *out = new sage_optimizer{std::unique_ptr<nn::Optimizer>(new nn::Adam(lr))};
     return SAGE_OK;
 }
+sage_status sage_adamw_create(double lr, double beta1, double beta2, double eps, double weight_decay, int32_t state_bits, sage_optimizer **out) {
+    return guarded([&]() -> sage_status {
+        auto w = std::make_unique<nn::AdamW>(lr, beta1, beta2, eps, weight_decay, state_bits);
+        *out = new sage_optimizer{std::move(w)};
+        return SAGE_OK;
+    });
+}
 sage_status sage_optimizer_set_weight_decay(sage_optimizer *o, float weight_decay) {
     if (auto *a = dynamic_cast<nn::Adam *>(o->impl.get())) a->weight_decay = weight_decay;
     else if (auto *g = dynamic_cast<nn::Sgd *>(o->impl.get())) g->weight_decay = weight_decay;
+    else if (auto *w = dynamic_cast<nn::AdamW *>(o->impl.get())) w->weight_decay = weight_decay;
     return SAGE_OK;
 }
 sage_status sage_optimizer_destroy(sage_optimizer *o) {

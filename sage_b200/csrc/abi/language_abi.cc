@@ -211,16 +211,9 @@ sage_status sage_adamw_step(sage_ctx *ctx, const sage_adamw_tensor *tensors, int
         if (o->step < 1) c.refuse("step", "is less than 1");
         if (!(o->beta1 >= 0.0 && o->beta1 < 1.0) || !(o->beta2 >= 0.0 && o->beta2 < 1.0)) c.refuse("beta1 or beta2", "is not in [0, 1)");
         if (!(o->eps >= 1e-15)) c.refuse("eps", "is less than 1e-15");
-        k::AdamWRule rule;
-        rule.beta1 = (float)o->beta1;
-        rule.one_minus_beta1 = (float)(1.0 - o->beta1);
-        rule.beta2 = (float)o->beta2;
-        rule.one_minus_beta2 = (float)(1.0 - o->beta2);
-        rule.keep = finite(c, "lr or weight_decay", 1.0 - o->lr * o->weight_decay);
-        rule.step_size = finite(c, "lr", o->lr / (1.0 - std::pow(o->beta1, (double)o->step)));
-        rule.root_factor = (float)(1.0 / std::sqrt(1.0 - std::pow(o->beta2, (double)o->step)));
-        rule.eps = finite(c, "eps", o->eps);
-        rule.grad_scale = finite(c, "grad_scale", o->grad_scale);
+        for (double x : {o->lr, o->weight_decay, o->lr * o->weight_decay, o->eps}) finite(c, "lr, weight_decay or eps", x);
+        finite(c, "grad_scale", o->grad_scale);
+        const k::AdamWRule rule = k::adamw_rule(o->lr, o->beta1, o->beta2, o->eps, o->weight_decay, o->grad_scale, o->step);
         std::vector<k::AdamWSlot> slots;
         slots.reserve((size_t)count);
         const bool states8 = count && tensors[0].m.dtype == SAGE_I8;

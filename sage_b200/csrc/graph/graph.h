@@ -348,6 +348,10 @@ Var softmax_cross_entropy(const Var &x, const Var &labels);
 Var layer_norm(const Var &x, const std::vector<long long> &axes, const Var &gamma, const Var &beta, float eps);
 // metric.rs
 Var accuracy(const Var &logits, const Var &labels);
+// language models (ops_language.cc)
+Var embedding(const Var &table, const Var &ids, float scale);
+Var token_log_probs(const Var &logits, const Var &ids, float scale);  // [rows, 4]: log probability, entropy, and what the gradient reads
+Var top_tokens(const Var &logits, long long k);
 // rand.rs (the seeds the reference draws per evaluation are arguments here)
 Var uniform(const Array &extents, unsigned seed_x, unsigned seed_y);
 Var normal(const Array &extents, unsigned seed_x, unsigned seed_y);

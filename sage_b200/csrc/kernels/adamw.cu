@@ -10,6 +10,8 @@
 // 16 with 8-bit states and f32 gradients.
 #include <cuda_runtime.h>
 
+#include <cmath>
+
 #include "language.h"
 #include "launch.h"
 #include "narrow.h"
@@ -377,6 +379,21 @@ __global__ void __launch_bounds__(256) adamw_states_kernel(const signed char *m,
 }
 
 }  // namespace
+
+// The constants of a step, from 64 bits.
+AdamWRule adamw_rule(double lr, double beta1, double beta2, double eps, double weight_decay, double grad_scale, long long step) {
+    AdamWRule r;
+    r.beta1 = (float)beta1;
+    r.one_minus_beta1 = (float)(1.0 - beta1);
+    r.beta2 = (float)beta2;
+    r.one_minus_beta2 = (float)(1.0 - beta2);
+    r.keep = (float)(1.0 - lr * weight_decay);
+    r.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+    r.root_factor = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+    r.eps = (float)eps;
+    r.grad_scale = (float)grad_scale;
+    return r;
+}
 
 template <int SLOTS>
 static sage_status step_batches(Context &ctx, const AdamWSlot *slots, int count, bool states8, const AdamWRule &rule) {

@@ -24,12 +24,12 @@ sage_status embedding(Context &ctx, const RowsArg &table, const VectorArg &ids, 
 sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids, float scale, bool add, const RowsArg &dtable);
 
 constexpr int kMaxTop = 32;
-struct LogProbs {
+struct LogProbs {  // what has no ptr is not wanted, or (ids) not given
     RowsArg logits;
     VectorArg ids;
     float scale = 1.f;
     VectorArg log_probs, entropy;  // f32
-    RowsArg stats;                 // [rows, 2] f32 {max of the logits, sum of exp(scale * (logit - max))}; ptr null = not wanted
+    RowsArg stats;                 // [rows, 2] f32 {max of the logits, sum of exp(scale * (logit - max))}
     int top = 0;
     RowsArg top_ids, top_log_probs;
 };
@@ -65,6 +65,7 @@ struct AdamWRule {
     float eps, grad_scale;
     float minus_zero = -0.f;
 };
+AdamWRule adamw_rule(double lr, double beta1, double beta2, double eps, double weight_decay, double grad_scale, long long step);
 sage_status adamw_step(Context &ctx, const AdamWSlot *slots, int count, bool states8, const AdamWRule &rule);
 sage_status adamw_states(Context &ctx, const void *m, const float *m_scale, const void *v, const float *v_scale, long long n, float *m_out, float *v_out);
 

@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     const float c2 = a.scale * 1.4426950408889634f;
     float own = 0.f;
     bool scored = false;
-    if (rank == 0 && threadIdx.x == 0) {
+    if (rank == 0 && threadIdx.x == 0 && a.ids.ptr) {
         const int id = ((const int *)a.ids.ptr)[r * a.ids.stride];
         scored = id >= 0 && id < a.logits.cols;
         if (scored) own = widen(x[id]);
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     const float base = base_of(all.m), ln_s = logf(all.s);
     const bool none = all.s == 0.f;
     if (threadIdx.x == 0) {
-        ((float *)a.log_probs.ptr)[r * a.log_probs.stride] = !scored ? 0.f : none ? -INFINITY : (own - base) * a.scale - ln_s;
+        if (a.log_probs.ptr) ((float *)a.log_probs.ptr)[r * a.log_probs.stride] = !scored ? 0.f : none ? -INFINITY : (own - base) * a.scale - ln_s;
         if (a.entropy.ptr) ((float *)a.entropy.ptr)[r * a.entropy.stride] = none ? 0.f : ln_s - kLn2 * (all.w / all.s);
         if (a.stats.ptr) {
             ((float *)a.stats.ptr)[r * a.stats.pitch] = all.m;
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     if (TOP && (int)threadIdx.x < a.top) {
         const unsigned long long key = top.best[lane];
         ((int *)a.top_ids.ptr)[r * a.top_ids.pitch + lane] = (int)(0xffffffffu - (unsigned)key);
-        ((float *)a.top_log_probs.ptr)[r * a.top_log_probs.pitch + lane] = none ? -INFINITY : (rank_logit(key) - base) * a.scale - ln_s;
+        if (a.top_log_probs.ptr) ((float *)a.top_log_probs.ptr)[r * a.top_log_probs.pitch + lane] = none ? -INFINITY : (rank_logit(key) - base) * a.scale - ln_s;
     }
 }
 

@@ -3,7 +3,9 @@
 
 #include <cmath>
 
-#include "../kernels/kernels.h"
+#include <cuda_runtime.h>
+
+#include "../kernels/language.h"
 
 namespace sage {
 namespace nn {
@@ -147,6 +149,64 @@ sage_status Adam::update(const std::vector<Var> &params, const std::vector<Var> 
     if (st) return st;
     t += 1.0f;  // optim.rs:176
     return SAGE_OK;
+}
+
+AdamW::AdamW(double lr_, double beta1_, double beta2_, double eps_, double weight_decay_, int state_bits_)
+    : lr(lr_), beta1(beta1_), beta2(beta2_), eps(eps_), weight_decay(weight_decay_), state_bits(state_bits_) {
+    if (state_bits != 32 && state_bits != 8) shape_fail("AdamW: states have 32 or 8 bits");
+    if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0)) shape_fail("AdamW: beta1 and beta2 lie in [0, 1)");
+    if (!(eps >= 1e-15) || !std::isfinite((float)eps)) shape_fail("AdamW: eps is 1e-15 at least, and finite");
+    if (!std::isfinite((float)lr) || !std::isfinite((float)(lr * weight_decay))) shape_fail("AdamW: lr and weight_decay are finite");
+}
+
+sage_status AdamW::init(Session &) {
+    state.clear();
+    step = 0;
+    return SAGE_OK;
+}
+
+sage_status AdamW::update(const std::vector<Var> &params, const std::vector<Var> &grads, Session &s) {
+    Context &C = s.ctx();
+    Prepared prep;
+    sage_status st = prepare(params, grads, s, &prep);
+    if (st) return st;
+    const auto zeroed = [&](long long words, Tensor *t) -> sage_status {
+        sage_status e = Tensor::uninit(C, TensorDesc(Array{words}, SAGE_F32), t);
+        if (e) return e;
+        C.note_memset();
+        return C.dry() ? SAGE_OK : C.check_cuda(cudaMemsetAsync(t->ptr(), 0, (size_t)words * 4, C.stream()), "adamw: states");
+    };
+    std::vector<k::AdamWSlot> slots;
+    for (size_t i = 0; i < params.size(); ++i) {
+        const long long n = prep.slots[i].n;
+        auto it = state.find(params[i].key());
+        if (it == state.end()) {
+            States z;
+            z.param = params[i];
+            const long long words = state_bits == 8 ? (n + 3) / 4 : n, blocks = (n + k::kAdamWBlock - 1) / k::kAdamWBlock;
+            st = zeroed(words, &z.m);
+            if (!st) st = zeroed(words, &z.v);
+            if (!st && state_bits == 8) st = zeroed(blocks, &z.m_scale);
+            if (!st && state_bits == 8) st = zeroed(blocks, &z.v_scale);
+            if (st) return st;
+            it = state.emplace(params[i].key(), z).first;
+        }
+        if (prep.slots[i].hi) params[i].origin->data.data->split.reset();  // tf32 planes of the old values: whoever reads the parameter next makes them
+        k::AdamWSlot slot;
+        slot.p = prep.slots[i].p;
+        slot.g = prep.slots[i].g;
+        slot.n = n;
+        slot.m = it->second.m.ptr();
+        slot.v = it->second.v.ptr();
+        if (state_bits == 8) {
+            slot.m_scale = (float *)it->second.m_scale.ptr();
+            slot.v_scale = (float *)it->second.v_scale.ptr();
+        }
+        if (n) slots.push_back(slot);
+    }
+    st = k::adamw_step(C, slots.data(), (int)slots.size(), state_bits == 8, k::adamw_rule(lr, beta1, beta2, eps, weight_decay, 1.0, step + 1));
+    if (!st) ++step;
+    return st;
 }
 
 }  // namespace nn

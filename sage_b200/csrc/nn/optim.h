@@ -42,5 +42,20 @@ struct Adam : Optimizer {  // optim.rs:97-178
     sage_status update(const std::vector<Var> &params, const std::vector<Var> &grads, Session &s) override;
 };
 
+// AdamW (not in the reference): the rule of kernels/adamw.cu over all parameters in one launch, states by parameter.
+struct AdamW : Optimizer {
+    double lr, beta1, beta2, eps, weight_decay;
+    int state_bits;
+    long long step = 0;  // updates so far
+    struct States {
+        Var param;  // keeps the key alive
+        Tensor m, v, m_scale, v_scale;
+    };
+    std::unordered_map<Origin *, States> state;
+    AdamW(double lr, double beta1, double beta2, double eps, double weight_decay, int state_bits);
+    sage_status init(Session &s) override;
+    sage_status update(const std::vector<Var> &params, const std::vector<Var> &grads, Session &s) override;
+};
+
 }  // namespace nn
 }  // namespace sage

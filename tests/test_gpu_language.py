@@ -125,6 +125,28 @@ def test_embedding_grad(ctx, kind, add, tokens, vocab, dim, how):
         assert np.array_equal(first.view(np.uint32), d2.numpy().view(np.uint32))  # the same bits every time
 
 
+@pytest.mark.parametrize("tokens,vocab,dim,how,stride", [
+    (40000, 11, 8, "any", 1), (40000, 5, 8, "one", 1), (17001, 200003, 4, "often", 1), (20000, 700001, 4, "any", 1), (70001, 3001, 20, "often", 2), (16384, 129, 12, "any", 1),
+    (16385, 128, 12, "often", 1), (9000, 40, 2052, "often", 1), (300000, 1000, 4, "often", 1)])
+def test_embedding_grad_of_long_batches(ctx, tokens, vocab, dim, how, stride):
+    """Sorting by one launch and by two, lists that overflow, rows that many blocks share, tables of more rows than a block counts."""
+    rng = np.random.default_rng(tokens)
+    ids = {"any": lambda: rng.integers(-1, vocab + 1, tokens), "one": lambda: np.full(tokens, vocab // 2),
+           "often": lambda: np.minimum(np.exp(rng.uniform(0, np.log(vocab + 1), tokens)).astype(np.int64) - 1, vocab - 1)}[how]().astype(np.int32)
+    with Held(ctx) as h:
+        g, val = h.rows(rng.standard_normal((tokens, dim)), "f32")
+        for add in (False, True):
+            start = np.full((vocab, dim), 0.25, np.float32)
+            d, i = h.put(start), h.vec(ids, stride)
+            L.embedding_grad(g, i, d, add=add)
+            want, bound = O.embedding_grad(val, ids, vocab, 1.0, start if add else None)
+            got = d.numpy()
+            close(got, want, bound)
+            d2 = h.put(start)
+            L.embedding_grad(g, i, d2, add=add)
+            assert np.array_equal(got.view(np.uint32), d2.numpy().view(np.uint32))
+
+
 @pytest.mark.parametrize("dim,pitch,lead,ld", [(64, 72, 8, 64), (50, 53, 1, 57), (129, 129, 0, 130), (8, 8, 4, 8)])
 def test_embedding_grad_of_views(ctx, dim, pitch, lead, ld):
     rng = np.random.default_rng(dim)
@@ -245,6 +267,52 @@ def test_token_log_probs(ctx, kind, mask, rows, vocab):
         lp2 = h.empty((rows,))
         L.token_log_probs(x, h.vec(ids), lp2, scale=scale)
         assert np.array_equal(lp.numpy().view(np.uint32), lp2.numpy().view(np.uint32))
+
+
+@pytest.mark.parametrize("kind,rows,vocab,top", [("f32", 2400, 5003, 5), ("bf16", 2500, 20000, 32), ("bf16", 2400, 40001, 3), ("f32", 100, 40003, 20), ("f16", 90, 70000, 0), ("f32", 700, 9001, 7),
+                                                 ("bf16", 74, 20001, 9), ("bf16", 20, 262144, 32)])
+@pytest.mark.parametrize("mask", ["", "inf", "ties", "few", "empty", "equal"])
+def test_token_log_probs_of_many_rows(ctx, kind, rows, vocab, top, mask):
+    """Blocks of every size, a row to each or several to a row; on top of the values of a few rows, all rows' tops and sums."""
+    rng = np.random.default_rng(rows)
+    base = logits_for(rng, 8, vocab, mask)
+    at = rng.integers(0, 8, rows)
+    with Held(ctx) as h:
+        raw, val = O.stored(base, kind)
+        x = h.put(raw[at], KIND[kind])
+        ids = rng.integers(-1, vocab + 1, rows).astype(np.int32)
+        lp, en, ti, tl = h.empty((rows,)), h.empty((rows,)), h.empty((rows, top), S.I32), h.empty((rows, top))
+        L.token_log_probs(x, h.vec(ids), lp, en, top_ids=ti, top_log_probs=tl)
+        eight = O.LogProbs(val, np.zeros(8, np.int64), 1.0)
+        ok = (ids >= 0) & (ids < vocab)
+        close(lp.numpy(), np.where(ok, eight.log_p[at, np.where(ok, ids, 0)], 0.0), eight.tol_log_p[at, np.where(ok, ids, 0)])
+        close(en.numpy(), eight.entropy[at], eight.tol_entropy[at])
+        if top:
+            tops, probs, bound = eight.top(top)
+            assert np.array_equal(ti.numpy(), tops[at])
+            close(tl.numpy(), probs[at], bound[at])
+
+
+@pytest.mark.parametrize("kind,rows,vocab", [("f32", 300, 5000), ("bf16", 1200, 9001), ("f16", 40, 50021), ("bf16", 300, 131072), ("f32", 9, 131075), ("bf16", 9, 262137), ("f32", 9, 140000), ("bf16", 700, 16400)])
+def test_gradient_of_many_rows(ctx, kind, rows, vocab):
+    """Rows in the registers of clusters of every size, and rows that no cluster holds."""
+    rng = np.random.default_rng(rows + vocab)
+    base = logits_for(rng, 4, vocab, "inf")
+    at = rng.integers(0, 4, rows)
+    with Held(ctx) as h:
+        raw, val = O.stored(base, kind)
+        x = h.put(raw[at], KIND[kind])
+        own = rng.integers(0, vocab, 4).astype(np.int32)
+        ids, gl, ge = own[at], np.array([0.5, -1.0, 0.25, 2.0], np.float32), np.array([0.1, 0.0, -0.3, 1.0], np.float32)
+        lp, en, dx = h.empty((rows,)), h.empty((rows,)), h.empty((rows, vocab), KIND[kind])
+        L.token_log_probs_and_grad(x, h.put(ids), h.put(gl[at]), h.put(ge[at]), lp, en, dx)
+        want = O.LogProbs(val, own, 1.0)
+        g, bound = want.grad(gl, ge, kind)
+        close(lp.numpy(), want.log_probs[at], want.tol_log_probs[at])
+        close(en.numpy(), want.entropy[at], want.tol_entropy[at])
+        got = O.values(dx.numpy(), kind)
+        for i in range(rows):  # rows of an odd length start at different places of a vector, so equal rows may differ in their last bits
+            close(got[i], g[at[i]], bound[at[i]])
 
 
 @pytest.mark.parametrize("top", range(1, 33))

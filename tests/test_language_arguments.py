@@ -152,3 +152,43 @@ def test_wrapped_memory_is_not_freed(ctx):
     assert ctx.mem_stats()["mem_used"] == used
     with pytest.raises(S.SageError):
         ctx.wrap(0, (4,))
+
+
+# ------------------------------------------------------------------------------------------ the lazy graph
+def test_graph_shapes_and_launches(ctx):
+    table, ids = ctx.var(np.zeros((10, 8), np.float32)), ctx.var(np.zeros((2, 3), np.uint32))
+    y = S.embedding(table, ids, 2.0)
+    assert y.extents == (2, 3, 8)
+    logits = S.view(y, [6, 8]).matmul(table.tr())
+    lp, h = S.token_log_probs(logits, ctx.var(np.zeros(6, np.int32)))
+    assert lp.extents == (6,) and h.extents == (6,)
+    top = S.top_tokens(logits, 3)
+    assert top.extents == (6, 3) and top.dtype == S.U32
+    loss = -(lp.mean([0]) + h.mean([0]) * 0.1)
+    ctx.trace_begin()
+    ctx.eval(loss, top, table.grad(loss))
+    names = ctx.trace()
+    for name in ("embedding", "token_log_probs", "token_log_probs_grad", "embedding_sort", "embedding_grad"):
+        assert name in names, names
+    opt = S.AdamW(1e-3, state_bits=8)
+    opt.init(ctx)
+    ctx.trace_begin()
+    opt.update({table: ctx.var(np.zeros((10, 8), np.float32))}, ctx)
+    assert "adamw_step" in ctx.trace()
+
+
+def test_graph_refusals(ctx):
+    table, ids = ctx.var(np.zeros((10, 8), np.float32)), ctx.var(np.zeros((6,), np.uint32))
+    f = ctx.var(np.zeros((6,), np.float32))
+    for call in (lambda: S.embedding(table, f), lambda: S.embedding(f, ids), lambda: S.token_log_probs(table, ids), lambda: S.token_log_probs(f, ids),
+                 lambda: S.token_log_probs(ctx.var(np.zeros((6, 8), np.float32)), f), lambda: S.token_log_probs(ctx.var(np.zeros((6, 8), np.float32)), ids, 0.0),
+                 lambda: S.top_tokens(table, 0), lambda: S.top_tokens(table, 9), lambda: S.top_tokens(f, 1),
+                 lambda: S.AdamW(1e-3, state_bits=16), lambda: S.AdamW(1e-3, beta1=1.0), lambda: S.AdamW(1e-3, eps=0.0), lambda: S.AdamW(float("nan"))):
+        with pytest.raises(S.SageError) as e:
+            call()
+        assert e.value.code == 1
+    lp, _ = S.token_log_probs(ctx.var(np.zeros((6, 8), np.float32)), ids)
+    x = ctx.var(np.zeros((6, 8), np.float32))
+    lp, _ = S.token_log_probs(x, ids)
+    with pytest.raises(S.SageError):
+        x.grad(x.grad(lp.sum(None)).sum(None))  # differentiated once
