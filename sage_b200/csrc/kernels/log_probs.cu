@@ -310,9 +310,9 @@ __device__ void block_top(const RowVectors<T> &row, int begin, int end, float th
     if (mine >= bound) sh.chosen[atomicAdd(&sh.sets, 1)] = (unsigned short)threadIdx.x;  // in any order: keys decide
     __syncthreads();
     const int sets = sh.sets;
-    // Vectors first, first + step ... in front of `end`, a vector to a lane; f(key, is it one)
-    auto each = [&](int first, int lane_step, int step, auto f) {
-        for (int base = first, i = first + lane * lane_step; base < end; base += step, i += step) {
+    // The warp's vectors i, i + step ... in front of `end`, each lane its own: f(key, is it one)
+    auto each = [&](int i, int step, auto f) {
+        for (; __any_sync(0xffffffffu, i < end); i += step) {
             const bool some = i < end;
             const uint4 v = some ? row.load(i) : RowVectors<T>::nothing();
             float2 x[N / 2];
@@ -330,19 +330,24 @@ __device__ void block_top(const RowVectors<T> &row, int begin, int end, float th
         }
     };
     const bool few = sets <= THREADS / 4;
-    if (few)
-        for (int q = warp; q < sets; q += W)
-            each(begin + sh.chosen[q], THREADS, 32 * THREADS, [&](unsigned long long key, bool in) {
+    if (few) {
+        int lanes = 32;  // to a thread's vectors: as many as it has, and the other lanes to other threads'
+        while (lanes > 1 && lanes / 2 * THREADS >= end - begin) lanes /= 2;
+        for (int q0 = 0; q0 < sets; q0 += W * (32 / lanes)) {
+            const int q = q0 + lane / lanes * W + warp;
+            each(q < sets ? begin + sh.chosen[q] + lane % lanes * THREADS : end, lanes * THREADS, [&](unsigned long long key, bool in) {
                 if (!in) return;
                 const int at = atomicAdd(&sh.found, 1);
                 if (at < kCandidates) sh.candidates[at] = key;
             });
+        }
+    }
     __syncthreads();
     if (few && sh.found <= kCandidates) {
         sort_by_rank(sh.candidates, sh.found, k, sh.best);
     } else {
         TopList list;
-        each(begin + warp * 32, 1, THREADS, [&](unsigned long long key, bool in) { list.offer(key, in, k); });
+        each(own, THREADS, [&](unsigned long long key, bool in) { list.offer(key, in, k); });
         sh.lists[warp][lane] = lane < k ? list.key : 0;
         __syncthreads();
         if (warp == 0) {
