@@ -29,14 +29,24 @@ struct Batch {
 };
 constexpr int kSlots = 400, kFewSlots = 40;  // 32 KB of kernel parameters, 3 KB
 
-__device__ __forceinline__ float fast_root(float x) {  // 2^-22 off at most, of subnormal numbers 0
+__device__ __forceinline__ float fast_root(float x) {  // 2^-23 off at most, of subnormal numbers 0
     float y;
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float largest(float a, float b) {  // NaN wins
+__device__ __forceinline__ float largest(float a, float b, float c) {  // NaN wins
     float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ float fast_reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float one_if_positive(float x) {
+    float y;
+    asm("set.gt.f32.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float warp_largest(float x) {
@@ -58,10 +68,11 @@ __device__ __forceinline__ float block_scale(float x, float *factor) {
 // whole number in the low bits.  `off` is the furthest that a root lies from its code: where that is within the approximation's error of
 // one half, another code might be nearer, and the caller takes the exact root.
 constexpr float kMagic = 12582912.f;
-__device__ __forceinline__ unsigned rounded(float root, float *off) {
-    const float n = __fadd_rn(root, kMagic);
-    *off = fmaxf(*off, fabsf(__fadd_rn(root, -__fadd_rn(n, -kMagic))));
-    return __float_as_uint(n);
+__device__ __forceinline__ void rounded(float2 root, float *off, unsigned *n) {
+    const float2 m = add2(root, both(kMagic)), d = add2(root, add2(both(kMagic), make_float2(-m.x, -m.y)));
+    *off = fmaxf(*off, fmaxf(fabsf(d.x), fabsf(d.y)));
+    n[0] = __float_as_uint(m.x);
+    n[1] = __float_as_uint(m.y);
 }
 __device__ __forceinline__ unsigned low_bytes(const unsigned *n) { return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410); }
 
@@ -79,7 +90,7 @@ __device__ __forceinline__ void update(const AdamWRule &k, Elements &e) {
         e.v[i] = add2(fma2(e.v[i], both(k.beta2), zero), fma2(mul2(g, g), both(k.one_minus_beta2), zero));
         e.root[i] = make_float2(fast_root(e.v[i].x), fast_root(e.v[i].y));
         const float2 below = fma2(e.root[i], both(k.root_factor), both(k.eps)), step = mul2(e.m[i], both(-k.step_size));
-        e.p[i] = fma2(e.p[i], both(k.keep), make_float2(__fdividef(step.x, below.x), __fdividef(step.y, below.y)));
+        e.p[i] = fma2(e.p[i], both(k.keep), mul2(step, make_float2(fast_reciprocal(below.x), fast_reciprocal(below.y))));
     }
 }
 __device__ __forceinline__ float &at(float2 *x, int i) { return i % 2 ? x[i / 2].y : x[i / 2].x; }
@@ -151,6 +162,10 @@ __device__ __forceinline__ void load_raw(const AdamWSlot &s, long long block, Ra
     r.vs = s.v_scale[block];
 }
 __device__ __forceinline__ float2 two(unsigned a, unsigned b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+// Bytes 2 j and 2 j + 1 of a word: behind the exponent of 2^23 they count from there.
+__device__ __forceinline__ float2 codes_of(unsigned word, int j, float zero) {
+    return add2(two(__byte_perm(word, 0x4b000000u, 0x7440 + 2 * j), __byte_perm(word, 0x4b000000u, 0x7441 + 2 * j)), both(-zero));
+}
 __device__ __forceinline__ void elements_of(const Raw &r, int g_dtype, Elements &e) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -166,10 +181,10 @@ __device__ __forceinline__ void elements_of(const Raw &r, int g_dtype, Elements 
             e.g[2 * h + 1] = __half22float2(*reinterpret_cast<const __half2 *>(&r.g[h].y));
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float c = (float)(signed char)(r.m[h] >> (8 * j));
-            at(e.m, 4 * h + j) = __fmul_rn(r.ms, c * fabsf(c));
-            at(e.v, 4 * h + j) = (float)(unsigned char)(r.v[h] >> (8 * j));
+        for (int j = 0; j < 2; ++j) {
+            const float2 c = codes_of(r.m[h] ^ 0x80808080u, j, 8388608.f + 128.f);
+            e.m[2 * h + j] = mul2(make_float2(c.x * fabsf(c.x), c.y * fabsf(c.y)), both(r.ms));
+            e.v[2 * h + j] = codes_of(r.v[h], j, 8388608.f);
         }
     }
 #pragma unroll
@@ -225,9 +240,9 @@ __device__ __forceinline__ void block_update(const AdamWSlot &s, const AdamWRule
     }
     float m_top = 0.f, v_top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        m_top = largest(m_top, fabsf(at(e.m, i)));
-        v_top = largest(v_top, at(e.v, i));
+    for (int i = 0; i < 4; ++i) {
+        m_top = largest(m_top, fabsf(e.m[i].x), fabsf(e.m[i].y));
+        v_top = largest(v_top, e.v[i].x, e.v[i].y);
     }
     m_top = warp_largest(m_top);
     v_top = __fsqrt_rn(warp_largest(v_top));
@@ -240,30 +255,36 @@ __device__ __forceinline__ void block_update(const AdamWSlot &s, const AdamWRule
     unsigned m[8], v[8];
     float m_off = 0.f, v_off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        m[i] = rounded(copysignf(fast_root(__fmul_rn(fabsf(at(e.m, i)), mf)), at(e.m, i)), &m_off);
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = mul2(make_float2(fabsf(e.m[i].x), fabsf(e.m[i].y)), both(mf)), u = mul2(e.root[i], both(vf));
+        rounded(make_float2(copysignf(fast_root(t.x), e.m[i].x), copysignf(fast_root(t.y), e.m[i].y)), &m_off, m + 2 * i);
         // one at least for what is not zero
-        v[i] = rounded(fmaxf(fast_root(__fmul_rn(at(e.root, i), vf)), at(e.v, i) > 0.f ? 0.75f : 0.f), &v_off);
+        rounded(make_float2(fmaxf(fast_root(u.x), one_if_positive(e.v[i].x)), fmaxf(fast_root(u.y), one_if_positive(e.v[i].y))), &v_off, v + 2 * i);
     }
-    // Two fast roots of up to 255 err by 2^-13 at most, one of up to 127 by 2^-15.  Where all of a block's v lie below 2^-80, subnormal ones count, which
-    // the fast root takes for zero.
-    if (m_off > 0.5f - 0x1p-14f || v_off > 0.5f - 0x1.8p-13f || v_top < 0x1p-40f) {
+    // A fast root is 2^-23 off at most: of up to 127 less than kMOff, two after another of up to 255 less than kVOff.  Where all of a block's v
+    // lie below 2^-80, subnormal ones count, which the fast root takes for zero.
+    constexpr float kMOff = 2.2e-5f, kVOff = 0x1p-14f;
+    if (m_off > 0.5f - kMOff || v_off > 0.5f - kVOff || v_top < 0x1p-40f) {
         float none = 0.f;
 #pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-            float x = at(e.m, 0), y = at(e.v, 0);
+        for (int i = 0; i < 4; ++i) {
+            float2 x = e.m[0], y = e.v[0];
 #pragma unroll
-            for (int j = 1; j < 8; ++j)
+            for (int j = 1; j < 4; ++j)
                 if (j == i) {
-                    x = at(e.m, j);
-                    y = at(e.v, j);
+                    x = e.m[j];
+                    y = e.v[j];
                 }
-            const unsigned c = rounded(copysignf(__fsqrt_rn(__fmul_rn(fabsf(x), mf)), x), &none), d = rounded(fmaxf(__fsqrt_rn(__fmul_rn(__fsqrt_rn(y), vf)), y > 0.f ? 0.75f : 0.f), &none);
+            unsigned c[2], d[2];
+            rounded(make_float2(copysignf(__fsqrt_rn(__fmul_rn(fabsf(x.x), mf)), x.x), copysignf(__fsqrt_rn(__fmul_rn(fabsf(x.y), mf)), x.y)), &none, c);
+            rounded(make_float2(fmaxf(__fsqrt_rn(__fmul_rn(__fsqrt_rn(y.x), vf)), one_if_positive(y.x)), fmaxf(__fsqrt_rn(__fmul_rn(__fsqrt_rn(y.y), vf)), one_if_positive(y.y))), &none, d);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 4; ++j)
                 if (j == i) {
-                    m[j] = c;
-                    v[j] = d;
+                    m[2 * j] = c[0];
+                    m[2 * j + 1] = c[1];
+                    v[2 * j] = d[0];
+                    v[2 * j + 1] = d[1];
                 }
         }
     }
