@@ -272,7 +272,7 @@ sage_status sage_conv2d_nhwc(sage_ctx *ctx, const sage_tensor *x, const sage_ten
  *
  * Operands are views (buffer, extents, strides, offset) that must lie inside their buffers; rows ([.., D] and [.., V]) are
  * contiguous along the last axis with any distance between rows that keeps them apart (inputs: any that is not negative), vectors
- * may have any stride (inputs: also 0, a broadcast value).  Outputs may not share memory with an operand unless it says so.
+ * may have any stride (inputs: also 0, a broadcast value).  No more than 2^31 - 2^16 rows or columns.  Outputs may not share memory with an operand unless it says so.
  * Calls with no rows return at once.  All sums are held in 32 bits in a fixed order: the same inputs, as far from 16-byte boundaries,
  * give the same bits. */
 
@@ -280,7 +280,8 @@ sage_status sage_conv2d_nhwc(sage_ctx *ctx, const sage_tensor *x, const sage_ten
  * outside [0, V) stands for no token: its row is zeros. */
 sage_status sage_embedding(sage_ctx *ctx, const sage_tensor *table, const sage_tensor *ids, float scale, const sage_tensor *y);
 /* Its gradient: dtable[v, :] = scale * (sum of g[t, :] over the tokens t with ids[t] = v), rows without a token zero; with `add`
- * the sums are added to what dtable holds.  g [T, D] f32 / f16 / bf16, dtable [V, D] f32. */
+ * the sums are added to what dtable holds, as the memory's atomic unit adds (results below 2^-126 in size become zero).  g [T, D] f32 /
+ * f16 / bf16, dtable [V, D] f32. */
 sage_status sage_embedding_grad(sage_ctx *ctx, const sage_tensor *g, const sage_tensor *ids, float scale, int32_t add, const sage_tensor *dtable);
 
 /* Over each row x = scale * logits[r, :] (logits [R, V] f32 / f16 / bf16, scale > 0, an inverse temperature):
@@ -309,7 +310,7 @@ sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logi
  *   param = param (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
  * param f32, grad f32 / f16 / bf16, contiguous, of the same number of elements.  The states m, v are f32 (m_scale, v_scale
  * unused, buf NULL), or m i8 and v u8 with f32 scales, one for each 256 elements of the tensor: |m| = m_scale code^2, sqrt(v) =
- * v_scale code^2; zeroed codes and scales are zero states.  A second moment that is not zero does not become zero; a block in which a
+ * v_scale code^2; zeroed codes and scales are zero states.  No tensor may appear twice in a call.  A second moment that is not zero does not become zero; a block in which a
  * moment is not finite has a scale that is NaN.  `copy` (buf NULL: none) receives the updated parameters in f16 / bf16.  States of all
  * tensors of a call have the same width.  step counts from 1; eps is 1e-15 at least. */
 typedef struct {

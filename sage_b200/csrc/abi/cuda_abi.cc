@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <cstring>
+#include <new>
 
 #include "../codegen/map_emit.h"
 #include "../kernels/kernels.h"
@@ -163,8 +164,8 @@ sage_status sage_buf_wrap(sage_ctx *ctx, void *device_ptr, size_t bytes, sage_bu
         if (!(a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged) || a.device != C.device())
             return C.fail(SAGE_ERR_INVALID, "buf_wrap: not memory of this context's device");
     }
-    *buf = new sage_buf{nullptr, device_ptr, bytes, &C};
-    return SAGE_OK;
+    *buf = new (std::nothrow) sage_buf{nullptr, device_ptr, bytes, &C};
+    return *buf ? SAGE_OK : C.fail(SAGE_ERR_OOM, "buf_wrap: out of host memory");
 }
 
 sage_status sage_last_oom(sage_ctx *ctx, uint64_t *needed, uint64_t *total) {
@@ -483,6 +484,7 @@ sage_status sage_pool2d(sage_ctx *ctx, int32_t is_max, const sage_tensor *x, con
 sage_status sage_ipc_export(sage_ctx *ctx, sage_buf *buf, uint8_t handle[64], uint64_t *offset) {
     CTX_OR_FAIL(ctx);
     if (C.dry()) return C.fail(SAGE_ERR_NO_DEVICE, "ipc on a planning context");
+    if (!buf->block) return C.fail(SAGE_ERR_INVALID, "ipc_export: memory that the caller owns");
     static_assert(sizeof(cudaIpcMemHandle_t) == 64, "handle size");
     cudaIpcMemHandle_t h;
     void *base = buf->block ? buf->block->segment : buf->ptr;

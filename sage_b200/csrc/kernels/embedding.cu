@@ -601,7 +601,8 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
                                 "embedding_deal");
     }
     ctx.note_launch("embedding_sort");
-    ctx.note_launch("embedding_grad");
+    const long long blocks = chunks * slices + zero_blocks;  // none: no tokens, and all of the table cleared early
+    if (blocks) ctx.note_launch("embedding_grad");
     if (!ctx.dry() && !st) {
         const auto sort = deal ? embedding_sort_kernel<kDealt> : ids.stride == 1 && reinterpret_cast<uintptr_t>(ids.ptr) % 16 == 0 ? embedding_sort_kernel<kQuads> : embedding_sort_kernel<kStrided>;
         st = ctx.check_cuda(cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortRows + 2 * kSortList) * kSortWarps * 4), "embedding_sort");
@@ -609,12 +610,12 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
             st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), sort, dim3((1u << bits) + (unsigned)((early_rows + warps - 1) / warps)), dim3(warps * 32), smem, source, bits, (int2 *)a.spans, (int *)a.total, (int *)a.order, (int *)a.sorted,
                                                  a.arrived, (int)counters, a.table, (int)late_rows),
                                 "embedding_sort");
-        if (!st)
+        if (!st && blocks)
             st = with_type(g.dtype, [&](auto t) {
                 typedef decltype(t) T;
                 const size_t smem_ahead = wide ? kAhead * threads * sizeof(Four<T>) : 0;  // 32 KB at most
                 return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? embedding_grad_kernel<T, true> : embedding_grad_kernel<T, false>,
-                                                       dim3((unsigned)(chunks * slices + zero_blocks)), dim3((unsigned)threads), smem_ahead, a),
+                                                       dim3((unsigned)blocks), dim3((unsigned)threads), smem_ahead, a),
                                       "embedding_grad");
             });
     }

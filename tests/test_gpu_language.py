@@ -147,6 +147,24 @@ def test_embedding_grad_of_long_batches(ctx, tokens, vocab, dim, how, stride):
             assert np.array_equal(got.view(np.uint32), d2.numpy().view(np.uint32))
 
 
+@pytest.mark.parametrize("vocab,dim", [(1, 1), (7, 12), (9000, 768)])
+def test_no_tokens(ctx, vocab, dim):
+    """A gradient of nothing is zeros, or leaves what is there; calls without rows do nothing."""
+    with Held(ctx) as h:
+        g, ids, d = h.empty((0, dim), S.BF16), h.empty((0,), S.I32), h.put(np.full((vocab, dim), 2.0, np.float32))
+        L.embedding_grad(g, ids, d, add=True)
+        assert (d.numpy() == 2.0).all()
+        L.embedding_grad(g, ids, d)
+        assert (d.numpy() == 0.0).all()
+        L.embedding(d, ids, h.empty((0, dim)))
+        L.embedding(h.empty((0, dim)), h.put(np.array([0, 1], np.int32)), y := h.empty((2, dim)))
+        assert (y.numpy() == 0.0).all()
+        x, f = h.empty((0, dim), S.F16), h.empty((0,))
+        L.token_log_probs(x, ids, f, f, stats=h.empty((0, 2)), top_ids=h.empty((0, 1), S.I32), top_log_probs=h.empty((0, 1)))
+        L.token_log_probs_grad(x, ids, h.empty((0, 2)), f, f, f, x)
+        L.token_log_probs_and_grad(x, ids, f, f, f, f, x)
+
+
 @pytest.mark.parametrize("dim,pitch,lead,ld", [(64, 72, 8, 64), (50, 53, 1, 57), (129, 129, 0, 130), (8, 8, 4, 8)])
 def test_embedding_grad_of_views(ctx, dim, pitch, lead, ld):
     rng = np.random.default_rng(dim)
