@@ -439,14 +439,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
 struct GradRow {
     float base, c2, slope, level, at_id;
     int id;
-    __device__ void set(float m, float s, float scale, float gl, float ge, float entropy, int id_) {
+    __device__ void set(float m, float s, float ln_s, float scale, float gl, float ge, float entropy, int id_) {
         base = base_of(m);
         c2 = scale * 1.4426950408889634f;
         id = id_;
         if (s == 0.f) gl = ge = 0.f;  // masked throughout
         const float share = s == 0.f ? 0.f : scale / s;
         slope = -share * (ge * kLn2);
-        level = -share * (ge != 0.f ? gl + ge * (entropy - logf(s)) : gl);  // NaN where s is: so is every gradient
+        level = -share * (ge != 0.f ? gl + ge * (entropy - ln_s) : gl);  // NaN where s is: so is every gradient
         at_id = scale * gl;
     }
     // The gradients at one vector's logits, in the logits' type; `own`: the token's place in the vector, if it is there.
@@ -525,17 +525,24 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
     const float *stats = (const float *)a.stats.ptr + r * a.stats.pitch;
     const int id = token_of(a, r);
     GradRow g;
-    g.set(stats[0], stats[1], a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), at_row(a.entropy, r), id);
+    g.set(stats[0], stats[1], logf(stats[1]), a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), at_row(a.entropy, r), id);
     const bool same = same_grid(x, dx);
     store_all<T, U, 256>(row, g, dx, same, v, i, row.count);
 }
 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
-// gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.
+// gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.  Bound by memory and by the joins
+// that each row waits for between its loads and its stores (8192 x 131072 bf16: 875 us, 4.9 TB/s; without the joins it would be
+// 657), so nothing else is left to be waited for there: what the row is asked about is fetched beside its logits (8192 x 50021
+// bf16: 384 us with those loads behind the join, 369 beside; 4096 x 131072 f32: 865 and 818).
 template <class T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int parts, const int each) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_kernel(const LogProbsGrad a, const VectorArg log_probs, const VectorArg entropy, const int parts, const int each) {
     __shared__ Sums sums[THREADS / 32], part_sums[kMaxCluster];
     __shared__ GradRow constants;
+    __shared__ struct {
+        int id;
+        float g_log_prob, g_entropy, own;
+    } asked;
     grid_dependency_sync();
     if (parts > 1) cluster_arrive_relaxed();
     const long long r = cluster_number();
@@ -545,19 +552,30 @@ __global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREA
     const RowVectors<T> row(x, a.logits.cols);
     const int begin = min((int)rank * each, row.count), end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
     const float c2 = a.scale * 1.4426950408889634f;
+    // What the row is asked about, fetched by the last thread while the logits are under way.
+    const bool asks = threadIdx.x == THREADS - 1;
+    int id = -1;
+    float g_log_prob = 0.f, g_entropy = 0.f, own = 0.f;
+    if (asks) {
+        id = ((const int *)a.ids.ptr)[r * a.ids.stride];
+        g_log_prob = at_row(a.g_log_probs, r);
+        g_entropy = at_row(a.g_entropy, r);
+    }
     uint4 v[NV];
     row.template load_all<NV, THREADS>(v, i, end);
+    if (asks && id >= 0 && id < a.logits.cols) own = widen(x[id]);
     Sums all;
     add_vectors<T, NV>(all, v, c2, (end - begin + THREADS - 1) / THREADS);
+    if (asks) {
+        const bool scored = id >= 0 && id < a.logits.cols;
+        asked.id = scored ? id : -1;
+        asked.g_log_prob = scored ? g_log_prob : 0.f;
+        asked.g_entropy = g_entropy;
+        asked.own = own;
+    }
 #pragma unroll
     for (int u = 0; u < NV; ++u) asm volatile("" : "+r"(v[u].x), "+r"(v[u].y), "+r"(v[u].z), "+r"(v[u].w));  // as loaded: unpacked twice rather than kept unpacked
     all = block_join<THREADS>(all, c2, sums);
-    int id = -1;
-    float own = 0.f;
-    if (threadIdx.x == 0) {
-        id = token_of(a, r);
-        if (rank == 0 && id >= 0) own = widen(x[id]);
-    }
     if (parts > 1) {
         cluster_wait();
         if ((int)threadIdx.x < parts) {
@@ -566,7 +584,7 @@ __global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREA
             peer_store(to + 4, all.s);
             peer_store(to + 8, all.w);
         }
-        // Behind the token's own logit too: from here on results may take the logits' place.
+        // Behind the token's own logit too, which was read in front of the block's join: from here on results may take the logits' place.
         if (threadIdx.x < 32) cluster_arrive();
         else cluster_arrive_relaxed();
         cluster_wait();
@@ -574,15 +592,14 @@ __global__ void __launch_bounds__(THREADS, NV > 8 ? 640 / THREADS : 1024 / THREA
     if (threadIdx.x < 32) {  // the row's constants once; a thread's other work is 64 elements
         const int lane = threadIdx.x;
         if (parts > 1) all = warp_join(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
+        const float ln_s = logf(all.s);
+        const bool none = all.s == 0.f;
+        const float h = none ? 0.f : ln_s - kLn2 * (all.w / all.s);
         if (lane == 0) {
-            const float ln_s = logf(all.s);
-            const bool none = all.s == 0.f;
-            const float h = none ? 0.f : ln_s - kLn2 * (all.w / all.s);
-            constants.set(all.m, all.s, a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), h, id);
-            if (rank == 0) {
-                ((float *)log_probs.ptr)[r * log_probs.stride] = id < 0 ? 0.f : none ? -INFINITY : (own - base_of(all.m)) * a.scale - ln_s;
-                if (entropy.ptr) ((float *)entropy.ptr)[r * entropy.stride] = h;
-            }
+            constants.set(all.m, all.s, ln_s, a.scale, asked.g_log_prob, asked.g_entropy, h, asked.id);
+        } else if (lane == 1 && rank == 0) {
+            ((float *)log_probs.ptr)[r * log_probs.stride] = asked.id < 0 ? 0.f : none ? -INFINITY : (asked.own - base_of(all.m)) * a.scale - ln_s;
+            if (entropy.ptr) ((float *)entropy.ptr)[r * entropy.stride] = h;
         }
     }
     __syncthreads();
