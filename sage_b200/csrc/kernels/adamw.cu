@@ -6,8 +6,9 @@
 // Codes and scales are those of the moments as f32 rounds them operation by operation, whatever shortcuts find them: the fast square
 // root decides a code unless its result lies so near the middle of two codes that it could err, where the exact one does.
 //
-// A warp takes a block of 256 elements at a time, eight to a lane.  Bound by memory: 28 bytes an element with f32 states and gradients,
-// 16 with 8-bit states and f32 gradients.
+// A warp takes a block of 256 elements at a time, eight to a lane.  Bound by memory: 28 bytes an element with f32 states and gradients (109 M:
+// 480 us, 6.4 TB/s), 16 with 8-bit states, bf16 gradients and a copy (334 M: 941 us, 5.7 TB/s, the instructions that find the codes at 64 %
+// of their slots beside it).
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(256, STATES8 ? 3 : 4) adamw_kernel(const __gri
     }
 }
 
-// Values of codes: four to a thread where `wide`, else one.
+// Values of codes: four to a thread where `wide`, else one.  Bound by memory: 2 bytes read, 8 written (334 M: 586 us, 5.7 TB/s).
 template <bool WIDE>
 __global__ void __launch_bounds__(256) adamw_states_kernel(const signed char *m, const float *m_scale, const unsigned char *v, const float *v_scale, long long n, float *m_out, float *v_out) {
     grid_dependency_sync();
