@@ -177,25 +177,30 @@ __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float 
     a.s = s.x + s.y;
     a.w = w.x + w.y;
 }
-// Of the warp's lanes, in all of them: the largest m first, then sums relative to it.
+// Of the warp's lanes: the largest m first, then sums relative to it.  In all lanes; or, where those behind the first LANES have nothing, in
+// these (8192 x 131072 bf16 with its gradient: 876 us with 32 everywhere, 861 with as many as there are warps and CTAs).
+template <int LANES = 32>
 __device__ __forceinline__ Sums warp_join(Sums a, float c2) {
     float m;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(a.m));
     move_to(a, m, c2);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
+    for (int o = LANES / 2; o; o >>= 1) {
         a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
         a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
     }
     return a;
 }
-// Of all threads, in warp 0.  `shared`: one for each warp.
+// Of all threads, in warp 0 (its first LANES lanes).  `shared`: one for each warp.
+constexpr int kMaxCluster = 8;  // CTAs that share a row
 template <int THREADS>
+constexpr int kJoinLanes = THREADS / 32 < kMaxCluster ? kMaxCluster : THREADS / 32;  // for each warp, and one to send to each CTA
+template <int THREADS, int LANES>
 __device__ __forceinline__ Sums block_join(Sums a, float c2, Sums *shared) {
     a = warp_join(a, c2);
     if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = a;
     __syncthreads();
-    return threadIdx.x < 32 ? warp_join((int)threadIdx.x < THREADS / 32 ? shared[threadIdx.x] : Sums(), c2) : a;
+    return threadIdx.x < 32 ? warp_join<LANES>((int)threadIdx.x < THREADS / 32 ? shared[threadIdx.x] : Sums(), c2) : a;
 }
 
 // ------------------------------------------------------------------------------------------ clusters: CTAs that share a row
@@ -359,8 +364,6 @@ __device__ void block_top(const RowVectors<T> &row, int begin, int end, float th
 }
 
 // ------------------------------------------------------------------------------------------ values
-constexpr int kMaxCluster = 8;
-
 // A cluster of 2^shift CTAs for each row; each reads a part of it once, and the running maximum and sums are joined over lanes, warps and CTAs.
 // Bound by memory in many rows (8192 x 50021 f32: 259 us, 6.3 TB/s), by the chain of joins in few (1 x 30522: 6 us with 5 alternatives).
 template <class T, int THREADS, bool TOP>
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
         add_vectors<T, U>(mine, v, c2);
     }
     const float thread_max = mine.m;
-    Sums all = block_join<THREADS>(mine, c2, sums);
+    Sums all = block_join<THREADS, TOP ? 32 : kJoinLanes<THREADS>>(mine, c2, sums);
     if constexpr (TOP) block_top<T, THREADS>(row, begin, end, thread_max, a.top, top);
     const int lane = threadIdx.x % 32;
     if (parts > 1) {  // everything to the first CTA, which has started when the wait ends
@@ -414,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
             sort_by_rank(part_lists, parts * a.top, a.top, top.best);
             __syncthreads();
         }
-        if (threadIdx.x < 32) all = warp_join(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
+        if (threadIdx.x < 32) all = warp_join<TOP ? 32 : kMaxCluster>(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
     }
     if (threadIdx.x >= 32) return;
     const float base = base_of(all.m), ln_s = logf(all.s);
@@ -534,7 +537,7 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
 // gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.  Bound by memory and by the joins
-// that each row waits for between its loads and its stores (8192 x 131072 bf16: 875 us, 4.9 TB/s; without the joins it would be
+// that each row waits for between its loads and its stores (8192 x 131072 bf16: 861 us, 5.0 TB/s; without the joins it would be
 // 657), so nothing else is left to be waited for there: what the row is asked about is fetched beside its logits (8192 x 50021
 // bf16: 384 us with those loads behind the join, 369 beside; 4096 x 131072 f32: 865 and 818).
 template <class T, int THREADS, int NV>
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
     }
 #pragma unroll
     for (int u = 0; u < NV; ++u) asm volatile("" : "+r"(v[u].x), "+r"(v[u].y), "+r"(v[u].z), "+r"(v[u].w));  // as loaded: unpacked twice rather than kept unpacked
-    all = block_join<THREADS>(all, c2, sums);
+    all = block_join<THREADS, kJoinLanes<THREADS>>(all, c2, sums);
     if (parts > 1) {
         cluster_wait();
         if ((int)threadIdx.x < parts) {
@@ -593,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
     }
     if (threadIdx.x < 32) {  // the row's constants once; a thread's other work is 64 elements
         const int lane = threadIdx.x;
-        if (parts > 1) all = warp_join(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
+        if (parts > 1) all = warp_join<kMaxCluster>(lane < parts ? part_sums[lane < parts ? lane : 0] : Sums(), c2);
         const float ln_s = logf(all.s);
         const bool none = all.s == 0.f;
         const float h = none ? 0.f : ln_s - kLn2 * (all.w / all.s);
