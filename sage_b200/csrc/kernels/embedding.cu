@@ -346,9 +346,9 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const I
 // row that began before block c, 2 c + 1: of one that goes on behind it), and the last block of such a row to arrive adds the pieces up,
 // in their order.  Further blocks write the rows that no token reaches.
 // Bound by memory: g once, the table once.  Each thread copies its own columns of the next tokens into shared memory asynchronously (no
-// barriers, and no registers that wait for them): kAhead rows of the block in flight, six blocks of 256 threads on an SM.
-// The whole gradient of 4096 x 768 f32 into 30522 rows: 24 us, of which sorting is 8; of 65521 x 1000 bf16 added to 50021 rows: 79 us, of which
-// the sums are 50 (half of the instruction slots: a token's columns are unpacked, added and, where its row ends, sent).
+// barriers, and no registers that wait for them): kAhead rows of the block in flight, five blocks of 256 threads on an SM.
+// The whole gradient of 4096 x 768 f32 into 30522 rows: 23.5 us, of which sorting is 8; of 65521 x 1000 bf16 added to 50021 rows: 67 us, of which
+// sorting is 15; of 65536 x 4096 bf16 added to 131072: 208 us, 5.6 TB/s.
 struct EmbeddingGrad {
     const void *g;
     long long ldg;
@@ -434,21 +434,31 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const __grid_consta
     if (WIDE) {
         Four<T> *mine = reinterpret_cast<Four<T> *>(ahead) + threadIdx.x;
         const bool some = cols.first < cols.dim;
-        auto fetch = [&](int i) {
-            if (some && i < n)
-                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((unsigned)__cvta_generic_to_shared(mine + i % kAhead * blockDim.x)), "l"(g + tokens[i] * a.ldg), "n"((int)sizeof(Four<T>)) : "memory");
+        const unsigned place = (unsigned)__cvta_generic_to_shared(mine), step = blockDim.x * sizeof(Four<T>);
+        auto fetch = [&](int i, int u) {
+            if (some && i < n) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(place + u * step), "l"(g + tokens[i] * a.ldg), "n"((int)sizeof(Four<T>)) : "memory");
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) fetch(i);
-        for (int i = 0; i < n; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-            if (i && rows[i + 1] != rows[i]) ended(i);
-            const Four<T> v = mine[i % kAhead * blockDim.x];
+        for (int u = 0; u < kAhead; ++u) fetch(u, u);
+        int row = rows[1];
+        for (int i0 = 0; i0 < n; i0 += kAhead) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] += widen(v.v[j]);
-            asm volatile("" ::"f"(sum[0]), "f"(sum[1]), "f"(sum[2]), "f"(sum[3]) : "memory");  // read before the place is taken again
-            fetch(i + kAhead);
+            for (int u = 0; u < kAhead; ++u) {  // the places of the ring at fixed offsets (4096 x 768 f32 25.5 -> 23.5 us, 65521 x 1000 bf16 69 -> 67)
+                const int i = i0 + u;
+                if (i >= n) break;
+                asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+                const int now = rows[i + 1];
+                if (now != row) {
+                    ended(i);
+                    row = now;
+                }
+                const Four<T> v = mine[u * blockDim.x];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] += widen(v.v[j]);
+                asm volatile("" ::"f"(sum[0]), "f"(sum[1]), "f"(sum[2]), "f"(sum[3]) : "memory");  // read before the place is taken again
+                fetch(i + kAhead, u);
+            }
         }
     } else {
         constexpr int U = 8;
@@ -545,9 +555,11 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     if (tokens > 0x7fff0000ll) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many tokens");
     const size_t size = g.dtype == SAGE_F32 ? 4 : 2;
     const bool wide = dim % 4 == 0 && on_boundary(g.ptr, g.pitch, size, 4 * size) && on_boundary(dtable.ptr, dtable.pitch, 4, 16);
-    // Four columns a thread, up to 256 threads; so many tokens a block that four blocks an SM take all of them in one go.
+    // Four columns a thread, up to 256 threads (eight 16-bit columns in half the threads: 65521 x 1000 bf16 113 us instead of 80).  So many tokens a
+    // block that there are seven blocks for each SM, of which five of 256 threads are resident: sums of few rows begin while others wait (four,
+    // seven, eight for each: 72, 67, 70 us).
     const long long threads = dim >= 1024 ? 256 : ((dim + 3) / 4 + 31) / 32 * 32, slices = (dim + 4 * threads - 1) / (4 * threads);
-    long long length = (tokens * slices + ctx.sm_count * 4 - 1) / (ctx.sm_count * 4);
+    long long length = (tokens * slices + ctx.sm_count * 7 - 1) / (ctx.sm_count * 7);
     length = length < 16 ? 16 : length > kMaxLength ? kMaxLength : (length + 7) / 8 * 8;
     const long long chunks = (tokens + length - 1) / length;
     // Rows that no token reaches become zero beside the sums.  24 MB of the table are cleared beside the sorting already, which leaves the memory
