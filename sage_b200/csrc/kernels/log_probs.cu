@@ -632,14 +632,17 @@ int threads_of_rows(long long rows, long long bytes, bool top, int sms) {
     return rows * kMaxCluster < 4ll * sms ? 512 : 256;
 }
 
-// How many CTAs share a row: the fewest steps of a grid of `slots` resident CTAs, each step the part's bytes and a fixed cost that
-// measures like 24 KB of them (joining, the cluster's barriers), 128 KB with alternatives (candidates found and ranked).
+// How many CTAs share a row: the fewest steps of the resident CTAs, each step the part's bytes and a fixed cost that measures like 24 KB of them
+// (joining), 128 KB with alternatives (candidates found and ranked); twice that where the cluster's barriers come in (32 x 30522 f32 with 20
+// alternatives: 14.2 us with eight CTAs a row, 8.4 with four; 1000 x 131072 bf16 without: 60 us with four, 53 with one).  Clusters of eight do not
+// fill all SMs: their number differs from one part of the GPU to the other.
 constexpr double kFixed = 24576, kFixedTop = 131072;  // of a block of 512 threads
 int parts_of_rows(long long rows, long long bytes, long long slots, double fixed) {
     int best = 1;
     double least = 0;
     for (int c = 1; c <= kMaxCluster; c *= 2) {
-        const double cost = (double)((rows * c + slots - 1) / slots) * ((double)bytes / c + fixed);
+        const long long resident = c == 1 ? slots : c < 8 ? slots * 15 / 16 : slots * 27 / 32;
+        const double cost = (double)((rows * c + resident - 1) / resident) * ((double)bytes / c + (c == 1 ? fixed : 2 * fixed));
         if (c == 1 || cost < least) {
             best = c;
             least = cost;
