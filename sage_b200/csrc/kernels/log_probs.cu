@@ -635,13 +635,16 @@ int threads_of_rows(long long rows, long long bytes, bool top, int sms) {
 // How many CTAs share a row: the fewest steps of the resident CTAs, each step the part's bytes and a fixed cost that measures like 24 KB of them
 // (joining), 128 KB with alternatives (candidates found and ranked); twice that where the cluster's barriers come in (32 x 30522 f32 with 20
 // alternatives: 14.2 us with eight CTAs a row, 8.4 with four; 1000 x 131072 bf16 without: 60 us with four, 53 with one).  Clusters of eight do not
-// fill all SMs: their number differs from one part of the GPU to the other.
+// fill all SMs: their number differs from one part of the GPU to the other.  So few rows that they are one step however they are cut have the same
+// parts, and the same bits, whether alternatives are asked for or not (without: 1 x 30522 f32 5.2 us with one CTA, 5.5 with eight).
 constexpr double kFixed = 24576, kFixedTop = 131072;  // of a block of 512 threads
-int parts_of_rows(long long rows, long long bytes, long long slots, double fixed) {
+int parts_of_rows(long long rows, long long bytes, int threads, bool top, int sms) {
+    const long long slots = sms * 1024ll / threads, slots8 = slots * 27 / 32;
+    const double fixed = (top || rows * kMaxCluster <= slots8 ? kFixedTop : kFixed) * threads / 512;
     int best = 1;
     double least = 0;
     for (int c = 1; c <= kMaxCluster; c *= 2) {
-        const long long resident = c == 1 ? slots : c < 8 ? slots * 15 / 16 : slots * 27 / 32;
+        const long long resident = c == 1 ? slots : c < kMaxCluster ? slots * 15 / 16 : slots8;
         const double cost = (double)((rows * c + resident - 1) / resident) * ((double)bytes / c + (c == 1 ? fixed : 2 * fixed));
         if (c == 1 || cost < least) {
             best = c;
@@ -661,7 +664,7 @@ sage_status token_log_probs(Context &ctx, const LogProbs &a) {
         typedef decltype(t) T;
         const long long bytes = a.logits.cols * (long long)sizeof(T);
         const int threads = threads_of_rows(a.logits.rows, bytes, a.top > 0, ctx.sm_count);
-        const int parts = threads == 128 ? 1 : parts_of_rows(a.logits.rows, bytes, ctx.sm_count * 1024ll / threads, (a.top ? kFixedTop : kFixed) * threads / 512);
+        const int parts = threads == 128 ? 1 : parts_of_rows(a.logits.rows, bytes, threads, a.top > 0, ctx.sm_count);
         auto launch = [&](auto kernel) {
             return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), parts, kernel, dim3((unsigned)(a.logits.rows * parts)), dim3(threads), 0, a, log2_of(parts)), "token_log_probs");
         };
