@@ -634,18 +634,20 @@ int threads_of_rows(long long rows, long long bytes, bool top, int sms) {
 
 // How many CTAs share a row: the fewest steps of the resident CTAs, each step the part's bytes and a fixed cost that measures like 24 KB of them
 // (joining), 128 KB with alternatives (candidates found and ranked); twice that where the cluster's barriers come in (32 x 30522 f32 with 20
-// alternatives: 14.2 us with eight CTAs a row, 8.4 with four; 1000 x 131072 bf16 without: 60 us with four, 53 with one).  Clusters of eight do not
+// alternatives: 13.8 us with eight CTAs a row, 8.2 with one; 1000 x 131072 bf16 without: 60 us with four, 53 with one).  Clusters of eight do not
 // fill all SMs: their number differs from one part of the GPU to the other.  So few rows that they are one step however they are cut have the same
-// parts, and the same bits, whether alternatives are asked for or not (without: 1 x 30522 f32 5.2 us with one CTA, 5.5 with eight).
+// parts, and the same bits, whether alternatives are asked for or not; there a CTA more costs what reading 7 KB does (one row of 8191 f32 with 20
+// alternatives: 6.2, 7.7 and 8.3 us with one, four and eight CTAs; of 30522 7.8, 7.8, 8.4; of 131072 14.4, 9.2, 8.8).
 constexpr double kFixed = 24576, kFixedTop = 131072;  // of a block of 512 threads
 int parts_of_rows(long long rows, long long bytes, int threads, bool top, int sms) {
     const long long slots = sms * 1024ll / threads, slots8 = slots * 27 / 32;
-    const double fixed = (top || rows * kMaxCluster <= slots8 ? kFixedTop : kFixed) * threads / 512;
+    const bool few = rows * kMaxCluster <= slots8;
+    const double fixed = (top ? kFixedTop : kFixed) * threads / 512;
     int best = 1;
     double least = 0;
     for (int c = 1; c <= kMaxCluster; c *= 2) {
         const long long resident = c == 1 ? slots : c < kMaxCluster ? slots * 15 / 16 : slots8;
-        const double cost = (double)((rows * c + resident - 1) / resident) * ((double)bytes / c + (c == 1 ? fixed : 2 * fixed));
+        const double one = (double)bytes / c, cost = few ? one + (c == 1 ? 0 : 6144 + 7168 * c) : (double)((rows * c + resident - 1) / resident) * (one + (c == 1 ? fixed : 2 * fixed));
         if (c == 1 || cost < least) {
             best = c;
             least = cost;
