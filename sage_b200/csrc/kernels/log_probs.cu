@@ -200,7 +200,8 @@ __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float 
 // Where the largest logit is of ordinary size, differences may be scaled first: t = fma(c2, x, -b) with b = c2 m, rounded once and the same for all,
 // is as exact, and one instruction less for two elements; and 16-bit logits can be held at m + kLeast / c2, two to an instruction, in place of t.
 // `least`: that bound, or Bits<T>::kFill where this form is not open (b large, its rounding then reaching kLeast; the bound not finite).  Values and
-// gradient of 8192 x 131072 bf16 for a second on end, with the clock down to 1.79 GHz at the power limit: 930 us without it, 886 with.
+// gradient: 4096 x 131072 f32 811 us without it, 796 with, 8192 x 32000 bf16 211 and 208, 8192 x 131072 bf16 864 and 867; for a second on end, with the
+// clock down to 1.8 GHz at the power limit, 4096 x 131072 f32 817 and 801, 8192 x 131072 bf16 890 and 886.
 template <class T>
 struct Ordinary {
     float b, rest;  // t relative to b is t relative to m, plus `rest`
@@ -509,7 +510,6 @@ struct GradRow {
     float base, c2, slope, level, at_id;
     int id;
     unsigned least;
-    template <class T>
     __device__ void set(float m, float s, float ln_s, float scale, float gl, float ge, float entropy, int id_) {
         base = base_of(m);
         c2 = scale * 1.4426950408889634f;
@@ -519,6 +519,10 @@ struct GradRow {
         slope = -share * (ge * kLn2);
         level = -share * (ge != 0.f ? gl + ge * (entropy - ln_s) : gl);  // NaN where s is: so is every gradient
         at_id = scale * gl;
+    }
+    // Behind set(): into the form with scaled differences, where it is open.
+    template <class T>
+    __device__ void scale_first() {
         const Ordinary<T> o(base, c2);
         least = o.least;
         if (o.open()) {  // relative to b
@@ -593,7 +597,7 @@ __device__ __forceinline__ int token_of(const LogProbsGrad &a, long long r) {
 }
 
 // From the forward pass's sums: `pieces` blocks for a row, kGradVectors vectors each.  Bound by memory: a read and a write (4096 x
-// 30522 f32: 151 us, 6.6 TB/s).
+// 30522 f32: 151 us, 6.6 TB/s; with scaled differences, worked out by each thread, 157).
 constexpr int kGradVectors = 1024;
 template <class T>
 __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad a, const unsigned pieces) {
@@ -610,9 +614,9 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
     const float *stats = (const float *)a.stats.ptr + r * a.stats.pitch;
     const int id = token_of(a, r);
     GradRow g;
-    g.set<T>(stats[0], stats[1], logf(stats[1]), a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), at_row(a.entropy, r), id);
+    g.set(stats[0], stats[1], logf(stats[1]), a.scale, id >= 0 ? at_row(a.g_log_probs, r) : 0.f, at_row(a.g_entropy, r), at_row(a.entropy, r), id);
     const bool same = same_grid(x, dx);
-    store_all<T, U, 256>(row, g, dx, same, v, i, row.count);
+    store_some<T, U, 256, false>(row, g, dx, same, v, i, row.count);
 }
 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
@@ -681,7 +685,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
         const bool none = all.s == 0.f;
         const float h = none ? 0.f : ln_s - kLn2 * (all.w / all.s);
         if (lane == 0) {
-            constants.set<T>(all.m, all.s, ln_s, a.scale, asked.g_log_prob, asked.g_entropy, h, asked.id);
+            constants.set(all.m, all.s, ln_s, a.scale, asked.g_log_prob, asked.g_entropy, h, asked.id);
+            constants.scale_first<T>();
         } else if (lane == 1 && rank == 0) {
             ((float *)log_probs.ptr)[r * log_probs.stride] = asked.id < 0 ? 0.f : none ? -INFINITY : (asked.own - base_of(all.m)) * a.scale - ln_s;
             if (entropy.ptr) ((float *)entropy.ptr)[r * entropy.stride] = h;
