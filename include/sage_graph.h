@@ -143,8 +143,8 @@ sage_status sage_op_accuracy(const sage_var *logits, const sage_var *labels, sag
 typedef struct sage_optimizer sage_optimizer;
 sage_status sage_sgd_create(float lr, sage_optimizer **out);
 sage_status sage_adam_create(float lr, sage_optimizer **out);
-/* AdamW (no reference counterpart; the rule is sage_adamw_step's): states in 32 or 8 bits, kept by parameter, zero before the first
- * update, which is step 1. */
+/* AdamW (no reference counterpart; the rule is sage_adamw_step's): states in 32 or 8 bits, kept by parameter and zero before
+ * the parameter's first update, which is its step 1 whenever it comes. */
 sage_status sage_adamw_create(double lr, double beta1, double beta2, double eps, double weight_decay, int32_t state_bits, sage_optimizer **out);
 /* The private fields of the reference's structs (optim.rs:14-26, 97-110); Sgd's momentum stays 0 (with
  * any other value the reference's update panics, optim.rs:68-69, and this one returns SAGE_ERR_UNSUPPORTED). */

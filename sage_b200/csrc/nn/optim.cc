@@ -2,6 +2,7 @@
 #include "optim.h"
 
 #include <cmath>
+#include <map>
 
 #include <cuda_runtime.h>
 
@@ -161,7 +162,6 @@ AdamW::AdamW(double lr_, double beta1_, double beta2_, double eps_, double weigh
 
 sage_status AdamW::init(Session &) {
     state.clear();
-    step = 0;
     return SAGE_OK;
 }
 
@@ -176,7 +176,11 @@ sage_status AdamW::update(const std::vector<Var> &params, const std::vector<Var>
         C.note_memset();
         return C.dry() ? SAGE_OK : C.check_cuda(cudaMemsetAsync(t->ptr(), 0, (size_t)words * 4, C.stream()), "adamw: states");
     };
-    std::vector<k::AdamWSlot> slots;
+    struct Group {  // parameters that have had the same number of updates: one rule, one launch
+        std::vector<k::AdamWSlot> slots;
+        std::vector<States *> states;
+    };
+    std::map<long long, Group> groups;
     for (size_t i = 0; i < params.size(); ++i) {
         const long long n = prep.slots[i].n;
         auto it = state.find(params[i].key());
@@ -202,11 +206,16 @@ sage_status AdamW::update(const std::vector<Var> &params, const std::vector<Var>
             slot.m_scale = (float *)it->second.m_scale.ptr();
             slot.v_scale = (float *)it->second.v_scale.ptr();
         }
-        if (n) slots.push_back(slot);
+        Group &group = groups[it->second.steps];
+        if (n) group.slots.push_back(slot);
+        group.states.push_back(&it->second);
     }
-    st = k::adamw_step(C, slots.data(), (int)slots.size(), state_bits == 8, k::adamw_rule(lr, beta1, beta2, eps, weight_decay, 1.0, step + 1));
-    if (!st) ++step;
-    return st;
+    for (auto &g : groups) {
+        st = k::adamw_step(C, g.second.slots.data(), (int)g.second.slots.size(), state_bits == 8, k::adamw_rule(lr, beta1, beta2, eps, weight_decay, 1.0, g.first + 1));
+        if (st) return st;
+        for (States *z : g.second.states) z->steps = g.first + 1;
+    }
+    return SAGE_OK;
 }
 
 }  // namespace nn

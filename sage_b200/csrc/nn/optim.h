@@ -42,13 +42,14 @@ struct Adam : Optimizer {  // optim.rs:97-178
     sage_status update(const std::vector<Var> &params, const std::vector<Var> &grads, Session &s) override;
 };
 
-// AdamW (not in the reference): the rule of kernels/adamw.cu over all parameters in one launch, states by parameter.
+// AdamW (not in the reference): the rule of kernels/adamw.cu over all parameters, states and steps by parameter; one launch for those
+// that have had as many updates, which is all of them unless calls name different ones.
 struct AdamW : Optimizer {
     double lr, beta1, beta2, eps, weight_decay;
     int state_bits;
-    long long step = 0;  // updates so far
     struct States {
-        Var param;  // keeps the key alive
+        Var param;            // keeps the key alive
+        long long steps = 0;  // updates so far
         Tensor m, v, m_scale, v_scale;
     };
     std::unordered_map<Origin *, States> state;
