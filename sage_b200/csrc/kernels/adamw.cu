@@ -262,9 +262,11 @@ __device__ __forceinline__ void block_update(const AdamWSlot &s, const AdamWRule
         // one at least for what is not zero
         rounded(make_float2(fmaxf(fast_root(u.x), one_if_positive(e.v[i].x)), fmaxf(fast_root(u.y), one_if_positive(e.v[i].y))), &v_off, v + 2 * i);
     }
-    // A fast root is 2^-23 off at most: of up to 127 less than kMOff, two after another of up to 255 less than kVOff.  Where all of a block's v
-    // lie below 2^-80, subnormal ones count, which the fast root takes for zero.
-    constexpr float kMOff = 2.2e-5f, kVOff = 0x1p-14f;
+    // How far a fast root can lie from the exact one's rounded result.  u = 2^-24 is one rounding, a fast root is 2 u off at most, and errors in
+    // front of a root halve.  Of m: 2 u of up to 127, and half an f32 step there, 1.9e-5.  Of v: the fast way has 2 u (outer root), u / 2 (product)
+    // and u (inner root), the exact way u, u / 2 and u / 2, in all 5.5 u of up to 255, 8.4e-5.  Where all of a block's v lie below 2^-80,
+    // subnormal ones count, which the fast root takes for zero.
+    constexpr float kMOff = 2.2e-5f, kVOff = 0x1.8p-14f;
     if (m_off > 0.5f - kMOff || v_off > 0.5f - kVOff || v_top < 0x1p-40f) {
         float none = 0.f;
 #pragma unroll 1

@@ -1,8 +1,10 @@
-"""Rules of the language-model operators on a B200 that single calls do not show: steps of an optimizer's parameters."""
+"""Rules of the language-model operators on a B200 that single calls do not show: steps of an optimizer's parameters, codes of states that
+lie midway between two."""
 import numpy as np
 import pytest
 
 import sage_b200 as S
+from sage_b200 import language as L
 
 import language_oracle as O
 
@@ -68,3 +70,32 @@ def test_groups_updated_by_calls_of_their_own(ctx, bits):
             opt.update({p.var: p.gradient() for p in group}, ctx)
             for p in group:
                 p.check()
+
+
+# ------------------------------------------------------------------------------------------ codes midway
+@pytest.mark.parametrize("first,last", [(0, 60), (60, 186), (186, 255)])
+@pytest.mark.parametrize("moment", ["m", "v"])
+def test_codes_near_the_middle_of_two(ctx, moment, first, last):
+    """Moments within a few f32 steps of where the code changes: the codes are those of the operations rounded one by one."""
+    top = 127 if moment == "m" else 255
+    first, last = (first // 2, last // 2) if moment == "m" else (first, last)
+    f, blocks = np.float32, 4096
+    rng = np.random.default_rng(first + top)
+    largest = np.exp2(rng.uniform(-3, 3, (blocks, 1))).astype(f)
+    c = rng.integers(first, last, (blocks, 256)) + 0.5
+    with np.errstate(divide="ignore"):
+        factor = f(1) / (largest if moment == "m" else np.sqrt(largest * largest)) * f(top * top)
+    g = (c * c / factor).astype(f)
+    g = (g.view(np.int32) + rng.integers(-12, 13, g.shape)).astype(np.int32).view(f)
+    g[:, 0] = largest[:, 0]
+    n = g.size
+    g = g.reshape(-1)
+    t = [ctx.tensor(np.zeros(n, f)), ctx.tensor(g), ctx.tensor(np.zeros(n, np.int8), S.I8), ctx.tensor(np.zeros(n, np.uint8), S.U8), ctx.tensor(np.zeros(blocks, f)), ctx.tensor(np.zeros(blocks, f))]
+    L.adamw_step(L.AdamWTensors(ctx, [L.adamw_tensor(*t)]), step=1, lr=1e-3, beta1=0.0, beta2=0.0)
+    m, v = O.adamw_f32(np.zeros(n, f), np.zeros(n, f), g, 0.0, 0.0, 1.0)
+    (mc, ms), (vc, vs) = O.adamw_encode(m, 127), O.adamw_encode(np.sqrt(v), 255)
+    got = [x.numpy() for x in t[2:]]
+    for x in t:
+        x.release()
+    assert np.array_equal(got[2], ms) and np.array_equal(got[3], vs)
+    assert (got[0] != mc).sum() == 0 and (got[1] != vc).sum() == 0

@@ -1,8 +1,13 @@
 """Rules of the language-model operators that a planning context shows: what is accepted, what is launched, whose memory is whose."""
+import os
+import re
+
 import numpy as np
 import pytest
 
 import sage_b200 as S
+
+KERNELS = os.path.join(os.path.dirname(os.path.abspath(S.__file__)), "csrc", "kernels")
 
 
 @pytest.fixture()
@@ -30,3 +35,14 @@ def test_adamw_launches_once_for_parameters_of_the_same_step(ctx):
     assert launches({a: ga, b: gb}) == 1  # both step 4
     opt.init(ctx)
     assert launches({a: ga}) == 1 and launches({a: ga, b: gb}) == 2
+
+
+def test_margins_within_which_codes_take_exact_roots():
+    """Codes of 8-bit states are found from square roots that are 2^-23 off at most (the instruction's bound); the margins around one half
+    within which exact roots decide have to cover all that separates the two ways: no run shows errors that this GPU's roots do not make."""
+    text = open(os.path.join(KERNELS, "adamw.cu")).read()
+    m_off, v_off = (float.fromhex(x) if "p" in x else float(x) for x in re.search(r"kMOff = ([^f;]*)f, kVOff = ([^f;]*)f;", text).groups())
+    u, fast = 2.0 ** -24, 2.0 ** -23
+    assert m_off > 127 * fast + 0.5 * 2.0 ** -17  # the exact root is rounded to the f32 grid, which has the middles
+    # root, product, root; an error in front of a root halves
+    assert v_off > 255 * ((fast + (u + fast) / 2) + (u + (u + u) / 2))
