@@ -164,7 +164,7 @@ Var ops::embedding(const Var &table, const Var &ids, float scale) {
 Var ops::token_log_probs(const Var &logits, const Var &ids, float scale) {
     if (logits.rank() != 2 || logits.dtype() != SAGE_F32) shape_fail("token_log_probs: logits must be f32 [rows, tokens]");
     check_ids(ids, "token_log_probs");
-    if (ids.size() != logits.extents()[0] || ids.extents()[0] != logits.extents()[0]) shape_fail("token_log_probs: one token id for each row is needed");
+    if (ids.rank() < 1 || ids.size() != logits.extents()[0] || ids.extents()[0] != logits.extents()[0]) shape_fail("token_log_probs: one token id for each row is needed");
     if (!(scale > 0.f) || !(scale < 3.4e38f)) shape_fail("token_log_probs: the scale must be positive and finite");
     if (!logits.extents()[1]) shape_fail("token_log_probs: rows without tokens");
     auto op = std::make_shared<TokenLogProbsOp>();

@@ -46,3 +46,15 @@ def test_margins_within_which_codes_take_exact_roots():
     assert m_off > 127 * fast + 0.5 * 2.0 ** -17  # the exact root is rounded to the f32 grid, which has the middles
     # root, product, root; an error in front of a root halves
     assert v_off > 255 * ((fast + (u + fast) / 2) + (u + (u + u) / 2))
+
+
+def test_token_ids_without_axes_are_refused(ctx):
+    """Logits of one row and an id that has no axis: refused, however the variable came to have none."""
+    logits = ctx.var(np.zeros((1, 8), np.float32))
+    one = ctx.var(np.zeros(1, np.int32))
+    S.token_log_probs(logits, one)
+    for ids in (S.squeeze(one, 0), S.squeeze(S.squeeze(ctx.var(np.zeros((1, 1), np.int32)), 0), 0), S.Var.empty([], S.I32)):
+        assert ids.extents == ()
+        with pytest.raises(S.SageError) as e:
+            S.token_log_probs(logits, ids)
+        assert e.value.code == 1 and "one token id for each row" in str(e.value)
