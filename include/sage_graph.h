@@ -147,7 +147,8 @@ sage_status sage_adam_create(float lr, sage_optimizer **out);
  * the parameter's first update, which is its step 1 whenever it comes. */
 sage_status sage_adamw_create(double lr, double beta1, double beta2, double eps, double weight_decay, int32_t state_bits, sage_optimizer **out);
 /* The private fields of the reference's structs (optim.rs:14-26, 97-110); Sgd's momentum stays 0 (with
- * any other value the reference's update panics, optim.rs:68-69, and this one returns SAGE_ERR_UNSUPPORTED). */
+ * any other value the reference's update panics, optim.rs:68-69, and this one returns SAGE_ERR_UNSUPPORTED).  AdamW refuses a decay
+ * that is not finite, by itself or times the learning rate. */
 sage_status sage_optimizer_set_weight_decay(sage_optimizer *o, float weight_decay);
 sage_status sage_optimizer_destroy(sage_optimizer *o);
 /* Optimizer::init — optim.rs:9,43-46,128-132: forgets the moments, step count back to 1 */

@@ -679,7 +679,7 @@ class Optimizer:
         ctx._ck(lib.sage_optimizer_update(self.h, ctx.s, p, g, len(params)))
 
     def set_weight_decay(self, weight_decay):
-        lib.sage_optimizer_set_weight_decay(self.h, ctypes.c_float(weight_decay))
+        _gck(lib.sage_optimizer_set_weight_decay(self.h, ctypes.c_float(weight_decay)))
 
 
 class Sgd(Optimizer):

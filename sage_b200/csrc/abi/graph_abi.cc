@@ -384,7 +384,7 @@ sage_status sage_adamw_create(double lr, double beta1, double beta2, double eps,
 sage_status sage_optimizer_set_weight_decay(sage_optimizer *o, float weight_decay) {
     if (auto *a = dynamic_cast<nn::Adam *>(o->impl.get())) a->weight_decay = weight_decay;
     else if (auto *g = dynamic_cast<nn::Sgd *>(o->impl.get())) g->weight_decay = weight_decay;
-    else if (auto *w = dynamic_cast<nn::AdamW *>(o->impl.get())) w->weight_decay = weight_decay;
+    else if (auto *w = dynamic_cast<nn::AdamW *>(o->impl.get())) return guarded([&]() -> sage_status { return w->set_weight_decay(weight_decay); });
     return SAGE_OK;
 }
 sage_status sage_optimizer_destroy(sage_optimizer *o) {

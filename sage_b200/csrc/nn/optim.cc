@@ -157,7 +157,18 @@ AdamW::AdamW(double lr_, double beta1_, double beta2_, double eps_, double weigh
     if (state_bits != 32 && state_bits != 8) shape_fail("AdamW: states have 32 or 8 bits");
     if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0)) shape_fail("AdamW: beta1 and beta2 lie in [0, 1)");
     if (!(eps >= 1e-15) || !std::isfinite((float)eps)) shape_fail("AdamW: eps is 1e-15 at least, and finite");
-    if (!std::isfinite((float)lr) || !std::isfinite((float)(lr * weight_decay))) shape_fail("AdamW: lr and weight_decay are finite");
+    check_finite(lr, weight_decay);
+}
+
+void AdamW::check_finite(double lr, double weight_decay) {
+    for (double x : {lr, weight_decay, lr * weight_decay})
+        if (!std::isfinite((float)x)) shape_fail("AdamW: lr and weight_decay are finite");
+}
+
+sage_status AdamW::set_weight_decay(double w) {
+    check_finite(lr, w);
+    weight_decay = w;
+    return SAGE_OK;
 }
 
 sage_status AdamW::init(Session &) {

@@ -54,6 +54,8 @@ struct AdamW : Optimizer {
     };
     std::unordered_map<Origin *, States> state;
     AdamW(double lr, double beta1, double beta2, double eps, double weight_decay, int state_bits);
+    static void check_finite(double lr, double weight_decay);  // throws ShapeError
+    sage_status set_weight_decay(double weight_decay);
     sage_status init(Session &s) override;
     sage_status update(const std::vector<Var> &params, const std::vector<Var> &grads, Session &s) override;
 };

@@ -58,3 +58,18 @@ def test_token_ids_without_axes_are_refused(ctx):
         with pytest.raises(S.SageError) as e:
             S.token_log_probs(logits, ids)
         assert e.value.code == 1 and "one token id for each row" in str(e.value)
+
+
+def test_adamw_refuses_weight_decay_that_is_not_finite(ctx):
+    """As the constructor does, so that no update can make parameters NaN; the old value stays."""
+    for opt, bad in ((S.AdamW(1e-3), (float("nan"), float("inf"), 1e39)), (S.AdamW(1e30), (1e20,))):
+        opt.set_weight_decay(0.5)
+        for w in bad:
+            with pytest.raises(S.SageError) as e:
+                opt.set_weight_decay(w)
+            assert e.value.code == 1 and "finite" in str(e.value)
+    for lr, w in ((1e-3, float("inf")), (0.0, float("nan")), (1e-40, 1e39)):
+        with pytest.raises(S.SageError):
+            S.AdamW(lr, weight_decay=w)
+    for opt in (S.Sgd(1e-3), S.Adam(1e-3)):
+        opt.set_weight_decay(0.5)
