@@ -124,7 +124,8 @@ sage_status sage_op_layer_norm(const sage_var *x, int32_t naxes, const int64_t *
 /* ---- language models (no reference counterpart; the kernels and their rules are sage_cuda.h's).
  * embedding: scale * table[ids], extents of ids + [width], gradient by sorted tokens.  token_log_probs: f32 [rows, 4] over logits
  * [rows, tokens] and one id for each row: column 0 the token's log probability under softmax(scale * logits), column 1 the row's
- * entropy, both differentiable, then what the gradient reads.  top_tokens: u32 [rows, k], the k <= 32 largest. */
+ * entropy, both differentiable, then what the gradient reads.  top_tokens: u32 [rows, k], the k <= 32 largest.  No more than 2^31 - 2^16 rows,
+ * tokens or columns. */
 sage_status sage_op_embedding(const sage_var *table, const sage_var *ids, float scale, sage_var **out);
 sage_status sage_op_token_log_probs(const sage_var *logits, const sage_var *ids, float scale, sage_var **out);
 sage_status sage_op_top_tokens(const sage_var *logits, int64_t k, sage_var **out);

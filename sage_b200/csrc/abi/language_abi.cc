@@ -56,7 +56,7 @@ struct Checks {
         r.pitch = t->strides[0];
         if (r.cols > 1 && t->strides[1] != 1) refuse(name, "is not contiguous along its rows");
         if (output && r.rows > 1 && r.pitch < r.cols) refuse(name, "has rows that overlap");
-        if (r.rows > 0x7fff0000ll || r.cols > 0x7fff0000ll) refuse(name, "has more than 2^31 - 2^16 rows or columns");
+        if (r.rows > k::kMaxRows || r.cols > k::kMaxRows) refuse(name, "has more than 2^31 - 2^16 rows or columns");
         return r;
     }
     k::RowsArg real_rows(const sage_tensor *t, const char *name, bool output) const {

@@ -37,6 +37,10 @@ void check_ids(const Var &ids, const char *what) {
     if (ids.dtype() != SAGE_I32 && ids.dtype() != SAGE_U32) shape_fail(std::string(what) + ": token ids must be i32 or u32");
 }
 
+void check_rows(long long rows, long long cols, const char *what) {
+    if (rows > k::kMaxRows || cols > k::kMaxRows) shape_fail(std::string(what) + ": more than 2^31 - 2^16 rows, tokens or columns");
+}
+
 struct EmbeddingGradOp : Operator {  // inputs gy [.., D], ids [..] -> [V, D]
     float scale;
     const char *name() const override { return "embedding_grad"; }
@@ -151,6 +155,8 @@ struct TopTokensOp : Operator {  // logits [R, V] -> [R, k] u32
 Var ops::embedding(const Var &table, const Var &ids, float scale) {
     if (table.rank() != 2 || table.dtype() != SAGE_F32) shape_fail("embedding: the table must be f32 [tokens, width]");
     check_ids(ids, "embedding");
+    check_rows(table.extents()[0], table.extents()[1], "embedding");
+    check_rows(ids.size(), 0, "embedding");
     auto op = std::make_shared<EmbeddingOp>();
     op->scale = scale;
     Array e = ids.extents();
@@ -164,6 +170,7 @@ Var ops::embedding(const Var &table, const Var &ids, float scale) {
 Var ops::token_log_probs(const Var &logits, const Var &ids, float scale) {
     if (logits.rank() != 2 || logits.dtype() != SAGE_F32) shape_fail("token_log_probs: logits must be f32 [rows, tokens]");
     check_ids(ids, "token_log_probs");
+    check_rows(logits.extents()[0], logits.extents()[1], "token_log_probs");
     if (ids.rank() < 1 || ids.size() != logits.extents()[0] || ids.extents()[0] != logits.extents()[0]) shape_fail("token_log_probs: one token id for each row is needed");
     if (!(scale > 0.f) || !(scale < 3.4e38f)) shape_fail("token_log_probs: the scale must be positive and finite");
     if (!logits.extents()[1]) shape_fail("token_log_probs: rows without tokens");
@@ -176,6 +183,7 @@ Var ops::token_log_probs(const Var &logits, const Var &ids, float scale) {
 
 Var ops::top_tokens(const Var &logits, long long k) {
     if (logits.rank() != 2 || logits.dtype() != SAGE_F32) shape_fail("top_tokens: logits must be f32 [rows, tokens]");
+    check_rows(logits.extents()[0], logits.extents()[1], "top_tokens");
     if (k < 1 || k > k::kMaxTop || k > logits.extents()[1]) shape_fail("top_tokens: 1 to 32 tokens of a row, and no more than it has");
     auto op = std::make_shared<TopTokensOp>();
     op->in = {logits.desc};

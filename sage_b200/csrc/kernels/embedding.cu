@@ -552,7 +552,7 @@ sage_status embedding(Context &ctx, const RowsArg &table, const VectorArg &ids, 
 sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids, float scale, bool add, const RowsArg &dtable) {
     const long long vocab = dtable.rows, dim = dtable.cols, tokens = g.rows;
     if (!vocab || !dim || (add && !tokens)) return SAGE_OK;
-    if (tokens > 0x7fff0000ll) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many tokens");
+    if (tokens > kMaxRows) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many tokens");
     const size_t size = g.dtype == SAGE_F32 ? 4 : 2;
     const bool wide = dim % 4 == 0 && on_boundary(g.ptr, g.pitch, size, 4 * size) && on_boundary(dtable.ptr, dtable.pitch, 4, 16);
     // Four columns a thread, up to 256 threads (eight 16-bit columns in half the threads: 65521 x 1000 bf16 113 us instead of 80).  So many tokens a

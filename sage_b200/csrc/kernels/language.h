@@ -8,6 +8,9 @@
 namespace sage {
 namespace k {
 
+// Rows, tokens or columns: the kernels number them in 32 bits, with room for a last round's.
+constexpr long long kMaxRows = 0x7fff0000;
+
 struct RowsArg {  // [rows, cols], contiguous along a row
     void *ptr = nullptr;
     int dtype = SAGE_F32;

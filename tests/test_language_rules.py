@@ -73,3 +73,18 @@ def test_adamw_refuses_weight_decay_that_is_not_finite(ctx):
             S.AdamW(lr, weight_decay=w)
     for opt in (S.Sgd(1e-3), S.Adam(1e-3)):
         opt.set_weight_decay(0.5)
+
+
+def test_graph_refuses_more_rows_or_columns_than_the_kernels_count(ctx):
+    """2^31 - 2^16 rows, tokens or columns, as the operators on tensors; the kernels number rows and columns in 32 bits."""
+    most = 2 ** 31 - 2 ** 16
+    f, i = (lambda *e: S.Var.empty(e)), (lambda *e: S.Var.empty(e, S.I32))
+    assert S.embedding(f(most, 1), i(1)).extents == (1, 1) and S.embedding(f(1, most), i(1)).extents == (1, most) and S.embedding(f(1, 1), i(most)).extents == (most, 1)
+    S.token_log_probs(f(most, 1), i(most))
+    S.token_log_probs(f(1, most), i(1))
+    S.top_tokens(f(most, 1), 1)
+    for call in (lambda: S.embedding(f(most + 1, 1), i(1)), lambda: S.embedding(f(1, most + 1), i(1)), lambda: S.embedding(f(1, 1), i(most + 1)), lambda: S.embedding(f(1, 1), i(2 ** 16, 2 ** 16)),
+                 lambda: S.token_log_probs(f(most + 1, 1), i(most + 1)), lambda: S.token_log_probs(f(1, most + 1), i(1)), lambda: S.top_tokens(f(most + 1, 1), 1), lambda: S.top_tokens(f(1, most + 1), 1)):
+        with pytest.raises(S.SageError) as e:
+            call()
+        assert e.value.code == 1 and "2^31 - 2^16" in str(e.value)
