@@ -33,16 +33,19 @@ struct Checks {
         if (t->dtype < SAGE_F32 || t->dtype > SAGE_U8) refuse(name, "has an unknown element type");
         if (t->ndim < 1 || t->ndim > SAGE_MAX_DIMS) refuse(name, "has no rank of 1 to 8");
         if (t->offset < 0) refuse(name, "starts in front of its buffer");
-        __int128 last = t->offset;
         bool empty = false;
         for (int i = 0; i < t->ndim; ++i) {
             if (t->extents[i] < 0 || t->strides[i] < 0) refuse(name, "has a negative extent or stride");
             empty |= t->extents[i] == 0;
-            if (t->extents[i] > 0) last += (__int128)(t->extents[i] - 1) * t->strides[i];
         }
         const size_t size = element_size(t->dtype);
-        if (!empty && (last + 1) * (__int128)size > (__int128)t->buf->size) refuse(name, "reaches behind the end of its buffer");
-        char *p = (char *)t->buf->ptr + t->offset * (long long)size;
+        const __int128 room = t->buf->size / size;
+        __int128 last = t->offset;
+        for (int i = 0; i < t->ndim && !empty; ++i) {  // a product has 126 bits at most
+            last += (__int128)(t->extents[i] - 1) * t->strides[i];
+            if (last >= room) refuse(name, "reaches behind the end of its buffer");
+        }
+        char *p = (char *)t->buf->ptr + (empty ? 0 : t->offset * (long long)size);
         if (!empty && (uintptr_t)p % size) refuse(name, "is not aligned to its elements");
         return p;
     }
@@ -79,7 +82,9 @@ struct Checks {
     void *flat(const sage_tensor *t, const char *name, long long n, long long *count = nullptr) const {
         void *p = view(t, name);
         long long s = 1;
-        for (int i = t->ndim - 1; i >= 0; --i) {
+        for (int i = 0; i < t->ndim; ++i)
+            if (!t->extents[i]) s = 0;
+        for (int i = t->ndim - 1; i >= 0 && s; --i) {
             if (t->extents[i] > 1 && t->strides[i] != s) refuse(name, "is not contiguous");
             s *= t->extents[i];
         }

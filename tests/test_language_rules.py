@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import sage_b200 as S
+from sage_b200 import language as L
 
 KERNELS = os.path.join(os.path.dirname(os.path.abspath(S.__file__)), "csrc", "kernels")
 
@@ -88,3 +89,16 @@ def test_graph_refuses_more_rows_or_columns_than_the_kernels_count(ctx):
         with pytest.raises(S.SageError) as e:
             call()
         assert e.value.code == 1 and "2^31 - 2^16" in str(e.value)
+
+
+def test_views_of_any_size_are_checked_without_overflow(ctx):
+    """Extents and strides whose products pass 64 and 128 bits reach behind the end of every buffer; views of nothing reach nowhere."""
+    most = 2 ** 63 - 1
+    step = lambda *t: L.adamw_step(L.AdamWTensors(ctx, [L.adamw_tensor(*t)]), step=1, lr=1e-3)  # noqa: E731
+    for extents, strides in (((most, most), (most, 1)), ((most,) * 8, (most,) * 7 + (1,)), ((1, most, most), (1, most, 1)), ((2 ** 62, 4), (4, 1))):
+        t = [ctx.empty((1,)).view(extents, strides) for _ in range(4)]
+        with pytest.raises(S.SageError) as e:
+            step(*t)
+        assert e.value.code == 1 and "behind the end" in str(e.value)
+    for extents, strides in (((0, most, most), (most, most, 1)), ((5, 0), (1, 1)), ((0,), (3,))):
+        step(*[ctx.empty((1,)).view(extents, strides) for _ in range(4)])
