@@ -284,7 +284,7 @@ sage_status sage_embedding(sage_ctx *ctx, const sage_tensor *table, const sage_t
  * f16 / bf16, dtable [V, D] f32. */
 sage_status sage_embedding_grad(sage_ctx *ctx, const sage_tensor *g, const sage_tensor *ids, float scale, int32_t add, const sage_tensor *dtable);
 
-/* Over each row x = scale * logits[r, :] (logits [R, V] f32 / f16 / bf16, scale > 0, an inverse temperature):
+/* Over each row x = scale * logits[r, :] (logits [R, V] f32 / f16 / bf16, scale > 0, an inverse temperature, up to 2.35e38):
  *   log_probs[r] = x[ids[r]] - log_sum_exp(x)         (ids[r] outside [0, V): no token is scored, 0)
  *   entropy[r]   = - sum of p log p, p = softmax(x)
  *   stats[r]     = { max of x / scale, sum of exp(x - max x) }, what the gradient reads

@@ -116,7 +116,7 @@ float finite(const Checks &c, const char *name, double x) {
 }
 
 float temperature_scale(const Checks &c, float scale) {
-    if (!(scale > 0.f) || !std::isfinite(scale)) c.refuse("scale", "is not positive and finite");
+    if (!k::is_scale(scale)) c.refuse("scale", "is not positive and finite, also times log2(e)");
     return scale;
 }
 

@@ -1,6 +1,8 @@
 // Language-model operators of the lazy graph: token embedding, log probabilities of given tokens with entropy, alternatives
 // (kernels/language.h).  No counterpart in the reference, whose embedding is a gather (layers.rs:427-452) with a scatter as its
 // gradient and whose loss is composed (nn.rs:70-82).
+#include <cmath>
+
 #include "../kernels/language.h"
 #include "graph.h"
 
@@ -157,6 +159,7 @@ Var ops::embedding(const Var &table, const Var &ids, float scale) {
     check_ids(ids, "embedding");
     check_rows(table.extents()[0], table.extents()[1], "embedding");
     check_rows(ids.size(), 0, "embedding");
+    if (!std::isfinite(scale)) shape_fail("embedding: the scale must be finite");
     auto op = std::make_shared<EmbeddingOp>();
     op->scale = scale;
     Array e = ids.extents();
@@ -172,7 +175,7 @@ Var ops::token_log_probs(const Var &logits, const Var &ids, float scale) {
     check_ids(ids, "token_log_probs");
     check_rows(logits.extents()[0], logits.extents()[1], "token_log_probs");
     if (ids.rank() < 1 || ids.size() != logits.extents()[0] || ids.extents()[0] != logits.extents()[0]) shape_fail("token_log_probs: one token id for each row is needed");
-    if (!(scale > 0.f) || !(scale < 3.4e38f)) shape_fail("token_log_probs: the scale must be positive and finite");
+    if (!k::is_scale(scale)) shape_fail("token_log_probs: the scale must be positive and finite, also times log2(e)");
     if (!logits.extents()[1]) shape_fail("token_log_probs: rows without tokens");
     auto op = std::make_shared<TokenLogProbsOp>();
     op->scale = scale;

@@ -27,6 +27,9 @@ sage_status embedding(Context &ctx, const RowsArg &table, const VectorArg &ids, 
 sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids, float scale, bool add, const RowsArg &dtable);
 
 constexpr int kMaxTop = 32;
+constexpr float kLog2E = 1.4426950408889634f;
+// Scales of logits: positive, and finite in base 2 too, in which exponentials are taken.
+inline bool is_scale(float scale) { return scale > 0.f && scale <= 3.4028235e38f / kLog2E; }
 struct LogProbs {  // what has no ptr is not wanted, or (ids) not given
     RowsArg logits;
     VectorArg ids;

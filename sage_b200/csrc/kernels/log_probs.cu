@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     const T *x = (const T *)a.logits.ptr + r * a.logits.pitch;
     const RowVectors<T> row(x, a.logits.cols);
     const int each = (row.count + parts - 1) >> shift, begin = (int)rank * each, end = min(begin + each, row.count);
-    const float c2 = a.scale * 1.4426950408889634f;
+    const float c2 = a.scale * kLog2E;
     float own = 0.f;
     bool scored = false;
     if (rank == 0 && threadIdx.x == 0 && a.ids.ptr) {
@@ -512,7 +512,7 @@ struct GradRow {
     unsigned least;
     __device__ void set(float m, float s, float ln_s, float scale, float gl, float ge, float entropy, int id_) {
         base = base_of(m);
-        c2 = scale * 1.4426950408889634f;
+        c2 = scale * kLog2E;
         id = id_;
         if (s == 0.f) gl = ge = 0.f;  // masked throughout
         const float share = s == 0.f ? 0.f : scale / s;
@@ -640,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
     T *dx = (T *)a.dlogits.ptr + r * a.dlogits.pitch;
     const RowVectors<T> row(x, a.logits.cols);
     const int begin = min((int)rank * each, row.count), end = min(begin + each, row.count), i = begin + (int)threadIdx.x;
-    const float c2 = a.scale * 1.4426950408889634f;
+    const float c2 = a.scale * kLog2E;
     // What the row is asked about, fetched by the last thread while the logits are under way.
     const bool asks = threadIdx.x == THREADS - 1;
     int id = -1;

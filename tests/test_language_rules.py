@@ -102,3 +102,22 @@ def test_views_of_any_size_are_checked_without_overflow(ctx):
         assert e.value.code == 1 and "behind the end" in str(e.value)
     for extents, strides in (((0, most, most), (most, most, 1)), ((5, 0), (1, 1)), ((0,), (3,))):
         step(*[ctx.empty((1,)).view(extents, strides) for _ in range(4)])
+
+
+def test_scales_whose_base_2_form_is_not_finite_are_refused(ctx):
+    """Above 2.35e38 scale * log2(e), by which differences of logits are multiplied, is infinite, and 0 times that is no number."""
+    x, i, v, st, dx = ctx.empty((3, 50)), ctx.empty((3,), S.I32), ctx.empty((3,)), ctx.empty((3, 2)), ctx.empty((3, 50))
+    xv, iv = ctx.var(np.zeros((3, 50), np.float32)), ctx.var(np.zeros(3, np.int32))
+    calls = (lambda s: L.token_log_probs(x, i, v, scale=s), lambda s: L.token_log_probs_grad(x, i, st, v, v, v, dx, scale=s),
+             lambda s: L.token_log_probs_and_grad(x, i, v, v, ctx.empty((3,)), None, dx, scale=s), lambda s: S.token_log_probs(xv, iv, s))
+    for call in calls:
+        call(2.3e38)
+        for scale in (2.4e38, 3.4e38):
+            with pytest.raises(S.SageError) as e:
+                call(scale)
+            assert e.value.code == 1 and "scale" in str(e.value)
+    table = ctx.var(np.zeros((3, 50), np.float32))
+    for scale in (float("nan"), float("inf")):
+        with pytest.raises(S.SageError) as e:  # as the operator on tensors
+            S.embedding(table, iv, scale)
+        assert e.value.code == 1 and "scale" in str(e.value)
