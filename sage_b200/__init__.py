@@ -311,11 +311,7 @@ class Context:
     def wrap(self, address, extents, dtype=F32, strides=None):
         """A DeviceTensor over device memory that something else owns and keeps: `address` is its first element's.  No copy."""
         t = DeviceTensor(self, None, dtype, extents, strides)
-        last = 0
-        for e, s in zip(t.extents, t.strides):
-            last += (e - 1) * s
-        t.buf = _P()
-        self._ck(_buf_wrap(self.h, address, (last + 1) * _SIZE[dtype] if 0 not in t.extents else 0, t.buf))
+        t.buf = _Handle(self, address, t.extents, t.strides, dtype, None)
         return t
 
     def borrow(self, t):
@@ -327,13 +323,29 @@ class Context:
                 raise SageError(1, "borrow: no element type for %s" % t.dtype)
             _BORROWED[t.dtype] = dtype
         extents, strides = tuple(t.shape) or (1,), t.stride() or (1,)
-        n = 1 + sum([(e - 1) * s for e, s in zip(extents, strides)]) if 0 not in extents else 0
-        buf = _P()
-        if _buf_wrap(self.h, t.data_ptr(), n * _SIZE[dtype], buf):
-            self._ck(1)
+        buf = _Handle(self, t.data_ptr(), extents, strides, dtype, t)
         d = DeviceTensor.__new__(DeviceTensor)  # programs borrow hundreds of tensors at a time
         d.__dict__ = {"ctx": self, "buf": buf, "dtype": dtype, "extents": extents, "strides": strides, "offset": 0, "owner": True, "base": t}
         return d
+
+
+class _Handle(_P):
+    """A sage_buf over memory that something else owns (`base`, kept alive): released with the last tensor, view or C struct that has it."""
+
+    def __init__(self, ctx, address, extents, strides, dtype, base):
+        super().__init__()
+        n = 1 + sum([(e - 1) * s for e, s in zip(extents, strides)]) if 0 not in extents else 0
+        st = _buf_wrap(ctx.h, address, n * _SIZE[dtype], self)
+        if st:
+            ctx._ck(1)
+        self.ctx, self.base = ctx, base
+
+    def __del__(self):
+        try:
+            if self.value and self.ctx.h:  # (behind the context there is nothing to release it with)
+                lib.sage_free(self.ctx.h, self)
+        except Exception:
+            pass
 
 
 class DeviceTensor:
@@ -353,6 +365,7 @@ class DeviceTensor:
         t.buf, t.dtype, t.ndim, t.offset = self.buf, self.dtype, len(self.extents), self.offset
         n = t.ndim
         t.extents[:n], t.strides[:n] = self.extents, self.strides
+        t.handle = self.buf  # the struct has the address alone
         return t
 
     def ref(self):
@@ -375,6 +388,8 @@ class DeviceTensor:
     def release(self):
         if self.owner and self.buf:
             self.ctx.free(self.buf)
+            if isinstance(self.buf, _Handle):
+                self.buf.value = None  # views have it too
             self.buf = self._ref = None
 
 

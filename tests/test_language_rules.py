@@ -121,3 +121,81 @@ def test_scales_whose_base_2_form_is_not_finite_are_refused(ctx):
         with pytest.raises(S.SageError) as e:  # as the operator on tensors
             S.embedding(table, iv, scale)
         assert e.value.code == 1 and "scale" in str(e.value)
+
+
+# ------------------------------------------------------------------------------------------ memory of something else
+class Foreign:
+    """What Context.borrow takes of another package's tensor."""
+
+    def __init__(self, shape=(4, 8), stride=(8, 1), dtype="float32", address=0x10000):
+        self.shape, self._stride, self.dtype, self._address = shape, stride, dtype, address
+
+    def stride(self):
+        return self._stride
+
+    def data_ptr(self):
+        return self._address
+
+
+@pytest.fixture()
+def freed(monkeypatch):
+    """The handles that were released so far."""
+    free, handles = S.lib.sage_free, []
+
+    def counted(ctx, buf):
+        handles.append(buf.value)
+        return free(ctx, buf)
+
+    monkeypatch.setattr(S.lib, "sage_free", counted)
+    return handles
+
+
+def test_handles_of_borrowed_memory_go_with_their_last_holder(ctx, freed):
+    for make in (lambda: ctx.borrow(Foreign()), lambda: ctx.wrap(0x10000, (4, 8))):
+        del freed[:]
+        t = make()
+        handle = t.buf.value
+        del t
+        assert freed == [handle]
+        view = make().view((8,), (1,), 8)  # a view, a struct and a reference each keep it
+        assert len(freed) == 1 and S.lib.sage_buf_size(view.buf) == 4 * 8 * 4
+        struct = view.c()
+        del view
+        assert len(freed) == 1 and struct.buf
+        del struct
+        assert len(freed) == 2
+        assert S.lib.sage_softmax(ctx.h, make().ref(), S.ctypes.c_int64(4), S.ctypes.c_int64(8), make().ref()) == 0
+        assert len(freed) == 4
+        tensors = L.AdamWTensors(ctx, [L.adamw_tensor(*[make() for _ in range(4)])])
+        L.adamw_step(tensors, step=1, lr=1e-3)
+        assert len(freed) == 4
+        del tensors
+        assert len(freed) == 8
+        t = make()
+        view = t.view((8,), (1,))
+        t.release()  # at once; nothing is left to release behind it, and views have lost it too
+        t.release()
+        assert len(freed) == 9
+        with pytest.raises(S.SageError):
+            L.embedding(view, view, view)
+        del t, view
+        assert len(freed) == 9
+
+
+def test_borrowed_memory_stays_while_a_view_has_it(ctx):
+    import weakref
+    foreign = Foreign()
+    alive = weakref.ref(foreign)
+    view = ctx.borrow(foreign).view((8,), (1,))
+    del foreign
+    assert alive() is not None
+    del view
+    assert alive() is None
+
+
+def test_handles_that_outlive_their_context(freed):
+    c = S.Context(-1)
+    t = c.borrow(Foreign())
+    c.close()
+    del t
+    assert not freed
