@@ -337,7 +337,7 @@ class _Handle(_P):
         n = 1 + sum([(e - 1) * s for e, s in zip(extents, strides)]) if 0 not in extents else 0
         st = _buf_wrap(ctx.h, address, n * _SIZE[dtype], self)
         if st:
-            ctx._ck(1)
+            ctx._ck(st)
         self.ctx, self.base = ctx, base
 
     def __del__(self):

@@ -199,3 +199,11 @@ def test_handles_that_outlive_their_context(freed):
     c.close()
     del t
     assert not freed
+
+
+def test_borrowing_reports_the_failure_that_it_met(ctx, monkeypatch):
+    monkeypatch.setattr(S, "_buf_wrap", lambda *a: 4)
+    for make in (lambda: ctx.borrow(Foreign()), lambda: ctx.wrap(0x10000, (4, 8))):
+        with pytest.raises(S.SageError) as e:
+            make()
+        assert e.value.code == 4
