@@ -334,6 +334,8 @@ class _Handle(_P):
 
     def __init__(self, ctx, address, extents, strides, dtype, base):
         super().__init__()
+        if min(extents, default=0) < 0 or min(strides, default=0) < 0:
+            raise SageError(1, "memory of something else: negative extents or strides")
         n = 1 + sum([(e - 1) * s for e, s in zip(extents, strides)]) if 0 not in extents else 0
         st = _buf_wrap(ctx.h, address, n * _SIZE[dtype], self)
         if st:

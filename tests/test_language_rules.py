@@ -207,3 +207,11 @@ def test_borrowing_reports_the_failure_that_it_met(ctx, monkeypatch):
         with pytest.raises(S.SageError) as e:
             make()
         assert e.value.code == 4
+
+
+def test_memory_of_something_else_has_no_negative_strides(ctx):
+    """A size worked out of them would reach over all memory."""
+    for make in (lambda: ctx.wrap(0x10000, (4,), S.F32, (-1,)), lambda: ctx.wrap(0x10000, (-4,)), lambda: ctx.borrow(Foreign((4, 8), (-8, 1)))):
+        with pytest.raises(S.SageError) as e:
+            make()
+        assert e.value.code == 1
