@@ -311,7 +311,7 @@ class Context:
     def wrap(self, address, extents, dtype=F32, strides=None):
         """A DeviceTensor over device memory that something else owns and keeps: `address` is its first element's.  No copy."""
         t = DeviceTensor(self, None, dtype, extents, strides)
-        t.buf = _Handle(self, address, t.extents, t.strides, dtype, None)
+        t.buf = _Handle.over(self, address, t.extents, t.strides, dtype, None)
         return t
 
     def borrow(self, t):
@@ -323,7 +323,7 @@ class Context:
                 raise SageError(1, "borrow: no element type for %s" % t.dtype)
             _BORROWED[t.dtype] = dtype
         extents, strides = tuple(t.shape) or (1,), t.stride() or (1,)
-        buf = _Handle(self, t.data_ptr(), extents, strides, dtype, t)
+        buf = _Handle.over(self, t.data_ptr(), extents, strides, dtype, t)
         d = DeviceTensor.__new__(DeviceTensor)  # programs borrow hundreds of tensors at a time
         d.__dict__ = {"ctx": self, "buf": buf, "dtype": dtype, "extents": extents, "strides": strides, "offset": 0, "owner": True, "base": t}
         return d
@@ -332,15 +332,19 @@ class Context:
 class _Handle(_P):
     """A sage_buf over memory that something else owns (`base`, kept alive): released with the last tensor, view or C struct that has it."""
 
-    def __init__(self, ctx, address, extents, strides, dtype, base):
-        super().__init__()
-        if min(extents, default=0) < 0 or min(strides, default=0) < 0:
-            raise SageError(1, "memory of something else: negative extents or strides")
-        n = 1 + sum([(e - 1) * s for e, s in zip(extents, strides)]) if 0 not in extents else 0
-        st = _buf_wrap(ctx.h, address, n * _SIZE[dtype], self)
+    @staticmethod
+    def over(ctx, address, extents, strides, dtype, base):
+        n = 1
+        for e, s in zip(extents, strides):
+            if e < 0 or s < 0:
+                raise SageError(1, "memory of something else: negative extents or strides")
+            n += (e - 1) * s
+        h = _Handle()
+        st = _buf_wrap(ctx.h, address, n * _SIZE[dtype] if 0 not in extents else 0, h)
         if st:
             ctx._ck(st)
-        self.ctx, self.base = ctx, base
+        h.ctx, h.base = ctx, base
+        return h
 
     def __del__(self):
         try:
