@@ -429,6 +429,12 @@ __device__ void block_top(const RowVectors<T> &row, int begin, int end, float th
     __syncthreads();
 }
 
+// scale (x - m) - ln S, where x - m is beyond f32 too.
+__device__ __forceinline__ float log_prob(float x, float base, float scale, float ln_s) {
+    const float d = x - base;
+    return (fabsf(d) <= FLT_MAX ? d * scale : x * scale - base * scale) - ln_s;
+}
+
 // ------------------------------------------------------------------------------------------ values
 // A cluster of 2^shift CTAs for each row; each reads a part of it once, and the running maximum and sums are joined over lanes, warps and CTAs.
 // Bound by memory in many rows (8192 x 50021 f32: 259 us, 6.3 TB/s), by the chain of joins in few (1 x 30522: 6 us with 5 alternatives).
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     const float base = base_of(all.m), ln_s = logf(all.s);
     const bool none = all.s == 0.f;
     if (threadIdx.x == 0) {
-        if (a.log_probs.ptr) ((float *)a.log_probs.ptr)[r * a.log_probs.stride] = !scored ? 0.f : none ? -INFINITY : (own - base) * a.scale - ln_s;
+        if (a.log_probs.ptr) ((float *)a.log_probs.ptr)[r * a.log_probs.stride] = !scored ? 0.f : none ? -INFINITY : log_prob(own, base, a.scale, ln_s);
         if (a.entropy.ptr) ((float *)a.entropy.ptr)[r * a.entropy.stride] = none ? 0.f : ln_s - kLn2 * (all.w / all.s);
         if (a.stats.ptr) {
             ((float *)a.stats.ptr)[r * a.stats.pitch] = all.m;
@@ -499,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(cons
     if (TOP && (int)threadIdx.x < a.top) {
         const unsigned long long key = top.best[lane];
         ((int *)a.top_ids.ptr)[r * a.top_ids.pitch + lane] = (int)(0xffffffffu - (unsigned)key);
-        if (a.top_log_probs.ptr) ((float *)a.top_log_probs.ptr)[r * a.top_log_probs.pitch + lane] = none ? -INFINITY : (rank_logit(key) - base) * a.scale - ln_s;
+        if (a.top_log_probs.ptr) ((float *)a.top_log_probs.ptr)[r * a.top_log_probs.pitch + lane] = none ? -INFINITY : log_prob(rank_logit(key), base, a.scale, ln_s);
     }
 }
 
@@ -688,7 +694,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_and_grad_ke
             constants.set(all.m, all.s, ln_s, a.scale, asked.g_log_prob, asked.g_entropy, h, asked.id);
             constants.scale_first<T>();
         } else if (lane == 1 && rank == 0) {
-            ((float *)log_probs.ptr)[r * log_probs.stride] = asked.id < 0 ? 0.f : none ? -INFINITY : (asked.own - base_of(all.m)) * a.scale - ln_s;
+            ((float *)log_probs.ptr)[r * log_probs.stride] = asked.id < 0 ? 0.f : none ? -INFINITY : log_prob(asked.own, base_of(all.m), a.scale, ln_s);
             if (entropy.ptr) ((float *)entropy.ptr)[r * entropy.stride] = h;
         }
     }

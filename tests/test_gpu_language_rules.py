@@ -99,3 +99,36 @@ def test_codes_near_the_middle_of_two(ctx, moment, first, last):
         x.release()
     assert np.array_equal(got[2], ms) and np.array_equal(got[3], vs)
     assert (got[0] != mc).sum() == 0 and (got[1] != vc).sum() == 0
+
+
+# ------------------------------------------------------------------------------------------ differences beyond f32
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(3, 40), (2, 70001)])
+def test_log_probabilities_of_logits_further_apart_than_f32_reaches(ctx, kind, rows, vocab):
+    """Masks of the type's lowest value beside logits of 2e38: their difference is beyond f32, a quarter of it is not."""
+    rng = np.random.default_rng(vocab)
+    x = np.full((rows, vocab), -3.38e38)
+    x[:, 3:9] = rng.uniform(1.9e38, 2e38, (rows, 6))
+    x[:, 7] = 2.5e38
+    raw, x = O.stored(x, kind)
+    ids = np.zeros(rows, np.int32)
+    ids[1] = 7
+    want = O.LogProbs(x, ids, 0.25)
+    t, i = ctx.tensor(raw, S.BF16 if kind == "bf16" else S.F32), ctx.tensor(ids)
+    lp, h, dx, one = ctx.empty((rows,)), ctx.empty((rows,)), ctx.empty((rows, vocab), t.dtype), ctx.tensor(np.ones(rows, np.float32))
+    top_ids, top = ctx.empty((rows, 8), S.I32), ctx.empty((rows, 8))
+
+    def close(got, value, bound):
+        assert np.isfinite(value).all() and (np.abs(got.astype(np.float64) - value) <= bound).all(), (got, value)
+
+    L.token_log_probs(t, i, lp, h, top_ids=top_ids, top_log_probs=top, scale=0.25)
+    close(lp.numpy(), want.log_probs, want.tol_log_probs)
+    order, value, bound = want.top(8)
+    assert np.array_equal(top_ids.numpy(), order)
+    close(top.numpy(), value, bound)
+    L.token_log_probs_and_grad(t, i, one, one, lp, h, dx, scale=0.25)
+    close(lp.numpy(), want.log_probs, want.tol_log_probs)
+    g, bound = want.grad(1.0, 1.0, kind)
+    close(O.values(dx.numpy(), kind), g, bound)
+    for x in (t, i, lp, h, dx, one, top_ids, top):
+        x.release()
