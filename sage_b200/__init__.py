@@ -115,6 +115,7 @@ class Context:
         st = lib.sage_ctx_create(int(device), ctypes.byref(o), ctypes.byref(self.h))
         if st:
             raise SageError(st, "cannot create a context on device %d (no CUDA device?)" % device)
+        self.released = 0  # device tensors so far: who has prepared some looks again when others have gone
         self.s = _P()
         self._ck(lib.sage_session_create(self.h, ctypes.byref(self.s)))
         self.device = device
@@ -375,8 +376,8 @@ class DeviceTensor:
         return t
 
     def ref(self):
-        """c() by reference, made once: a handle's view does not change."""
-        if getattr(self, "_ref", None) is None:
+        """c() by reference, made once: a handle's view does not change until it is released."""
+        if getattr(self, "_ref", None) is None or not self.buf:
             self._c = self.c()
             self._ref = ctypes.byref(self._c)
         return self._ref
@@ -394,9 +395,10 @@ class DeviceTensor:
     def release(self):
         if self.owner and self.buf:
             self.ctx.free(self.buf)
-            if isinstance(self.buf, _Handle):
+            if isinstance(self.buf, _P):
                 self.buf.value = None  # views have it too
             self.buf = self._ref = None
+            self.ctx.released += 1
 
 
 # --------------------------------------------------------------------------- Var

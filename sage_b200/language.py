@@ -8,7 +8,7 @@ forms of the same operators are `sage_b200.embedding`, `token_log_probs`, `top_t
 """
 import ctypes
 
-from . import CTensor, lib
+from . import CTensor, SageError, lib
 
 _F = ctypes.c_float
 
@@ -62,7 +62,7 @@ def adamw_tensor(param, grad, m, v, m_scale=None, v_scale=None, copy=None):
 
 
 class AdamWTensors:
-    """The tensors of an update as the library takes them; made once, used for every step."""
+    """The tensors of an update as the library takes them; made once, used for every step until one of them is released."""
 
     def __init__(self, ctx, tensors):
         self.ctx, self.tensors = ctx, list(tensors)  # keeps the operands alive
@@ -71,12 +71,21 @@ class AdamWTensors:
             for name, t in zip(_OPERANDS, operands):
                 if t is not None:
                     setattr(slot, name, t.c())
+        self.released = ctx.released
+
+    def ready(self):
+        """The array, behind a look at the operands if any tensor was released since the last one."""
+        if self.released != self.ctx.released:
+            if any(t is not None and not t.buf for operands in self.tensors for t in operands):
+                raise SageError(1, "adamw_step: an operand was released")
+            self.released = self.ctx.released
+        return self.array
 
 
 def adamw_step(tensors, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, grad_scale=1.0):
     """One AdamW update of all tensors in place; `step` counts from 1."""
     o = _AdamWOpts(lr, beta1, beta2, eps, weight_decay, grad_scale, step)
-    tensors.ctx._ck(lib.sage_adamw_step(tensors.ctx.h, tensors.array, len(tensors.tensors), ctypes.byref(o)))
+    tensors.ctx._ck(lib.sage_adamw_step(tensors.ctx.h, tensors.ready(), len(tensors.tensors), ctypes.byref(o)))
 
 
 def adamw_states(m, m_scale, v, v_scale, m_out, v_out):

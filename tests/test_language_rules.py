@@ -215,3 +215,23 @@ def test_memory_of_something_else_has_no_negative_strides(ctx):
         with pytest.raises(S.SageError) as e:
             make()
         assert e.value.code == 1
+
+
+def test_released_tensors_are_refused_wherever_they_were_prepared(ctx):
+    """Views, references and prepared updates hold a buffer's address; once it is released there is nothing behind it."""
+    make = (lambda: ctx.empty((8,))), (lambda: ctx.borrow(Foreign((8,), (1,))))
+    for new in make:
+        t = [new() for _ in range(4)]
+        update = L.AdamWTensors(ctx, [L.adamw_tensor(*t)])
+        parts = L.AdamWTensors(ctx, [L.adamw_tensor(*[x.view((4,), (1,), 4) for x in t])])
+        view, ids, y = t[0].view((2, 4), (4, 1)), ctx.empty((1,), S.I32), ctx.empty((1, 4))
+        L.embedding(view, ids, y)
+        L.adamw_step(update, step=1, lr=1e-3)
+        new().release()  # others do not matter
+        L.adamw_step(update, step=2, lr=1e-3)
+        t[0].release()
+        for call in (lambda: L.adamw_step(update, step=3, lr=1e-3), lambda: L.adamw_step(parts, step=3, lr=1e-3), lambda: L.embedding(view, ids, y), lambda: L.embedding(t[0], ids, y)):
+            for _ in range(2):
+                with pytest.raises(S.SageError) as e:
+                    call()
+                assert e.value.code == 1 and ("released" in str(e.value) or "missing" in str(e.value)), str(e.value)
