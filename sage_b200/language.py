@@ -71,12 +71,13 @@ class AdamWTensors:
             for name, t in zip(_OPERANDS, operands):
                 if t is not None:
                     setattr(slot, name, t.c())
+        self.handles = [t.buf for operands in self.tensors for t in operands if t is not None]
         self.released = ctx.released
 
     def ready(self):
         """The array, behind a look at the operands if any tensor was released since the last one."""
         if self.released != self.ctx.released:
-            if any(t is not None and not t.buf for operands in self.tensors for t in operands):
+            if not all(self.handles):
                 raise SageError(1, "adamw_step: an operand was released")
             self.released = self.ctx.released
         return self.array
