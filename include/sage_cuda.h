@@ -310,8 +310,9 @@ sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logi
  *   param = param (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
  * param f32, grad f32 / f16 / bf16, contiguous, of the same number of elements.  The states m, v are f32 (m_scale, v_scale
  * unused, buf NULL), or m i8 and v u8 with f32 scales, one for each 256 elements of the tensor: |m| = m_scale code^2, sqrt(v) =
- * v_scale code^2; zeroed codes and scales are zero states.  No tensor may appear twice in a call.  A second moment that is not zero does not become zero; a block in which a
- * moment is not finite has a scale that is NaN.  `copy` (buf NULL: none) receives the updated parameters in f16 / bf16.  States of all
+ * v_scale code^2; zeroed codes and scales are zero states.  No tensor may appear twice in a call.  A second moment that is not zero has a code of 1 at least, so it does not become
+ * zero where its block's largest is 2^-117 or more; a block in which a moment is not finite has a scale that is NaN.  Second moments below 2^-126 count as zero
+ * beside eps.  `copy` (buf NULL: none) receives the updated parameters in f16 / bf16.  States of all
  * tensors of a call have the same width.  step counts from 1; eps is 1e-15 at least. */
 typedef struct {
     sage_tensor param, grad, m, v, m_scale, v_scale, copy;

@@ -316,7 +316,8 @@ class Context:
         return t
 
     def borrow(self, t):
-        """wrap() of a device tensor of another package (a torch.Tensor: data_ptr(), shape, stride(), dtype), which is kept alive."""
+        """wrap() of a device tensor of another package (a torch.Tensor: data_ptr(), shape, stride(), dtype), which is kept alive
+        until the last tensor or view over it goes."""
         dtype = _BORROWED.get(t.dtype)
         if dtype is None:
             dtype = _BY_NAME.get(str(t.dtype).split(".")[-1])

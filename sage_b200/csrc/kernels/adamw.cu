@@ -7,7 +7,7 @@
 // root decides a code unless its result lies so near the middle of two codes that it could err, where the exact one does.
 //
 // A warp takes a block of 256 elements at a time, eight to a lane.  Bound by memory: 28 bytes an element with f32 states and gradients (109 M:
-// 480 us, 6.4 TB/s), 16 with 8-bit states, bf16 gradients and a copy (334 M: 941 us, 5.7 TB/s, the instructions that find the codes at 64 %
+// 483 us, 6.3 TB/s), 16 with 8-bit states, bf16 gradients and a copy (334 M: 957 us, 5.6 TB/s, the instructions that find the codes at 64 %
 // of their slots beside it).
 #include <cuda_runtime.h>
 
@@ -28,7 +28,9 @@ struct Batch {
     unsigned first[SLOTS + 1];  // prefix sums of the slots' blocks of 256 elements
     int count;
 };
-constexpr int kSlots = 400, kFewSlots = 40;  // 32 KB of kernel parameters, 3 KB
+// 32 KB of kernel parameters, or 3 KB for short lists: a launch's parameters are copied with it (4, 20 and 38 tensors of 4000 elements: 3.9, 4.1 and 4.5 us
+// a step with the short list, 5.3, 5.7 and 6.2 with the long one; 54 tensors 6.5, 300 13).
+constexpr int kSlots = 400, kFewSlots = 40;
 
 __device__ __forceinline__ float fast_root(float x) {  // 2^-23 off at most, of subnormal numbers 0
     float y;
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(256, STATES8 ? 3 : 4) adamw_kernel(const __gri
     }
 }
 
-// Values of codes: four to a thread where `wide`, else one.  Bound by memory: 2 bytes read, 8 written (334 M: 586 us, 5.7 TB/s).
+// Values of codes: four to a thread where `wide`, else one.  Bound by memory: 2 bytes read, 8 written (334 M: 580 us, 5.8 TB/s).
 template <bool WIDE>
 __global__ void __launch_bounds__(256) adamw_states_kernel(const signed char *m, const float *m_scale, const unsigned char *v, const float *v_scale, long long n, float *m_out, float *v_out) {
     grid_dependency_sync();
@@ -448,7 +450,6 @@ static sage_status step_batches(Context &ctx, const AdamWSlot *slots, int count,
 }
 
 sage_status adamw_step(Context &ctx, const AdamWSlot *slots, int count, bool states8, const AdamWRule &rule) {
-    // Parameters of a launch are copied with it: a short list where it holds all tensors.
     return count <= kFewSlots ? step_batches<kFewSlots>(ctx, slots, count, states8, rule) : step_batches<kSlots>(ctx, slots, count, states8, rule);
 }
 

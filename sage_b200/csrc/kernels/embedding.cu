@@ -14,7 +14,7 @@ namespace {
 
 // ------------------------------------------------------------------------------------------ lookup
 // A thread moves V elements at a time (16 bytes of the table, or one element where rows do not lie on 16-byte boundaries), four of
-// them in flight.  Bound by memory: the tokens' rows read, the results written (32768 x 4096 bf16: 92 us, 5.8 TB/s; 8 x 768: 4.1, a launch).
+// them in flight.  Bound by memory: the tokens' rows read, the results written (32768 x 4096 bf16: 91 us, 5.9 TB/s; 8 x 768: 4.0, a launch).
 constexpr int kLookups = 4;
 template <class T, class Y, int V>
 __global__ void __launch_bounds__(256) embedding_kernel(const T *__restrict__ table, long long vocab, long long ld, const int *__restrict__ ids, long long ids_stride, float scale, Y *__restrict__ y,
@@ -97,8 +97,11 @@ struct Zeros {
 // Sorting.  Each of 2^bits blocks owns the table rows whose numbers end in its own (frequent tokens have low numbers: neighbours go to
 // different blocks).  Its warps, each over a share of the tokens, count its rows' tokens, the counts become places (in front of them
 // all tokens of the blocks before), and a second pass puts the tokens there.  Up to kDealFrom tokens every block reads all ids for that: one
-// launch, but 128 times the ids out of L2 (65 521 of them: sorting 19 us, dealt out first 15 in all).  Above, a launch in front deals the ids out, 1024 to a
-// block, so that a sorting block finds its tokens of them together.
+// launch, but the ids once for each sorting block out of L2, 128 times for tables of up to 131 072 rows.  Above, a launch in front deals the ids out,
+// 1024 to a block, so that a sorting block finds its tokens of them together.  The whole gradient, added, undealt and dealt: 16 384 x 768 f32 into
+// 30 522 rows 31 and 36 us, 32 768 44 and 49, 65 536 70 and 72, 131 072 151 and 113; 32 768 x 256 bf16 into 131 072 rows 32 and 32; 262 144 x 256 f32 into as many
+// 244 and 166.  Dealing knows 2^kDealBits sorting blocks, those of up to 524 288 rows.  Larger tables have 1024 and more, which read all ids
+// whatever their number: 65 536 x 128 f32 into 524 288 rows 53 us, into one row more 95; 262 144 103 us, into 1 048 576 rows 293.
 constexpr int kSortWarps = 32, kSortRows = 1024, kSortList = 256;  // rows of a block and own tokens of a warp that shared memory holds
 constexpr int kDealFrom = 16384, kDealTokens = 1024, kDealThreads = 256, kDealBits = 9;
 
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) embedding_sort_kernel(const I
 // in their order.  Further blocks write the rows that no token reaches.
 // Bound by memory: g once, the table once.  Each thread copies its own columns of the next tokens into shared memory asynchronously (no
 // barriers, and no registers that wait for them): kAhead rows of the block in flight, five blocks of 256 threads on an SM.
-// The whole gradient of 4096 x 768 f32 into 30522 rows: 23.5 us, of which sorting is 8; of 65521 x 1000 bf16 added to 50021 rows: 67 us, of which
+// The whole gradient of 4096 x 768 f32 into 30522 rows: 22.5 us, of which sorting is 8; of 65521 x 1000 bf16 added to 50021 rows: 66 us, of which
 // sorting is 15; of 65536 x 4096 bf16 added to 131072: 208 us, 5.6 TB/s.
 struct EmbeddingGrad {
     const void *g;
@@ -444,7 +447,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const __grid_consta
         int row = rows[1];
         for (int i0 = 0; i0 < n; i0 += kAhead) {
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {  // the places of the ring at fixed offsets (4096 x 768 f32 25.5 -> 23.5 us, 65521 x 1000 bf16 69 -> 67)
+            for (int u = 0; u < kAhead; ++u) {  // the places of the ring at fixed offsets: 2 us less in both of the cases above
                 const int i = i0 + u;
                 if (i >= n) break;
                 asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
@@ -563,8 +566,9 @@ sage_status embedding_grad(Context &ctx, const RowsArg &g, const VectorArg &ids,
     length = length < 16 ? 16 : length > kMaxLength ? kMaxLength : (length + 7) / 8 * 8;
     const long long chunks = (tokens + length - 1) / length;
     // Rows that no token reaches become zero beside the sums.  24 MB of the table are cleared beside the sorting already, which leaves the memory
-    // idle, whether tokens reach them or not: the last rows, since frequent tokens have low numbers (4096 x 768 into 30522 rows: 25.4 us, none
-    // early 28.3, 36 MB 28.6, all 32.3).
+    // idle, whether tokens reach them or not: the last rows, since frequent tokens have low numbers (with 0, 12, 24 and 48 MB: 512 x 768
+    // into 30522 rows 21.1, 19.9, 19.4, 20.1 us; 4096 24.9, 23.6, 22.7, 23.6; 16384 44.7, 43.4, 40.2, 41.9; 65536 74.5, 74.6, 72.2, 72.5; 4096 x 1024 into
+    // 131072 86.3, 84.6, 83.3, 82.6; 8192 x 512 into 8000, 16 MB in all, 20.2, 21.0, 21.5, 21.8; 32768 x 4096 into 131072 403, 409, 408, 406).
     const long long early_rows = add ? 0 : std::min(vocab, (24ll << 20) / (dim * 4)), late_rows = add ? 0 : vocab - early_rows, zero_blocks = (late_rows + kZeroRows - 1) / kZeroRows;
     if (chunks * slices + zero_blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "embedding_grad: too many rows");
     const auto rounded = [](long long words) { return (words + 63) / 64 * 64; };

@@ -200,8 +200,8 @@ __device__ __forceinline__ void add_vectors(Sums &a, const uint4 (&v)[U], float 
 // Where the largest logit is of ordinary size, differences may be scaled first: t = fma(c2, x, -b) with b = c2 m, rounded once and the same for all,
 // is as exact, and one instruction less for two elements; and 16-bit logits can be held at m + kLeast / c2, two to an instruction, in place of t.
 // `least`: that bound, or Bits<T>::kFill where this form is not open (b large, its rounding then reaching kLeast; the bound not finite).  Values and
-// gradient: 4096 x 131072 f32 811 us without it, 796 with, 8192 x 32000 bf16 211 and 208, 8192 x 131072 bf16 864 and 867; for a second on end, with the
-// clock down to 1.8 GHz at the power limit, 4096 x 131072 f32 817 and 801, 8192 x 131072 bf16 890 and 886.
+// gradient without it and with it, on one GPU: 4096 x 131072 f32 811 and 796 us, 8192 x 32000 bf16 211 and 208; for a second on end, with the clock down
+// to 1.8 GHz at the power limit, 4096 x 131072 f32 817 and 801.  8192 x 131072 bf16 is the same with both.
 template <class T>
 struct Ordinary {
     float b, rest;  // t relative to b is t relative to m, plus `rest`
@@ -244,7 +244,7 @@ __device__ __forceinline__ void sum_vectors(Sums &a, const uint4 (&v)[U], float 
     a.w = f * (w.x + w.y - o.rest * all);
 }
 // Of the warp's lanes: the largest m first, then sums relative to it.  In all lanes; or, where those behind the first LANES have nothing, in
-// these (8192 x 131072 bf16 with its gradient: 876 us with 32 everywhere, 861 with as many as there are warps and CTAs).
+// these (8192 x 131072 bf16 with its gradient: 1.7 % less with as many lanes as there are warps and CTAs than with 32 everywhere).
 template <int LANES = 32>
 __device__ __forceinline__ Sums warp_join(Sums a, float c2) {
     float m;
@@ -437,7 +437,7 @@ __device__ __forceinline__ float log_prob(float x, float base, float scale, floa
 
 // ------------------------------------------------------------------------------------------ values
 // A cluster of 2^shift CTAs for each row; each reads a part of it once, and the running maximum and sums are joined over lanes, warps and CTAs.
-// Bound by memory in many rows (8192 x 50021 f32: 259 us, 6.3 TB/s), by the chain of joins in few (1 x 30522: 6 us with 5 alternatives).
+// Bound by memory in many rows (8192 x 50021 f32: 268 us, 6.1 TB/s), by the chain of joins in few (1 x 30522: 6 us with 5 alternatives).
 template <class T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(const LogProbs a, const int shift) {
     constexpr int U = 4;
@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(256) log_probs_grad_kernel(const LogProbsGrad 
 
 // Values and gradient together: a cluster holds its row in registers (NV vectors for each thread) between the sums and the
 // gradient, so the logits are read once.  All CTAs of the cluster give their sums to all.  Bound by memory and by the joins
-// that each row waits for between its loads and its stores (8192 x 131072 bf16: 865 us, 5.0 TB/s; without the joins it would be
+// that each row waits for between its loads and its stores (8192 x 131072 bf16: 915 us, 4.7 TB/s; without the joins it would be
 // 657), so nothing else is left to be waited for there: what the row is asked about is fetched beside its logits (8192 x 50021
 // bf16: 384 us with those loads behind the join, 369 beside; 4096 x 131072 f32: 865 and 818).
 template <class T, int THREADS, int NV>
@@ -716,8 +716,9 @@ int log2_of(int power) { return __builtin_ctz((unsigned)power); }
 
 // The block's size: small blocks, of which more run on an SM, interleave reading and joining better, as long as there are rows for them (8192 x
 // 50021 f32: 259, 269 and 283 us with 128, 256 and 512 threads; 16384 x 8000: 85, 103 and 148); with few rows the largest, a cluster of eight of
-// which reads a row fastest (64 x 131072 bf16 with 20 alternatives: 15.5 us with 256 threads, 12.1 with 512).  Alternatives are found
-// by few threads, which have more to read again in long rows of small blocks (3000 x 131072 bf16 with 20: 234 us with 128 threads, 191 with 256).
+// which reads a row fastest (64 x 131072 bf16 with 20 alternatives: 14.4 us with 256 threads, 10.8 with 512; 19.2 and 16.7 where masks leave parts of
+// rows empty; 73 rows 14.8 and 17.5).  Alternatives are found by few threads, which have more to read again in long rows of small
+// blocks (3000 x 131072 bf16 with 20: 234 us with 128 threads, 191 with 256).
 int threads_of_rows(long long rows, long long bytes, bool top, int sms) {
     if (bytes <= 16384 || (rows >= 16ll * sms && (!top || bytes <= 65536))) return 128;
     return rows * kMaxCluster < 4ll * sms ? 512 : 256;
@@ -796,7 +797,7 @@ sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const 
     constexpr int NV = 8;
     const long long vectors = most_vectors(a.logits);
     // The smallest blocks eight of which hold a row: more of them run on an SM, and loads, sums and stores of different ones interleave (8192
-    // x 131072 bf16: 852 us with 256 threads, 992 with 512; 8192 x 50021: 387, 484 and 540 with 128, 256 and 512).
+    // x 131072 bf16: 16 % more time with 512 threads than with 256; 8192 x 50021: 25 % more with 256 than with 128, 40 % with 512).
     const int threads = vectors <= kMaxCluster * 128 * NV ? 128 : vectors <= kMaxCluster * 256 * NV ? 256 : 512;
     int parts = (int)std::min((vectors + threads * NV - 1) / (threads * NV), kMaxCluster + 1ll);
     // Rows that fit the registers of a cluster.
