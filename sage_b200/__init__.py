@@ -368,11 +368,15 @@ class DeviceTensor:
                 p *= e
         self.strides = tuple(map(int, strides))
 
+    def fill(self, t):
+        """The fields of a C struct; who keeps it keeps this tensor's buffer."""
+        t.buf, t.dtype, t.offset = self.buf, self.dtype, self.offset
+        t.ndim = n = len(self.extents)
+        t.extents[:n], t.strides[:n] = self.extents, self.strides
+
     def c(self):
         t = CTensor()
-        t.buf, t.dtype, t.ndim, t.offset = self.buf, self.dtype, len(self.extents), self.offset
-        n = t.ndim
-        t.extents[:n], t.strides[:n] = self.extents, self.strides
+        self.fill(t)
         t.handle = self.buf  # the struct has the address alone
         return t
 

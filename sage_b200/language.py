@@ -70,7 +70,7 @@ class AdamWTensors:
         for slot, operands in zip(self.array, self.tensors):
             for name, t in zip(_OPERANDS, operands):
                 if t is not None:
-                    setattr(slot, name, t.c())
+                    t.fill(getattr(slot, name))
         self.handles = [t.buf for operands in self.tensors for t in operands if t is not None]
         self.released = ctx.released
 
