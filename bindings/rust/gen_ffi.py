@@ -14,7 +14,8 @@ OUT = os.path.join(HERE, "src", "backend", "cuda", "ffi.rs")
 SCALARS = {"sage_status": "i32", "int32_t": "i32", "int64_t": "i64", "uint64_t": "u64", "uint32_t": "u32", "uint8_t": "u8",
            "size_t": "usize", "float": "f32", "double": "f64", "char": "c_char", "void": "c_void"}
 OPAQUE = ["sage_ctx", "sage_buf", "sage_module"]
-STRUCTS = ["sage_tensor", "sage_ctx_opts", "sage_mem_stats_t", "sage_arg", "sage_window", "sage_adamw_tensor", "sage_adamw_opts"]
+STRUCTS = ["sage_tensor", "sage_ctx_opts", "sage_mem_stats_t", "sage_arg", "sage_window", "sage_adamw_tensor", "sage_adamw_opts", "sage_block_norms_opts",
+           "sage_block_norms_sums"]
 
 PRELUDE = '''// GENERATED by bindings/rust/gen_ffi.py from include/sage_cuda.h — do not edit by hand.
 //
@@ -68,6 +69,13 @@ pub struct sage_adamw_tensor {
 }
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct sage_adamw_opts { pub lr: f64, pub beta1: f64, pub beta2: f64, pub eps: f64, pub weight_decay: f64, pub grad_scale: f64, pub step: i64 }
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sage_block_norms_opts {
+    pub after_weight: sage_tensor, pub after_bias: sage_tensor, pub before_weight: sage_tensor, pub before_bias: sage_tensor, pub gate: sage_tensor, pub seed: sage_tensor,
+    pub after: i32, pub before: i32, pub residual_scale: f32, pub eps: f32, pub p: f32, pub site: u64,
+}
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sage_block_norms_sums { pub after_weight: sage_tensor, pub after_bias: sage_tensor, pub before_weight: sage_tensor, pub before_bias: sage_tensor, pub gate: sage_tensor }
 
 #[link(name = "sagecuda")]
 extern "C" {

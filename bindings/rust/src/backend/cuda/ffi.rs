@@ -50,6 +50,13 @@ pub struct sage_adamw_tensor {
 }
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct sage_adamw_opts { pub lr: f64, pub beta1: f64, pub beta2: f64, pub eps: f64, pub weight_decay: f64, pub grad_scale: f64, pub step: i64 }
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sage_block_norms_opts {
+    pub after_weight: sage_tensor, pub after_bias: sage_tensor, pub before_weight: sage_tensor, pub before_bias: sage_tensor, pub gate: sage_tensor, pub seed: sage_tensor,
+    pub after: i32, pub before: i32, pub residual_scale: f32, pub eps: f32, pub p: f32, pub site: u64,
+}
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct sage_block_norms_sums { pub after_weight: sage_tensor, pub after_bias: sage_tensor, pub before_weight: sage_tensor, pub before_bias: sage_tensor, pub gate: sage_tensor }
 
 #[link(name = "sagecuda")]
 extern "C" {
@@ -104,6 +111,9 @@ extern "C" {
     pub fn sage_token_log_probs(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, log_probs: *const sage_tensor, entropy: *const sage_tensor, stats: *const sage_tensor, top_ids: *const sage_tensor, top_log_probs: *const sage_tensor) -> i32;
     pub fn sage_token_log_probs_grad(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, stats: *const sage_tensor, entropy: *const sage_tensor, g_log_probs: *const sage_tensor, g_entropy: *const sage_tensor, dlogits: *const sage_tensor) -> i32;
     pub fn sage_token_log_probs_and_grad(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, g_log_probs: *const sage_tensor, g_entropy: *const sage_tensor, log_probs: *const sage_tensor, entropy: *const sage_tensor, dlogits: *const sage_tensor) -> i32;
+    pub fn sage_dropout(ctx: *mut sage_ctx, x: *const sage_tensor, y: *const sage_tensor, seed: *const sage_tensor, p: f32, site: u64) -> i32;
+    pub fn sage_block_norms(ctx: *mut sage_ctx, opts: *const sage_block_norms_opts, x: *const sage_tensor, y: *const sage_tensor, out: *const sage_tensor, h: *const sage_tensor, stats: *const sage_tensor) -> i32;
+    pub fn sage_block_norms_grad(ctx: *mut sage_ctx, opts: *const sage_block_norms_opts, out: *const sage_tensor, y: *const sage_tensor, stats: *const sage_tensor, g_out: *const sage_tensor, g_h: *const sage_tensor, dx: *const sage_tensor, dy: *const sage_tensor, sums: *const sage_block_norms_sums) -> i32;
     pub fn sage_adamw_step(ctx: *mut sage_ctx, tensors: *const sage_adamw_tensor, count: i32, opts: *const sage_adamw_opts) -> i32;
     pub fn sage_adamw_states(ctx: *mut sage_ctx, m: *const sage_tensor, m_scale: *const sage_tensor, v: *const sage_tensor, v_scale: *const sage_tensor, m_out: *const sage_tensor, v_out: *const sage_tensor) -> i32;
     pub fn sage_ipc_export(ctx: *mut sage_ctx, buf: *mut sage_buf, handle: *mut u8, offset: *mut u64) -> i32;

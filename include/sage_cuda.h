@@ -305,6 +305,39 @@ sage_status sage_token_log_probs_grad(sage_ctx *ctx, const sage_tensor *logits, 
 sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logits, const sage_tensor *ids, float scale, const sage_tensor *g_log_probs,
                                           const sage_tensor *g_entropy, const sage_tensor *log_probs, const sage_tensor *entropy, const sage_tensor *dlogits);
 
+/* Dropout: y = x * 65536 / (65536 - T) where an element stays and 0 elsewhere (whatever x held), T = p * 65536 rounded to the nearest whole
+ * number, 65535 at most.  x, y [R, C] f32 / f16 / bf16 of one type; y may be x's own memory.  Element i = r * C + c stays where 16 bits are T or more: half i % 2 of word
+ * i / 2 % 4 of Philox4x32-10 with counter (i / 8, site), 64 bits each, low words first, and the key `seed`, i32 / u32 [2] in device memory.  The mask
+ * depends on nothing else, so the gradient is the same call on the gradient that arrives; a captured call draws by what `seed` holds when it is
+ * replayed.  0 <= p < 1; with p = 0 everything stays and `seed` may be NULL.  `site` tells places of a model apart that draw with the same seed. */
+sage_status sage_dropout(sage_ctx *ctx, const sage_tensor *x, const sage_tensor *y, const sage_tensor *seed, float p, uint64_t site);
+
+/* The norms before and after a block of a model, with what joins the block to the residual stream.  For each row:
+ *   out = residual_scale * x + gate * dropout(A(y)),  h = B(out)
+ * x, out [R, D] (the stream) f32 or of the type of y, h [R, D] (the block's output, the next block's input; f32 / f16 / bf16).  A = `after`, B =
+ * `before`: a sage_norm over the row, (v - mean) / sqrt(variance + eps) (layer) or v / sqrt(mean of v^2 + eps) (rms), times the weight, plus the bias
+ * (f32 [D]; either may be absent; none with SAGE_NORM_NONE).  B reads `out` as it is stored.  gate: f32 [D], or [G, D] whose row g serves the rows
+ * g * R / G and following.  Dropout as sage_dropout's, over [R, D], with `seed` absent where p = 0.  y may be NULL: out = residual_scale * x (no norm
+ * after, gate or dropout then, and `out` may be NULL where residual_scale is 1).  h is given exactly where there is a norm before.  stats, f32 [R, 4], what
+ * the gradient reads: mean and 1 / deviation under A, under B (0 and 1 where there is none); may be NULL.  out may be x's own memory, h that of y (same rows).
+ * eps is positive; D is 1 to 16384. */
+typedef enum { SAGE_NORM_NONE = 0, SAGE_NORM_RMS = 1, SAGE_NORM_LAYER = 2 } sage_norm;
+typedef struct { /* buf NULL: absent */
+    sage_tensor after_weight, after_bias, before_weight, before_bias, gate, seed;
+    int32_t after, before; /* sage_norm */
+    float residual_scale, eps, p;
+    uint64_t site;
+} sage_block_norms_opts;
+sage_status sage_block_norms(sage_ctx *ctx, const sage_block_norms_opts *opts, const sage_tensor *x, const sage_tensor *y, const sage_tensor *out, const sage_tensor *h, const sage_tensor *stats);
+/* Its gradient, from `out` (x where that was NULL), y and stats as they are behind the call, and the gradients g_out and g_h of both results (either may be NULL: zero):
+ * dx and dy (of the types of x and y; NULL: not wanted), and the sums over rows that `sums` asks for (buf NULL: not wanted; f32, of the operand's shape),
+ * in a fixed order.  Without y: dy, the gate's and the norm after's sums are NULL. */
+typedef struct {
+    sage_tensor after_weight, after_bias, before_weight, before_bias, gate;
+} sage_block_norms_sums;
+sage_status sage_block_norms_grad(sage_ctx *ctx, const sage_block_norms_opts *opts, const sage_tensor *out, const sage_tensor *y, const sage_tensor *stats, const sage_tensor *g_out,
+                                  const sage_tensor *g_h, const sage_tensor *dx, const sage_tensor *dy, const sage_block_norms_sums *sums);
+
 /* AdamW over many tensors in one call.  For every element, g = grad * grad_scale:
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)

@@ -1,4 +1,5 @@
 // extern "C" surface of the language-model operators of include/sage_cuda.h: argument checks, then kernels/language.h.
+#include <algorithm>
 #include <cmath>
 #include <exception>
 #include <new>
@@ -77,6 +78,29 @@ struct Checks {
         v.stride = t->strides[0];
         if (output && n > 1 && v.stride < 1) refuse(name, "has elements that overlap");
         return v;
+    }
+    // f32 [dim], or [groups, dim] whose groups divide `n` rows.
+    k::RowsArg gate(const sage_tensor *t, const char *name, long long n, long long dim, bool output) const {
+        k::RowsArg r;
+        if (t->ndim == 1) {
+            r.ptr = flat(t, name, dim);
+            r.rows = 1;
+            r.cols = r.pitch = dim;
+            r.dtype = t->dtype;
+        } else {
+            r = rows(t, name, output);
+            if (r.cols != dim) refuse(name, "does not have one element for each column");
+            if (r.rows < 1 || n % r.rows) refuse(name, "has a number of rows that does not divide theirs");
+        }
+        if (r.dtype != SAGE_F32) refuse(name, "is not f32");
+        return r;
+    }
+    // f32 [n, 4]
+    k::RowsArg stats4(const sage_tensor *t, long long n, bool output, bool optional) const {
+        if (!t && optional) return k::RowsArg{};
+        const k::RowsArg r = rows(t, "stats", output);
+        if (r.rows != n || r.cols != 4 || r.dtype != SAGE_F32) refuse("stats", "is not f32 [rows, 4]");
+        return r;
     }
     // Contiguous memory of n elements (n < 0: as many as it has, left in *count).
     void *flat(const sage_tensor *t, const char *name, long long n, long long *count = nullptr) const {
@@ -206,6 +230,129 @@ sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logi
         const k::VectorArg lp = c.vector(log_probs, "log_probs", a.logits.rows, false, true, false);
         const k::VectorArg h = c.vector(entropy, "entropy", a.logits.rows, false, true, true);
         return k::token_log_probs_and_grad(c.C, a, lp, h);
+    });
+}
+
+static k::Dropout dropout_args(const Checks &c, const sage_tensor *seed, float p, uint64_t site) {
+    k::Dropout d;
+    if (!(p >= 0.f && p < 1.f)) c.refuse("p", "is not in [0, 1)");
+    d.bar = (unsigned)std::min(65535.0, std::nearbyint((double)p * 65536.0));
+    d.factor = (float)(65536.0 / (65536.0 - d.bar));
+    d.site = site;
+    if (p > 0.f || seed) {
+        const k::VectorArg v = c.vector(seed, "seed", 2, true, false, false);
+        d.seed = (const unsigned *)v.ptr;
+        d.seed_stride = v.stride;
+    }
+    return d;
+}
+
+sage_status sage_dropout(sage_ctx *ctx, const sage_tensor *x, const sage_tensor *y, const sage_tensor *seed, float p, uint64_t site) {
+    return guarded(ctx, "dropout", [&](const Checks &c) {
+        const k::RowsArg in = c.real_rows(x, "x", false), o = c.real_rows(y, "y", true);
+        if (o.rows != in.rows || o.cols != in.cols || o.dtype != in.dtype) c.refuse("y", "does not have the shape and type of x");
+        return k::dropout(c.C, in, o, dropout_args(c, seed, p, site));
+    });
+}
+
+static const sage_tensor *given(const sage_tensor &t) { return t.buf ? &t : nullptr; }
+
+// The description of both directions, for rows of `dim` columns; `branch`: there is a y.
+static k::BlockNorms norms_args(const Checks &c, const sage_block_norms_opts *o, long long rows, long long dim, bool branch) {
+    if (!o) c.refuse("opts", "is missing");
+    k::BlockNorms n;
+    if (dim < 1 || dim > k::kMaxNormColumns) c.refuse("x", "does not have 1 to 16384 columns");
+    n.dim = dim;
+    for (int kind : {o->after, o->before})
+        if (kind < SAGE_NORM_NONE || kind > SAGE_NORM_LAYER) c.refuse("after or before", "is no sage_norm");
+    n.after = o->after;
+    n.before = o->before;
+    const auto row = [&](const sage_tensor &t, const char *name, int kind) -> const float * {
+        if (!t.buf) return nullptr;
+        if (kind == SAGE_NORM_NONE) c.refuse(name, "is given without its norm");
+        if (t.dtype != SAGE_F32) c.refuse(name, "is not f32");
+        if (t.ndim != 1) c.refuse(name, "does not have rank 1");
+        return (const float *)c.flat(&t, name, dim);
+    };
+    n.after_weight = row(o->after_weight, "after_weight", n.after);
+    n.after_bias = row(o->after_bias, "after_bias", n.after);
+    n.before_weight = row(o->before_weight, "before_weight", n.before);
+    n.before_bias = row(o->before_bias, "before_bias", n.before);
+    n.eps = o->eps;
+    if (!(n.eps > 0.f) || !std::isfinite(n.eps)) c.refuse("eps", "is not positive and finite");
+    n.scale = finite(c, "residual_scale", o->residual_scale);
+    n.drop = dropout_args(c, given(o->seed), o->p, o->site);
+    if (o->gate.buf) n.gate = c.gate(&o->gate, "gate", rows, dim, false);
+    if (!branch && (n.after != SAGE_NORM_NONE || o->gate.buf || o->p > 0.f)) c.refuse("y", "is missing, which the norm after, the gate and dropout need");
+    return n;
+}
+
+sage_status sage_block_norms(sage_ctx *ctx, const sage_block_norms_opts *opts, const sage_tensor *x, const sage_tensor *y, const sage_tensor *out, const sage_tensor *h, const sage_tensor *stats) {
+    return guarded(ctx, "block_norms", [&](const Checks &c) {
+        const k::RowsArg xs = c.real_rows(x, "x", false);
+        const auto like = [&](const sage_tensor *t, const char *name, bool output) {
+            k::RowsArg r;
+            if (!t) return r;
+            r = c.real_rows(t, name, output);
+            if (r.rows != xs.rows || r.cols != xs.cols) c.refuse(name, "does not have the shape of x");
+            return r;
+        };
+        const k::RowsArg ys = like(y, "y", false), os = like(out, "out", true), hs = like(h, "h", true);
+        k::BlockNorms n = norms_args(c, opts, xs.rows, xs.cols, y != nullptr);
+        n.x_dtype = xs.dtype;
+        n.dtype = y ? ys.dtype : h ? hs.dtype : xs.dtype;
+        if (out && os.dtype != xs.dtype) c.refuse("out", "does not have the type of x");
+        if (xs.dtype != SAGE_F32 && xs.dtype != n.dtype) c.refuse("x", "is neither f32 nor of the type of y and h");
+        if (y && h && hs.dtype != ys.dtype) c.refuse("h", "does not have the type of y");
+        if (!h != (n.before == SAGE_NORM_NONE)) c.refuse("h", h ? "is given without a norm before" : "is missing, which the norm before writes");
+        if (!out && (y || n.scale != 1.f || !h)) c.refuse("out", "is missing");
+        return k::block_norms(c.C, n, xs, ys, os, hs, c.stats4(stats, xs.rows, true, true));
+    });
+}
+
+sage_status sage_block_norms_grad(sage_ctx *ctx, const sage_block_norms_opts *opts, const sage_tensor *out, const sage_tensor *y, const sage_tensor *stats, const sage_tensor *g_out,
+                                  const sage_tensor *g_h, const sage_tensor *dx, const sage_tensor *dy, const sage_block_norms_sums *sums) {
+    return guarded(ctx, "block_norms_grad", [&](const Checks &c) {
+        const k::RowsArg os = c.real_rows(out, "out", false);
+        const auto like = [&](const sage_tensor *t, const char *name, bool output) {
+            k::RowsArg r;
+            if (!t) return r;
+            r = c.real_rows(t, name, output);
+            if (r.rows != os.rows || r.cols != os.cols) c.refuse(name, "does not have the shape of out");
+            return r;
+        };
+        const k::RowsArg ys = like(y, "y", false), go = like(g_out, "g_out", false), gh = like(g_h, "g_h", false), xs = like(dx, "dx", true), d = like(dy, "dy", true);
+        k::BlockNorms n = norms_args(c, opts, os.rows, os.cols, y != nullptr);
+        n.x_dtype = os.dtype;
+        n.dtype = y ? ys.dtype : g_h ? gh.dtype : os.dtype;
+        if (os.dtype != SAGE_F32 && os.dtype != n.dtype) c.refuse("out", "is neither f32 nor of the type of y and g_h");
+        if (g_out && go.dtype != os.dtype) c.refuse("g_out", "does not have the type of out");
+        if (dx && xs.dtype != os.dtype) c.refuse("dx", "does not have the type of out");
+        if (y && g_h && gh.dtype != ys.dtype) c.refuse("g_h", "does not have the type of y");
+        if (dy && (!y || d.dtype != n.dtype)) c.refuse("dy", y ? "does not have the type of y" : "is given without y");
+        if (g_h && n.before == SAGE_NORM_NONE) c.refuse("g_h", "is given without a norm before");
+        if (!g_out && !g_h) c.refuse("g_out", "and g_h are both missing");
+        const k::RowsArg st = c.stats4(stats, os.rows, false, false);
+        k::BlockNormsSums s;
+        if (sums) {
+            const auto row = [&](const sage_tensor &t, const char *name, int kind) -> float * {
+                if (!t.buf) return nullptr;
+                if (kind == SAGE_NORM_NONE) c.refuse(name, "is given without its norm");
+                if (t.dtype != SAGE_F32) c.refuse(name, "is not f32");
+                if (t.ndim != 1) c.refuse(name, "does not have rank 1");
+                return (float *)c.flat(&t, name, os.cols);
+            };
+            s.after_weight = row(sums->after_weight, "sums of after_weight", n.after);
+            s.after_bias = row(sums->after_bias, "sums of after_bias", n.after);
+            s.before_weight = row(sums->before_weight, "sums of before_weight", n.before);
+            s.before_bias = row(sums->before_bias, "sums of before_bias", n.before);
+            if (sums->gate.buf) {
+                if (!n.gate.ptr) c.refuse("sums of gate", "is given without a gate");
+                s.gate = c.gate(&sums->gate, "sums of gate", os.rows, os.cols, true);
+                if (s.gate.rows != n.gate.rows) c.refuse("sums of gate", "does not have the gate's shape");
+            }
+        }
+        return k::block_norms_grad(c.C, n, os, ys, st, go, gh, xs, d, s);
     });
 }
 

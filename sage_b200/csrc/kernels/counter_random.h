@@ -1,0 +1,57 @@
+// Random bits by position: Philox4x32-10 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011), keyed by
+// two words of device memory, so that what a captured graph draws follows what the program wrote there before the replay.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace sage {
+namespace k {
+
+// Which elements dropout keeps, and the factor on them.  `bar` of 65536 are dropped.
+struct Dropout {
+    const unsigned *seed = nullptr;  // two words, `seed_stride` apart
+    long long seed_stride = 1;
+    unsigned long long site = 0;
+    unsigned bar = 0;
+    float factor = 1.f;
+};
+
+struct Key {
+    unsigned a, b;
+};
+__device__ __forceinline__ Key key_of(const Dropout &d) { return d.bar ? Key{__ldg(d.seed), __ldg(d.seed + d.seed_stride)} : Key{0u, 0u}; }
+
+__device__ __forceinline__ uint4 philox(Key k, unsigned long long count, unsigned long long site) {
+    uint4 x = make_uint4((unsigned)count, (unsigned)(count >> 32), (unsigned)site, (unsigned)(site >> 32));
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+        const unsigned long long p = (unsigned long long)x.x * 0xD2511F53u, q = (unsigned long long)x.z * 0xCD9E8D57u;
+        x = make_uint4((unsigned)(q >> 32) ^ x.y ^ k.a, (unsigned)q, (unsigned)(p >> 32) ^ x.w ^ k.b, (unsigned)p);
+        k.a += 0x9E3779B9u;
+        k.b += 0xBB67AE85u;
+    }
+    return x;
+}
+
+// Bit e: element 8 * block + e stays.  Sixteen bits an element, four words a block: a draw of ten rounds serves eight elements (one draw for
+// four, with 32 bits each, is more arithmetic than the memory leaves time for), and shares are multiples of 2^-16.
+__device__ __forceinline__ unsigned keep8(const Dropout &d, Key k, unsigned long long block) {
+    const uint4 w = philox(k, block, d.site);
+    const unsigned words[4] = {w.x, w.y, w.z, w.w};
+    unsigned keep = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        keep |= ((words[i] & 0xffffu) >= d.bar ? 1u : 0u) << (2 * i);
+        keep |= ((words[i] >> 16) >= d.bar ? 1u : 0u) << (2 * i + 1);
+    }
+    return keep;
+}
+// ... of eight elements from `first` on, wherever that lies in a block.
+__device__ __forceinline__ unsigned keep_from(const Dropout &d, Key k, unsigned long long first) {
+    if (!d.bar) return 0xffu;
+    const unsigned at = (unsigned)first & 7u;
+    const unsigned low = keep8(d, k, first >> 3);
+    return at ? (low >> at | keep8(d, k, (first >> 3) + 1) << (8 - at)) & 0xffu : low;
+}
+
+}  // namespace k
+}  // namespace sage

@@ -1,8 +1,10 @@
 // Host launchers of the language-model operators: token embedding and its gradient (embedding.cu), log probabilities of given
-// tokens with entropy, alternatives and gradient (log_probs.cu), AdamW over many tensors (adamw.cu).  Pointers are raw device
+// tokens with entropy, alternatives and gradient (log_probs.cu), the same from hidden states (head.cu), dropout (dropout.cu), norms around a
+// block (block_norms.cu), AdamW over many tensors (adamw.cu).  Pointers are raw device
 // addresses with the offset applied, strides in elements; the caller (abi/language_abi.cc, graph/ops_language.cc) has checked
 // types, extents and that views lie in their buffers.
 #pragma once
+#include "counter_random.h"
 #include "kernels.h"
 
 namespace sage {
@@ -51,6 +53,27 @@ struct LogProbsGrad {
 sage_status token_log_probs_grad(Context &ctx, const LogProbsGrad &a);
 // Both at once: `a.stats` and `a.entropy` are not read; log_probs and entropy (null = not wanted) are written.
 sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const VectorArg &log_probs, const VectorArg &entropy);
+
+// y = x where an element stays, times the factor, else 0
+sage_status dropout(Context &ctx, const RowsArg &x, const RowsArg &y, const Dropout &d);
+
+constexpr long long kMaxNormColumns = 16384;
+struct BlockNorms {  // block_norms.cu says what of what; null: none
+    int after = SAGE_NORM_NONE, before = SAGE_NORM_NONE;
+    const float *after_weight = nullptr, *after_bias = nullptr, *before_weight = nullptr, *before_bias = nullptr;  // [dim], contiguous
+    RowsArg gate;  // f32 [groups, dim]: a row for each rows / groups rows
+    float scale = 1.f, eps = 0.f;
+    Dropout drop;
+    long long dim = 0;
+    int x_dtype = SAGE_F32, dtype = SAGE_F32;  // of the stream; of the block's input and output
+};
+sage_status block_norms(Context &ctx, const BlockNorms &n, const RowsArg &x, const RowsArg &y, const RowsArg &out, const RowsArg &h, const RowsArg &stats);
+struct BlockNormsSums {  // null: not wanted
+    float *after_weight = nullptr, *after_bias = nullptr, *before_weight = nullptr, *before_bias = nullptr;
+    RowsArg gate;
+};
+sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &out, const RowsArg &y, const RowsArg &stats, const RowsArg &g_out, const RowsArg &g_h, const RowsArg &dx,
+                             const RowsArg &dy, const BlockNormsSums &sums);
 
 constexpr int kAdamWBlock = 256;  // elements of an 8-bit state that share a scale
 struct AdamWSlot {

@@ -11,6 +11,7 @@ import ctypes
 from . import CTensor, SageError, lib
 
 _F = ctypes.c_float
+_U64 = ctypes.c_uint64
 
 
 def _ref(t):
@@ -42,6 +43,73 @@ def token_log_probs_grad(logits, ids, stats, entropy, g_log_probs, g_entropy, dl
 def token_log_probs_and_grad(logits, ids, g_log_probs, g_entropy, log_probs, entropy, dlogits, scale=1.0):
     """Values and gradient in one call, for weights g_log_probs and g_entropy that are known before the values."""
     logits.ctx._ck(lib.sage_token_log_probs_and_grad(logits.ctx.h, logits.ref(), ids.ref(), _F(scale), _ref(g_log_probs), _ref(g_entropy), log_probs.ref(), _ref(entropy), dlogits.ref()))
+
+
+def dropout(x, y, seed, p, site=0):
+    """y = x / (1 - p) where an element stays, else 0; the same call makes the gradient of it.  Which elements stay follows from their places, `site`
+    and what `seed` (u32 or i32 [2]) holds when the call is run; shares are multiples of 2^-16.  y may be x."""
+    x.ctx._ck(lib.sage_dropout(x.ctx.h, x.ref(), y.ref(), _ref(seed), _F(p), _U64(site)))
+
+
+_NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
+_NORM_OPERANDS = ("after_weight", "after_bias", "before_weight", "before_bias", "gate", "seed")
+
+
+class _BlockNormsOpts(ctypes.Structure):
+    _fields_ = [(n, CTensor) for n in _NORM_OPERANDS] + [("after", ctypes.c_int32), ("before", ctypes.c_int32)] + \
+               [(n, _F) for n in ("residual_scale", "eps", "p")] + [("site", _U64)]
+
+
+class _BlockNormsSums(ctypes.Structure):
+    _fields_ = [(n, CTensor) for n in _NORM_OPERANDS[:-1]]
+
+
+def _filled(struct, names, operands):
+    """The struct with those operands that are there, and their handles, which it needs alive."""
+    held = [t for t in operands if t is not None]
+    for name, t in zip(names, operands):
+        if t is not None:
+            if not t.buf:
+                raise SageError(1, "block_norms: %s was released" % name)
+            t.fill(getattr(struct, name))
+    return [t.buf for t in held], held
+
+
+class BlockNorms:
+    """How a block of a model is joined to its residual stream, made once and used for every call until one of its tensors is released:
+    out = residual_scale * x + gate * dropout(A(y)), h = B(out), with A = `after` and B = `before` one of "rms", "layer" and None.  Weights and
+    biases are f32 [D], the gate f32 [D] or [G, D], `seed` and `site` dropout's."""
+
+    def __init__(self, ctx, after=None, after_weight=None, after_bias=None, before=None, before_weight=None, before_bias=None, gate=None, residual_scale=1.0, eps=1e-5,
+                 p=0.0, seed=None, site=0):
+        for name in (after, before):
+            if name not in _NORMS:
+                raise SageError(1, "block_norms: no norm is called %r" % (name,))
+        self.ctx, self.opts = ctx, _BlockNormsOpts(after=_NORMS[after], before=_NORMS[before], residual_scale=residual_scale, eps=eps, p=p, site=site)
+        self.handles, self.held = _filled(self.opts, _NORM_OPERANDS, (after_weight, after_bias, before_weight, before_bias, gate, seed))
+        self.released = ctx.released
+
+    def ready(self):
+        """The struct, behind a look at the operands if any tensor was released since the last one."""
+        if self.released != self.ctx.released:
+            if not all(self.handles):
+                raise SageError(1, "block_norms: an operand was released")
+            self.released = self.ctx.released
+        return ctypes.byref(self.opts)
+
+
+def block_norms(norms, x, y, out, h=None, stats=None):
+    """One call for all rows [R, D]: the stream x and the block's output y give the stream behind the block, the next block's input, and what the gradient
+    reads (stats, [R, 4]).  y None: just h = B(x).  out may be x, h may be y."""
+    norms.ctx._ck(lib.sage_block_norms(norms.ctx.h, norms.ready(), x.ref(), _ref(y), _ref(out), _ref(h), _ref(stats)))
+
+
+def block_norms_grad(norms, out, y, stats, g_out, g_h, dx=None, dy=None, dgate=None, dafter_weight=None, dafter_bias=None, dbefore_weight=None, dbefore_bias=None):
+    """From what block_norms left in out and stats, y, and the gradients of out and h (either may be None): those of x, of y, and the sums over rows that
+    are those of the gate, the weights and the biases (f32), each where it is asked for."""
+    sums = _BlockNormsSums()
+    _filled(sums, _NORM_OPERANDS, (dafter_weight, dafter_bias, dbefore_weight, dbefore_bias, dgate))
+    norms.ctx._ck(lib.sage_block_norms_grad(norms.ctx.h, norms.ready(), out.ref(), _ref(y), stats.ref(), _ref(g_out), _ref(g_h), _ref(dx), _ref(dy), ctypes.byref(sums)))
 
 
 _OPERANDS = ("param", "grad", "m", "v", "m_scale", "v_scale", "copy")
