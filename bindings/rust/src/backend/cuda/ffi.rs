@@ -111,6 +111,8 @@ extern "C" {
     pub fn sage_token_log_probs(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, log_probs: *const sage_tensor, entropy: *const sage_tensor, stats: *const sage_tensor, top_ids: *const sage_tensor, top_log_probs: *const sage_tensor) -> i32;
     pub fn sage_token_log_probs_grad(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, stats: *const sage_tensor, entropy: *const sage_tensor, g_log_probs: *const sage_tensor, g_entropy: *const sage_tensor, dlogits: *const sage_tensor) -> i32;
     pub fn sage_token_log_probs_and_grad(ctx: *mut sage_ctx, logits: *const sage_tensor, ids: *const sage_tensor, scale: f32, g_log_probs: *const sage_tensor, g_entropy: *const sage_tensor, log_probs: *const sage_tensor, entropy: *const sage_tensor, dlogits: *const sage_tensor) -> i32;
+    pub fn sage_head_log_probs(ctx: *mut sage_ctx, hidden: *const sage_tensor, weight: *const sage_tensor, ids: *const sage_tensor, scale: f32, log_probs: *const sage_tensor, entropy: *const sage_tensor, stats: *const sage_tensor) -> i32;
+    pub fn sage_head_log_probs_grad(ctx: *mut sage_ctx, hidden: *const sage_tensor, weight: *const sage_tensor, ids: *const sage_tensor, scale: f32, stats: *const sage_tensor, entropy: *const sage_tensor, g_log_probs: *const sage_tensor, g_entropy: *const sage_tensor, dhidden: *const sage_tensor, dweight: *const sage_tensor) -> i32;
     pub fn sage_dropout(ctx: *mut sage_ctx, x: *const sage_tensor, y: *const sage_tensor, seed: *const sage_tensor, p: f32, site: u64) -> i32;
     pub fn sage_block_norms(ctx: *mut sage_ctx, opts: *const sage_block_norms_opts, x: *const sage_tensor, y: *const sage_tensor, out: *const sage_tensor, h: *const sage_tensor, stats: *const sage_tensor) -> i32;
     pub fn sage_block_norms_grad(ctx: *mut sage_ctx, opts: *const sage_block_norms_opts, out: *const sage_tensor, y: *const sage_tensor, stats: *const sage_tensor, g_out: *const sage_tensor, g_h: *const sage_tensor, dx: *const sage_tensor, dy: *const sage_tensor, sums: *const sage_block_norms_sums) -> i32;

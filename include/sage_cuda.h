@@ -305,6 +305,17 @@ sage_status sage_token_log_probs_grad(sage_ctx *ctx, const sage_tensor *logits, 
 sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logits, const sage_tensor *ids, float scale, const sage_tensor *g_log_probs,
                                           const sage_tensor *g_entropy, const sage_tensor *log_probs, const sage_tensor *entropy, const sage_tensor *dlogits);
 
+/* The same from hidden states, without keeping the logits: sage_token_log_probs and its gradient of logits = hidden weight^T, hidden [R, D], weight [V, D]
+ * f32 / f16 / bf16 of one type, which are made in pieces of the vocabulary and never stored as a whole (an embedding table that is tied to the
+ * head is `weight`).  Products are summed in f32 (f32 operands: with f32's accuracy).  The gradient reads the stats and the entropy that the values left and makes
+ * the logits again; with q = d / d logits, dhidden = q weight and dweight = q^T hidden are of the operands' type or f32 (NULL: not wanted).  Between 16-bit operands q is
+ * rounded to their type (f16: by a power of two that brings its largest near 2^14), an operand like the others of both products.  The order of all sums is fixed.
+ * Memory for a call comes from the context's pool: up to 512 MB for the values, 256 MB for a piece of q and f32 sums of [R, D] for the gradient. */
+sage_status sage_head_log_probs(sage_ctx *ctx, const sage_tensor *hidden, const sage_tensor *weight, const sage_tensor *ids, float scale, const sage_tensor *log_probs,
+                                const sage_tensor *entropy, const sage_tensor *stats);
+sage_status sage_head_log_probs_grad(sage_ctx *ctx, const sage_tensor *hidden, const sage_tensor *weight, const sage_tensor *ids, float scale, const sage_tensor *stats,
+                                     const sage_tensor *entropy, const sage_tensor *g_log_probs, const sage_tensor *g_entropy, const sage_tensor *dhidden, const sage_tensor *dweight);
+
 /* Dropout: y = x * 65536 / (65536 - T) where an element stays and 0 elsewhere (whatever x held), T = p * 65536 rounded to the nearest whole
  * number, 65535 at most.  x, y [R, C] f32 / f16 / bf16 of one type; y may be x's own memory.  Element i = r * C + c stays where 16 bits are T or more: half i % 2 of word
  * i / 2 % 4 of Philox4x32-10 with counter (i / 8, site), 64 bits each, low words first, and the key `seed`, i32 / u32 [2] in device memory.  The mask

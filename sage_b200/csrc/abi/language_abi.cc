@@ -233,6 +233,56 @@ sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logi
     });
 }
 
+static k::Head head_args(const Checks &c, const sage_tensor *hidden, const sage_tensor *weight, const sage_tensor *ids, float scale) {
+    k::Head a;
+    a.hidden = c.real_rows(hidden, "hidden", false);
+    a.weight = c.real_rows(weight, "weight", false);
+    if (a.weight.dtype != a.hidden.dtype) c.refuse("weight", "does not have the type of hidden");
+    if (a.weight.cols != a.hidden.cols) c.refuse("weight", "does not have the width of hidden");
+    if (!a.weight.cols) c.refuse("hidden", "has rows without elements");
+    if (!a.weight.rows) c.refuse("weight", "has no rows");
+    a.ids = c.vector(ids, "ids", a.hidden.rows, true, false, false);
+    a.scale = temperature_scale(c, scale);
+    return a;
+}
+
+sage_status sage_head_log_probs(sage_ctx *ctx, const sage_tensor *hidden, const sage_tensor *weight, const sage_tensor *ids, float scale, const sage_tensor *log_probs,
+                                const sage_tensor *entropy, const sage_tensor *stats) {
+    return guarded(ctx, "head_log_probs", [&](const Checks &c) {
+        const k::Head a = head_args(c, hidden, weight, ids, scale);
+        const long long n = a.hidden.rows;
+        const k::VectorArg lp = c.vector(log_probs, "log_probs", n, false, true, false), h = c.vector(entropy, "entropy", n, false, true, true);
+        k::RowsArg st;
+        if (stats) {
+            st = c.rows(stats, "stats", true);
+            if (st.rows != n || st.cols != 2 || st.dtype != SAGE_F32) c.refuse("stats", "is not f32 [rows, 2]");
+        }
+        return k::head_log_probs(c.C, a, lp, h, st);
+    });
+}
+
+sage_status sage_head_log_probs_grad(sage_ctx *ctx, const sage_tensor *hidden, const sage_tensor *weight, const sage_tensor *ids, float scale, const sage_tensor *stats,
+                                     const sage_tensor *entropy, const sage_tensor *g_log_probs, const sage_tensor *g_entropy, const sage_tensor *dhidden, const sage_tensor *dweight) {
+    return guarded(ctx, "head_log_probs_grad", [&](const Checks &c) {
+        const k::Head a = head_args(c, hidden, weight, ids, scale);
+        const long long n = a.hidden.rows;
+        const k::RowsArg st = c.rows(stats, "stats", false);
+        if (st.rows != n || st.cols != 2 || st.dtype != SAGE_F32) c.refuse("stats", "is not f32 [rows, 2]");
+        if (g_entropy && !entropy) c.refuse("entropy", "is missing, which g_entropy needs");
+        const k::VectorArg h = c.vector(entropy, "entropy", n, false, false, true), gl = c.vector(g_log_probs, "g_log_probs", n, false, false, true), ge = c.vector(g_entropy, "g_entropy", n, false, false, true);
+        const auto like = [&](const sage_tensor *t, const char *name, const k::RowsArg &of) {
+            k::RowsArg r;
+            if (!t) return r;
+            r = c.real_rows(t, name, true);
+            if (r.rows != of.rows || r.cols != of.cols) c.refuse(name, "does not have its operand's shape");
+            if (r.dtype != SAGE_F32 && r.dtype != of.dtype) c.refuse(name, "is neither f32 nor of its operand's type");
+            return r;
+        };
+        const k::RowsArg dh = like(dhidden, "dhidden", a.hidden), dw = like(dweight, "dweight", a.weight);
+        return k::head_log_probs_grad(c.C, a, st, h, gl, ge, dh, dw);
+    });
+}
+
 static k::Dropout dropout_args(const Checks &c, const sage_tensor *seed, float p, uint64_t site) {
     k::Dropout d;
     if (!(p >= 0.f && p < 1.f)) c.refuse("p", "is not in [0, 1)");

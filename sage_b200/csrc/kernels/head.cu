@@ -1,0 +1,558 @@
+// Log probabilities of given tokens straight from hidden states, x = scale hidden weight^T, without keeping the logits, and the gradient:
+//   log p_j = x_j - m - ln S,  m = max x,  S = sum exp(x_j - m),  H = ln S - sum (x_j - m) exp(x_j - m) / S
+//   q_j = gl (delta(j, id) - p_j) - ge p_j (ln p_j + H);   dhidden = scale q weight,   dweight = scale q^T hidden
+//
+// 16-bit operands (head_device.h).  Forward: one product whose tiles are finished in registers; each half tile leaves a row's {m, S, sum} and a second
+// launch joins them.  Gradient: the vocabulary in pieces; of each piece the product again, q into a buffer (16 bits: q is an operand of two
+// products, rounded like the operands beside it; the sums of both are f32), then its two products.
+// Bound by the tensor cores: 2 rows vocab width operations forward, three times that for the gradient, which makes the logits again.
+// f32 operands: the same pieces as the framework's own f32 products around kernels over a piece of the logits.
+#include <algorithm>
+#include <cmath>
+
+#include "head_device.h"
+#include "language.h"
+
+namespace sage {
+void *driver_symbol(const char *name);  // runtime/context.cc
+namespace k {
+namespace head {
+namespace {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr size_t kPartBytes = (size_t)512 << 20;   // what half tiles leave of a run of rows
+constexpr size_t kPieceBytes = (size_t)256 << 20;  // a piece of q
+
+__device__ __forceinline__ float exp2_of(float x) { return exp2f(x); }
+
+// One row's sums, joined: (m, S, A) with A = sum (x - m) c2 2^((x - m) c2).
+struct Sums {
+    float m, s, a;
+};
+__device__ __forceinline__ Sums joined(Sums x, Sums y, float c2) {
+    const float m = fmaxf(x.m, y.m);  // of two numbers the larger; nan only beside sums that are nan
+    const float fx = x.m == -INFINITY ? 0.f : (x.m - m) * c2, fy = y.m == -INFINITY ? 0.f : (y.m - m) * c2;
+    const float ex = x.m == -INFINITY ? 1.f : exp2_of(fx), ey = y.m == -INFINITY ? 1.f : exp2_of(fy);  // (sums of nothing are zero, or nan)
+    const float ax = ex > 0.f ? fmaf(x.s * ex, fx, x.a * ex) : x.s * ex, ay = ey > 0.f ? fmaf(y.s * ey, fy, y.a * ey) : y.s * ey;
+    return Sums{m, x.s * ex + y.s * ey, ax + ay};
+}
+
+struct Values {
+    float *log_probs, *entropy, *stats;
+    long long log_probs_stride, entropy_stride, stats_pitch;
+};
+
+// 32 rows a block, its warps share the parts.
+__global__ void __launch_bounds__(1024) head_join_kernel(const float4 *parts, int count, int rows, const float *asked, const int *ids, long long ids_stride, int vocab, float scale, float c2,
+                                                         Values y) {
+    __shared__ Sums all[32][33];
+    grid_dependency_sync();
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, warps = (int)blockDim.x >> 5, row = (int)blockIdx.x * 32 + lane;
+    Sums x{-INFINITY, 0.f, 0.f};
+    if (row < rows) {
+#pragma unroll 4
+        for (int i = warp; i < count; i += warps) {
+            const float4 p = __ldg(parts + (long long)i * rows + row);
+            x = joined(x, Sums{p.x, p.y, p.z}, c2);
+        }
+    }
+    all[warp][lane] = x;
+    __syncthreads();
+    if (warp || row >= rows) return;
+    for (int w = 1; w < warps; ++w) x = joined(x, all[w][lane], c2);
+    const bool none = x.m == -INFINITY && x.s == 0.f;  // no token has a chance
+    const float ln_s = logf(x.s);
+    const int id = __ldg(ids + row * ids_stride);
+    const bool scored = id >= 0 && id < vocab;
+    if (y.log_probs) y.log_probs[row * y.log_probs_stride] = !scored ? 0.f : none ? -INFINITY : (asked[row] - x.m) * scale - ln_s;
+    if (y.entropy) y.entropy[row * y.entropy_stride] = none ? 0.f : ln_s - kLn2 * x.a / x.s;
+    if (y.stats) {
+        y.stats[row * y.stats_pitch] = x.m;
+        y.stats[row * y.stats_pitch + 1] = x.s;
+    }
+}
+
+// What the gradient needs of each row, once.
+__global__ void __launch_bounds__(256) head_rows_kernel(const float *stats, long long stats_pitch, VectorArg entropy, VectorArg gl, VectorArg ge, const int *ids, long long ids_stride, int rows,
+                                                        int vocab, float4 *about, float *gls, unsigned *gmax) {
+    grid_dependency_sync();
+    const int row = (int)blockIdx.x * 256 + (int)threadIdx.x;
+    float size = 0.f;
+    if (row < rows) {
+        const float m = stats[row * stats_pitch], s = stats[row * stats_pitch + 1];
+        const int id = __ldg(ids + row * ids_stride);
+        const bool none = m == -INFINITY && s == 0.f;
+        const float g = gl.ptr && !none && id >= 0 && id < vocab ? ((const float *)gl.ptr)[row * gl.stride] : 0.f;
+        const float e = ge.ptr && !none ? ((const float *)ge.ptr)[row * ge.stride] : 0.f, h = e != 0.f ? ((const float *)entropy.ptr)[row * entropy.stride] : 0.f;
+        about[row] = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(m, -log2f(s), -fmaf(e, h, g), -e * kLn2);
+        gls[row] = g;
+        size = fabsf(g) + fabsf(e) * (fabsf(h) + 0.5f);
+        if (!(size < INFINITY)) size = 0.f;
+    }
+    if (gmax) {
+#pragma unroll
+        for (int off = 16; off; off >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, off));
+        if (!(threadIdx.x & 31) && size > 0.f) atomicMax(gmax, __float_as_uint(size));  // (a largest value: in any order)
+    }
+}
+
+// Rows into others: the sum of `slices` that lie apart, in another type, with another pitch.
+template <class A, class B>
+__global__ void __launch_bounds__(256) head_rows_copy_kernel(const A *x, long long px, B *y, long long py, long long rows, int cols, int slices, long long slice) {
+    grid_dependency_sync();
+    const int per = (cols + 3) / 4;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * per; i += gridDim.x * 256ll) {
+        const long long r = i / per, c = (i - r * per) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < slices; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < cols) v[e] += widen(x[s * slice + r * px + c + e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < cols) y[r * py + c + e] = narrowed<B>(v[e]);
+    }
+}
+template <class A, class B>
+sage_status copy_rows(Context &ctx, const A *x, long long px, B *y, long long py, long long rows, int cols, int slices, long long slice) {
+    ctx.note_launch("head_rows_copy");
+    if (ctx.dry()) return SAGE_OK;
+    const long long blocks = std::min<long long>((rows * ((cols + 3) / 4) + 255) / 256, ctx.sm_count * 16ll);
+    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_rows_copy_kernel<A, B>, dim3((unsigned)blocks), dim3(256), 0, x, px, y, py, rows, cols, slices, slice), "head_rows_copy");
+}
+
+// f32: a piece of the logits becomes the rows' sums over it ...
+__global__ void __launch_bounds__(256) head_stats_kernel(const float *x, int rows, int cols, const int *ids, long long ids_stride, int first, float c2, float4 *parts, float *asked) {
+    __shared__ Sums all[8];
+    grid_dependency_sync();
+    const int row = (int)blockIdx.x;
+    const float *p = x + (long long)row * cols;
+    Sums t{-INFINITY, 0.f, 0.f};
+    for (int c = (int)threadIdx.x; c < cols; c += 256 * 8) {
+        float v[8], high = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = c + e * 256 < cols ? __ldg(p + c + e * 256) : -INFINITY;
+            high = fmaxf(high, v[e]);
+        }
+        Sums u{high, 0.f, 0.f};
+        const float from = high == -INFINITY ? 0.f : high;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float d = (v[e] - from) * c2, y = exp2_of(d);
+            u.s += y;
+            u.a = fmaf(y, fmaxf(d, kFar), u.a);
+        }
+        t = joined(t, u, c2);
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) t = joined(t, Sums{__shfl_xor_sync(0xffffffffu, t.m, off), __shfl_xor_sync(0xffffffffu, t.s, off), __shfl_xor_sync(0xffffffffu, t.a, off)}, c2);
+    if (!(threadIdx.x & 31)) all[threadIdx.x >> 5] = t;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 8; ++w) t = joined(t, all[w], c2);
+    parts[row] = make_float4(t.m, t.s, t.a, 0.f);
+    const int id = __ldg(ids + row * ids_stride);
+    if (id >= first && id - first < cols) asked[row] = p[id - first];
+}
+// ... or q, in its place.
+__global__ void __launch_bounds__(256) head_probs_kernel(float *x, int rows, int cols, const int *ids, long long ids_stride, int first, float c2, float scale, const float4 *about, const float *gls) {
+    grid_dependency_sync();
+    const int row = (int)blockIdx.x;
+    const float4 t = __ldg(about + row);
+    const float gl = __ldg(gls + row);
+    const int id = __ldg(ids + row * ids_stride), at = id < first ? -1 : id - first;
+    float *p = x + (long long)row * cols;
+#pragma unroll 8
+    for (int c = (int)blockIdx.y * 256 + (int)threadIdx.x; c < cols; c += 256 * (int)gridDim.y) {
+        const float d = fmaf(p[c] - t.x, c2, t.y), y = exp2_of(d);
+        p[c] = scale * (y * fmaf(t.w, fmaxf(d, kFar), t.z) + (c == at ? gl : 0.f));
+    }
+}
+__global__ void __launch_bounds__(256) head_add_kernel(const float *x, float *y, long long py, long long rows, int cols, int add) {
+    grid_dependency_sync();
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * cols; i += gridDim.x * 256ll) {
+        const long long r = i / cols, c = i - r * cols;
+        y[r * py + c] = add ? y[r * py + c] + x[i] : x[i];
+    }
+}
+
+// ------------------------------------------------------------------------------------------ host
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Rows of 128 bytes of a matrix, boxes of `box_rows` of them.
+sage_status map_of(Context &ctx, int dtype, const void *base, long long cols, long long rows, long long pitch, int box_rows, CUtensorMap *map) {
+    static const EncodeTiled encode = reinterpret_cast<EncodeTiled>(driver_symbol("cuTensorMapEncodeTiled"));
+    if (!encode) return ctx.fail(SAGE_ERR_DEVICE, "cuTensorMapEncodeTiled is not available");
+    const int size = dtype == SAGE_F32 ? 4 : 2;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(pitch * size)};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const CUtensorMapDataType type = dtype == SAGE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == SAGE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (encode(map, type, 2, const_cast<void *>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return ctx.fail(SAGE_ERR_DEVICE, "head_log_probs: cuTensorMapEncodeTiled failed");
+    return SAGE_OK;
+}
+
+// Memory of the call, given back with it: the stream orders its next use.
+struct Scratch {
+    Context &ctx;
+    std::vector<Block *> blocks;
+    explicit Scratch(Context &c) : ctx(c) {}
+    ~Scratch() {
+        for (Block *b : blocks) ctx.allocator().free(b);
+    }
+    template <class P>
+    sage_status get(size_t bytes, P **out) {
+        Block *b = ctx.allocator().alloc(bytes);
+        if (!b) return ctx.fail(SAGE_ERR_OOM, "head_log_probs: out of memory");
+        blocks.push_back(b);
+        *out = (P *)b->ptr;
+        return SAGE_OK;
+    }
+};
+
+struct Matrix {  // rows x cols, cols contiguous
+    const void *p = nullptr;
+    long long rows = 0, cols = 0, pitch = 0;
+};
+bool on_16(const void *p, long long pitch, int size) { return (uintptr_t)p % 16 == 0 && pitch * size % 16 == 0; }
+
+// The operand as TMA reads it: rows on 16-byte boundaries, copied where they are not.
+template <class T>
+sage_status aligned(Context &ctx, Scratch &scratch, const RowsArg &r, Matrix *m) {
+    *m = Matrix{r.ptr, r.rows, r.cols, r.rows > 1 ? r.pitch : (r.cols + 7) / 8 * 8};
+    if (on_16(m->p, m->pitch, 2) && m->pitch >= r.cols) return SAGE_OK;
+    const long long pitch = (r.cols + 7) / 8 * 8;
+    T *to = nullptr;
+    sage_status st = scratch.get((size_t)(r.rows * pitch) * 2, &to);
+    if (!st) st = copy_rows<T, T>(ctx, (const T *)r.ptr, r.rows > 1 ? r.pitch : r.cols, to, pitch, r.rows, (int)r.cols, 1, 0);
+    m->p = to;
+    m->pitch = pitch;
+    return st;
+}
+
+Product shape_of(Context &ctx, long long m, long long n, long long k) {
+    Product p{};
+    p.m = (int)m;
+    p.n = (int)n;
+    p.k = (int)k;
+    p.bn = n <= 128 || (n + 255) / 256 * 256 - (n + 127) / 128 * 128 > 0 && n < 1024 ? 128 : 256;  // fewer columns that are not there
+    p.tiles_m = (int)((m + 255) / 256);
+    p.tiles_n = (int)((n + p.bn - 1) / p.bn);
+    p.slices = 1;
+    p.slice_blocks = (int)((k + kK - 1) / kK);
+    p.band = 8;
+    p.status = ctx.status_word_dev;
+    return p;
+}
+
+template <class T, bool A_MN, bool B_MN, End END>
+sage_status launch(Context &ctx, const char *name, Product p, int dtype, const Matrix &a, const Matrix &b, int out_type, const Matrix &c) {
+    ctx.note_launch(name);
+    if (ctx.dry()) return SAGE_OK;
+    p.band = std::min(p.band, p.tiles_m);
+    CUtensorMap ma, mb, mc;
+    sage_status st = map_of(ctx, dtype, a.p, a.cols, a.rows, a.pitch, A_MN ? kK : 128, &ma);
+    if (!st) st = map_of(ctx, dtype, b.p, b.cols, b.rows, b.pitch, B_MN ? kK : p.bn / 2, &mb);
+    if (!st && END != kStats) st = map_of(ctx, out_type, c.p, c.cols, c.rows, c.pitch, 32, &mc);
+    else mc = ma;
+    const auto kernel = head_product_kernel<T, A_MN, B_MN, END>;
+    if (!st) st = ctx.check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem), name);
+    if (st) return st;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n * p.slices;
+    const unsigned grid = 2 * (unsigned)std::min<long long>(tiles, ctx.sm_count / 2);
+    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), 2, kernel, dim3(grid), dim3(kBlock), kSmem, ma, mb, mc, p), name);
+}
+
+// out = alpha * the product, rounded once.  Pieces of K come in calls of their own, the first with `first`, the last with `last`; where tiles are few, slices
+// of K are worked on side by side.  `held`: f32 sums between the calls, made here where they are needed.
+struct Result {
+    RowsArg out;
+    float *sums = nullptr;
+    long long pitch = 0;
+    int slices = 1, slice_rows = 0;
+    bool wide = false;  // sums are kept in f32
+};
+void plan(Context &ctx, const Product &p, long long k, bool pieces, Result *r) {
+    const int pairs = ctx.sm_count / 2, tiles = p.tiles_m * p.tiles_n;
+    const int blocks = (int)((k + kK - 1) / kK);
+    r->slices = tiles >= pairs ? 1 : std::max(1, std::min(pairs / tiles, blocks / 8));
+    r->slice_rows = p.tiles_m * 256;
+    r->wide = pieces || r->slices > 1 || !on_16(r->out.ptr, r->out.pitch, r->out.dtype == SAGE_F32 ? 4 : 2);
+}
+template <class T, bool A_MN, bool B_MN>
+sage_status multiply(Context &ctx, Scratch &scratch, const char *name, Product p, int dtype, const Matrix &a, const Matrix &b, bool first, bool last, Result *r) {
+    sage_status st = SAGE_OK;
+    const long long rows = r->out.rows, cols = r->out.cols;
+    const bool f32 = r->out.dtype == SAGE_F32, direct = f32 && r->slices == 1 && on_16(r->out.ptr, r->out.pitch, 4);  // sums may be the result itself
+    if (!r->wide && !f32) return launch<T, A_MN, B_MN, kNarrow>(ctx, name, p, dtype, a, b, dtype, Matrix{r->out.ptr, rows, cols, r->out.pitch});
+    p.add = !first;
+    if (direct) return launch<T, A_MN, B_MN, kWide>(ctx, name, p, dtype, a, b, SAGE_F32, Matrix{r->out.ptr, rows, cols, r->out.pitch});
+    if (first) {
+        r->pitch = (cols + 7) / 8 * 8;
+        st = scratch.get((size_t)r->slices * r->slice_rows * r->pitch * 4, &r->sums);
+        if (st) return st;
+    }
+    const int blocks = p.slice_blocks;
+    p.slice_blocks = (blocks + r->slices - 1) / r->slices;
+    p.slices = (blocks + p.slice_blocks - 1) / p.slice_blocks;
+    if (first) r->slices = p.slices;  // (pieces that follow are no longer: a slice of the last one may have nothing to add)
+    p.slice_rows = r->slice_rows;
+    st = launch<T, A_MN, B_MN, kWide>(ctx, name, p, dtype, a, b, SAGE_F32, Matrix{r->sums, (long long)r->slices * r->slice_rows, cols, r->pitch});
+    if (st || !last) return st;
+    const long long slice = (long long)r->slice_rows * r->pitch;
+    if (f32) return copy_rows<float, float>(ctx, r->sums, r->pitch, (float *)r->out.ptr, r->out.pitch, rows, (int)cols, r->slices, slice);
+    return copy_rows<float, T>(ctx, r->sums, r->pitch, (T *)r->out.ptr, r->out.pitch, rows, (int)cols, r->slices, slice);
+}
+
+sage_status join(Context &ctx, const float4 *parts, int count, long long rows, const float *asked, const VectorArg &ids, long long vocab, float scale, const Values &y) {
+    ctx.note_launch("head_join");
+    if (ctx.dry()) return SAGE_OK;
+    const int warps = count >= 64 && rows < 32 * 296 ? 32 : 8;
+    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_join_kernel, dim3((unsigned)((rows + 31) / 32)), dim3(32 * warps), 0, parts, count, (int)rows, asked, (const int *)ids.ptr,
+                                           ids.stride, (int)vocab, scale, scale * kLog2E, y),
+                          "head_join");
+}
+
+// Rows [at, at + count) of the operands and results.
+RowsArg cut(const RowsArg &r, long long at, long long count) {
+    RowsArg c = r;
+    if (r.ptr) c.ptr = (char *)r.ptr + at * r.pitch * (r.dtype == SAGE_F32 ? 4 : 2);
+    c.rows = count;
+    return c;
+}
+VectorArg cut(const VectorArg &v, long long at) { return v.ptr ? VectorArg{(char *)v.ptr + at * v.stride * 4, v.stride} : v; }
+
+template <class T>
+sage_status forward16(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
+    Scratch scratch(ctx);
+    const long long rows = a.hidden.rows, vocab = a.weight.rows, width = a.hidden.cols;
+    Matrix w;
+    sage_status st = aligned<T>(ctx, scratch, a.weight, &w);
+    if (st) return st;
+    Product p = shape_of(ctx, rows, vocab, width);
+    const long long parts_of_row = 2ll * p.tiles_n;
+    const long long most = std::max<long long>(256, (long long)(kPartBytes / (16 * parts_of_row)) / 256 * 256);  // rows at a time
+    float4 *parts = nullptr;
+    float *asked = nullptr;
+    st = scratch.get((size_t)(std::min(rows, most) * parts_of_row) * 16, &parts);
+    if (!st) st = scratch.get((size_t)std::min(rows, most) * 4, &asked);
+    for (long long at = 0; at < rows && !st; at += most) {
+        const long long count = std::min(most, rows - at);
+        Matrix x;
+        st = aligned<T>(ctx, scratch, cut(a.hidden, at, count), &x);
+        if (st) return st;
+        p.m = (int)count;
+        p.tiles_m = (int)((count + 255) / 256);
+        p.band = (int)std::max<long long>(8, ((long long)48 << 20) / (256 * width * 2));  // rows of hidden states that stay in L2 while the weights go by
+        const VectorArg ids = cut(a.ids, at);
+        p.ids = (const int *)ids.ptr;
+        p.ids_stride = ids.stride;
+        p.c2 = a.scale * kLog2E;
+        p.parts = parts;
+        p.asked = asked;
+        st = launch<T, false, false, kStats>(ctx, "head_log_probs", p, a.hidden.dtype, x, w, 0, Matrix{});
+        const VectorArg lp = cut(log_probs, at), h = cut(entropy, at);
+        const RowsArg s = cut(stats, at, count);
+        if (!st) st = join(ctx, parts, (int)parts_of_row, count, asked, ids, vocab, a.scale, Values{(float *)lp.ptr, (float *)h.ptr, (float *)s.ptr, lp.stride, h.stride, s.pitch});
+    }
+    return st;
+}
+
+// The rows' part of the gradient; gmax where P is stored by a scale of its own.
+sage_status rows_about(Context &ctx, Scratch &scratch, const Head &a, const RowsArg &stats, const VectorArg &entropy, const VectorArg &gl, const VectorArg &ge, bool scaled, float4 **about,
+                       float **gls, unsigned **gmax) {
+    const long long rows = a.hidden.rows;
+    sage_status st = scratch.get((size_t)rows * 16, about);
+    if (!st) st = scratch.get((size_t)rows * 4, gls);
+    *gmax = nullptr;
+    if (!st && scaled) {
+        st = scratch.get(4, gmax);
+        ctx.note_memset();
+        if (!st && !ctx.dry()) st = ctx.check_cuda(cudaMemsetAsync(*gmax, 0, 4, ctx.stream()), "head_log_probs_grad");
+    }
+    if (st) return st;
+    ctx.note_launch("head_rows");
+    if (ctx.dry()) return SAGE_OK;
+    return ctx.check_cuda(launch_dependent(ctx.pdl && !scaled, ctx.stream(), head_rows_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, (const float *)stats.ptr,
+                                           rows > 1 ? stats.pitch : 2, entropy, gl, ge, (const int *)a.ids.ptr, a.ids.stride, (int)rows, (int)a.weight.rows, *about, *gls, *gmax),
+                          "head_rows");
+}
+
+template <class T>
+sage_status grad16(Context &ctx, const Head &a, const RowsArg &stats, const VectorArg &entropy, const VectorArg &gl, const VectorArg &ge, const RowsArg &dhidden, const RowsArg &dweight) {
+    Scratch scratch(ctx);
+    const long long rows = a.hidden.rows, vocab = a.weight.rows, width = a.hidden.cols;
+    const int dtype = a.hidden.dtype;
+    Matrix x, w;
+    float4 *about;
+    float *gls;
+    unsigned *gmax;
+    T *probs = nullptr;
+    // Pieces of equal size, whole tiles
+    const long long tiles = (vocab + 255) / 256, most = std::max<long long>(1, (long long)(kPieceBytes / ((size_t)rows * 512))), pieces = (tiles + most - 1) / most,
+                    piece = (tiles + pieces - 1) / pieces * 256, pitch = std::min(piece, (vocab + 63) / 64 * 64);
+    sage_status st = aligned<T>(ctx, scratch, a.hidden, &x);
+    if (!st) st = aligned<T>(ctx, scratch, a.weight, &w);
+    if (!st) st = rows_about(ctx, scratch, a, stats, entropy, gl, ge, dtype == SAGE_F16, &about, &gls, &gmax);
+    if (!st) st = scratch.get((size_t)(rows * pitch) * 2, &probs);
+    Result to_hidden;
+    to_hidden.out = dhidden;
+    for (long long at = 0; at < vocab && !st; at += piece) {
+        const long long n = std::min(piece, vocab - at);
+        const bool first = at == 0, last = at + n == vocab;
+        const Matrix here{(const T *)w.p + at * w.pitch, n, width, w.pitch}, q{probs, rows, n, pitch};
+        Product p = shape_of(ctx, rows, n, width);
+        p.ids = (const int *)a.ids.ptr;
+        p.ids_stride = a.ids.stride;
+        p.first = (int)at;
+        p.c2 = a.scale * kLog2E;
+        p.rows = about;
+        p.gl = gls;
+        p.gmax = gmax;
+        p.band = (int)std::max<long long>(8, ((long long)48 << 20) / (256 * width * 2));
+        st = launch<T, false, false, kProbs>(ctx, "head_probs", p, dtype, x, here, dtype, q);
+        if (!st && dhidden.ptr) {
+            p = shape_of(ctx, rows, width, n);
+            p.gmax = gmax;
+            p.alpha = a.scale;
+            if (first) plan(ctx, p, n, !last, &to_hidden);
+            st = multiply<T, false, true>(ctx, scratch, "head_dhidden", p, dtype, q, here, first, last, &to_hidden);
+        }
+        if (!st && dweight.ptr) {
+            p = shape_of(ctx, n, width, rows);
+            p.gmax = gmax;
+            p.alpha = a.scale;
+            Result r;
+            r.out = cut(dweight, at, n);
+            plan(ctx, p, rows, false, &r);
+            st = multiply<T, true, true>(ctx, scratch, "head_dweight", p, dtype, q, x, true, true, &r);
+        }
+    }
+    return st;
+}
+
+// ------------------------------------------------------------------------------------------ f32
+// The f32 products' operands: one row has any pitch, rows that overlap are laid out anew.
+sage_status apart(Context &ctx, Scratch &scratch, RowsArg *r) {
+    if (r->rows == 1) r->pitch = r->cols;
+    if (r->pitch >= r->cols) return SAGE_OK;
+    float *to = nullptr;
+    sage_status st = scratch.get((size_t)(r->rows * r->cols) * 4, &to);
+    if (!st) st = copy_rows<float, float>(ctx, (const float *)r->ptr, r->pitch, to, r->cols, r->rows, (int)r->cols, 1, 0);
+    r->ptr = to;
+    r->pitch = r->cols;
+    return st;
+}
+
+GemmArgs product_of(bool ta, bool tb, long long m, long long n, long long k, const float *a, long long lda, const float *b, long long ldb, float *c, long long ldc) {
+    return GemmArgs{ta, tb, m, n, k, a, lda, 0, b, ldb, 0, c, ldc, 0, 1};
+}
+struct Pieces {
+    long long rows, cols;  // at a time
+};
+// A piece of f32 logits: all rows where they leave room for at least 1024 columns.
+Pieces pieces_of(long long rows, long long vocab) {
+    const long long room = (long long)(kPieceBytes / 4), r = std::min(rows, std::max<long long>(256, room / std::min<long long>(vocab, 1024)));
+    const long long most = std::max<long long>(1, std::min(vocab, room / r)), count = (vocab + most - 1) / most;
+    return Pieces{r, std::min(vocab, ((vocab + count - 1) / count + 63) / 64 * 64)};
+}
+
+sage_status forward32(Context &ctx, Head a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
+    Scratch scratch(ctx);
+    sage_status st = apart(ctx, scratch, &a.hidden);
+    if (!st) st = apart(ctx, scratch, &a.weight);
+    const long long rows = a.hidden.rows, vocab = a.weight.rows, width = a.hidden.cols;
+    const Pieces piece = pieces_of(rows, vocab);
+    const int count = (int)((vocab + piece.cols - 1) / piece.cols);
+    float *logits, *asked;
+    float4 *parts;
+    if (!st) st = scratch.get((size_t)(piece.rows * piece.cols) * 4, &logits);
+    if (!st) st = scratch.get((size_t)(piece.rows * count) * 16, &parts);
+    if (!st) st = scratch.get((size_t)piece.rows * 4, &asked);
+    for (long long at = 0; at < rows && !st; at += piece.rows) {
+        const long long r = std::min(piece.rows, rows - at);
+        const RowsArg x = cut(a.hidden, at, r);
+        const VectorArg ids = cut(a.ids, at), lp = cut(log_probs, at), h = cut(entropy, at);
+        const RowsArg s = cut(stats, at, r);
+        for (int i = 0; i < count && !st; ++i) {
+            const long long v = i * piece.cols, n = std::min(piece.cols, vocab - v);
+            st = gemm(ctx, product_of(false, true, r, n, width, (const float *)x.ptr, x.pitch, (const float *)a.weight.ptr + v * a.weight.pitch, a.weight.pitch, logits, n));
+            ctx.note_launch("head_stats");
+            if (!st && !ctx.dry())
+                st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_stats_kernel, dim3((unsigned)r), dim3(256), 0, (const float *)logits, (int)r, (int)n, (const int *)ids.ptr, ids.stride, (int)v,
+                                                     a.scale * kLog2E, parts + i * r, asked),
+                                    "head_stats");
+        }
+        if (!st) st = join(ctx, parts, count, r, asked, ids, vocab, a.scale, Values{(float *)lp.ptr, (float *)h.ptr, (float *)s.ptr, lp.stride, h.stride, s.pitch});
+    }
+    return st;
+}
+
+sage_status grad32(Context &ctx, Head a, const RowsArg &stats, const VectorArg &entropy, const VectorArg &gl, const VectorArg &ge, const RowsArg &dhidden, const RowsArg &dweight) {
+    Scratch scratch(ctx);
+    sage_status st = apart(ctx, scratch, &a.hidden);
+    if (!st) st = apart(ctx, scratch, &a.weight);
+    const long long rows = a.hidden.rows, vocab = a.weight.rows, width = a.hidden.cols;
+    const long long most = std::max<long long>(1, std::min(vocab, (long long)(kPieceBytes / 4) / rows)), count = (vocab + most - 1) / most, piece = std::min(vocab, ((vocab + count - 1) / count + 63) / 64 * 64);
+    float4 *about;
+    float *gls, *q, *part = nullptr;
+    unsigned *gmax;
+    const float *x = (const float *)a.hidden.ptr;
+    if (!st) st = rows_about(ctx, scratch, a, stats, entropy, gl, ge, false, &about, &gls, &gmax);
+    if (!st) st = scratch.get((size_t)(rows * piece) * 4, &q);
+    if (!st && dhidden.ptr && piece < vocab) st = scratch.get((size_t)(rows * width) * 4, &part);
+    for (long long v = 0; v < vocab && !st; v += piece) {
+        const long long n = std::min(piece, vocab - v);
+        const float *w = (const float *)a.weight.ptr + v * a.weight.pitch;
+        st = gemm(ctx, product_of(false, true, rows, n, width, x, a.hidden.pitch, w, a.weight.pitch, q, n));
+        ctx.note_launch("head_probs");
+        if (!st && !ctx.dry()) {
+            const unsigned across = (unsigned)std::max<long long>(1, std::min<long long>((n + 2047) / 2048, ctx.sm_count * 16 / rows));
+            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_probs_kernel, dim3((unsigned)rows, across), dim3(256), 0, q, (int)rows, (int)n, (const int *)a.ids.ptr, a.ids.stride, (int)v,
+                                                 a.scale * kLog2E, a.scale, (const float4 *)about, (const float *)gls),
+                                "head_probs");
+        }
+        if (!st && dhidden.ptr) {
+            st = gemm(ctx, product_of(false, false, rows, width, n, q, n, w, a.weight.pitch, part ? part : (float *)dhidden.ptr, part ? width : dhidden.pitch));
+            if (part) ctx.note_launch("head_add");
+            if (!st && part && !ctx.dry())
+                st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_add_kernel, dim3((unsigned)std::min<long long>((rows * width + 255) / 256, ctx.sm_count * 16ll)), dim3(256), 0, (const float *)part,
+                                                     (float *)dhidden.ptr, dhidden.pitch, rows, (int)width, v ? 1 : 0),
+                                    "head_add");
+        }
+        if (!st && dweight.ptr)
+            st = gemm(ctx, product_of(true, false, n, width, rows, q, n, x, a.hidden.pitch, (float *)dweight.ptr + v * dweight.pitch, dweight.pitch));
+    }
+    return st;
+}
+
+}  // namespace
+}  // namespace head
+
+sage_status head_log_probs(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
+    if (!a.hidden.rows) return SAGE_OK;
+    if (a.hidden.dtype == SAGE_F32) return head::forward32(ctx, a, log_probs, entropy, stats);
+    return a.hidden.dtype == SAGE_F16 ? head::forward16<__half>(ctx, a, log_probs, entropy, stats) : head::forward16<__nv_bfloat16>(ctx, a, log_probs, entropy, stats);
+}
+
+sage_status head_log_probs_grad(Context &ctx, const Head &a, const RowsArg &stats, const VectorArg &entropy, const VectorArg &g_log_probs, const VectorArg &g_entropy, const RowsArg &dhidden,
+                                const RowsArg &dweight) {
+    RowsArg dh = dhidden, dw = dweight;
+    if (dh.rows <= 1) dh.pitch = (dh.cols + 7) / 8 * 8;
+    if (dw.rows <= 1) dw.pitch = (dw.cols + 7) / 8 * 8;
+    if (!a.hidden.rows) {
+        if (!dw.ptr) return SAGE_OK;
+        ctx.note_memset();
+        const size_t size = dw.dtype == SAGE_F32 ? 4 : 2;
+        return ctx.dry() ? SAGE_OK : ctx.check_cuda(cudaMemset2DAsync(dw.ptr, dw.pitch * size, 0, dw.cols * size, (size_t)dw.rows, ctx.stream()), "head_log_probs_grad");
+    }
+    if (a.hidden.dtype == SAGE_F32) return head::grad32(ctx, a, stats, entropy, g_log_probs, g_entropy, dh, dw);
+    if (a.hidden.dtype == SAGE_F16) return head::grad16<__half>(ctx, a, stats, entropy, g_log_probs, g_entropy, dh, dw);
+    return head::grad16<__nv_bfloat16>(ctx, a, stats, entropy, g_log_probs, g_entropy, dh, dw);
+}
+
+}  // namespace k
+}  // namespace sage

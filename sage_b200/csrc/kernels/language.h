@@ -54,6 +54,17 @@ sage_status token_log_probs_grad(Context &ctx, const LogProbsGrad &a);
 // Both at once: `a.stats` and `a.entropy` are not read; log_probs and entropy (null = not wanted) are written.
 sage_status token_log_probs_and_grad(Context &ctx, const LogProbsGrad &a, const VectorArg &log_probs, const VectorArg &entropy);
 
+// token_log_probs of the logits hidden weight^T, which are made in pieces and not kept (head.cu)
+struct Head {
+    RowsArg hidden, weight;  // [rows, width], [vocab, width], of one type
+    VectorArg ids;
+    float scale = 1.f;
+};
+sage_status head_log_probs(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats);
+// dhidden, dweight: null = not wanted
+sage_status head_log_probs_grad(Context &ctx, const Head &a, const RowsArg &stats, const VectorArg &entropy, const VectorArg &g_log_probs, const VectorArg &g_entropy, const RowsArg &dhidden,
+                                const RowsArg &dweight);
+
 // y = x where an element stays, times the factor, else 0
 sage_status dropout(Context &ctx, const RowsArg &x, const RowsArg &y, const Dropout &d);
 

@@ -45,6 +45,18 @@ def token_log_probs_and_grad(logits, ids, g_log_probs, g_entropy, log_probs, ent
     logits.ctx._ck(lib.sage_token_log_probs_and_grad(logits.ctx.h, logits.ref(), ids.ref(), _F(scale), _ref(g_log_probs), _ref(g_entropy), log_probs.ref(), _ref(entropy), dlogits.ref()))
 
 
+def head_log_probs(hidden, weight, ids, log_probs, entropy=None, stats=None, scale=1.0):
+    """token_log_probs of the logits hidden weight^T [rows, vocab], which are made in pieces and not kept: hidden [rows, D], weight [vocab, D]."""
+    hidden.ctx._ck(lib.sage_head_log_probs(hidden.ctx.h, hidden.ref(), weight.ref(), ids.ref(), _F(scale), log_probs.ref(), _ref(entropy), _ref(stats)))
+
+
+def head_log_probs_grad(hidden, weight, ids, stats, entropy, g_log_probs, g_entropy, dhidden=None, dweight=None, scale=1.0):
+    """The gradient of g_log_probs . log_probs + g_entropy . entropy with respect to the hidden states and the weight, from what head_log_probs left in
+    `stats` and `entropy`."""
+    hidden.ctx._ck(lib.sage_head_log_probs_grad(hidden.ctx.h, hidden.ref(), weight.ref(), ids.ref(), _F(scale), stats.ref(), _ref(entropy), _ref(g_log_probs), _ref(g_entropy),
+                                                _ref(dhidden), _ref(dweight)))
+
+
 def dropout(x, y, seed, p, site=0):
     """y = x / (1 - p) where an element stays, else 0; the same call makes the gradient of it.  Which elements stay follows from their places, `site`
     and what `seed` (u32 or i32 [2]) holds when the call is run; shares are multiples of 2^-16.  y may be x."""

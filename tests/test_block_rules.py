@@ -161,3 +161,45 @@ def test_the_oracles_gradient_against_differences(after, before, gate):
                 ends.append(value(**{**a, arg: moved}))
             want[i] = (ends[0] - ends[1]) / (2 * eps)
         assert np.allclose(found[name][0], want, rtol=1e-6, atol=1e-6), name
+
+
+# ------------------------------------------------------------------------------------------ log probabilities from hidden states
+def test_head_refusals(ctx):
+    f = lambda *s, d=S.BF16: ctx.empty(s, d)  # noqa: E731
+    h, w, i, lp, st = f(6, 8), f(50, 8), f(6, d=S.I32), f(6, d=S.F32), f(6, 2, d=S.F32)
+    L.head_log_probs(h, w, i, lp, lp, st)
+    go = lambda *a, **k: refused(L.head_log_probs, *a, **k)  # noqa: E731
+    go(h, f(50, 8, d=S.F16), i, lp, match="type of hidden")
+    go(h, f(50, 9), i, lp, match="width")
+    go(f(6, 0), f(50, 0), i, lp, match="without elements")
+    go(h, f(0, 8), i, lp, match="no rows")
+    go(f(6, 8, d=S.I8), w, i, lp, match="hidden")
+    go(h, w, f(5, d=S.I32), lp, match="ids")
+    go(h, w, lp, lp, match="i32")
+    go(h, w, i, f(6), match="log_probs")
+    go(h, w, i, lp, f(5, d=S.F32), match="entropy")
+    go(h, w, i, lp, stats=f(6, 3, d=S.F32), match="stats")
+    for scale in (0.0, -1.0, float("nan"), float("inf"), 3e38):
+        go(h, w, i, lp, scale=scale, match="scale")
+    go(h.view((6, 8), (1, 6)), w, i, lp, match="contiguous")
+    L.head_log_probs_grad(h, w, i, st, lp, lp, lp, f(6, 8), f(50, 8))
+    L.head_log_probs_grad(h, w, i, st, None, lp, None, f(6, 8, d=S.F32), None)
+    go = lambda *a, **k: refused(L.head_log_probs_grad, *a, **k)  # noqa: E731
+    go(h, w, i, st, None, lp, lp, h, match="entropy")
+    go(h, w, i, f(6, 4, d=S.F32), lp, lp, lp, h, match="stats")
+    go(h, w, i, st, lp, f(5, d=S.F32), None, h, match="g_log_probs")
+    go(h, w, i, st, lp, lp, lp, f(6, 8, d=S.F16), match="dhidden")
+    go(h, w, i, st, lp, lp, lp, f(6, 7), match="dhidden")
+    go(h, w, i, st, lp, lp, lp, None, f(50, 9), match="dweight")
+    go(h, w, i, st, lp, lp, lp, None, w.view((50, 8), (0, 1)), match="overlap")
+
+
+def test_head_launches(ctx):
+    f = lambda *s, d=S.BF16: ctx.empty(s, d)  # noqa: E731
+    h, w, i, v, st = f(300, 64), f(1000, 64), f(300, d=S.I32), f(300, d=S.F32), f(300, 2, d=S.F32)
+    ctx.trace_begin()
+    L.head_log_probs(h, w, i, v, v, st)
+    assert ctx.trace() == ["head_log_probs", "head_join"]
+    ctx.trace_begin()
+    L.head_log_probs_grad(h, w, i, st, v, v, v, f(300, 64), f(1000, 64))
+    assert ctx.trace() == ["head_rows", "head_probs", "head_dhidden", "head_rows_copy", "head_dweight"], ctx.trace()
