@@ -1,0 +1,361 @@
+// What the norms around a block (block_norms.cu) and their gradient (block_norms_grad.cu) have in common: teams of threads that go through rows.
+//
+// A thread owns NV runs of eight neighbouring columns and a team of threads a row, so that the sums over rows stay in registers, a sum over a row is
+// one shuffle tree and, in teams of several warps, one exchange in shared memory, and a block of dropout's mask is one draw.  Teams go through rows in
+// steps of their number; what a thread reads of its team's next rows is copied into places of its own in shared memory while the present row
+// is worked on (no barrier: only the thread that asked reads them).  Arithmetic is on pairs of columns, two f32 operations an instruction.
+#pragma once
+#include <algorithm>
+
+#include "counter_random.h"
+#include "language.h"
+#include "launch.h"
+#include "narrow.h"
+
+namespace sage {
+namespace k {
+namespace norms {
+
+constexpr int kMaxThreads = 512, kMaxTeams = 15;  // of a CTA; named barriers 1 to 15
+constexpr int kRingBytes = 216 * 1024;            // of an SM's shared memory, for rows on their way
+
+struct Rows {
+    void *p;
+    long long pitch;
+};
+
+struct NormsArgs {
+    Rows x, y, out, h;     // forward: x, y in, out, h out; backward: out, y in
+    Rows go, gh, dx, dy;   // backward
+    float *stats;          // [rows, 4]: mean and 1 / deviation of A's operand, of B's
+    long long stats_pitch;
+    const float *wa, *ba, *wb, *bb, *gate;
+    long long gate_pitch;
+    int after, before;     // sage_norm
+    float eps, scale;
+    Dropout d;
+    int rows, dim;
+    int group_rows;        // rows that share a row of the gate
+    int team, teams;       // threads that share a row, teams of a CTA
+    int stages;            // of the ring: a row worked on, the others on their way
+    int splits;            // of a group's rows
+    float *partial;        // backward: [CTA][sum][dim]
+    float *gate_partial;   // ... and for gates of several groups [group * splits + split][dim]
+    int sums;              // bits: which of kSums are wanted
+};
+enum { kSumWb, kSumBb, kSumWa, kSumBa, kSumGate, kSums };
+
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the `stages - 1` youngest groups have arrived.
+__device__ __forceinline__ void copies_wait(int stages) {
+    if (stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Sums over a team, two at a time, the same bits in all of its threads.
+struct Team {
+    int index, lane, warp, warps, threads;
+    float2 *slots;  // [2][16], zero where there are no warps
+    int turn;
+    __device__ __forceinline__ void open() {
+        if (warps == 1) return;
+        if (!warp) slots[lane] = make_float2(0.f, 0.f);
+        asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(threads) : "memory");
+    }
+    __device__ __forceinline__ float2 sum(float2 v) {
+#pragma unroll
+        for (int off = 16; off; off >>= 1) v = add2(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, off), __shfl_xor_sync(0xffffffffu, v.y, off)));
+        if (warps == 1) return v;
+        if (!lane) slots[turn + warp] = v;
+        return met();
+    }
+    __device__ __forceinline__ float sum(float v) {
+#pragma unroll
+        for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+        if (warps == 1) return v;
+        if (!lane) slots[turn + warp].x = v;
+        return met().x;
+    }
+    __device__ __forceinline__ float2 met() {
+        const float4 *q = (const float4 *)(slots + turn);
+        turn ^= 16;  // (the next sum but one writes here again, behind the next one's barrier)
+        asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(threads) : "memory");
+        float4 a = q[0], b = q[1];
+        float2 t = add2(add2(make_float2(a.x, a.y), make_float2(a.z, a.w)), add2(make_float2(b.x, b.y), make_float2(b.z, b.w)));
+        for (int w = 4; w < warps; w += 4) {
+            a = q[w / 2], b = q[w / 2 + 1];
+            t = add2(t, add2(add2(make_float2(a.x, a.y), make_float2(a.z, a.w)), add2(make_float2(b.x, b.y), make_float2(b.z, b.w))));
+        }
+        return t;
+    }
+};
+constexpr int kSlots = 32 * kMaxTeams;
+
+// Pairs of columns.
+template <class T>
+__device__ __forceinline__ float2 pair_at(const Pack<T> &p, int i) { return make_float2(widen(p.v[2 * i]), widen(p.v[2 * i + 1])); }
+template <>
+__device__ __forceinline__ float2 pair_at<__nv_bfloat16>(const Pack<__nv_bfloat16> &p, int i) {
+    const unsigned u = ((const unsigned *)&p)[i];
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 pair_at<__half>(const Pack<__half> &p, int i) { return __half22float2(((const __half2 *)&p)[i]); }
+template <class T>
+__device__ __forceinline__ void put_pair(Pack<T> &p, int i, float2 x) {
+    p.v[2 * i] = narrowed<T>(x.x);
+    p.v[2 * i + 1] = narrowed<T>(x.y);
+}
+template <>
+__device__ __forceinline__ void put_pair<__nv_bfloat16>(Pack<__nv_bfloat16> &p, int i, float2 x) { ((__nv_bfloat162 *)&p)[i] = __float22bfloat162_rn(x); }
+template <>
+__device__ __forceinline__ void put_pair<__half>(Pack<__half> &p, int i, float2 x) { ((__half2 *)&p)[i] = __float22half2_rn(x); }
+
+template <class T>
+struct Eight {  // columns, as they are stored
+    static constexpr int kPacks = 8 / Pack<T>::N;
+    Pack<T> p[kPacks];
+    __device__ __forceinline__ void load(const char *from) {
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) p[i] = ((const Pack<T> *)from)[i];
+    }
+    __device__ __forceinline__ void store(char *to) const {
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) ((Pack<T> *)to)[i] = p[i];
+    }
+    __device__ __forceinline__ void open(float2 (&v)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = pair_at<T>(p[i / (4 / kPacks)], i % (4 / kPacks));
+    }
+    __device__ __forceinline__ void close(const float2 (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put_pair<T>(p[i / (4 / kPacks)], i % (4 / kPacks), v[i]);
+    }
+};
+template <class T>
+__device__ __forceinline__ void load8(const T *p, int count, bool wide, float2 (&v)[4]) {
+    Eight<T> q;
+    if (wide && count == 8) {
+#pragma unroll
+        for (int i = 0; i < Eight<T>::kPacks; ++i) q.p[i] = ((const Pack<T> *)p)[i];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q.p[e / Pack<T>::N].v[e % Pack<T>::N] = e < count ? p[e] : narrowed<T>(0.f);
+    }
+    q.open(v);
+}
+template <class T>
+__device__ __forceinline__ void store8(T *p, int count, bool wide, const float2 (&v)[4]) {
+    Eight<T> q;
+    q.close(v);
+    if (wide && count == 8) {
+#pragma unroll
+        for (int i = 0; i < Eight<T>::kPacks; ++i) ((Pack<T> *)p)[i] = q.p[i];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < count) p[e] = q.p[e / Pack<T>::N].v[e % Pack<T>::N];
+    }
+}
+// Weights, biases and gates: f32, through L1.  There is one.
+__device__ __forceinline__ void weights8(const float *p, int count, bool wide, float2 (&v)[4]) {
+    if (wide && count == 8) {
+        const float4 a = __ldg((const float4 *)p), b = __ldg((const float4 *)p + 1);
+        v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = make_float2(2 * i < count ? __ldg(p + 2 * i) : 0.f, 2 * i + 1 < count ? __ldg(p + 2 * i + 1) : 0.f);
+    }
+}
+// Columns behind the row's end hold nothing.
+__device__ __forceinline__ void only(float2 (&v)[4], int count) {
+    if (count == 8) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(2 * i < count ? v[i].x : 0.f, 2 * i + 1 < count ? v[i].y : 0.f);
+}
+__device__ __forceinline__ void only_kept(float2 (&v)[4], unsigned keep) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(keep >> (2 * i) & 1u ? v[i].x : 0.f, keep >> (2 * i + 1) & 1u ? v[i].y : 0.f);
+}
+
+// The rows a team goes through: of each of its shares (a group's rows, every `splits`-th from the share's first on).
+struct Walk {
+    int share, shares, stride, row, end, group;  // shares: groups * splits
+    int splits, group_rows;
+    __device__ __forceinline__ void enter() {
+        group = share / splits;
+        row = group * group_rows + share % splits;
+        end = (group + 1) * group_rows;
+    }
+    __device__ __forceinline__ bool more() const { return share < shares; }
+    __device__ __forceinline__ bool last_of_share() const { return end - row <= splits; }
+    __device__ __forceinline__ void next() {
+        if (!last_of_share()) {
+            row += splits;
+            return;
+        }
+        share += stride;
+        if (more()) enter();
+    }
+};
+__device__ __forceinline__ Walk walk_of(const NormsArgs &a, int unit, int units) {
+    Walk w;
+    w.splits = a.splits;
+    w.group_rows = a.group_rows;
+    w.shares = a.rows / a.group_rows * a.splits;
+    w.stride = units;
+    w.share = unit;
+    w.row = w.end = w.group = 0;
+    if (w.more()) w.enter();
+    return w;
+}
+
+template <class T>
+__host__ __device__ constexpr int pieces(int nv) { return nv * 8 * (int)sizeof(T) / 16; }
+
+// One of a row's operands, eight columns at a time.
+template <class T>
+struct Operand {
+    const T *base;  // at the thread's first column
+    long long pitch;
+    int run;        // elements between its runs
+    __device__ __forceinline__ void get(int row, int v, int count, bool wide, float2 (&x)[4]) const { load8(base + row * pitch + v * run, count, wide, x); }
+};
+
+struct Place {
+    int column, run;  // of the thread's first run; elements between its runs
+    Team team;
+    int unit, units;
+};
+__device__ __forceinline__ Place place_of(const NormsArgs &a, float2 *slots) {
+    Place p;
+    const int index = (int)threadIdx.x / a.team, t = (int)threadIdx.x - index * a.team;
+    p.column = 8 * t;
+    p.run = 8 * a.team;
+    p.team = Team{index, t & 31, t >> 5, a.team / 32, a.team, slots + index * 32, 0};
+    p.team.open();
+    p.unit = (int)blockIdx.x * a.teams + index;
+    p.units = (int)gridDim.x * a.teams;
+    return p;
+}
+// Which of a thread's eight columns of a row stay.
+__device__ __forceinline__ unsigned kept(const Dropout &d, Key key, int row, int dim, int col) { return keep_from(d, key, (unsigned long long)row * dim + col); }
+
+// ---- rows that come through shared memory: 8 | dim, rows on 16-byte boundaries less than 4 GB apart.  All but a thread's last run of columns are
+// there; `last` says whether that one is.  Addresses are made from the kernel's parameters where they are used: held in registers they
+// took more of them than the sums over rows do.
+template <class T>
+__device__ __forceinline__ char *at_row(const Rows &r, int row, int col) {
+    return (char *)r.p + (unsigned long long)(unsigned)row * (unsigned)(r.pitch * (long long)sizeof(T)) + (unsigned)(col * (int)sizeof(T));
+}
+template <class T, int NV>
+__device__ __forceinline__ void ring_ask(const Rows &r, int row, int col, int run, bool last, unsigned to, unsigned piece) {
+    const char *from = at_row<T>(r, row, col);
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+        if (v + 1 < NV || last)
+#pragma unroll
+            for (int i = 0; i < Eight<T>::kPacks; ++i)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (v * Eight<T>::kPacks + i) * piece), "l"(from + (unsigned)(v * run * (int)sizeof(T)) + i * 16) : "memory");
+}
+template <class T>
+__device__ __forceinline__ void ring_get(unsigned from, int v, unsigned piece, float2 (&x)[4]) {
+    Eight<T> q;
+#pragma unroll
+    for (int i = 0; i < Eight<T>::kPacks; ++i) {
+        uint4 u;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(from + (v * Eight<T>::kPacks + i) * piece) : "memory");
+        *(uint4 *)&q.p[i] = u;
+    }
+    q.open(x);
+}
+template <class T>
+__device__ __forceinline__ void put8(char *to, const float2 (&v)[4]) {
+    Eight<T> q;
+    q.close(v);
+#pragma unroll
+    for (int i = 0; i < Eight<T>::kPacks; ++i) ((Pack<T> *)to)[i] = q.p[i];
+}
+__device__ __forceinline__ void get8(const float *p, float2 (&v)[4]) {  // weights, biases, gates
+    const float4 a = __ldg((const float4 *)p), b = __ldg((const float4 *)p + 1);
+    v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
+}
+// Eight columns of which some are dropped, by the sixteen bits of each.
+__device__ __forceinline__ void drop8(float2 (&v)[4], const uint4 &w, unsigned bar) {
+    const unsigned words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2((words[i] & 0xffffu) >= bar ? v[i].x : 0.f, (words[i] >> 16) >= bar ? v[i].y : 0.f);
+}
+
+inline bool boundary(const Rows &r, long long size) { return (uintptr_t)r.p % 16 == 0 && r.pitch * size % 16 == 0 && r.pitch * size < 0x100000000ll; }
+inline bool boundary(const float *p) { return (uintptr_t)p % 16 == 0; }
+inline Rows of(const RowsArg &r) { return Rows{r.ptr, r.rows > 1 ? r.pitch : r.cols}; }
+
+// Threads of a row: of the numbers of runs a thread may own, the one that leaves the fewest without columns, and of those the largest, since what a row
+// costs each thread is shared by its columns; teams of a CTA: up to 256 threads.
+inline int shape_of(NormsArgs *a, int least, int most) {
+    const int runs = (a->dim + 7) / 8;
+    int slots = 0;
+    for (int n = least; n <= most; ++n) {
+        const int team = std::max(32, ((runs + n - 1) / n + 31) / 32 * 32), taken = team * ((runs + team - 1) / team);
+        if (team > kMaxThreads || (slots && taken > slots)) continue;
+        slots = taken;
+        a->team = team;
+    }
+    a->teams = std::max(1, std::min(256 / a->team, kMaxTeams));
+    return (runs + a->team - 1) / a->team;  // all of a thread's runs but the last are whole
+}
+// How many CTAs, and how deep the ring: `row_bytes` of what a row reads, `registers` of a thread.
+inline int grid_of(Context &ctx, NormsArgs *a, int nv, size_t operand_bytes, int registers, bool ring, size_t *smem) {
+    const int threads = a->team * a->teams;
+    int fit = std::max(1, 65536 / (registers * threads));
+    const size_t stage = (size_t)threads * nv * 8 * operand_bytes;
+    const long long wanted = (a->rows + a->teams - 1) / a->teams;
+    a->stages = 4;
+    if (ring) {
+        while (a->stages > 2 && stage * a->stages * fit > (size_t)kRingBytes) --a->stages;
+        while (fit > 1 && stage * a->stages * fit > (size_t)kRingBytes) --fit;
+    }
+    *smem = ring ? stage * a->stages : 0;
+    const int grid = (int)std::min<long long>(wanted, (long long)ctx.sm_count * fit);
+    a->splits = std::max(1, std::min(a->group_rows, grid * a->teams / (a->rows / a->group_rows)));
+    return grid;
+}
+
+inline NormsArgs args_of(const BlockNorms &n, long long rows, long long dim) {
+    NormsArgs a{};
+    a.wa = n.after_weight;
+    a.ba = n.after_bias;
+    a.wb = n.before_weight;
+    a.bb = n.before_bias;
+    a.gate = n.gate.ptr ? (const float *)n.gate.ptr : nullptr;
+    const long long groups = n.gate.ptr ? n.gate.rows : 1;
+    a.gate_pitch = n.gate.pitch;
+    a.after = n.after;
+    a.before = n.before;
+    a.eps = n.eps;
+    a.scale = n.scale;
+    a.d = n.drop;
+    a.rows = (int)rows;
+    a.dim = (int)dim;
+    a.group_rows = (int)(rows / groups);
+    return a;
+}
+
+inline bool weights_wide(const NormsArgs &a) {
+    return boundary(a.wa) && boundary(a.ba) && boundary(a.wb) && boundary(a.bb) && boundary(a.gate) && (!a.gate || a.rows == a.group_rows || a.gate_pitch % 4 == 0);
+}
+
+template <class F>
+sage_status with_types(int x, int t, F f) {
+    return with_type(t, [&](auto b) {
+        typedef decltype(b) T;
+        return x == t ? f(T(), T()) : f(float(), T());
+    });
+}
+
+}  // namespace norms
+}  // namespace k
+}  // namespace sage

@@ -1,0 +1,516 @@
+// The gradient of the norms around a block (block_norms.cu), for arrivals go (of out) and gh (of h), with u = the unit rows of B's operand, v of A's:
+//   q = gh wb;   G = go + rstd (q - mean(q u) u [- mean q], layer norms);   dx = c G
+//   K = G keep / (1 - p);   d gate = sum over rows of K n;   t = K gate;   dy from t as G - go from gh
+// and the weights' and biases' gradients: sums over rows of gh u, gh, t v, t.
+//
+// Bound by memory, with as many operations beside it as the instruction slots hold: sums over rows take eight registers for each run of columns and kind, of
+// which programs without a norm after the block and without a gate (FULL false) have two.  They are joined in a fixed order: team by team within a
+// CTA, then CTA by CTA in a second launch.
+#include "block_norms.h"
+
+namespace sage {
+namespace k {
+namespace norms {
+namespace {
+
+constexpr int kRegisters = 112;  // of a thread of the general form
+
+// The teams' sums of a CTA, team by team, through shared memory (a kind at a time: dim floats).
+template <int KINDS, int NV>
+__device__ __forceinline__ void join_teams(const NormsArgs &a, const Place &at, float2 (&sum)[KINDS][NV][4], const int (&count)[NV], bool wide, float *shared) {
+#pragma unroll
+    for (int s = 0; s < KINDS; ++s) {
+        if (!(a.sums >> s & 1)) continue;
+        for (int t = 0; t < a.teams; ++t) {
+            if (a.teams > 1) __syncthreads();
+            if (t != at.team.index) continue;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int col = at.column + v * at.run;
+                float2 x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = sum[s][v][i];
+                if (t && count[v]) {
+                    float2 y[4];
+                    load8(shared + col, count[v], wide, y);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = add2(x[i], y[i]);
+                }
+                store8(t + 1 == a.teams ? a.partial + ((long long)blockIdx.x * kSums + s) * a.dim + col : shared + col, count[v], wide, x);
+            }
+        }
+    }
+}
+
+__host__ __device__ constexpr int ring_registers(int nv, bool full) { return full ? (nv == 1 ? 96 : 128) : nv == 1 ? 80 : nv == 2 ? 96 : 128; }
+
+// What models call: both gradients arrive, there is a norm before the next block and norms have weights; whole runs of columns on
+// 16-byte boundaries.
+template <class TX, class T, int NV, bool FULL>
+__global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kernel(const NormsArgs a) {
+    extern __shared__ __align__(16) char ring[];
+    __shared__ __align__(16) float2 slots[kSlots];
+    Place at = place_of(a, slots);
+    grid_dependency_sync();
+    Team &team = at.team;
+    const int col = at.column, run = at.run;
+    const bool last = col + (NV - 1) * run < a.dim;
+    // a stage: out, gh, go and (FULL) y
+    const unsigned piece = blockDim.x * 16;
+    constexpr int kGh = pieces<TX>(NV), kGo = kGh + pieces<T>(NV), kY = kGo + pieces<TX>(NV), kStage = kY + (FULL ? pieces<T>(NV) : 0);
+    const unsigned stage = kStage * piece, ring0 = (unsigned)__cvta_generic_to_shared(ring) + threadIdx.x * 16, ring1 = ring0 + a.stages * stage;
+    const Key key = key_of(a.d);
+    const float per = 1.f / (float)a.dim;
+    const float2 zero = make_float2(0.f, 0.f);
+    constexpr int kKept = FULL ? (int)kSums : 2;
+    float2 sum[kKept][NV][4];
+#pragma unroll
+    for (int s = 0; s < kKept; ++s)
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[s][v][i] = zero;
+    const int shares = a.rows / a.group_rows * a.splits;
+    for (int share = at.unit; share < shares; share += at.units) {
+        const int group = share / a.splits, end = (group + 1) * a.group_rows, row0 = group * a.group_rows + share % a.splits;
+        unsigned put = ring0, take = ring0;
+        int ahead = row0;
+        const auto ask = [&]() {
+            if (ahead < end) {
+                ring_ask<TX, NV>(a.out, ahead, col, run, last, put, piece);
+                ring_ask<T, NV>(a.gh, ahead, col, run, last, put + kGh * piece, piece);
+                ring_ask<TX, NV>(a.go, ahead, col, run, last, put + kGo * piece, piece);
+                if (FULL) ring_ask<T, NV>(a.y, ahead, col, run, last, put + kY * piece, piece);
+                put = put + stage == ring1 ? ring0 : put + stage;
+                ahead += a.splits;
+            }
+            copies_end();
+        };
+        for (int i = 1; i < a.stages; ++i) ask();
+        float next[4];
+#pragma unroll
+        for (int i = FULL ? 0 : 2; i < 4; ++i) next[i] = __ldg(a.stats + row0 * a.stats_pitch + i);
+        for (int row = row0; row < end; row += a.splits) {
+            const float mean_a = FULL ? next[0] : 0.f, rstd_a = FULL ? next[1] : 1.f, mean_b = next[2], rstd_b = next[3];
+            if (end - row > a.splits)
+#pragma unroll
+                for (int i = FULL ? 0 : 2; i < 4; ++i) next[i] = __ldg(a.stats + (row + a.splits) * a.stats_pitch + i);
+            ask();
+            copies_wait(a.stages);
+            float2 q[NV][4], along = zero, all = zero;  // what arrives through the norm
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (v + 1 < NV || last) {
+                    float2 u[4], w[4];
+                    ring_get<TX>(take, v, piece, u);
+                    ring_get<T>(take + kGh * piece, v, piece, q[v]);
+                    get8(a.wb + col + v * run, w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        u[i] = mul2(add2(u[i], both(-mean_b)), both(rstd_b));
+                        sum[kSumWb][v][i] = fma2(q[v][i], u[i], sum[kSumWb][v][i]);
+                        sum[kSumBb][v][i] = add2(sum[kSumBb][v][i], q[v][i]);
+                        q[v][i] = mul2(q[v][i], w[i]);
+                        along = fma2(q[v][i], u[i], along);
+                        all = add2(all, q[v][i]);
+                    }
+                }
+            const float2 s1 = team.sum(make_float2(along.x + along.y, all.x + all.y));
+            const float along_u = s1.x * per, mean_q = a.before == SAGE_NORM_LAYER ? s1.y * per : 0.f;
+            float2 along_t = zero, all_t = zero;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (v + 1 < NV || last) {
+                    const int at_col = col + v * run;
+                    float2 G[4], u[4];
+                    ring_get<TX>(take + kGo * piece, v, piece, G);
+                    ring_get<TX>(take, v, piece, u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        u[i] = mul2(add2(u[i], both(-mean_b)), both(rstd_b));
+                        G[i] = fma2(fma2(u[i], both(-along_u), add2(q[v][i], both(-mean_q))), both(rstd_b), G[i]);
+                        u[i] = mul2(G[i], both(a.scale));
+                    }
+                    if (a.dx.p) put8<TX>(at_row<TX>(a.dx, row, at_col), u);
+                    if (a.d.bar) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) G[i] = mul2(G[i], both(a.d.factor));
+                        drop8(G, philox(key, ((unsigned long long)(unsigned)row * (unsigned)a.dim + at_col) >> 3, a.d.site), a.d.bar);
+                    }
+                    if (!FULL) {
+                        if (a.dy.p) put8<T>(at_row<T>(a.dy, row, at_col), G);
+                        continue;
+                    }
+                    float2 n[4], w[4], b[4];
+                    ring_get<T>(take + kY * piece, v, piece, n);
+                    if (a.after != SAGE_NORM_NONE) {
+                        get8(a.wa + at_col, w);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) n[i] = mul2(add2(n[i], both(-mean_a)), both(rstd_a));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = both(1.f);
+                        if (a.d.bar)  // a value that is dropped may be anything (a norm would have spread it)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) n[i] = make_float2(G[i].x == 0.f ? 0.f : n[i].x, G[i].y == 0.f ? 0.f : n[i].y);
+                    }
+                    if (a.gate) {
+                        float2 by[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) by[i] = mul2(n[i], w[i]);
+                        if (a.ba) {
+                            get8(a.ba + at_col, b);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) by[i] = add2(by[i], b[i]);
+                        }
+                        get8(a.gate + (long long)group * a.gate_pitch + at_col, b);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            sum[kKept - 1][v][i] = fma2(G[i], by[i], sum[kKept - 1][v][i]);
+                            G[i] = mul2(G[i], b[i]);
+                        }
+                    }
+                    constexpr int kWa = FULL ? (int)kSumWa : 0, kBa = FULL ? (int)kSumBa : 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sum[kBa][v][i] = add2(sum[kBa][v][i], G[i]);
+                        sum[kWa][v][i] = fma2(G[i], n[i], sum[kWa][v][i]);
+                        q[v][i] = mul2(G[i], w[i]);
+                        along_t = fma2(q[v][i], n[i], along_t);
+                        all_t = add2(all_t, q[v][i]);
+                    }
+                }
+            if (FULL && a.dy.p) {
+                float2 s2 = zero;
+                if (a.after != SAGE_NORM_NONE) s2 = team.sum(make_float2(along_t.x + along_t.y, all_t.x + all_t.y));
+                const float along_v = s2.x * per, mean_t = a.after == SAGE_NORM_LAYER ? s2.y * per : 0.f;
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+                    if (v + 1 < NV || last) {
+                        if (a.after != SAGE_NORM_NONE) {
+                            float2 n[4];
+                            ring_get<T>(take + kY * piece, v, piece, n);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                q[v][i] = mul2(fma2(mul2(add2(n[i], both(-mean_a)), both(rstd_a)), both(-along_v), add2(q[v][i], both(-mean_t))), both(rstd_a));
+                        }
+                        put8<T>(at_row<T>(a.dy, row, col + v * run), q[v]);
+                    }
+            }
+            take = take + stage == ring1 ? ring0 : take + stage;
+        }
+        if (FULL && a.gate_partial) {
+            float *to = a.gate_partial + (long long)share * a.dim + col;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                if (v + 1 < NV || last) store8(to + v * run, 8, true, sum[kKept - 1][v]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[kKept - 1][v][i] = zero;
+            }
+        }
+    }
+    if (!a.partial) return;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    int count[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) count[v] = v + 1 < NV || last ? 8 : 0;
+    join_teams(a, at, sum, count, true, (float *)ring);
+}
+
+// Any layout: rows are read where they are used, as vectors if `wide`.
+template <class TX, class T, int NV, bool FULL>
+__global__ void __maxnreg__(kRegisters) block_norms_grad_kernel(const NormsArgs a, const bool wide, const bool wide_weights) {
+    extern __shared__ __align__(16) char ring[];
+    __shared__ __align__(16) float2 slots[kSlots];
+    Place at = place_of(a, slots);
+    grid_dependency_sync();
+    Team &team = at.team;
+    int count[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) count[v] = max(0, min(8, a.dim - at.column - v * at.run));
+    const bool branch = a.y.p != nullptr, second = a.gh.p != nullptr, carried = a.go.p != nullptr;
+    const Operand<TX> r{(const TX *)a.out.p + at.column, a.out.pitch, at.run}, go{(const TX *)a.go.p + at.column, a.go.pitch, at.run};
+    const Operand<T> gh{(const T *)a.gh.p + at.column, a.gh.pitch, at.run}, y{(const T *)a.y.p + at.column, a.y.pitch, at.run};
+    const Key key = key_of(a.d);
+    const float per = 1.f / (float)a.dim;
+    const float2 zero = make_float2(0.f, 0.f);
+    constexpr int kKept = FULL ? (int)kSums : 2;
+    float2 sum[kKept][NV][4];
+#pragma unroll
+    for (int s = 0; s < kKept; ++s)
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[s][v][i] = zero;
+    Walk now = walk_of(a, at.unit, at.units);
+    while (now.more()) {
+        const int row = now.row;
+        const float *st = a.stats + row * a.stats_pitch;
+        const float mean_a = __ldg(st), rstd_a = __ldg(st + 1), mean_b = __ldg(st + 2), rstd_b = __ldg(st + 3);
+        // (drawn here: nothing waits for it, and the sums below wait for others)
+        unsigned keep[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) keep[v] = a.d.bar && count[v] ? kept(a.d, key, row, a.dim, at.column + v * at.run) : 0xffu;
+        float2 s1 = zero;
+        if (second) {
+            float2 along = zero, all = zero;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                if (!count[v]) continue;
+                float2 u[4], g[4], w[4];
+                r.get(row, v, count[v], wide, u);
+                gh.get(row, v, count[v], wide, g);  // (zero behind the row's end)
+                if (a.wb) weights8(a.wb + at.column + v * at.run, count[v], wide_weights, w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 n = mul2(add2(u[i], both(-mean_b)), both(rstd_b)), q = a.wb ? mul2(g[i], w[i]) : g[i];
+                    sum[kSumWb][v][i] = fma2(g[i], n, sum[kSumWb][v][i]);
+                    sum[kSumBb][v][i] = add2(sum[kSumBb][v][i], g[i]);
+                    along = fma2(q, n, along);
+                    all = add2(all, q);
+                }
+            }
+            s1 = make_float2(along.x + along.y, all.x + all.y);
+            if (a.before != SAGE_NORM_NONE) s1 = team.sum(s1);
+        }
+        const float along_u = s1.x * per * rstd_b, mean_q = a.before == SAGE_NORM_LAYER ? s1.y * per : 0.f;
+        const float *gate = FULL && a.gate ? a.gate + now.group * a.gate_pitch : nullptr;
+        float2 q[NV][4], along_t = zero, all_t = zero;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (!count[v]) continue;
+            const int col = at.column + v * at.run;
+            float2 G[4];
+            if (carried) {
+                go.get(row, v, count[v], wide, G);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) G[i] = zero;
+            }
+            if (second) {
+                float2 u[4], g[4], w[4];
+                r.get(row, v, count[v], wide, u);
+                gh.get(row, v, count[v], wide, g);
+                if (a.wb) weights8(a.wb + col, count[v], wide_weights, w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 n = mul2(add2(u[i], both(-mean_b)), both(rstd_b));
+                    const float2 e = a.wb ? fma2(g[i], w[i], both(-mean_q)) : add2(g[i], both(-mean_q));
+                    G[i] = add2(G[i], fma2(n, both(-along_u), mul2(e, both(rstd_b))));
+                }
+            }
+            if (a.dx.p) {
+                float2 d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = mul2(G[i], both(a.scale));
+                store8((TX *)a.dx.p + row * a.dx.pitch + col, count[v], wide, d);
+            }
+            if (!branch) continue;
+            if (a.d.bar) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) G[i] = mul2(G[i], both(a.d.factor));
+                only_kept(G, keep[v]);
+            }
+            if (!FULL) {
+                if (a.dy.p) store8((T *)a.dy.p + row * a.dy.pitch + col, count[v], wide, G);
+                continue;
+            }
+            only(G, count[v]);
+            float2 n[4], w[4], b[4], t[4];
+            y.get(row, v, count[v], wide, n);
+            if (a.wa) weights8(a.wa + col, count[v], wide_weights, w);
+            if (gate) {
+                if (a.ba) weights8(a.ba + col, count[v], wide_weights, b);
+                weights8(gate + col, count[v], wide_weights, t);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                n[i] = mul2(add2(n[i], both(-mean_a)), both(rstd_a));
+                if (gate) {
+                    float2 by = a.wa ? a.ba ? fma2(n[i], w[i], b[i]) : mul2(n[i], w[i]) : a.ba ? add2(n[i], b[i]) : n[i];
+                    if (a.d.bar) by = make_float2(keep[v] >> (2 * i) & 1u ? by.x : 0.f, keep[v] >> (2 * i + 1) & 1u ? by.y : 0.f);  // (a value that is dropped may be anything)
+                    sum[kSumGate][v][i] = fma2(G[i], by, sum[kSumGate][v][i]);
+                    t[i] = mul2(t[i], G[i]);
+                } else {
+                    t[i] = G[i];
+                }
+                sum[kSumBa][v][i] = add2(sum[kSumBa][v][i], t[i]);
+                sum[kSumWa][v][i] = fma2(t[i], n[i], sum[kSumWa][v][i]);
+                q[v][i] = a.wa ? mul2(t[i], w[i]) : t[i];
+                along_t = fma2(q[v][i], n[i], along_t);
+                all_t = add2(all_t, q[v][i]);
+            }
+        }
+        if (FULL && branch && a.dy.p) {
+            float2 s2 = make_float2(along_t.x + along_t.y, all_t.x + all_t.y);
+            if (a.after != SAGE_NORM_NONE) s2 = team.sum(s2);
+            const float along_v = s2.x * per * rstd_a, mean_t = a.after == SAGE_NORM_LAYER ? s2.y * per : 0.f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                if (!count[v]) continue;
+                if (a.after != SAGE_NORM_NONE) {
+                    float2 n[4];
+                    y.get(row, v, count[v], wide, n);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        q[v][i] = fma2(mul2(add2(n[i], both(-mean_a)), both(rstd_a)), both(-along_v), mul2(add2(q[v][i], both(-mean_t)), both(rstd_a)));
+                }
+                store8((T *)a.dy.p + row * a.dy.pitch + at.column + v * at.run, count[v], wide, q[v]);
+            }
+        }
+        if (FULL && a.gate_partial && now.last_of_share()) {
+            float *to = a.gate_partial + (long long)now.share * a.dim;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                store8(to + at.column + v * at.run, count[v], wide, sum[FULL ? kSumGate : 0][v]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[FULL ? kSumGate : 0][v][i] = zero;
+            }
+        }
+        now.next();
+    }
+    if (!a.partial) return;
+    join_teams(a, at, sum, count, wide, (float *)ring);
+}
+
+// y[j] = the sum over i of x[i * pitch + j], in a fixed order: sixteen runs of i, then their sums.
+struct Join {
+    const float *x[kSums];
+    float *y[kSums];
+    int count[kSums];       // addends
+    long long pitch[kSums];
+    int dim;
+};
+constexpr int kJoinParts = 16;
+__global__ void __launch_bounds__(32 * kJoinParts) block_norms_join_kernel(const Join a) {
+    __shared__ float part[kJoinParts][33];
+    grid_dependency_sync();
+    const int s = (int)blockIdx.y, lane = (int)threadIdx.x & 31, w = (int)threadIdx.x >> 5, col = (int)blockIdx.x * 32 + lane;
+    float sum = 0.f;
+    if (col < a.dim) {
+        const float *x = a.x[s] + col;
+#pragma unroll 4
+        for (int i = w; i < a.count[s]; i += kJoinParts) sum += x[i * a.pitch[s]];
+    }
+    part[w][lane] = sum;
+    __syncthreads();
+    if (w || col >= a.dim) return;
+#pragma unroll
+    for (int i = 1; i < kJoinParts; ++i) sum += part[i][lane];
+    a.y[s][col] = sum;
+}
+// Gates of several groups: y[g, j] = the sum over `splits` rows of x.
+__global__ void __launch_bounds__(256) block_norms_gates_kernel(const float *x, float *y, int splits, int dim, long long total, long long pitch) {
+    grid_dependency_sync();
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+        const long long g = i / dim, col = i - g * dim;
+        float sum = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) sum += x[(g * splits + s) * dim + col];
+        y[g * pitch + col] = sum;
+    }
+}
+
+}  // namespace
+}  // namespace norms
+
+sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &out, const RowsArg &y, const RowsArg &stats, const RowsArg &g_out, const RowsArg &g_h, const RowsArg &dx,
+                             const RowsArg &dy, const BlockNormsSums &sums) {
+    using namespace norms;
+    const long long rows = stats.rows, dim = n.dim;
+    float *const to[kSums] = {sums.before_weight, sums.before_bias, sums.after_weight, sums.after_bias, (float *)sums.gate.ptr};
+    const long long groups = n.gate.ptr ? n.gate.rows : 1;
+    if (!rows) {  // sums of nothing
+        for (int s = 0; s < kSums; ++s) {
+            if (!to[s] || (s == kSumGate && !groups)) continue;
+            ctx.note_memset();
+            if (ctx.dry()) continue;
+            const long long pitch = s == kSumGate && groups > 1 ? sums.gate.pitch : dim;
+            sage_status st = ctx.check_cuda(cudaMemset2DAsync(to[s], (size_t)pitch * 4, 0, (size_t)dim * 4, (size_t)(s == kSumGate ? groups : 1), ctx.stream()), "block_norms_grad");
+            if (st) return st;
+        }
+        return SAGE_OK;
+    }
+    NormsArgs a = args_of(n, rows, dim);
+    a.out = of(out);
+    a.y = of(y);
+    a.go = of(g_out);
+    a.gh = of(g_h);
+    a.dx = of(dx);
+    a.dy = of(dy);
+    a.stats = (float *)stats.ptr;
+    a.stats_pitch = rows > 1 ? stats.pitch : 4;
+    const int tx = n.x_dtype, t = n.dtype, sx = tx == SAGE_F32 ? 4 : 2, st = t == SAGE_F32 ? 4 : 2;
+    // Without a norm after the block or a gate its values are not read, and two kinds of sums are kept.
+    const bool full = a.y.p && (a.after != SAGE_NORM_NONE || a.gate);
+    const int nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, 1, full ? (a.dim > 8 * kMaxThreads ? 2 : 1) : 4), threads = a.team * a.teams;
+    const bool wide = a.dim % 8 == 0 && boundary(a.out, sx) && boundary(a.go, sx) && boundary(a.dx, sx) && boundary(a.y, st) && boundary(a.gh, st) && boundary(a.dy, st);
+    size_t smem;
+    const size_t bytes = (a.gh.p ? sx + st : 0) + (a.go.p ? sx : 0) + (full ? st : 0);
+    const bool usual = a.y.p && a.gh.p && a.go.p && a.wb && (a.wa || a.after == SAGE_NORM_NONE);
+    const bool ring = wide && usual && weights_wide(a) && !(full && nv > 2) && grid_of(ctx, &a, nv, bytes, ring_registers(nv, full), true, &smem) && smem <= kRingBytes;
+    const int grid = grid_of(ctx, &a, nv, bytes, ring ? ring_registers(nv, full) : kRegisters, ring, &smem);
+    const bool by_group = a.gate && groups > 1 && to[kSumGate];
+    int partials = 0;
+    Join join{};
+    for (int s = 0; s < kSums; ++s)
+        if (to[s] && !(s == kSumGate && by_group)) {
+            a.sums |= 1 << s;
+            join.y[partials++] = to[s];
+        }
+    const size_t partial_bytes = partials ? (size_t)grid * kSums * dim * 4 : 0, gate_bytes = by_group ? (size_t)(groups * a.splits) * dim * 4 : 0, first = (partial_bytes + 255) / 256 * 256;
+    Block *scratch = nullptr;
+    if (partial_bytes + gate_bytes) {
+        scratch = ctx.allocator().alloc(first + gate_bytes);
+        if (!scratch) return ctx.fail(SAGE_ERR_OOM, "block_norms_grad: out of memory");
+    }
+    a.partial = partials ? (float *)scratch->ptr : nullptr;
+    a.gate_partial = by_group ? (float *)(scratch->ptr + first) : nullptr;
+    join.dim = a.dim;
+    for (int s = 0, i = 0; s < kSums; ++s)
+        if (a.sums >> s & 1) {
+            join.x[i] = a.partial + (long long)s * dim;
+            join.count[i] = grid;
+            join.pitch[i++] = (long long)kSums * dim;
+        }
+    ctx.note_launch("block_norms_grad");
+    if (partials) ctx.note_launch("block_norms_join");
+    if (by_group) ctx.note_launch("block_norms_gates");
+    sage_status status = SAGE_OK;
+    if (!ctx.dry()) {
+        if (partials && a.teams > 1) smem = std::max(smem, (size_t)dim * 4);
+        status = with_types(tx, t, [&](auto txv, auto tv) {
+            typedef decltype(txv) TX;
+            typedef decltype(tv) T;
+            const auto by_ring = [&](auto kernel) {
+                sage_status s = ctx.check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes), "block_norms_grad");
+                return s ? s : ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3((unsigned)grid), dim3((unsigned)threads), smem, a), "block_norms_grad");
+            };
+            const auto any = [&](auto kernel) { return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3((unsigned)grid), dim3((unsigned)threads), smem, a, wide, weights_wide(a)), "block_norms_grad"); };
+            if (ring) {
+                if (full) return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, true>) : by_ring(block_norms_grad_ring_kernel<TX, T, 2, true>);
+                return nv == 1   ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, false>)
+                       : nv == 2 ? by_ring(block_norms_grad_ring_kernel<TX, T, 2, false>)
+                       : nv == 3 ? by_ring(block_norms_grad_ring_kernel<TX, T, 3, false>)
+                                 : by_ring(block_norms_grad_ring_kernel<TX, T, 4, false>);
+            }
+            if (full) return nv == 1 ? any(block_norms_grad_kernel<TX, T, 1, true>) : nv == 2 ? any(block_norms_grad_kernel<TX, T, 2, true>) : any(block_norms_grad_kernel<TX, T, 4, true>);
+            return nv == 1   ? any(block_norms_grad_kernel<TX, T, 1, false>)
+                   : nv == 2 ? any(block_norms_grad_kernel<TX, T, 2, false>)
+                             : any(block_norms_grad_kernel<TX, T, 4, false>);
+        });
+        if (!status && partials)
+            status = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), block_norms_join_kernel, dim3((unsigned)((dim + 31) / 32), (unsigned)partials), dim3(32 * kJoinParts), 0, join), "block_norms_join");
+        if (!status && by_group) {
+            const long long total = groups * dim;
+            status = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), block_norms_gates_kernel, dim3((unsigned)std::min((total + 255) / 256, (long long)ctx.sm_count * 8)), dim3(256), 0,
+                                                     (const float *)a.gate_partial, (float *)sums.gate.ptr, a.splits, a.dim, total, sums.gate.pitch),
+                                    "block_norms_gates");
+        }
+    }
+    if (scratch) ctx.allocator().free(scratch);
+    return status;
+}
+
+}  // namespace k
+}  // namespace sage

@@ -18,7 +18,11 @@ struct Dropout {
 struct Key {
     unsigned a, b;
 };
-__device__ __forceinline__ Key key_of(const Dropout &d) { return d.bar ? Key{__ldg(d.seed), __ldg(d.seed + d.seed_stride)} : Key{0u, 0u}; }
+// (the shuffle tells the compiler that a warp has one key, whose sums with the rounds' constants it then keeps once for all lanes)
+__device__ __forceinline__ Key key_of(const Dropout &d) {
+    if (!d.bar) return Key{0u, 0u};
+    return Key{__shfl_sync(0xffffffffu, __ldg(d.seed), 0), __shfl_sync(0xffffffffu, __ldg(d.seed + d.seed_stride), 0)};
+}
 
 __device__ __forceinline__ uint4 philox(Key k, unsigned long long count, unsigned long long site) {
     uint4 x = make_uint4((unsigned)count, (unsigned)(count >> 32), (unsigned)site, (unsigned)(site >> 32));

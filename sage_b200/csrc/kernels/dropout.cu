@@ -26,6 +26,7 @@ constexpr int kThreads = 256;
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs a) {
     grid_dependency_sync();
+    const Key key = key_of(a.d);
     const long long block = (long long)blockIdx.x * kThreads + threadIdx.x, first = 8 * block;
     if (first >= a.n) return;
     const T *x = (const T *)a.x;
@@ -36,7 +37,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs a) 
         Pack<T> p[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) p[i] = *(const Pack<T> *)(x + row * a.px + col + i * N);
-        const unsigned keep = a.d.bar ? keep8(a.d, key_of(a.d), block) : 0xffu;
+        const unsigned keep = a.d.bar ? keep8(a.d, key, block) : 0xffu;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
 #pragma unroll
@@ -44,7 +45,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs a) 
             *(Pack<T> *)(y + row * a.py + col + i * N) = p[i];
         }
     } else {
-        const unsigned keep = a.d.bar ? keep8(a.d, key_of(a.d), block) : 0xffu;
+        const unsigned keep = a.d.bar ? keep8(a.d, key, block) : 0xffu;
         long long row = first / a.cols, col = first - row * a.cols;
         const int count = (int)min(8ll, a.n - first);
         for (int e = 0; e < count; ++e) {
