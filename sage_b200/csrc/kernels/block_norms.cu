@@ -16,8 +16,10 @@ __host__ __device__ constexpr int wide_registers(int nv) { return nv <= 2 ? 64 :
 // Whole runs of eight columns on 16-byte boundaries: a team takes one row, all of whose columns are asked for before anything waits.  Teams enough for
 // the memory's latency are there at once, and the weights stay in L1 (with rows brought through rings in shared memory by teams that stay,
 // 16384 x 4096 took 232 us: what is left of L1 then does not hold the weights).
+__device__ __forceinline__ void prefetch_row(const char *p, int bytes) { asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory"); }
+
 template <class TX, class T, int NV>
-__global__ void __maxnreg__(wide_registers(NV)) block_norms_wide_kernel(const NormsArgs a) {
+__global__ void __maxnreg__(wide_registers(NV)) block_norms_wide_kernel(const NormsArgs a, const int ahead) {
     __shared__ __align__(16) float2 slots[kSlots];
     Place at = place_of(a, slots);
     grid_dependency_sync();
@@ -35,6 +37,10 @@ __global__ void __maxnreg__(wide_registers(NV)) block_norms_wide_kernel(const No
 #pragma unroll
     for (int v = 0; v < NV; ++v)
         if (v + 1 < NV || last) xs[v].load(from_x + v * run * (int)sizeof(TX));
+    if (!col && row < a.rows - ahead) {  // the rows of the CTAs that come when these have gone, into L2
+        prefetch_row(at_row<TX>(a.x, row + ahead, 0), a.dim * (int)sizeof(TX));
+        if (branch) prefetch_row(at_row<T>(a.y, row + ahead, 0), a.dim * (int)sizeof(T));
+    }
     const Key key = key_of(a.d);
     const float per = 1.f / (float)a.dim;
     float2 r[NV][4];
@@ -268,12 +274,13 @@ sage_status block_norms(Context &ctx, const BlockNorms &n, const RowsArg &x, con
     size_t none;
     a.teams = std::max(1, std::min(128 / a.team, kMaxTeams));
     const int threads = a.team * a.teams, grid = vectors ? (a.rows + a.teams - 1) / a.teams : grid_of(ctx, &a, nv, 0, kRegisters, false, &none);
+    const int ahead = ctx.sm_count * (65536 / (wide_registers(nv) * threads)) * a.teams;  // rows that are worked on at once
     ctx.note_launch("block_norms");
     if (ctx.dry()) return SAGE_OK;
     return with_types(x.dtype, t, [&](auto tx, auto tt) {
         typedef decltype(tx) TX;
         typedef decltype(tt) T;
-        const auto by_vectors = [&](auto kernel) { return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3((unsigned)grid), dim3((unsigned)threads), 0, a), "block_norms"); };
+        const auto by_vectors = [&](auto kernel) { return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3((unsigned)grid), dim3((unsigned)threads), 0, a, ahead), "block_norms"); };
         const auto any = [&](auto kernel) { return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3((unsigned)grid), dim3((unsigned)threads), 0, a, wide, weights_wide(a)), "block_norms"); };
         if (vectors)
             return nv == 1 ? by_vectors(block_norms_wide_kernel<TX, T, 1>) : nv == 2 ? by_vectors(block_norms_wide_kernel<TX, T, 2>) : nv == 3 ? by_vectors(block_norms_wide_kernel<TX, T, 3>) : by_vectors(block_norms_wide_kernel<TX, T, 4>);

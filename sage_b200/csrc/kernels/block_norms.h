@@ -8,9 +8,9 @@
 #include <algorithm>
 
 #include "counter_random.h"
+#include "eight.h"
 #include "language.h"
 #include "launch.h"
-#include "narrow.h"
 
 namespace sage {
 namespace k {
@@ -22,6 +22,7 @@ constexpr int kRingBytes = 216 * 1024;            // of an SM's shared memory, f
 struct Rows {
     void *p;
     long long pitch;
+    unsigned bytes;  // of a pitch, where that is less than 4 GB
 };
 
 struct NormsArgs {
@@ -93,47 +94,6 @@ struct Team {
 };
 constexpr int kSlots = 32 * kMaxTeams;
 
-// Pairs of columns.
-template <class T>
-__device__ __forceinline__ float2 pair_at(const Pack<T> &p, int i) { return make_float2(widen(p.v[2 * i]), widen(p.v[2 * i + 1])); }
-template <>
-__device__ __forceinline__ float2 pair_at<__nv_bfloat16>(const Pack<__nv_bfloat16> &p, int i) {
-    const unsigned u = ((const unsigned *)&p)[i];
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ float2 pair_at<__half>(const Pack<__half> &p, int i) { return __half22float2(((const __half2 *)&p)[i]); }
-template <class T>
-__device__ __forceinline__ void put_pair(Pack<T> &p, int i, float2 x) {
-    p.v[2 * i] = narrowed<T>(x.x);
-    p.v[2 * i + 1] = narrowed<T>(x.y);
-}
-template <>
-__device__ __forceinline__ void put_pair<__nv_bfloat16>(Pack<__nv_bfloat16> &p, int i, float2 x) { ((__nv_bfloat162 *)&p)[i] = __float22bfloat162_rn(x); }
-template <>
-__device__ __forceinline__ void put_pair<__half>(Pack<__half> &p, int i, float2 x) { ((__half2 *)&p)[i] = __float22half2_rn(x); }
-
-template <class T>
-struct Eight {  // columns, as they are stored
-    static constexpr int kPacks = 8 / Pack<T>::N;
-    Pack<T> p[kPacks];
-    __device__ __forceinline__ void load(const char *from) {
-#pragma unroll
-        for (int i = 0; i < kPacks; ++i) p[i] = ((const Pack<T> *)from)[i];
-    }
-    __device__ __forceinline__ void store(char *to) const {
-#pragma unroll
-        for (int i = 0; i < kPacks; ++i) ((Pack<T> *)to)[i] = p[i];
-    }
-    __device__ __forceinline__ void open(float2 (&v)[4]) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = pair_at<T>(p[i / (4 / kPacks)], i % (4 / kPacks));
-    }
-    __device__ __forceinline__ void close(const float2 (&v)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) put_pair<T>(p[i / (4 / kPacks)], i % (4 / kPacks), v[i]);
-    }
-};
 template <class T>
 __device__ __forceinline__ void load8(const T *p, int count, bool wide, float2 (&v)[4]) {
     Eight<T> q;
@@ -248,7 +208,7 @@ __device__ __forceinline__ unsigned kept(const Dropout &d, Key key, int row, int
 // took more of them than the sums over rows do.
 template <class T>
 __device__ __forceinline__ char *at_row(const Rows &r, int row, int col) {
-    return (char *)r.p + (unsigned long long)(unsigned)row * (unsigned)(r.pitch * (long long)sizeof(T)) + (unsigned)(col * (int)sizeof(T));
+    return (char *)r.p + ((unsigned long long)(unsigned)row * r.bytes + (unsigned)(col * (int)sizeof(T)));
 }
 template <class T, int NV>
 __device__ __forceinline__ void ring_ask(const Rows &r, int row, int col, int run, bool last, unsigned to, unsigned piece) {
@@ -282,16 +242,12 @@ __device__ __forceinline__ void get8(const float *p, float2 (&v)[4]) {  // weigh
     const float4 a = __ldg((const float4 *)p), b = __ldg((const float4 *)p + 1);
     v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
 }
-// Eight columns of which some are dropped, by the sixteen bits of each.
-__device__ __forceinline__ void drop8(float2 (&v)[4], const uint4 &w, unsigned bar) {
-    const unsigned words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = make_float2((words[i] & 0xffffu) >= bar ? v[i].x : 0.f, (words[i] >> 16) >= bar ? v[i].y : 0.f);
-}
-
 inline bool boundary(const Rows &r, long long size) { return (uintptr_t)r.p % 16 == 0 && r.pitch * size % 16 == 0 && r.pitch * size < 0x100000000ll; }
 inline bool boundary(const float *p) { return (uintptr_t)p % 16 == 0; }
-inline Rows of(const RowsArg &r) { return Rows{r.ptr, r.rows > 1 ? r.pitch : r.cols}; }
+inline Rows of(const RowsArg &r) {
+    const long long pitch = r.rows > 1 ? r.pitch : r.cols;
+    return Rows{r.ptr, pitch, (unsigned)(pitch * (r.dtype == SAGE_F32 ? 4 : 2))};
+}
 
 // Threads of a row: of the numbers of runs a thread may own, the one that leaves the fewest without columns, and of those the largest, since what a row
 // costs each thread is shared by its columns; teams of a CTA: up to 256 threads.

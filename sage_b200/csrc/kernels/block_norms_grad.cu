@@ -58,7 +58,18 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
     // a stage: out, gh, go and (FULL) y
     const unsigned piece = blockDim.x * 16;
     constexpr int kGh = pieces<TX>(NV), kGo = kGh + pieces<T>(NV), kY = kGo + pieces<TX>(NV), kStage = kY + (FULL ? pieces<T>(NV) : 0);
+    const int wcol = last ? col + (NV - 1) * run : 0;  // of the last run's weights: threads without one work on zeros, and on any weights
     const unsigned stage = kStage * piece, ring0 = (unsigned)__cvta_generic_to_shared(ring) + threadIdx.x * 16, ring1 = ring0 + a.stages * stage;
+    if (!last)
+        for (int s = 0; s < a.stages; ++s) {
+            const auto clear = [&](int first, int packs) {
+                for (int p = first + (NV - 1) * packs; p < first + NV * packs; ++p) *(uint4 *)(ring + threadIdx.x * 16 + s * stage + p * piece) = make_uint4(0u, 0u, 0u, 0u);
+            };
+            clear(0, Eight<TX>::kPacks);
+            clear(kGh, Eight<T>::kPacks);
+            clear(kGo, Eight<TX>::kPacks);
+            if (FULL) clear(kY, Eight<T>::kPacks);
+        }
     const Key key = key_of(a.d);
     const float per = 1.f / (float)a.dim;
     const float2 zero = make_float2(0.f, 0.f);
@@ -92,6 +103,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
         for (int i = FULL ? 0 : 2; i < 4; ++i) next[i] = __ldg(a.stats + row0 * a.stats_pitch + i);
         for (int row = row0; row < end; row += a.splits) {
             const float mean_a = FULL ? next[0] : 0.f, rstd_a = FULL ? next[1] : 1.f, mean_b = next[2], rstd_b = next[3];
+            const float from_a = -mean_a * rstd_a, from_b = -mean_b * rstd_b;  // unit rows are x * rstd + these
             if (end - row > a.splits)
 #pragma unroll
                 for (int i = FULL ? 0 : 2; i < 4; ++i) next[i] = __ldg(a.stats + (row + a.splits) * a.stats_pitch + i);
@@ -99,15 +111,14 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
             copies_wait(a.stages);
             float2 q[NV][4], along = zero, all = zero;  // what arrives through the norm
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
-                if (v + 1 < NV || last) {
+            for (int v = 0; v < NV; ++v) {
                     float2 u[4], w[4];
                     ring_get<TX>(take, v, piece, u);
                     ring_get<T>(take + kGh * piece, v, piece, q[v]);
-                    get8(a.wb + col + v * run, w);
+                    get8(a.wb + (v + 1 < NV ? col + v * run : wcol), w);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        u[i] = mul2(add2(u[i], both(-mean_b)), both(rstd_b));
+                        u[i] = fma2(u[i], both(rstd_b), both(from_b));
                         sum[kSumWb][v][i] = fma2(q[v][i], u[i], sum[kSumWb][v][i]);
                         sum[kSumBb][v][i] = add2(sum[kSumBb][v][i], q[v][i]);
                         q[v][i] = mul2(q[v][i], w[i]);
@@ -119,26 +130,27 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
             const float along_u = s1.x * per, mean_q = a.before == SAGE_NORM_LAYER ? s1.y * per : 0.f;
             float2 along_t = zero, all_t = zero;
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
-                if (v + 1 < NV || last) {
-                    const int at_col = col + v * run;
+            for (int v = 0; v < NV; ++v) {
+                    const bool there = v + 1 < NV || last;
+                    const int at_col = v + 1 < NV ? col + v * run : wcol;
+                    const float through = there ? rstd_b : 0.f;
                     float2 G[4], u[4];
                     ring_get<TX>(take + kGo * piece, v, piece, G);
                     ring_get<TX>(take, v, piece, u);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        u[i] = mul2(add2(u[i], both(-mean_b)), both(rstd_b));
-                        G[i] = fma2(fma2(u[i], both(-along_u), add2(q[v][i], both(-mean_q))), both(rstd_b), G[i]);
+                        u[i] = fma2(u[i], both(rstd_b), both(from_b));
+                        G[i] = fma2(fma2(u[i], both(-along_u), add2(q[v][i], both(-mean_q))), both(through), G[i]);
                         u[i] = mul2(G[i], both(a.scale));
                     }
-                    if (a.dx.p) put8<TX>(at_row<TX>(a.dx, row, at_col), u);
+                    if (a.dx.p && there) put8<TX>(at_row<TX>(a.dx, row, at_col), u);
                     if (a.d.bar) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) G[i] = mul2(G[i], both(a.d.factor));
                         drop8(G, philox(key, ((unsigned long long)(unsigned)row * (unsigned)a.dim + at_col) >> 3, a.d.site), a.d.bar);
                     }
                     if (!FULL) {
-                        if (a.dy.p) put8<T>(at_row<T>(a.dy, row, at_col), G);
+                        if (a.dy.p && there) put8<T>(at_row<T>(a.dy, row, at_col), G);
                         continue;
                     }
                     float2 n[4], w[4], b[4];
@@ -146,7 +158,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
                     if (a.after != SAGE_NORM_NONE) {
                         get8(a.wa + at_col, w);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) n[i] = mul2(add2(n[i], both(-mean_a)), both(rstd_a));
+                        for (int i = 0; i < 4; ++i) n[i] = fma2(n[i], both(rstd_a), both(from_a));
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) w[i] = both(1.f);
@@ -192,7 +204,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
                             ring_get<T>(take + kY * piece, v, piece, n);
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                q[v][i] = mul2(fma2(mul2(add2(n[i], both(-mean_a)), both(rstd_a)), both(-along_v), add2(q[v][i], both(-mean_t))), both(rstd_a));
+                                q[v][i] = mul2(fma2(fma2(n[i], both(rstd_a), both(from_a)), both(-along_v), add2(q[v][i], both(-mean_t))), both(rstd_a));
                         }
                         put8<T>(at_row<T>(a.dy, row, col + v * run), q[v]);
                     }
@@ -373,42 +385,52 @@ __global__ void __maxnreg__(kRegisters) block_norms_grad_kernel(const NormsArgs 
     join_teams(a, at, sum, count, wide, (float *)ring);
 }
 
-// y[j] = the sum over i of x[i * pitch + j], in a fixed order: sixteen runs of i, then their sums.
+// The sums that CTAs, and shares of a group's rows, left: y[j] = the sum over i of x[i * pitch + j], in a fixed order: warp by warp every 16th, then
+// the warps'.  A row of blocks for each kind, and for each group of a gate.
 struct Join {
     const float *x[kSums];
     float *y[kSums];
-    int count[kSums];       // addends
-    long long pitch[kSums];
-    int dim;
+    int kinds, count;         // addends
+    long long pitch;
+    const float *gate_x;      // gates of several groups: `splits` addends each, dim apart
+    float *gate_y;
+    long long gate_pitch;
+    int splits, dim;
 };
 constexpr int kJoinParts = 16;
 __global__ void __launch_bounds__(32 * kJoinParts) block_norms_join_kernel(const Join a) {
-    __shared__ float part[kJoinParts][33];
+    __shared__ float2 part[kJoinParts][32];
     grid_dependency_sync();
-    const int s = (int)blockIdx.y, lane = (int)threadIdx.x & 31, w = (int)threadIdx.x >> 5, col = (int)blockIdx.x * 32 + lane;
-    float sum = 0.f;
-    if (col < a.dim) {
-        const float *x = a.x[s] + col;
-#pragma unroll 4
-        for (int i = w; i < a.count[s]; i += kJoinParts) sum += x[i * a.pitch[s]];
+    const int lane = (int)threadIdx.x & 31, w = (int)threadIdx.x >> 5, col = ((int)blockIdx.x * 32 + lane) * 2, s = (int)blockIdx.y;
+    const bool kind = s < a.kinds;
+    const int count = kind ? a.count : a.splits;
+    const long long group = s - a.kinds, pitch = kind ? a.pitch : a.dim;
+    const float *x = (kind ? a.x[s] : a.gate_x + group * a.splits * a.dim) + col;
+    const bool two = a.dim % 2 == 0 && col < a.dim, one = col < a.dim;  // (the partial sums lie on 256-byte boundaries)
+    float2 sum = make_float2(0.f, 0.f);
+    int i = w;
+    for (; i + 3 * kJoinParts < count; i += 4 * kJoinParts) {
+        float2 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float *p = x + (i + k * kJoinParts) * pitch;
+            v[k] = two ? *(const float2 *)p : make_float2(one ? p[0] : 0.f, col + 1 < a.dim ? p[1] : 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum = add2(sum, v[k]);
+    }
+    for (; i < count; i += kJoinParts) {
+        const float *p = x + i * pitch;
+        sum = add2(sum, two ? *(const float2 *)p : make_float2(one ? p[0] : 0.f, col + 1 < a.dim ? p[1] : 0.f));
     }
     part[w][lane] = sum;
     __syncthreads();
-    if (w || col >= a.dim) return;
+    if (w || !one) return;
 #pragma unroll
-    for (int i = 1; i < kJoinParts; ++i) sum += part[i][lane];
-    a.y[s][col] = sum;
-}
-// Gates of several groups: y[g, j] = the sum over `splits` rows of x.
-__global__ void __launch_bounds__(256) block_norms_gates_kernel(const float *x, float *y, int splits, int dim, long long total, long long pitch) {
-    grid_dependency_sync();
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        const long long g = i / dim, col = i - g * dim;
-        float sum = 0.f;
-#pragma unroll 4
-        for (int s = 0; s < splits; ++s) sum += x[(g * splits + s) * dim + col];
-        y[g * pitch + col] = sum;
-    }
+    for (int k = 1; k < kJoinParts; ++k) sum = add2(sum, part[k][lane]);
+    float *y = (kind ? a.y[s] : a.gate_y + group * a.gate_pitch) + col;
+    y[0] = sum.x;
+    if (col + 1 < a.dim) y[1] = sum.y;
 }
 
 }  // namespace
@@ -469,13 +491,20 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
     join.dim = a.dim;
     for (int s = 0, i = 0; s < kSums; ++s)
         if (a.sums >> s & 1) {
-            join.x[i] = a.partial + (long long)s * dim;
-            join.count[i] = grid;
-            join.pitch[i++] = (long long)kSums * dim;
+            join.x[i++] = a.partial + (long long)s * dim;
         }
     ctx.note_launch("block_norms_grad");
-    if (partials) ctx.note_launch("block_norms_join");
-    if (by_group) ctx.note_launch("block_norms_gates");
+    join.kinds = partials;
+    join.count = grid;
+    join.pitch = (long long)kSums * dim;
+    join.splits = a.splits;
+    if (by_group) {
+        join.gate_x = a.gate_partial;
+        join.gate_y = (float *)sums.gate.ptr;
+        join.gate_pitch = sums.gate.pitch;
+    }
+    const long long joins = partials + (by_group ? groups : 0), once = 32768;  // rows of blocks, as many as a launch may have
+    for (long long at = 0; at < joins; at += once) ctx.note_launch("block_norms_join");
     sage_status status = SAGE_OK;
     if (!ctx.dry()) {
         if (partials && a.teams > 1) smem = std::max(smem, (size_t)dim * 4);
@@ -499,13 +528,14 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
                    : nv == 2 ? any(block_norms_grad_kernel<TX, T, 2, false>)
                              : any(block_norms_grad_kernel<TX, T, 4, false>);
         });
-        if (!status && partials)
-            status = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), block_norms_join_kernel, dim3((unsigned)((dim + 31) / 32), (unsigned)partials), dim3(32 * kJoinParts), 0, join), "block_norms_join");
-        if (!status && by_group) {
-            const long long total = groups * dim;
-            status = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), block_norms_gates_kernel, dim3((unsigned)std::min((total + 255) / 256, (long long)ctx.sm_count * 8)), dim3(256), 0,
-                                                     (const float *)a.gate_partial, (float *)sums.gate.ptr, a.splits, a.dim, total, sums.gate.pitch),
-                                    "block_norms_gates");
+        for (long long at = 0; at < joins && !status; at += once) {
+            status = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), block_norms_join_kernel, dim3((unsigned)((dim + 63) / 64), (unsigned)std::min(once, joins - at)), dim3(32 * kJoinParts), 0, join), "block_norms_join");
+            const long long done = std::min(once, joins - at) - join.kinds;  // groups
+            join.kinds = 0;
+            if (join.gate_x) {
+                join.gate_x += done * a.splits * dim;
+                join.gate_y += done * join.gate_pitch;
+            }
         }
     }
     if (scratch) ctx.allocator().free(scratch);

@@ -6,9 +6,9 @@
 #include <algorithm>
 
 #include "counter_random.h"
+#include "eight.h"
 #include "language.h"
 #include "launch.h"
-#include "narrow.h"
 
 namespace sage {
 namespace k {
@@ -21,32 +21,42 @@ struct DropoutArgs {
     Dropout d;
 };
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kBlocks = 4;  // of a CTA; blocks of eight elements to a thread
 
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs a) {
     grid_dependency_sync();
     const Key key = key_of(a.d);
-    const long long block = (long long)blockIdx.x * kThreads + threadIdx.x, first = 8 * block;
-    if (first >= a.n) return;
+    const long long block0 = (long long)blockIdx.x * (kThreads * kBlocks) + threadIdx.x;
     const T *x = (const T *)a.x;
     T *y = (T *)a.y;
-    if (WIDE && first + 8 <= a.n) {
-        const long long row = a.cols == a.n ? 0 : a.n <= 0xffffffffll ? (unsigned)first / (unsigned)a.cols : first / a.cols, col = first - row * a.cols;
-        constexpr int N = Pack<T>::N, P = 8 / N;
-        Pack<T> p[P];
+    const auto row_of = [&](long long i) { return a.cols == a.n ? 0 : a.n <= 0xffffffffll ? (long long)((unsigned)i / (unsigned)a.cols) : i / a.cols; };
+    if (WIDE && 8 * (block0 + (kBlocks - 1) * kThreads) + 8 <= a.n) {  // whole blocks, all of them asked for at once
+        Eight<T> v[kBlocks];
+        long long to[kBlocks];
 #pragma unroll
-        for (int i = 0; i < P; ++i) p[i] = *(const Pack<T> *)(x + row * a.px + col + i * N);
-        const unsigned keep = a.d.bar ? keep8(a.d, key, block) : 0xffu;
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) p[i].v[e] = narrowed<T>(keep >> (i * N + e) & 1u ? widen(p[i].v[e]) * a.d.factor : 0.f);
-            *(Pack<T> *)(y + row * a.py + col + i * N) = p[i];
+        for (int b = 0; b < kBlocks; ++b) {
+            const long long first = 8 * (block0 + b * kThreads), row = row_of(first), col = first - row * a.cols;
+            v[b].load((const char *)(x + row * a.px + col));
+            to[b] = row * a.py + col;
         }
-    } else {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            float2 f[4];
+            v[b].open(f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = mul2(f[i], both(a.d.factor));
+            if (a.d.bar) drop8(f, philox(key, block0 + b * kThreads, a.d.site), a.d.bar);
+            v[b].close(f);
+            v[b].store((char *)(y + to[b]));
+        }
+        return;
+    }
+    for (int b = 0; b < kBlocks; ++b) {
+        const long long block = block0 + b * kThreads, first = 8 * block;
+        if (first >= a.n) return;
         const unsigned keep = a.d.bar ? keep8(a.d, key, block) : 0xffu;
-        long long row = first / a.cols, col = first - row * a.cols;
+        long long row = row_of(first), col = first - row * a.cols;
         const int count = (int)min(8ll, a.n - first);
         for (int e = 0; e < count; ++e) {
             y[row * a.py + col] = narrowed<T>(keep >> e & 1u ? widen(x[row * a.px + col]) * a.d.factor : 0.f);
@@ -64,8 +74,8 @@ sage_status dropout(Context &ctx, const RowsArg &x, const RowsArg &y, const Drop
     if (!x.rows || !x.cols) return SAGE_OK;
     DropoutArgs a{x.ptr, y.ptr, x.rows * x.cols, x.cols, x.pitch, y.pitch, d};
     if (x.rows == 1 || (x.pitch == x.cols && y.pitch == x.cols)) a.cols = a.n;
-    const long long size = x.dtype == SAGE_F32 ? 4 : 2, blocks = (a.n + 8 * kThreads - 1) / (8 * kThreads);
-    if (blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "dropout: more than 2^42 elements");
+    const long long size = x.dtype == SAGE_F32 ? 4 : 2, blocks = (a.n + 8 * kThreads * kBlocks - 1) / (8 * kThreads * kBlocks);
+    if (blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "dropout: more than 2^44 elements");
     const bool one = a.cols == a.n;
     const bool wide = (uintptr_t)x.ptr % 16 == 0 && (uintptr_t)y.ptr % 16 == 0 && (one || (a.cols % 8 == 0 && x.pitch * size % 16 == 0 && y.pitch * size % 16 == 0));
     ctx.note_launch("dropout");

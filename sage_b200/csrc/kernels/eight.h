@@ -1,0 +1,49 @@
+// Eight neighbouring elements in 16 or 32 bits each, as four pairs of f32 values and back.
+#pragma once
+#include "narrow.h"
+
+namespace sage {
+namespace k {
+
+template <class T>
+__device__ __forceinline__ float2 pair_at(const Pack<T> &p, int i) { return make_float2(widen(p.v[2 * i]), widen(p.v[2 * i + 1])); }
+template <>
+__device__ __forceinline__ float2 pair_at<__nv_bfloat16>(const Pack<__nv_bfloat16> &p, int i) {
+    const unsigned u = ((const unsigned *)&p)[i];
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 pair_at<__half>(const Pack<__half> &p, int i) { return __half22float2(((const __half2 *)&p)[i]); }
+template <class T>
+__device__ __forceinline__ void put_pair(Pack<T> &p, int i, float2 x) {
+    p.v[2 * i] = narrowed<T>(x.x);
+    p.v[2 * i + 1] = narrowed<T>(x.y);
+}
+template <>
+__device__ __forceinline__ void put_pair<__nv_bfloat16>(Pack<__nv_bfloat16> &p, int i, float2 x) { ((__nv_bfloat162 *)&p)[i] = __float22bfloat162_rn(x); }
+template <>
+__device__ __forceinline__ void put_pair<__half>(Pack<__half> &p, int i, float2 x) { ((__half2 *)&p)[i] = __float22half2_rn(x); }
+
+template <class T>
+struct Eight {  // columns, as they are stored
+    static constexpr int kPacks = 8 / Pack<T>::N;
+    Pack<T> p[kPacks];
+    __device__ __forceinline__ void load(const char *from) {
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) p[i] = ((const Pack<T> *)from)[i];
+    }
+    __device__ __forceinline__ void store(char *to) const {
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) ((Pack<T> *)to)[i] = p[i];
+    }
+    __device__ __forceinline__ void open(float2 (&v)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = pair_at<T>(p[i / (4 / kPacks)], i % (4 / kPacks));
+    }
+    __device__ __forceinline__ void close(const float2 (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put_pair<T>(p[i / (4 / kPacks)], i % (4 / kPacks), v[i]);
+    }
+};
+}  // namespace k
+}  // namespace sage
