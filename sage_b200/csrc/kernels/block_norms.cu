@@ -273,7 +273,7 @@ sage_status block_norms(Context &ctx, const BlockNorms &n, const RowsArg &x, con
     const bool vectors = wide && weights_wide(a);
     size_t none;
     a.teams = std::max(1, std::min(128 / a.team, kMaxTeams));
-    const int threads = a.team * a.teams, grid = vectors ? (a.rows + a.teams - 1) / a.teams : grid_of(ctx, &a, nv, 0, kRegisters, false, &none);
+    const int grid = vectors ? (a.rows + a.teams - 1) / a.teams : grid_of(ctx, &a, nv, 0, kRegisters, false, &none), threads = a.team * a.teams;  // (grid_of sets the teams)
     const int ahead = ctx.sm_count * (65536 / (wide_registers(nv) * threads)) * a.teams;  // rows that are worked on at once
     ctx.note_launch("block_norms");
     if (ctx.dry()) return SAGE_OK;

@@ -47,12 +47,10 @@ struct NormsArgs {
 enum { kSumWb, kSumBb, kSumWa, kSumBa, kSumGate, kSums };
 
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the `stages - 1` youngest groups have arrived.
+// All but the `stages - 1` youngest groups have arrived (two stages or four).
 __device__ __forceinline__ void copies_wait(int stages) {
     if (stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else asm volatile("cp.async.wait_group 1;" ::: "memory");
 }
 
 // Sums over a team, two at a time, the same bits in all of its threads.
@@ -83,12 +81,13 @@ struct Team {
         const float4 *q = (const float4 *)(slots + turn);
         turn ^= 16;  // (the next sum but one writes here again, behind the next one's barrier)
         asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(threads) : "memory");
-        float4 a = q[0], b = q[1];
-        float2 t = add2(add2(make_float2(a.x, a.y), make_float2(a.z, a.w)), add2(make_float2(b.x, b.y), make_float2(b.z, b.w)));
-        for (int w = 4; w < warps; w += 4) {
-            a = q[w / 2], b = q[w / 2 + 1];
-            t = add2(t, add2(add2(make_float2(a.x, a.y), make_float2(a.z, a.w)), add2(make_float2(b.x, b.y), make_float2(b.z, b.w))));
-        }
+        const auto eight = [&](int at) {
+            const float4 a = q[at], b = q[at + 1], c = q[at + 2], d = q[at + 3];
+            return add2(add2(add2(make_float2(a.x, a.y), make_float2(a.z, a.w)), add2(make_float2(b.x, b.y), make_float2(b.z, b.w))),
+                        add2(add2(make_float2(c.x, c.y), make_float2(c.z, c.w)), add2(make_float2(d.x, d.y), make_float2(d.z, d.w))));
+        };
+        float2 t = eight(0);
+        if (warps > 8) t = add2(t, eight(4));
         return t;
     }
 };
@@ -210,15 +209,10 @@ template <class T>
 __device__ __forceinline__ char *at_row(const Rows &r, int row, int col) {
     return (char *)r.p + ((unsigned long long)(unsigned)row * r.bytes + (unsigned)(col * (int)sizeof(T)));
 }
-template <class T, int NV>
-__device__ __forceinline__ void ring_ask(const Rows &r, int row, int col, int run, bool last, unsigned to, unsigned piece) {
-    const char *from = at_row<T>(r, row, col);
+template <class T>
+__device__ __forceinline__ void ring_ask(const char *from, unsigned to, unsigned piece) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-        if (v + 1 < NV || last)
-#pragma unroll
-            for (int i = 0; i < Eight<T>::kPacks; ++i)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (v * Eight<T>::kPacks + i) * piece), "l"(from + (unsigned)(v * run * (int)sizeof(T)) + i * 16) : "memory");
+    for (int i = 0; i < Eight<T>::kPacks; ++i) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * piece), "l"(from + i * 16) : "memory");
 }
 template <class T>
 __device__ __forceinline__ void ring_get(unsigned from, int v, unsigned piece, float2 (&x)[4]) {
@@ -250,7 +244,7 @@ inline Rows of(const RowsArg &r) {
 }
 
 // Threads of a row: of the numbers of runs a thread may own, the one that leaves the fewest without columns, and of those the largest, since what a row
-// costs each thread is shared by its columns; teams of a CTA: up to 256 threads.
+// costs each thread is shared by its columns.
 inline int shape_of(NormsArgs *a, int least, int most) {
     const int runs = (a->dim + 7) / 8;
     int slots = 0;
@@ -260,22 +254,33 @@ inline int shape_of(NormsArgs *a, int least, int most) {
         slots = taken;
         a->team = team;
     }
-    a->teams = std::max(1, std::min(256 / a->team, kMaxTeams));
     return (runs + a->team - 1) / a->team;  // all of a thread's runs but the last are whole
 }
-// How many CTAs, and how deep the ring: `row_bytes` of what a row reads, `registers` of a thread.
+// How many teams a CTA has and how many CTAs there are, and how deep the ring: `operand_bytes` of what a column reads, `registers` of a thread.  As many
+// teams at once as an SM's registers hold (each quarter of it has 16384), in few CTAs, which leave few sums behind.
 inline int grid_of(Context &ctx, NormsArgs *a, int nv, size_t operand_bytes, int registers, bool ring, size_t *smem) {
-    const int threads = a->team * a->teams;
-    int fit = std::max(1, 65536 / (registers * threads));
-    const size_t stage = (size_t)threads * nv * 8 * operand_bytes;
-    const long long wanted = (a->rows + a->teams - 1) / a->teams;
+    const int team_warps = a->team / 32, warps = 16384 / (registers * 32) * 4;
+    int fit = 0;
+    a->teams = 1;
+    for (int t = 1; t * a->team <= 1024 && t <= kMaxTeams; ++t) {
+        const int ctas = warps / (t * team_warps);
+        if (ctas && ctas * t >= fit * a->teams) {
+            fit = ctas;
+            a->teams = t;
+        }
+    }
+    fit = std::max(1, fit);
+    const size_t stage = (size_t)a->team * nv * 8 * operand_bytes;  // of a team
     a->stages = 4;
     if (ring) {
-        while (a->stages > 2 && stage * a->stages * fit > (size_t)kRingBytes) --a->stages;
-        while (fit > 1 && stage * a->stages * fit > (size_t)kRingBytes) --fit;
+        if (stage * 4 * a->teams * fit > (size_t)kRingBytes) a->stages = 2;
+        while (fit > 1 && stage * a->stages * a->teams * fit > (size_t)kRingBytes) --fit;
+        while (a->teams > 1 && stage * a->stages * a->teams > (size_t)kRingBytes) --a->teams;
     }
-    *smem = ring ? stage * a->stages : 0;
-    const int grid = (int)std::min<long long>(wanted, (long long)ctx.sm_count * fit);
+    *smem = ring ? stage * a->stages * a->teams : 0;
+    while (a->teams > 1 && (a->rows + a->teams - 1) / a->teams < ctx.sm_count) --a->teams;  // few rows: on all SMs
+    const int grid = (int)std::min<long long>((a->rows + a->teams - 1) / a->teams, (long long)ctx.sm_count * fit);
+    if (ring) *smem = stage * a->stages * a->teams;
     a->splits = std::max(1, std::min(a->group_rows, grid * a->teams / (a->rows / a->group_rows)));
     return grid;
 }

@@ -46,7 +46,7 @@ __host__ __device__ constexpr int ring_registers(int nv, bool full) { return ful
 
 // What models call: both gradients arrive, there is a norm before the next block and norms have weights; whole runs of columns on
 // 16-byte boundaries.
-template <class TX, class T, int NV, bool FULL>
+template <class TX, class T, int NV, bool FULL, bool BIAS>
 __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kernel(const NormsArgs a) {
     extern __shared__ __align__(16) char ring[];
     __shared__ __align__(16) float2 slots[kSlots];
@@ -70,7 +70,11 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
             clear(kGo, Eight<TX>::kPacks);
             if (FULL) clear(kY, Eight<T>::kPacks);
         }
-    const Key key = key_of(a.d);
+    __shared__ RoundKeys keys;
+    if (a.d.bar) {
+        round_keys(&keys, Key{__ldg(a.d.seed), __ldg(a.d.seed + a.d.seed_stride)}, (int)threadIdx.x);
+        __syncthreads();
+    }
     const float per = 1.f / (float)a.dim;
     const float2 zero = make_float2(0.f, 0.f);
     constexpr int kKept = FULL ? (int)kSums : 2;
@@ -88,10 +92,16 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
         int ahead = row0;
         const auto ask = [&]() {
             if (ahead < end) {
-                ring_ask<TX, NV>(a.out, ahead, col, run, last, put, piece);
-                ring_ask<T, NV>(a.gh, ahead, col, run, last, put + kGh * piece, piece);
-                ring_ask<TX, NV>(a.go, ahead, col, run, last, put + kGo * piece, piece);
-                if (FULL) ring_ask<T, NV>(a.y, ahead, col, run, last, put + kY * piece, piece);
+                const unsigned long long x_at = (unsigned long long)(unsigned)ahead * a.out.bytes + (unsigned)(col * (int)sizeof(TX)), t_at = (unsigned long long)(unsigned)ahead * a.gh.bytes + (unsigned)(col * (int)sizeof(T));
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+                    if (v + 1 < NV || last) {
+                        const unsigned x_run = (unsigned)(v * run * (int)sizeof(TX)), t_run = (unsigned)(v * run * (int)sizeof(T));
+                        ring_ask<TX>((const char *)a.out.p + x_at + x_run, put + v * Eight<TX>::kPacks * piece, piece);
+                        ring_ask<T>((const char *)a.gh.p + t_at + t_run, put + (kGh + v * Eight<T>::kPacks) * piece, piece);
+                        ring_ask<TX>((const char *)a.go.p + x_at + x_run, put + (kGo + v * Eight<TX>::kPacks) * piece, piece);
+                        if (FULL) ring_ask<T>((const char *)a.y.p + t_at + t_run, put + (kY + v * Eight<T>::kPacks) * piece, piece);
+                    }
                 put = put + stage == ring1 ? ring0 : put + stage;
                 ahead += a.splits;
             }
@@ -109,6 +119,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
                 for (int i = FULL ? 0 : 2; i < 4; ++i) next[i] = __ldg(a.stats + (row + a.splits) * a.stats_pitch + i);
             ask();
             copies_wait(a.stages);
+            const unsigned long long x_at = (unsigned long long)(unsigned)row * a.out.bytes + (unsigned)(col * (int)sizeof(TX)), t_at = (unsigned long long)(unsigned)row * a.gh.bytes + (unsigned)(col * (int)sizeof(T));
             float2 q[NV][4], along = zero, all = zero;  // what arrives through the norm
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
@@ -143,14 +154,14 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
                         G[i] = fma2(fma2(u[i], both(-along_u), add2(q[v][i], both(-mean_q))), both(through), G[i]);
                         u[i] = mul2(G[i], both(a.scale));
                     }
-                    if (a.dx.p && there) put8<TX>(at_row<TX>(a.dx, row, at_col), u);
+                    if (a.dx.p && there) put8<TX>((char *)a.dx.p + x_at + (unsigned)(v * run * (int)sizeof(TX)), u);
                     if (a.d.bar) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) G[i] = mul2(G[i], both(a.d.factor));
-                        drop8(G, philox(key, ((unsigned long long)(unsigned)row * (unsigned)a.dim + at_col) >> 3, a.d.site), a.d.bar);
+                        drop8(G, philox(keys, ((unsigned long long)(unsigned)row * (unsigned)a.dim + at_col) >> 3, a.d.site), a.d.bar);
                     }
                     if (!FULL) {
-                        if (a.dy.p && there) put8<T>(at_row<T>(a.dy, row, at_col), G);
+                        if (a.dy.p && there) put8<T>((char *)a.dy.p + t_at + (unsigned)(v * run * (int)sizeof(T)), G);
                         continue;
                     }
                     float2 n[4], w[4], b[4];
@@ -185,7 +196,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
                     constexpr int kWa = FULL ? (int)kSumWa : 0, kBa = FULL ? (int)kSumBa : 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        sum[kBa][v][i] = add2(sum[kBa][v][i], G[i]);
+                        if (BIAS) sum[kBa][v][i] = add2(sum[kBa][v][i], G[i]);
                         sum[kWa][v][i] = fma2(G[i], n[i], sum[kWa][v][i]);
                         q[v][i] = mul2(G[i], w[i]);
                         along_t = fma2(q[v][i], n[i], along_t);
@@ -206,7 +217,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
                             for (int i = 0; i < 4; ++i)
                                 q[v][i] = mul2(fma2(fma2(n[i], both(rstd_a), both(from_a)), both(-along_v), add2(q[v][i], both(-mean_t))), both(rstd_a));
                         }
-                        put8<T>(at_row<T>(a.dy, row, col + v * run), q[v]);
+                        put8<T>((char *)a.dy.p + t_at + (unsigned)(v * run * (int)sizeof(T)), q[v]);
                     }
             }
             take = take + stage == ring1 ? ring0 : take + stage;
@@ -385,7 +396,7 @@ __global__ void __maxnreg__(kRegisters) block_norms_grad_kernel(const NormsArgs 
     join_teams(a, at, sum, count, wide, (float *)ring);
 }
 
-// The sums that CTAs, and shares of a group's rows, left: y[j] = the sum over i of x[i * pitch + j], in a fixed order: warp by warp every 16th, then
+// The sums that CTAs, and shares of a group's rows, left: y[j] = the sum over i of x[i * pitch + j], in a fixed order: warp by warp every 32nd, then
 // the warps'.  A row of blocks for each kind, and for each group of a gate.
 struct Join {
     const float *x[kSums];
@@ -397,8 +408,8 @@ struct Join {
     long long gate_pitch;
     int splits, dim;
 };
-constexpr int kJoinParts = 16;
-__global__ void __launch_bounds__(32 * kJoinParts) block_norms_join_kernel(const Join a) {
+constexpr int kJoinParts = 32;
+__global__ void __launch_bounds__(32 * kJoinParts) block_norms_join_kernel(const __grid_constant__ Join a) {
     __shared__ float2 part[kJoinParts][32];
     grid_dependency_sync();
     const int lane = (int)threadIdx.x & 31, w = (int)threadIdx.x >> 5, col = ((int)blockIdx.x * 32 + lane) * 2, s = (int)blockIdx.y;
@@ -408,20 +419,21 @@ __global__ void __launch_bounds__(32 * kJoinParts) block_norms_join_kernel(const
     const float *x = (kind ? a.x[s] : a.gate_x + group * a.splits * a.dim) + col;
     const bool two = a.dim % 2 == 0 && col < a.dim, one = col < a.dim;  // (the partial sums lie on 256-byte boundaries)
     float2 sum = make_float2(0.f, 0.f);
-    int i = w;
-    for (; i + 3 * kJoinParts < count; i += 4 * kJoinParts) {
-        float2 v[4];
+    if (two) {
+        const float2 *p = (const float2 *)x;
+        const long long step = pitch / 2;
+        int i = w;
+        for (; i + 7 * kJoinParts < count; i += 8 * kJoinParts) {
+            float2 v[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float *p = x + (i + k * kJoinParts) * pitch;
-            v[k] = two ? *(const float2 *)p : make_float2(one ? p[0] : 0.f, col + 1 < a.dim ? p[1] : 0.f);
+            for (int k = 0; k < 8; ++k) v[k] = p[(i + k * kJoinParts) * step];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum = add2(sum, v[k]);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sum = add2(sum, v[k]);
-    }
-    for (; i < count; i += kJoinParts) {
-        const float *p = x + i * pitch;
-        sum = add2(sum, two ? *(const float2 *)p : make_float2(one ? p[0] : 0.f, col + 1 < a.dim ? p[1] : 0.f));
+#pragma unroll 4
+        for (; i < count; i += kJoinParts) sum = add2(sum, p[i * step]);
+    } else if (one) {
+        for (int i = w; i < count; i += kJoinParts) sum = add2(sum, make_float2(x[i * pitch], col + 1 < a.dim ? x[i * pitch + 1] : 0.f));
     }
     part[w][lane] = sum;
     __syncthreads();
@@ -465,13 +477,15 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
     const int tx = n.x_dtype, t = n.dtype, sx = tx == SAGE_F32 ? 4 : 2, st = t == SAGE_F32 ? 4 : 2;
     // Without a norm after the block or a gate its values are not read, and two kinds of sums are kept.
     const bool full = a.y.p && (a.after != SAGE_NORM_NONE || a.gate);
-    const int nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, 1, full ? (a.dim > 8 * kMaxThreads ? 2 : 1) : 4), threads = a.team * a.teams;
+    const int nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, 1, a.dim > 8 * kMaxThreads ? 2 : 1);
     const bool wide = a.dim % 8 == 0 && boundary(a.out, sx) && boundary(a.go, sx) && boundary(a.dx, sx) && boundary(a.y, st) && boundary(a.gh, st) && boundary(a.dy, st);
     size_t smem;
     const size_t bytes = (a.gh.p ? sx + st : 0) + (a.go.p ? sx : 0) + (full ? st : 0);
-    const bool usual = a.y.p && a.gh.p && a.go.p && a.wb && (a.wa || a.after == SAGE_NORM_NONE);
+    // Rows of the stream have one pitch, those of the block another.
+    const auto like = [](const Rows &r, const Rows &of) { return !r.p || r.pitch == of.pitch; };
+    const bool usual = a.y.p && a.gh.p && a.go.p && a.wb && like(a.go, a.out) && like(a.dx, a.out) && like(a.y, a.gh) && like(a.dy, a.gh) && (a.wa || a.after == SAGE_NORM_NONE);
     const bool ring = wide && usual && weights_wide(a) && !(full && nv > 2) && grid_of(ctx, &a, nv, bytes, ring_registers(nv, full), true, &smem) && smem <= kRingBytes;
-    const int grid = grid_of(ctx, &a, nv, bytes, ring ? ring_registers(nv, full) : kRegisters, ring, &smem);
+    const int grid = grid_of(ctx, &a, nv, bytes, ring ? ring_registers(nv, full) : kRegisters, ring, &smem), threads = a.team * a.teams;
     const bool by_group = a.gate && groups > 1 && to[kSumGate];
     int partials = 0;
     Join join{};
@@ -517,11 +531,9 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
             };
             const auto any = [&](auto kernel) { return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3((unsigned)grid), dim3((unsigned)threads), smem, a, wide, weights_wide(a)), "block_norms_grad"); };
             if (ring) {
-                if (full) return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, true>) : by_ring(block_norms_grad_ring_kernel<TX, T, 2, true>);
-                return nv == 1   ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, false>)
-                       : nv == 2 ? by_ring(block_norms_grad_ring_kernel<TX, T, 2, false>)
-                       : nv == 3 ? by_ring(block_norms_grad_ring_kernel<TX, T, 3, false>)
-                                 : by_ring(block_norms_grad_ring_kernel<TX, T, 4, false>);
+                if (full && to[kSumBa]) return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, true, true>) : by_ring(block_norms_grad_ring_kernel<TX, T, 2, true, true>);
+                if (full) return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, true, false>) : by_ring(block_norms_grad_ring_kernel<TX, T, 2, true, false>);
+                return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, false, false>) : nv == 2 ? by_ring(block_norms_grad_ring_kernel<TX, T, 2, false, false>) : by_ring(block_norms_grad_ring_kernel<TX, T, 4, false, false>);
             }
             if (full) return nv == 1 ? any(block_norms_grad_kernel<TX, T, 1, true>) : nv == 2 ? any(block_norms_grad_kernel<TX, T, 2, true>) : any(block_norms_grad_kernel<TX, T, 4, true>);
             return nv == 1   ? any(block_norms_grad_kernel<TX, T, 1, false>)

@@ -36,6 +36,26 @@ __device__ __forceinline__ uint4 philox(Key k, unsigned long long count, unsigne
     return x;
 }
 
+// ... with the rounds' keys made once (a block of threads keeps them in shared memory: five loads instead of twenty additions).
+struct RoundKeys {
+    uint2 k[10];
+};
+__device__ __forceinline__ void round_keys(RoundKeys *to, Key k, int thread) {
+    if (thread < 10) to->k[thread] = make_uint2(k.a + (unsigned)thread * 0x9E3779B9u, k.b + (unsigned)thread * 0xBB67AE85u);
+}
+__device__ __forceinline__ uint4 philox(const RoundKeys &keys, unsigned long long count, unsigned long long site) {
+    uint4 x = make_uint4((unsigned)count, (unsigned)(count >> 32), (unsigned)site, (unsigned)(site >> 32));
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        const uint4 two = ((const uint4 *)keys.k)[i];
+        unsigned long long p = (unsigned long long)x.x * 0xD2511F53u, q = (unsigned long long)x.z * 0xCD9E8D57u;
+        x = make_uint4((unsigned)(q >> 32) ^ x.y ^ two.x, (unsigned)q, (unsigned)(p >> 32) ^ x.w ^ two.y, (unsigned)p);
+        p = (unsigned long long)x.x * 0xD2511F53u, q = (unsigned long long)x.z * 0xCD9E8D57u;
+        x = make_uint4((unsigned)(q >> 32) ^ x.y ^ two.z, (unsigned)q, (unsigned)(p >> 32) ^ x.w ^ two.w, (unsigned)p);
+    }
+    return x;
+}
+
 // Bit e: element 8 * block + e stays.  Sixteen bits an element, four words a block: a draw of ten rounds serves eight elements (one draw for
 // four, with 32 bits each, is more arithmetic than the memory leaves time for), and shares are multiples of 2^-16.
 __device__ __forceinline__ unsigned keep8(const Dropout &d, Key k, unsigned long long block) {
