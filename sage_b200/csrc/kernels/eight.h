@@ -32,6 +32,19 @@ struct Eight {  // columns, as they are stored
 #pragma unroll
         for (int i = 0; i < kPacks; ++i) p[i] = ((const Pack<T> *)from)[i];
     }
+    // ... what nothing reads again
+    __device__ __forceinline__ void load_once(const char *from) {
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) {
+            uint4 u;
+            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(from + i * 16));
+            *(uint4 *)&p[i] = u;
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) *(uint4 *)&p[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
     __device__ __forceinline__ void store(char *to) const {
 #pragma unroll
         for (int i = 0; i < kPacks; ++i) ((Pack<T> *)to)[i] = p[i];

@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "eight.h"
 #include "head_device.h"
 #include "language.h"
 
@@ -69,6 +70,98 @@ __global__ void __launch_bounds__(1024) head_join_kernel(const float4 *parts, in
     if (y.stats) {
         y.stats[row * y.stats_pitch] = x.m;
         y.stats[row * y.stats_pitch + 1] = x.s;
+    }
+}
+
+// Few rows (one token of each of a few sequences): a warp takes four rows of the weights at a time, straight from memory in order, with the hidden states in
+// shared memory.  Bound by the weights' bytes.  A lane sums its columns in f32; of the 4 x RB sums of a warp every lane ends up with one (half of
+// what it has goes to another lane at each step), and keeps the sums of exponentials for those of its place.
+template <class T, int RB>
+__global__ void __launch_bounds__(256, 2) head_few_kernel(const T *hidden, long long hidden_pitch, const T *weight, long long weight_pitch, int rows, int vocab, int width, const int *ids,
+                                                          long long ids_stride, float c2, float4 *parts, float *asked) {
+    extern __shared__ __align__(16) char smem[];
+    __shared__ Sums all[8][RB];
+    grid_dependency_sync();
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, runs = width / 8;
+    Eight<T> *states = (Eight<T> *)smem;
+    for (int i = (int)threadIdx.x; i < RB * runs; i += 256) {
+        const int r = i / runs;
+        if (r < rows) states[i].load((const char *)(hidden + r * hidden_pitch + (i - r * runs) * 8));
+        else states[i].clear();
+    }
+    __syncthreads();
+    constexpr int N = 4 * RB, kLanes = 32 / N;  // sums; lanes that end up with the same one
+    const int index = lane / kLanes, mine = index % RB, which = index / RB;
+    const int id = mine < rows ? __ldg(ids + mine * ids_stride) : -1;
+    Sums kept{-INFINITY, 0.f, 0.f};
+    for (long long first = 4ll * ((long long)blockIdx.x * 8 + warp); first < vocab; first += 32ll * gridDim.x) {
+        const char *row[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) row[k] = (const char *)(weight + min(first + k, vocab - 1ll) * weight_pitch);
+        float2 sum[4][RB];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int r = 0; r < RB; ++r) sum[k][r] = make_float2(0.f, 0.f);
+#pragma unroll(RB <= 2 ? 4 : 2)
+        for (int c = lane; c < runs; c += 32) {
+            float2 x[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                Eight<T> v;
+                v.load_once(row[k] + (long long)c * (8 * (int)sizeof(T)));
+                v.open(x[k]);
+            }
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+                float2 h[4];
+                states[r * runs + c].open(h);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[k][r] = fma2(x[k][i], h[i], sum[k][r]);
+            }
+        }
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = sum[i / RB][i % RB].x + sum[i / RB][i % RB].y;
+        int n = N;
+#pragma unroll
+        for (int off = 16; off; off >>= 1) {
+            if (n > 1) {
+                n /= 2;
+                const bool upper = lane & off;
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i)
+                    if (i < n) v[i] = (upper ? v[i + n] : v[i]) + __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + n], off);
+            } else {
+                v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+            }
+        }
+        const long long token = first + which;
+        if (token < vocab) {
+            const float x = v[0];
+            if (x > kept.m) {
+                const float by = kept.m == -INFINITY ? 0.f : (kept.m - x) * c2, f = kept.m == -INFINITY ? 0.f : exp2_of(by);
+                kept.a = f > 0.f ? fmaf(kept.s * f, by, kept.a * f) : kept.s * f;  // (zero, or not a number)
+                kept.s *= f;
+                kept.m = x;
+            }
+            const float d = (x - (kept.m == -INFINITY ? 0.f : kept.m)) * c2, e = exp2_of(d);
+            kept.s += e;
+            kept.a = fmaf(e, fmaxf(d, kFar), kept.a);
+            if (token == id) asked[mine] = x;
+        }
+    }
+#pragma unroll
+    for (int off = 16; off >= 8; off >>= 1)  // the four weights' rows of a hidden state
+        kept = joined(kept, Sums{__shfl_xor_sync(0xffffffffu, kept.m, off), __shfl_xor_sync(0xffffffffu, kept.s, off), __shfl_xor_sync(0xffffffffu, kept.a, off)}, c2);
+    if (lane < 8 && lane % kLanes == 0) all[warp][mine] = kept;
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+        Sums t = all[0][threadIdx.x];
+        for (int w = 1; w < 8; ++w) t = joined(t, all[w][threadIdx.x], c2);
+        parts[(long long)blockIdx.x * rows + threadIdx.x] = make_float4(t.m, t.s, t.a, 0.f);
     }
 }
 
@@ -242,7 +335,7 @@ Product shape_of(Context &ctx, long long m, long long n, long long k) {
     p.tiles_m = (int)((m + 255) / 256);
     p.tiles_n = (int)((n + p.bn - 1) / p.bn);
     p.slices = 1;
-    p.slice_blocks = (int)((k + kK - 1) / kK);
+    p.slice_blocks = p.chain = (int)((k + kK - 1) / kK);
     p.band = 8;
     p.status = ctx.status_word_dev;
     return p;
@@ -316,6 +409,38 @@ sage_status join(Context &ctx, const float4 *parts, int count, long long rows, c
                           "head_join");
 }
 
+// Rows that are few enough for the product by way of dot products.
+constexpr long long kFewRows = 8;
+bool few(const Head &a) {
+    const int size = a.hidden.dtype == SAGE_F32 ? 4 : 2;
+    const long long rows = a.hidden.rows > 4 ? 8 : a.hidden.rows > 2 ? 4 : a.hidden.rows;
+    return a.hidden.rows <= kFewRows && a.hidden.cols % 8 == 0 && rows * a.hidden.cols * size <= 96 * 1024 && on_16(a.hidden.ptr, a.hidden.rows > 1 ? a.hidden.pitch : 0, size) &&
+           on_16(a.weight.ptr, a.weight.rows > 1 ? a.weight.pitch : 0, size);
+}
+template <class T>
+sage_status forward_few(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
+    Scratch scratch(ctx);
+    const long long rows = a.hidden.rows, vocab = a.weight.rows;
+    const unsigned grid = (unsigned)std::min<long long>((vocab + 31) / 32, 2ll * ctx.sm_count);
+    float4 *parts = nullptr;
+    float *asked = nullptr;
+    sage_status st = scratch.get((size_t)(grid * rows) * 16, &parts);
+    if (!st) st = scratch.get((size_t)rows * 4, &asked);
+    if (st) return st;
+    ctx.note_launch("head_few");
+    const auto run = [&](auto kernel, int padded) {
+        const size_t smem = (size_t)padded * a.hidden.cols * sizeof(T);
+        sage_status s = ctx.check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024), "head_few");
+        return s ? s
+                 : ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3(grid), dim3(256), smem, (const T *)a.hidden.ptr, a.hidden.pitch, (const T *)a.weight.ptr, a.weight.pitch, (int)rows, (int)vocab,
+                                                   (int)a.hidden.cols, (const int *)a.ids.ptr, a.ids.stride, a.scale * kLog2E, parts, asked),
+                                  "head_few");
+    };
+    if (!ctx.dry()) st = rows > 4 ? run(head_few_kernel<T, 8>, 8) : rows > 2 ? run(head_few_kernel<T, 4>, 4) : rows > 1 ? run(head_few_kernel<T, 2>, 2) : run(head_few_kernel<T, 1>, 1);
+    if (st) return st;
+    return join(ctx, parts, (int)grid, rows, asked, a.ids, vocab, a.scale, Values{(float *)log_probs.ptr, (float *)entropy.ptr, (float *)stats.ptr, log_probs.stride, entropy.stride, stats.pitch});
+}
+
 // Rows [at, at + count) of the operands and results.
 RowsArg cut(const RowsArg &r, long long at, long long count) {
     RowsArg c = r;
@@ -351,6 +476,7 @@ sage_status forward16(Context &ctx, const Head &a, const VectorArg &log_probs, c
         p.ids = (const int *)ids.ptr;
         p.ids_stride = ids.stride;
         p.c2 = a.scale * kLog2E;
+        p.chain = (p.slice_blocks + (p.slice_blocks + 7) / 8 - 1) / ((p.slice_blocks + 7) / 8);  // of equal length
         p.parts = parts;
         p.asked = asked;
         st = launch<T, false, false, kStats>(ctx, "head_log_probs", p, a.hidden.dtype, x, w, 0, Matrix{});
@@ -534,6 +660,8 @@ sage_status grad32(Context &ctx, Head a, const RowsArg &stats, const VectorArg &
 
 sage_status head_log_probs(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
     if (!a.hidden.rows) return SAGE_OK;
+    if (head::few(a))
+        return with_type(a.hidden.dtype, [&](auto t) { return head::forward_few<decltype(t)>(ctx, a, log_probs, entropy, stats); });
     if (a.hidden.dtype == SAGE_F32) return head::forward32(ctx, a, log_probs, entropy, stats);
     return a.hidden.dtype == SAGE_F16 ? head::forward16<__half>(ctx, a, log_probs, entropy, stats) : head::forward16<__nv_bfloat16>(ctx, a, log_probs, entropy, stats);
 }

@@ -41,6 +41,7 @@ struct Product {
     int bn;                       // 256 or 128
     int tiles_m, tiles_n, slices; // slices of K, each a result of its own: `slice_rows` rows further
     int slice_blocks, slice_rows; // K-blocks of a slice
+    int chain;                    // K-blocks that the tensor cores add up
     int band;                     // row tiles that column tiles are gone through for
     unsigned *status;
     const int *ids;
@@ -211,34 +212,37 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         const unsigned long long desc_a = smem_desc(0u, A_MN ? kK * 128u : 16u, 1024u, 2u), desc_b = smem_desc(0u, B_MN ? kK * 128u : 16u, 1024u, 2u);
         constexpr unsigned kStepA = A_MN ? 128u : 2u, kStepB = B_MN ? 128u : 2u;
         const unsigned base = smem_u32(smem);
-        int i = 0, tiles = 0;
+        int i = 0, chains = 0;
         bool live = !__any_sync(0xffffffffu, given_up != 0);
-        for (int t = pair; t < all && live; t += pairs, ++tiles) {
+        for (int t = pair; t < all && live; t += pairs) {
             const int slice = t / (p.tiles_m * p.tiles_n), first = slice * p.slice_blocks, last = min(all_blocks, first + p.slice_blocks);
-            const int buffer = tiles & 1;
-            if (!mbar_wait_warp(&freed[buffer], ((tiles >> 1) & 1) ^ 1)) {
-                if (lane == 0) give_up(16);
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned d = tmem + (unsigned)buffer * 256u;
-            for (int b = first; b < last; ++b, ++i) {
-                const int s = i % kStages;
-                if (!mbar_wait_warp(&full[s], (i / kStages) & 1)) {
-                    if (lane == 0 && !given_up) give_up(4);
+            for (int from = first; from < last && live; from += p.chain, ++chains) {
+                const int buffer = chains & 1, to = min(last, from + p.chain);
+                if (!mbar_wait_warp(&freed[buffer], ((chains >> 1) & 1) ^ 1)) {
+                    if (lane == 0) give_up(16);
                     live = false;
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned at = base + (unsigned)(s * kStageSize);
-                const unsigned long long a = desc_a + (at >> 4), bb = desc_b + ((at + kOperandBytes) >> 4);
-                if (elect_one()) {
+                const unsigned d = tmem + (unsigned)buffer * 256u;
+                for (int b = from; b < to; ++b, ++i) {
+                    const int s = i % kStages;
+                    if (!mbar_wait_warp(&full[s], (i / kStages) & 1)) {
+                        if (lane == 0 && !given_up) give_up(4);
+                        live = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned at = base + (unsigned)(s * kStageSize);
+                    const unsigned long long a = desc_a + (at >> 4), bb = desc_b + ((at + kOperandBytes) >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < kK / 16; ++k) mma_pair(d, a + k * kStepA, bb + k * kStepB, idesc, b > first || k > 0 ? 1u : 0u);
-                    umma_commit_pair(&empty[s]);
-                    if (b + 1 == last) umma_commit_pair(&done[buffer]);
+                        for (int k = 0; k < kK / 16; ++k) mma_pair(d, a + k * kStepA, bb + k * kStepB, idesc, b > from || k > 0 ? 1u : 0u);
+                        umma_commit_pair(&empty[s]);
+                        if (b + 1 == to) umma_commit_pair(&done[buffer]);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
     } else if (warp >= 2) {
@@ -248,39 +252,67 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         float factor = 1.f;
         if (END == kProbs && p.gmax) factor = power_of_two(stored_exponent(p.gmax));
         if (END == kNarrow || END == kWide) factor = p.gmax ? p.alpha * power_of_two(-stored_exponent(p.gmax)) : p.alpha;
-        int tiles = 0;
-        for (int t = pair; t < all; t += pairs, ++tiles) {
+        int chains = 0;
+        bool live = true;
+        // Waits for a chain's sums; gives their tensor memory back.
+        const auto arrived = [&]() {
+            if (!mbar_wait_warp(&done[chains & 1], (chains >> 1) & 1)) {
+                if (lane == 0 && !given_up) give_up(8);
+                live = false;
+                return 0u;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            return tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)((chains & 1) * 256 + side * half);
+        };
+        const auto drained = [&]() {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 0) mbar_arrive(&freed[chains & 1]);
+                else mbar_arrive_remote_tmem(peer_addr(smem_u32(&freed[chains & 1]), 0));
+            }
+            ++chains;
+        };
+        for (int t = pair; t < all && live; t += pairs) {
             const Tile tile = tile_of(p, t);
-            const int buffer = tiles & 1, row0 = tile.m0 + rank * 128 + quarter * 32, row = row0 + lane, col0 = tile.n0 + side * half;
+            const int row0 = tile.m0 + rank * 128 + quarter * 32, row = row0 + lane, col0 = tile.n0 + side * half;
             const bool there = row < p.m;
-            float4 about = make_float4(0.f, 0.f, 0.f, 0.f);
             int id = -1;
             if ((END == kStats || END == kProbs) && there) {
                 id = __ldg(p.ids + row * p.ids_stride);
                 id = id < p.first ? -1 : id - p.first;
-                if (END == kProbs) about = __ldg(p.rows + row);
-                about.z *= factor, about.w *= factor;
             }
-            if (!mbar_wait_warp(&done[buffer], (tiles >> 1) & 1)) {
-                if (lane == 0 && !given_up) give_up(8);
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(buffer * 256 + side * half);
-            float largest = -INFINITY, sum = 0.f, along = 0.f;
-            for (int j = 0; j < half; j += 32) {
-                float v[32];
-                tmem_ld32(at + j, v);
-                const int col = col0 + j;
-                if (END == kStats) {
+            if constexpr (END == kStats) {
+                // The tensor cores cut what lies below a sum's last place at every addition: log probabilities of 4096 k in one chain were 4e-6 off.
+                // Chains of 512 k at most are added up here, to nearest.
+                float acc[128];
+                for (int from = 0; from < all_blocks && live; from += p.chain) {
+                    const unsigned at = arrived();
+                    if (!live) break;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j * 32 < half) {
+                            float v[32];
+                            tmem_ld32(at + j * 32, v);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) acc[j * 32 + e] = from ? acc[j * 32 + e] + v[e] : v[e];
+                        }
+                    drained();
+                }
+                if (!live) break;
+                float largest = -INFINITY, sum = 0.f, along = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j * 32 >= half) break;
+                    const int col = col0 + j * 32;
                     if (col + 32 > p.n) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (col + e >= p.n) v[e] = -INFINITY;
+                            if (col + e >= p.n) acc[j * 32 + e] = -INFINITY;
                     }
-                    float high = v[0];
+                    float high = acc[j * 32];
 #pragma unroll
-                    for (int e = 1; e < 32; ++e) high = fmaxf(high, v[e]);
+                    for (int e = 1; e < 32; ++e) high = fmaxf(high, acc[j * 32 + e]);
                     if (high > largest) {  // what there is so far, seen from the new largest
                         const float by = largest == -INFINITY ? 0.f : (largest - high) * p.c2, f = largest == -INFINITY ? 0.f : exp2_fast(by);
                         along = f > 0.f ? fmaf(sum * f, by, along * f) : 0.f;
@@ -291,7 +323,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     float s[4] = {0.f, 0.f, 0.f, 0.f}, a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const float d = (v[e] - from) * p.c2, x = exp2_fast(d);
+                        const float d = (acc[j * 32 + e] - from) * p.c2, x = exp2_fast(d);
                         s[e & 3] += x;
                         a[e & 3] = fmaf(x, fmaxf(d, kFar), a[e & 3]);
                     }
@@ -301,10 +333,23 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     if (__any_sync(0xffffffffu, want >= 0 && want < 32)) {
                         float x = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x = e == want ? v[e] : x;
+                        for (int e = 0; e < 32; ++e) x = e == want ? acc[j * 32 + e] : x;
                         if (want >= 0 && want < 32 && col + want < p.n) p.asked[row] = x;
                     }
-                } else {
+                }
+                if (there) p.parts[(long long)(tile.n0 / half + side) * p.m + row] = make_float4(largest, sum, along, 0.f);
+            } else {
+                float4 about = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (END == kProbs && there) {
+                    about = __ldg(p.rows + row);
+                    about.z *= factor, about.w *= factor;
+                }
+                const unsigned at = arrived();
+                if (!live) break;
+                for (int j = 0; j < half; j += 32) {
+                    float v[32];
+                    tmem_ld32(at + j, v);
+                    const int col = col0 + j;
                     const int want = END == kProbs ? id - col : -1;
                     if (END == kProbs) {
 #pragma unroll
@@ -348,14 +393,8 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         __syncwarp();
                     }
                 }
+                drained();
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                if (rank == 0) mbar_arrive(&freed[buffer]);
-                else mbar_arrive_remote_tmem(peer_addr(smem_u32(&freed[buffer]), 0));
-            }
-            if (END == kStats && there) p.parts[(long long)(tile.n0 / half + side) * p.m + row] = make_float4(largest, sum, along, 0.f);
         }
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
