@@ -6,7 +6,7 @@
 // launch joins them.  Gradient: the vocabulary in pieces; of each piece the product again, q into a buffer (16 bits: q is an operand of two
 // products, rounded like the operands beside it; the sums of both are f32), then its two products.
 // Bound by the tensor cores: 2 rows vocab width operations forward, three times that for the gradient, which makes the logits again.
-// f32 operands: the same pieces as the framework's own f32 products around kernels over a piece of the logits.
+// f32 operands: the same products of their pieces, which a pass over them makes first.
 #include <algorithm>
 #include <cmath>
 
@@ -214,59 +214,29 @@ sage_status copy_rows(Context &ctx, const A *x, long long px, B *y, long long py
     return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_rows_copy_kernel<A, B>, dim3((unsigned)blocks), dim3(256), 0, x, px, y, py, rows, cols, slices, slice), "head_rows_copy");
 }
 
-// f32: a piece of the logits becomes the rows' sums over it ...
-__global__ void __launch_bounds__(256) head_stats_kernel(const float *x, int rows, int cols, const int *ids, long long ids_stride, int first, float c2, float4 *parts, float *asked) {
-    __shared__ Sums all[8];
+// Three bf16 pieces of each f32 element, eight to a thread.
+template <bool WIDE>
+__global__ void __launch_bounds__(256) head_pieces_kernel(const float *x, long long px, __nv_bfloat16 *y, long long py, long long plane, long long rows, int cols) {
     grid_dependency_sync();
-    const int row = (int)blockIdx.x;
-    const float *p = x + (long long)row * cols;
-    Sums t{-INFINITY, 0.f, 0.f};
-    for (int c = (int)threadIdx.x; c < cols; c += 256 * 8) {
-        float v[8], high = -INFINITY;
+    const long long per = py / 8;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * per; i += gridDim.x * 256ll) {
+        const long long r = i / per, c = (i - r * per) * 8;
+        const float *from = x + r * px + c;
+        float v[8];
+        if (WIDE) {
+            const float4 a = *(const float4 *)from, b = *((const float4 *)from + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[e] = c + e * 256 < cols ? __ldg(p + c + e * 256) : -INFINITY;
-            high = fmaxf(high, v[e]);
+            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? from[e] : 0.f;
         }
-        Sums u{high, 0.f, 0.f};
-        const float from = high == -INFINITY ? 0.f : high;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float d = (v[e] - from) * c2, y = exp2_of(d);
-            u.s += y;
-            u.a = fmaf(y, fmaxf(d, kFar), u.a);
+        for (int n = 0; n < 3; ++n) {
+            unsigned w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = take_piece(v[2 * e], v[2 * e + 1]);
+            *(uint4 *)(y + n * plane + r * py + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        t = joined(t, u, c2);
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) t = joined(t, Sums{__shfl_xor_sync(0xffffffffu, t.m, off), __shfl_xor_sync(0xffffffffu, t.s, off), __shfl_xor_sync(0xffffffffu, t.a, off)}, c2);
-    if (!(threadIdx.x & 31)) all[threadIdx.x >> 5] = t;
-    __syncthreads();
-    if (threadIdx.x) return;
-    for (int w = 1; w < 8; ++w) t = joined(t, all[w], c2);
-    parts[row] = make_float4(t.m, t.s, t.a, 0.f);
-    const int id = __ldg(ids + row * ids_stride);
-    if (id >= first && id - first < cols) asked[row] = p[id - first];
-}
-// ... or q, in its place.
-__global__ void __launch_bounds__(256) head_probs_kernel(float *x, int rows, int cols, const int *ids, long long ids_stride, int first, float c2, float scale, const float4 *about, const float *gls) {
-    grid_dependency_sync();
-    const int row = (int)blockIdx.x;
-    const float4 t = __ldg(about + row);
-    const float gl = __ldg(gls + row);
-    const int id = __ldg(ids + row * ids_stride), at = id < first ? -1 : id - first;
-    float *p = x + (long long)row * cols;
-#pragma unroll 8
-    for (int c = (int)blockIdx.y * 256 + (int)threadIdx.x; c < cols; c += 256 * (int)gridDim.y) {
-        const float d = fmaf(p[c] - t.x, c2, t.y), y = exp2_of(d);
-        p[c] = scale * (y * fmaf(t.w, fmaxf(d, kFar), t.z) + (c == at ? gl : 0.f));
-    }
-}
-__global__ void __launch_bounds__(256) head_add_kernel(const float *x, float *y, long long py, long long rows, int cols, int add) {
-    grid_dependency_sync();
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * cols; i += gridDim.x * 256ll) {
-        const long long r = i / cols, c = i - r * cols;
-        y[r * py + c] = add ? y[r * py + c] + x[i] : x[i];
     }
 }
 
@@ -274,16 +244,16 @@ __global__ void __launch_bounds__(256) head_add_kernel(const float *x, float *y,
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Rows of 128 bytes of a matrix, boxes of `box_rows` of them.
-sage_status map_of(Context &ctx, int dtype, const void *base, long long cols, long long rows, long long pitch, int box_rows, CUtensorMap *map) {
+// Boxes of `box_rows` rows, `box_bytes` of each, of a matrix (of each of several, `plane` elements apart).
+sage_status map_of(Context &ctx, int dtype, const void *base, long long cols, long long rows, long long pitch, int box_rows, CUtensorMap *map, int box_bytes = 128, int planes = 0, long long plane = 0) {
     static const EncodeTiled encode = reinterpret_cast<EncodeTiled>(driver_symbol("cuTensorMapEncodeTiled"));
     if (!encode) return ctx.fail(SAGE_ERR_DEVICE, "cuTensorMapEncodeTiled is not available");
     const int size = dtype == SAGE_F32 ? 4 : 2;
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(pitch * size)};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)std::max(planes, 1)}, strides[2] = {(cuuint64_t)(pitch * size), (cuuint64_t)((plane ? plane : pitch) * size)};
+    const cuuint32_t box[3] = {(cuuint32_t)(box_bytes / size), (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
     const CUtensorMapDataType type = dtype == SAGE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == SAGE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    if (encode(map, type, 2, const_cast<void *>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    if (encode(map, type, planes ? 3 : 2, const_cast<void *>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return ctx.fail(SAGE_ERR_DEVICE, "head_log_probs: cuTensorMapEncodeTiled failed");
     return SAGE_OK;
 }
@@ -306,9 +276,9 @@ struct Scratch {
     }
 };
 
-struct Matrix {  // rows x cols, cols contiguous
+struct Matrix {  // rows x cols, cols contiguous; f32: in pieces, `plane` elements apart
     const void *p = nullptr;
-    long long rows = 0, cols = 0, pitch = 0;
+    long long rows = 0, cols = 0, pitch = 0, plane = 0;
 };
 bool on_16(const void *p, long long pitch, int size) { return (uintptr_t)p % 16 == 0 && pitch * size % 16 == 0; }
 
@@ -341,17 +311,22 @@ Product shape_of(Context &ctx, long long m, long long n, long long k) {
     return p;
 }
 
-template <class T, bool A_MN, bool B_MN, End END>
+template <class T, bool A_MN, bool B_MN, End END, bool F32 = false>
 sage_status launch(Context &ctx, const char *name, Product p, int dtype, const Matrix &a, const Matrix &b, int out_type, const Matrix &c) {
     ctx.note_launch(name);
     if (ctx.dry()) return SAGE_OK;
     p.band = std::min(p.band, p.tiles_m);
     CUtensorMap ma, mb, mc;
-    sage_status st = map_of(ctx, dtype, a.p, a.cols, a.rows, a.pitch, A_MN ? kK : 128, &ma);
-    if (!st) st = map_of(ctx, dtype, b.p, b.cols, b.rows, b.pitch, B_MN ? kK : p.bn / 2, &mb);
-    if (!st && END != kStats) st = map_of(ctx, out_type, c.p, c.cols, c.rows, c.pitch, 32, &mc);
+    constexpr int kPlanes = F32 ? 3 : 1;
+    sage_status st = map_of(ctx, dtype, a.p, a.cols, a.rows, a.pitch, A_MN ? kK : 128, &ma, 128, kPlanes, a.plane);
+    if (!st) st = map_of(ctx, dtype, b.p, b.cols, b.rows, b.pitch, B_MN ? kK : p.bn / 2, &mb, 128, kPlanes, b.plane);
+    if (!st && END != kStats) st = map_of(ctx, out_type, c.p, c.cols, c.rows, c.pitch, 32, &mc, F32 && END == kProbs ? 64 : 128);
     else mc = ma;
-    const auto kernel = head_product_kernel<T, A_MN, B_MN, END>;
+    if (F32) {
+        p.slice_blocks *= kProducts;
+        p.chain = kProducts;
+    }
+    const auto kernel = head_product_kernel<T, A_MN, B_MN, END, F32>;
     if (!st) st = ctx.check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem), name);
     if (st) return st;
     const long long tiles = (long long)p.tiles_m * p.tiles_n * p.slices;
@@ -375,14 +350,15 @@ void plan(Context &ctx, const Product &p, long long k, bool pieces, Result *r) {
     r->slice_rows = p.tiles_m * 256;
     r->wide = pieces || r->slices > 1 || !on_16(r->out.ptr, r->out.pitch, r->out.dtype == SAGE_F32 ? 4 : 2);
 }
-template <class T, bool A_MN, bool B_MN>
+template <class T, bool A_MN, bool B_MN, bool F32 = false>
 sage_status multiply(Context &ctx, Scratch &scratch, const char *name, Product p, int dtype, const Matrix &a, const Matrix &b, bool first, bool last, Result *r) {
     sage_status st = SAGE_OK;
     const long long rows = r->out.rows, cols = r->out.cols;
     const bool f32 = r->out.dtype == SAGE_F32, direct = f32 && r->slices == 1 && on_16(r->out.ptr, r->out.pitch, 4);  // sums may be the result itself
-    if (!r->wide && !f32) return launch<T, A_MN, B_MN, kNarrow>(ctx, name, p, dtype, a, b, dtype, Matrix{r->out.ptr, rows, cols, r->out.pitch});
+    if constexpr (!F32)
+        if (!r->wide && !f32) return launch<T, A_MN, B_MN, kNarrow>(ctx, name, p, dtype, a, b, dtype, Matrix{r->out.ptr, rows, cols, r->out.pitch});
     p.add = !first;
-    if (direct) return launch<T, A_MN, B_MN, kWide>(ctx, name, p, dtype, a, b, SAGE_F32, Matrix{r->out.ptr, rows, cols, r->out.pitch});
+    if (direct) return launch<T, A_MN, B_MN, kWide, F32>(ctx, name, p, dtype, a, b, SAGE_F32, Matrix{r->out.ptr, rows, cols, r->out.pitch});
     if (first) {
         r->pitch = (cols + 7) / 8 * 8;
         st = scratch.get((size_t)r->slices * r->slice_rows * r->pitch * 4, &r->sums);
@@ -393,7 +369,7 @@ sage_status multiply(Context &ctx, Scratch &scratch, const char *name, Product p
     p.slices = (blocks + p.slice_blocks - 1) / p.slice_blocks;
     if (first) r->slices = p.slices;  // (pieces that follow are no longer: a slice of the last one may have nothing to add)
     p.slice_rows = r->slice_rows;
-    st = launch<T, A_MN, B_MN, kWide>(ctx, name, p, dtype, a, b, SAGE_F32, Matrix{r->sums, (long long)r->slices * r->slice_rows, cols, r->pitch});
+    st = launch<T, A_MN, B_MN, kWide, F32>(ctx, name, p, dtype, a, b, SAGE_F32, Matrix{r->sums, (long long)r->slices * r->slice_rows, cols, r->pitch});
     if (st || !last) return st;
     const long long slice = (long long)r->slice_rows * r->pitch;
     if (f32) return copy_rows<float, float>(ctx, r->sums, r->pitch, (float *)r->out.ptr, r->out.pitch, rows, (int)cols, r->slices, slice);
@@ -561,96 +537,94 @@ sage_status grad16(Context &ctx, const Head &a, const RowsArg &stats, const Vect
 }
 
 // ------------------------------------------------------------------------------------------ f32
-// The f32 products' operands: one row has any pitch, rows that overlap are laid out anew.
-sage_status apart(Context &ctx, Scratch &scratch, RowsArg *r) {
-    if (r->rows == 1) r->pitch = r->cols;
-    if (r->pitch >= r->cols) return SAGE_OK;
-    float *to = nullptr;
-    sage_status st = scratch.get((size_t)(r->rows * r->cols) * 4, &to);
-    if (!st) st = copy_rows<float, float>(ctx, (const float *)r->ptr, r->pitch, to, r->cols, r->rows, (int)r->cols, 1, 0);
-    r->ptr = to;
-    r->pitch = r->cols;
-    return st;
+typedef __nv_bfloat16 Piece;
+
+// The operand's pieces, in planes of their own.
+sage_status pieces_of(Context &ctx, Scratch &scratch, const RowsArg &r, Matrix *m) {
+    Piece *to = nullptr;
+    *m = Matrix{nullptr, r.rows, r.cols, (r.cols + 7) / 8 * 8, 0};
+    m->plane = r.rows * m->pitch;
+    sage_status st = scratch.get((size_t)(3 * m->plane) * 2, &to);
+    if (st) return st;
+    m->p = to;
+    ctx.note_launch("head_pieces");
+    if (ctx.dry()) return SAGE_OK;
+    const long long pitch = r.rows > 1 ? r.pitch : r.cols, blocks = std::min<long long>((r.rows * (m->pitch / 8) + 255) / 256, ctx.sm_count * 16ll);
+    const bool wide = r.cols % 8 == 0 && on_16(r.ptr, pitch, 4);
+    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? head_pieces_kernel<true> : head_pieces_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, (const float *)r.ptr, pitch, to, m->pitch, m->plane,
+                                           r.rows, (int)r.cols),
+                          "head_pieces");
 }
 
-GemmArgs product_of(bool ta, bool tb, long long m, long long n, long long k, const float *a, long long lda, const float *b, long long ldb, float *c, long long ldc) {
-    return GemmArgs{ta, tb, m, n, k, a, lda, 0, b, ldb, 0, c, ldc, 0, 1};
-}
-struct Pieces {
-    long long rows, cols;  // at a time
-};
-// A piece of f32 logits: all rows where they leave room for at least 1024 columns.
-Pieces pieces_of(long long rows, long long vocab) {
-    const long long room = (long long)(kPieceBytes / 4), r = std::min(rows, std::max<long long>(256, room / std::min<long long>(vocab, 1024)));
-    const long long most = std::max<long long>(1, std::min(vocab, room / r)), count = (vocab + most - 1) / most;
-    return Pieces{r, std::min(vocab, ((vocab + count - 1) / count + 63) / 64 * 64)};
-}
-
-sage_status forward32(Context &ctx, Head a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
+sage_status forward32(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
     Scratch scratch(ctx);
-    sage_status st = apart(ctx, scratch, &a.hidden);
-    if (!st) st = apart(ctx, scratch, &a.weight);
     const long long rows = a.hidden.rows, vocab = a.weight.rows, width = a.hidden.cols;
-    const Pieces piece = pieces_of(rows, vocab);
-    const int count = (int)((vocab + piece.cols - 1) / piece.cols);
-    float *logits, *asked;
-    float4 *parts;
-    if (!st) st = scratch.get((size_t)(piece.rows * piece.cols) * 4, &logits);
-    if (!st) st = scratch.get((size_t)(piece.rows * count) * 16, &parts);
-    if (!st) st = scratch.get((size_t)piece.rows * 4, &asked);
-    for (long long at = 0; at < rows && !st; at += piece.rows) {
-        const long long r = std::min(piece.rows, rows - at);
-        const RowsArg x = cut(a.hidden, at, r);
+    Product p = shape_of(ctx, rows, vocab, width);
+    const long long parts_of_row = 2ll * p.tiles_n, most = std::max<long long>(256, (long long)(kPartBytes / (16 * parts_of_row)) / 256 * 256);  // rows at a time
+    Matrix x, w;
+    sage_status st = pieces_of(ctx, scratch, a.weight, &w);
+    if (!st) st = scratch.get((size_t)(std::min(rows, most) * parts_of_row) * 16, &p.parts);
+    if (!st) st = scratch.get((size_t)std::min(rows, most) * 4, &p.asked);
+    p.c2 = a.scale * kLog2E;
+    p.ids_stride = a.ids.stride;
+    for (long long at = 0; at < rows && !st; at += most) {
+        const long long count = std::min(most, rows - at);
         const VectorArg ids = cut(a.ids, at), lp = cut(log_probs, at), h = cut(entropy, at);
-        const RowsArg s = cut(stats, at, r);
-        for (int i = 0; i < count && !st; ++i) {
-            const long long v = i * piece.cols, n = std::min(piece.cols, vocab - v);
-            st = gemm(ctx, product_of(false, true, r, n, width, (const float *)x.ptr, x.pitch, (const float *)a.weight.ptr + v * a.weight.pitch, a.weight.pitch, logits, n));
-            ctx.note_launch("head_stats");
-            if (!st && !ctx.dry())
-                st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_stats_kernel, dim3((unsigned)r), dim3(256), 0, (const float *)logits, (int)r, (int)n, (const int *)ids.ptr, ids.stride, (int)v,
-                                                     a.scale * kLog2E, parts + i * r, asked),
-                                    "head_stats");
-        }
-        if (!st) st = join(ctx, parts, count, r, asked, ids, vocab, a.scale, Values{(float *)lp.ptr, (float *)h.ptr, (float *)s.ptr, lp.stride, h.stride, s.pitch});
+        const RowsArg s = cut(stats, at, count);
+        st = pieces_of(ctx, scratch, cut(a.hidden, at, count), &x);
+        p.m = (int)count;
+        p.tiles_m = (int)((count + 255) / 256);
+        p.band = (int)std::max<long long>(8, ((long long)48 << 20) / (256 * width * 6));
+        p.ids = (const int *)ids.ptr;
+        if (!st) st = launch<Piece, false, false, kStats, true>(ctx, "head_log_probs", p, SAGE_BF16, x, w, 0, Matrix{});
+        if (!st) st = join(ctx, p.parts, (int)parts_of_row, count, p.asked, ids, vocab, a.scale, Values{(float *)lp.ptr, (float *)h.ptr, (float *)s.ptr, lp.stride, h.stride, s.pitch});
     }
     return st;
 }
 
-sage_status grad32(Context &ctx, Head a, const RowsArg &stats, const VectorArg &entropy, const VectorArg &gl, const VectorArg &ge, const RowsArg &dhidden, const RowsArg &dweight) {
+sage_status grad32(Context &ctx, const Head &a, const RowsArg &stats, const VectorArg &entropy, const VectorArg &gl, const VectorArg &ge, const RowsArg &dhidden, const RowsArg &dweight) {
     Scratch scratch(ctx);
-    sage_status st = apart(ctx, scratch, &a.hidden);
-    if (!st) st = apart(ctx, scratch, &a.weight);
-    const long long rows = a.hidden.rows, vocab = a.weight.rows, width = a.hidden.cols;
-    const long long most = std::max<long long>(1, std::min(vocab, (long long)(kPieceBytes / 4) / rows)), count = (vocab + most - 1) / most, piece = std::min(vocab, ((vocab + count - 1) / count + 63) / 64 * 64);
+    const long long rows = a.hidden.rows, vocab = a.weight.rows, width = a.hidden.cols, padded = (rows + 255) / 256 * 256;
+    const long long tiles = (vocab + 255) / 256, most = std::max<long long>(1, (long long)(kPieceBytes / ((size_t)padded * 512 * 3))), pieces = (tiles + most - 1) / most, piece = (tiles + pieces - 1) / pieces * 256,
+                    pitch = std::min(piece, (vocab + 63) / 64 * 64);
     float4 *about;
-    float *gls, *q, *part = nullptr;
+    float *gls;
     unsigned *gmax;
-    const float *x = (const float *)a.hidden.ptr;
+    Piece *probs = nullptr;
+    Matrix x, w;
+    sage_status st = pieces_of(ctx, scratch, a.hidden, &x);
+    if (!st) st = pieces_of(ctx, scratch, a.weight, &w);
     if (!st) st = rows_about(ctx, scratch, a, stats, entropy, gl, ge, false, &about, &gls, &gmax);
-    if (!st) st = scratch.get((size_t)(rows * piece) * 4, &q);
-    if (!st && dhidden.ptr && piece < vocab) st = scratch.get((size_t)(rows * width) * 4, &part);
-    for (long long v = 0; v < vocab && !st; v += piece) {
-        const long long n = std::min(piece, vocab - v);
-        const float *w = (const float *)a.weight.ptr + v * a.weight.pitch;
-        st = gemm(ctx, product_of(false, true, rows, n, width, x, a.hidden.pitch, w, a.weight.pitch, q, n));
-        ctx.note_launch("head_probs");
-        if (!st && !ctx.dry()) {
-            const unsigned across = (unsigned)std::max<long long>(1, std::min<long long>((n + 2047) / 2048, ctx.sm_count * 16 / rows));
-            st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_probs_kernel, dim3((unsigned)rows, across), dim3(256), 0, q, (int)rows, (int)n, (const int *)a.ids.ptr, a.ids.stride, (int)v,
-                                                 a.scale * kLog2E, a.scale, (const float4 *)about, (const float *)gls),
-                                "head_probs");
-        }
+    if (!st) st = scratch.get((size_t)(3 * padded * pitch) * 2, &probs);
+    Result to_hidden;
+    to_hidden.out = dhidden;
+    for (long long at = 0; at < vocab && !st; at += piece) {
+        const long long n = std::min(piece, vocab - at);
+        const bool first = at == 0, last = at + n == vocab;
+        const Matrix here{(const Piece *)w.p + at * w.pitch, n, width, w.pitch, w.plane}, q{probs, rows, n, pitch, padded * pitch};
+        Product p = shape_of(ctx, rows, n, width);
+        p.ids = (const int *)a.ids.ptr;
+        p.ids_stride = a.ids.stride;
+        p.first = (int)at;
+        p.c2 = a.scale * kLog2E;
+        p.rows = about;
+        p.gl = gls;
+        p.band = (int)std::max<long long>(8, ((long long)48 << 20) / (256 * width * 6));
+        p.slice_rows = (int)padded;  // of a plane
+        p.alpha = a.scale;
+        st = launch<Piece, false, false, kProbs, true>(ctx, "head_probs", p, SAGE_BF16, x, here, SAGE_BF16, Matrix{probs, 3 * padded, n, pitch});
         if (!st && dhidden.ptr) {
-            st = gemm(ctx, product_of(false, false, rows, width, n, q, n, w, a.weight.pitch, part ? part : (float *)dhidden.ptr, part ? width : dhidden.pitch));
-            if (part) ctx.note_launch("head_add");
-            if (!st && part && !ctx.dry())
-                st = ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_add_kernel, dim3((unsigned)std::min<long long>((rows * width + 255) / 256, ctx.sm_count * 16ll)), dim3(256), 0, (const float *)part,
-                                                     (float *)dhidden.ptr, dhidden.pitch, rows, (int)width, v ? 1 : 0),
-                                    "head_add");
+            p = shape_of(ctx, rows, width, n);
+            if (first) plan(ctx, p, n, !last, &to_hidden);
+            st = multiply<Piece, false, true, true>(ctx, scratch, "head_dhidden", p, SAGE_BF16, q, here, first, last, &to_hidden);
         }
-        if (!st && dweight.ptr)
-            st = gemm(ctx, product_of(true, false, n, width, rows, q, n, x, a.hidden.pitch, (float *)dweight.ptr + v * dweight.pitch, dweight.pitch));
+        if (!st && dweight.ptr) {
+            p = shape_of(ctx, n, width, rows);
+            Result r;
+            r.out = cut(dweight, at, n);
+            plan(ctx, p, rows, false, &r);
+            st = multiply<Piece, true, true, true>(ctx, scratch, "head_dweight", p, SAGE_BF16, q, x, true, true, &r);
+        }
     }
     return st;
 }

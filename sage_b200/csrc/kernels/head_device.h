@@ -4,6 +4,14 @@
 // Two CTAs work on one tile of 256 rows and BN columns (cta_group::2): each loads its 128 rows of A and its half of B's rows, 64 k at a time,
 // through a ring of TMA stages; the first of them issues the MMAs, whose sums lie 128 rows to a CTA in tensor memory, two tiles' worth, so that
 // eight warps finish a tile while the next one's sums are made.  Either operand may be stored with K or with its rows contiguous.
+//
+// f32 operands (F32), with f32's accuracy: every element is the sum of three bf16 numbers, x = x0 + x1 + x2 (8 bits each, to nearest, 24 in all, in f32's
+// whole range), which lie in three planes, and of the nine products of pieces the six that reach 2^-24 of the result are made,
+//   x2 y0 + x0 y2 + x1 y1 + x1 y0 + x0 y1 + x0 y0,
+// in this order for each 64 k, so that the tensor cores, which cut what lies below the last place of a sum, add the small ones to small sums; the sum of
+// each 64 k is then added to registers, to nearest.  (Two f16 pieces would need three products, but a scale for each row, and what is far below a row's
+// largest would lose bits: the gradient of rare tokens is.  Pieces made inside the product, tile by tile, from f32 operands: 640 x 30522 x 768, values and
+// gradient, 1015 us.)
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -53,7 +61,7 @@ struct Product {
     const float4 *rows;           // kProbs: [m] {largest, -log2 sum, -(gl + ge H), -ge ln 2}
     const float *gl;              // ... [m]
     const unsigned *gmax;         // f16: the bits of the largest |gl| + |ge| (H + 1/2), for the scale that P is stored with; null: 1
-    float alpha;                  // kNarrow, kWide: of the product
+    float alpha;                  // kNarrow, kWide: of the product (f32 operands: kProbs)
     int add;                      // kWide
 };
 
@@ -64,9 +72,9 @@ __device__ __forceinline__ int stored_exponent(const unsigned *gmax) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
-__device__ __forceinline__ void load_2d_pair(void *dst, const CUtensorMap *map, unsigned bar, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(x),
-                 "r"(y)
+__device__ __forceinline__ void load_3d_pair(void *dst, const CUtensorMap *map, unsigned bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(x),
+                 "r"(y), "r"(z)
                  : "memory");
 }
 __device__ __forceinline__ void store_2d(const CUtensorMap *map, const void *src, int x, int y) {
@@ -112,15 +120,19 @@ __device__ __forceinline__ Tile tile_of(const Product &p, int index) {
 
 // One operand's rows of a stage: with K contiguous one box of 64 k, otherwise a box of 64 k for every 64 rows.
 template <bool MN>
-__device__ __forceinline__ void load_rows(char *to, const CUtensorMap *map, unsigned bar, int row, int rows, int k) {
+__device__ __forceinline__ void load_rows(char *to, const CUtensorMap *map, unsigned bar, int row, int rows, int k, int plane) {
     if (MN)
-        for (int i = 0; i < rows; i += 64) load_2d_pair(to + i * (kK * 2), map, bar, row + i, k);
+        for (int i = 0; i < rows; i += 64) load_3d_pair(to + i * (kK * 2), map, bar, row + i, k, plane);
     else
-        load_2d_pair(to, map, bar, k, row);
+        load_3d_pair(to, map, bar, k, row, plane);
 }
+constexpr int kProducts = 6;  // of pieces, for each 64 k of f32 operands
 
 // A warp's 32 rows of 128 bytes as TMA's 128-byte swizzle has them: 16-byte chunk c of row r lies at chunk c ^ (r % 8).
 __device__ __forceinline__ void put_chunk(char *out, int row, int chunk, uint4 v) { *(uint4 *)(out + row * 128 + ((chunk ^ (row & 7)) << 4)) = v; }
+
+// ... 32 rows of 64 bytes, its 64-byte swizzle: chunk c of row r at c ^ (r / 2 % 4).
+__device__ __forceinline__ void put_chunk64(char *out, int row, int chunk, uint4 v) { *(uint4 *)(out + row * 64 + ((chunk ^ (row >> 1 & 3)) << 4)) = v; }
 
 template <class T>
 __device__ __forceinline__ unsigned pair16(float a, float b);
@@ -137,7 +149,72 @@ __device__ __forceinline__ unsigned pair16<__half>(float a, float b) {
     return r;
 }
 
-template <class T, bool A_MN, bool B_MN, End END>
+// The largest bf16 piece of each of two numbers, which keep the rest.  (An infinity is its first piece alone: what is left of it is not a number.)
+__device__ __forceinline__ unsigned take_piece(float &a, float &b) {
+    const unsigned w = pair16<__nv_bfloat16>(a, b);
+    const float x = __uint_as_float(w << 16), y = __uint_as_float(w & 0xffff0000u);
+    a = fabsf(x) < INFINITY ? a - x : x == x ? 0.f : x;
+    b = fabsf(y) < INFINITY ? b - y : y == y ? 0.f : y;
+    return w;
+}
+
+// What a row's 32 * count columns from col0 on come to: largest, sum of exponentials, sum of those times their exponents; the asked-for logit where it is here.
+template <int N>
+__device__ __forceinline__ float4 stats_of(const Product &p, float (&acc)[N][32], int count, int col0, int id, int row) {
+    float largest = -INFINITY, sum = 0.f, along = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        if (j >= count) break;
+        const int col = col0 + j * 32;
+        if (col + 32 > p.n) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (col + e >= p.n) acc[j][e] = -INFINITY;
+        }
+        float high = acc[j][0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) high = fmaxf(high, acc[j][e]);
+        if (high > largest) {  // what there is so far, seen from the new largest
+            const float by = largest == -INFINITY ? 0.f : (largest - high) * p.c2, f = largest == -INFINITY ? 0.f : exp2_fast(by);
+            along = f > 0.f ? fmaf(sum * f, by, along * f) : 0.f;
+            sum *= f;
+            largest = high;
+        }
+        const float from = largest == -INFINITY ? 0.f : largest;
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            const float d = (acc[j][e] - from) * p.c2, x = exp2_fast(d);
+            s[e & 3] += x;
+            a[e & 3] = fmaf(x, fmaxf(d, kFar), a[e & 3]);
+        }
+        sum += (s[0] + s[1]) + (s[2] + s[3]);
+        along += (a[0] + a[1]) + (a[2] + a[3]);
+        const int want = id - col;
+        if (__any_sync(0xffffffffu, want >= 0 && want < 32)) {
+            float x = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x = e == want ? acc[j][e] : x;
+            if (want >= 0 && want < 32 && col + want < p.n) p.asked[row] = x;
+        }
+    }
+    return make_float4(largest, sum, along, 0.f);
+}
+// d / d logits of 32 columns, in place of the logits.
+__device__ __forceinline__ void probs_of(const Product &p, float (&v)[32], const float4 &about, int want, int row, bool there, float factor) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        const float d = fmaf(v[e] - about.x, p.c2, about.y), x = exp2_fast(d);
+        v[e] = x * fmaf(about.w, fmaxf(d, kFar), about.z);
+    }
+    if (__any_sync(0xffffffffu, want >= 0 && want < 32)) {
+        const float gl = there ? __ldg(p.gl + row) * factor : 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] += e == want ? gl : 0.f;
+    }
+}
+
+template <class T, bool A_MN, bool B_MN, End END, bool F32>
 __global__ void __launch_bounds__(kBlock, 1)
 head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c, const Product p) {
     extern __shared__ __align__(1024) char smem_raw[];
@@ -173,7 +250,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         atomicOr(p.status, 0x100u | where);
         given_up = 1;
     };
-    const int all = p.tiles_m * p.tiles_n * p.slices, all_blocks = (p.k + kK - 1) / kK, half = p.bn / 2;
+    const int all = p.tiles_m * p.tiles_n * p.slices, all_blocks = (p.k + kK - 1) / kK * (F32 ? kProducts : 1), half = p.bn / 2;
 
     if (warp == 0) {
         // ------------------------------------------------------------------ loads
@@ -193,8 +270,9 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 const unsigned bar = peer_addr(smem_u32(&full[s]), 0);
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(&full[s], (unsigned)(2 * (128 + half) * kK * 2));
-                    load_rows<A_MN>(to, &map_a, bar, tile.m0 + rank * 128, 128, b * kK);
-                    load_rows<B_MN>(to + kOperandBytes, &map_b, bar, tile.n0 + rank * half, half, b * kK);
+                    const int k = (F32 ? b / kProducts : b) * kK, n = F32 ? b % kProducts : 0;
+                    load_rows<A_MN>(to, &map_a, bar, tile.m0 + rank * 128, 128, k, F32 ? (0x001102 >> 4 * n) & 3 : 0);  // 2 0 1 1 0 0
+                    load_rows<B_MN>(to + kOperandBytes, &map_b, bar, tile.n0 + rank * half, half, k, F32 ? (0x010120 >> 4 * n) & 3 : 0);  // 0 2 1 0 1 0
                 }
                 __syncwarp();
             }
@@ -282,11 +360,15 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 id = __ldg(p.ids + row * p.ids_stride);
                 id = id < p.first ? -1 : id - p.first;
             }
-            if constexpr (END == kStats) {
+            if constexpr (END == kStats || F32) {
                 // The tensor cores cut what lies below a sum's last place at every addition: log probabilities of 4096 k in one chain were 4e-6 off.
                 // Chains of 512 k at most are added up here, to nearest.
-                float acc[128];
-                for (int from = 0; from < all_blocks && live; from += p.chain) {
+                float acc[4][32];
+#pragma unroll
+                for (int e = 0; e < 128; ++e) acc[e / 32][e % 32] = 0.f;
+                const int first = tile.slice * p.slice_blocks, last = min(all_blocks, first + p.slice_blocks);
+#pragma unroll 1
+                for (int from = first; from < last && live; from += p.chain) {
                     const unsigned at = arrived();
                     if (!live) break;
 #pragma unroll
@@ -295,49 +377,59 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                             float v[32];
                             tmem_ld32(at + j * 32, v);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) acc[j * 32 + e] = from ? acc[j * 32 + e] + v[e] : v[e];
+                            for (int e = 0; e < 32; ++e) acc[j][e] += v[e];
                         }
                     drained();
                 }
                 if (!live) break;
-                float largest = -INFINITY, sum = 0.f, along = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j * 32 >= half) break;
-                    const int col = col0 + j * 32;
-                    if (col + 32 > p.n) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (col + e >= p.n) acc[j * 32 + e] = -INFINITY;
+                if constexpr (END == kStats) {
+                const float4 found = stats_of(p, acc, half / 32, col0, id, row);
+                if (there) p.parts[(long long)(tile.n0 / half + side) * p.m + row] = found;
+                } else {
+                    float4 about = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (END == kProbs && there) {
+                        about = __ldg(p.rows + row);
+                        about.z *= p.alpha, about.w *= p.alpha;  // q with its scale: the products of f32 operands have none
                     }
-                    float high = acc[j * 32];
+                    // 32 columns at a time: the sums as they are, or q in three planes
+                    const auto open = [&]() {  // the warp's last store has been read
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+                    };
+                    const auto close = [&](int col, int y) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (row0 < p.m && col < p.n && elect_one()) {
+                            if (END == kWide && p.add) add_2d(&map_c, out, col, y);
+                            else store_2d(&map_c, out, col, y);
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        }
+                        __syncwarp();
+                    };
 #pragma unroll
-                    for (int e = 1; e < 32; ++e) high = fmaxf(high, acc[j * 32 + e]);
-                    if (high > largest) {  // what there is so far, seen from the new largest
-                        const float by = largest == -INFINITY ? 0.f : (largest - high) * p.c2, f = largest == -INFINITY ? 0.f : exp2_fast(by);
-                        along = f > 0.f ? fmaf(sum * f, by, along * f) : 0.f;
-                        sum *= f;
-                        largest = high;
-                    }
-                    const float from = largest == -INFINITY ? 0.f : largest;
-                    float s[4] = {0.f, 0.f, 0.f, 0.f}, a[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int j = 0; j < 4; ++j)
+                        if (j * 32 < half) {
+                            const int col = col0 + j * 32;
+                            if constexpr (END == kProbs) {
+                                probs_of(p, acc[j], about, id - col, row, there, p.alpha);
+#pragma unroll 1
+                                for (int n = 0; n < 3; ++n) {
+                                    open();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const float d = (acc[j * 32 + e] - from) * p.c2, x = exp2_fast(d);
-                        s[e & 3] += x;
-                        a[e & 3] = fmaf(x, fmaxf(d, kFar), a[e & 3]);
-                    }
-                    sum += (s[0] + s[1]) + (s[2] + s[3]);
-                    along += (a[0] + a[1]) + (a[2] + a[3]);
-                    const int want = id - col;
-                    if (__any_sync(0xffffffffu, want >= 0 && want < 32)) {
-                        float x = 0.f;
+                                    for (int c = 0; c < 4; ++c)
+                                        put_chunk64(out, lane, c, make_uint4(take_piece(acc[j][8 * c], acc[j][8 * c + 1]), take_piece(acc[j][8 * c + 2], acc[j][8 * c + 3]),
+                                                                             take_piece(acc[j][8 * c + 4], acc[j][8 * c + 5]), take_piece(acc[j][8 * c + 6], acc[j][8 * c + 7])));
+                                    close(col, row0 + n * p.slice_rows);
+                                }
+                            } else {
+                                open();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x = e == want ? acc[j * 32 + e] : x;
-                        if (want >= 0 && want < 32 && col + want < p.n) p.asked[row] = x;
-                    }
+                                for (int c = 0; c < 8; ++c)
+                                    put_chunk(out, lane, c, make_uint4(__float_as_uint(acc[j][4 * c]), __float_as_uint(acc[j][4 * c + 1]), __float_as_uint(acc[j][4 * c + 2]), __float_as_uint(acc[j][4 * c + 3])));
+                                close(col, row0 + tile.slice * p.slice_rows);
+                            }
+                        }
                 }
-                if (there) p.parts[(long long)(tile.n0 / half + side) * p.m + row] = make_float4(largest, sum, along, 0.f);
             } else {
                 float4 about = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (END == kProbs && there) {
@@ -350,19 +442,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     float v[32];
                     tmem_ld32(at + j, v);
                     const int col = col0 + j;
-                    const int want = END == kProbs ? id - col : -1;
-                    if (END == kProbs) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float d = fmaf(v[e] - about.x, p.c2, about.y), x = exp2_fast(d);
-                            v[e] = x * fmaf(about.w, fmaxf(d, kFar), about.z);
-                        }
-                        if (__any_sync(0xffffffffu, want >= 0 && want < 32)) {
-                            const float gl = there ? __ldg(p.gl + row) * factor : 0.f;
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] += e == want ? gl : 0.f;
-                        }
-                    }
+                    if (END == kProbs) probs_of(p, v, about, id - col, row, there, factor);
                     constexpr int kPer = END == kWide ? 1 : 2;  // loads of 32 columns to a store of 128 bytes
                     const int part = (j / 32) % kPer;
                     if (part == 0) {  // the warp's last store has been read
