@@ -385,38 +385,17 @@ sage_status join(Context &ctx, const float4 *parts, int count, long long rows, c
                           "head_join");
 }
 
-// Rows that are few enough for the product by way of dot products.
-constexpr long long kFewRows = 8;
-bool few(const Head &a) {
+// Rows that are few enough for dot products, and how many of them a pass over the weights takes: eight, or what 96 KB of shared memory hold.  16-bit operands
+// up to four rows (one, four, eight rows of 131072 x 4096 164, 208, 290 us, the tensor cores 203; 30522 x 768 20, 22, 27 and 23); f32 operands up
+// to four passes (16 rows of 131072 x 4096 in four 1250 us, the tensor cores, which need the weights in pieces first, 1820; 32 of 50021 x 2048 460 and 475).
+long long few(const Head &a) {
     const int size = a.hidden.dtype == SAGE_F32 ? 4 : 2;
-    const long long rows = a.hidden.rows > 4 ? 8 : a.hidden.rows > 2 ? 4 : a.hidden.rows;
-    return a.hidden.rows <= kFewRows && a.hidden.cols % 8 == 0 && rows * a.hidden.cols * size <= 96 * 1024 && on_16(a.hidden.ptr, a.hidden.rows > 1 ? a.hidden.pitch : 0, size) &&
-           on_16(a.weight.ptr, a.weight.rows > 1 ? a.weight.pitch : 0, size);
+    if (a.hidden.cols % 8 || !on_16(a.hidden.ptr, a.hidden.rows > 1 ? a.hidden.pitch : 0, size) || !on_16(a.weight.ptr, a.weight.rows > 1 ? a.weight.pitch : 0, size)) return 0;
+    long long pass = 8;
+    while (pass && pass * a.hidden.cols * size > 96 * 1024) pass /= 2;
+    while (pass > 1 && pass / 2 >= a.hidden.rows) pass /= 2;
+    return a.hidden.rows <= (size == 4 ? 4 * pass : std::min(4ll, pass)) ? pass : 0;
 }
-template <class T>
-sage_status forward_few(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
-    Scratch scratch(ctx);
-    const long long rows = a.hidden.rows, vocab = a.weight.rows;
-    const unsigned grid = (unsigned)std::min<long long>((vocab + 31) / 32, 2ll * ctx.sm_count);
-    float4 *parts = nullptr;
-    float *asked = nullptr;
-    sage_status st = scratch.get((size_t)(grid * rows) * 16, &parts);
-    if (!st) st = scratch.get((size_t)rows * 4, &asked);
-    if (st) return st;
-    ctx.note_launch("head_few");
-    const auto run = [&](auto kernel, int padded) {
-        const size_t smem = (size_t)padded * a.hidden.cols * sizeof(T);
-        sage_status s = ctx.check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024), "head_few");
-        return s ? s
-                 : ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3(grid), dim3(256), smem, (const T *)a.hidden.ptr, a.hidden.pitch, (const T *)a.weight.ptr, a.weight.pitch, (int)rows, (int)vocab,
-                                                   (int)a.hidden.cols, (const int *)a.ids.ptr, a.ids.stride, a.scale * kLog2E, parts, asked),
-                                  "head_few");
-    };
-    if (!ctx.dry()) st = rows > 4 ? run(head_few_kernel<T, 8>, 8) : rows > 2 ? run(head_few_kernel<T, 4>, 4) : rows > 1 ? run(head_few_kernel<T, 2>, 2) : run(head_few_kernel<T, 1>, 1);
-    if (st) return st;
-    return join(ctx, parts, (int)grid, rows, asked, a.ids, vocab, a.scale, Values{(float *)log_probs.ptr, (float *)entropy.ptr, (float *)stats.ptr, log_probs.stride, entropy.stride, stats.pitch});
-}
-
 // Rows [at, at + count) of the operands and results.
 RowsArg cut(const RowsArg &r, long long at, long long count) {
     RowsArg c = r;
@@ -425,6 +404,38 @@ RowsArg cut(const RowsArg &r, long long at, long long count) {
     return c;
 }
 VectorArg cut(const VectorArg &v, long long at) { return v.ptr ? VectorArg{(char *)v.ptr + at * v.stride * 4, v.stride} : v; }
+
+template <class T>
+sage_status forward_few(Context &ctx, const Head &all, long long pass, const VectorArg &all_log_probs, const VectorArg &all_entropy, const RowsArg &all_stats) {
+    for (long long at = 0; at < all.hidden.rows; at += pass) {
+        Scratch scratch(ctx);
+        Head a = all;
+        a.hidden = cut(all.hidden, at, std::min(pass, all.hidden.rows - at));
+        a.ids = cut(all.ids, at);
+        const VectorArg log_probs = cut(all_log_probs, at), entropy = cut(all_entropy, at);
+        const RowsArg stats = cut(all_stats, at, a.hidden.rows);
+        const long long rows = a.hidden.rows, vocab = a.weight.rows;
+        const unsigned grid = (unsigned)std::min<long long>((vocab + 31) / 32, 2ll * ctx.sm_count);
+        float4 *parts = nullptr;
+        float *asked = nullptr;
+        sage_status st = scratch.get((size_t)(grid * rows) * 16, &parts);
+        if (!st) st = scratch.get((size_t)rows * 4, &asked);
+        if (st) return st;
+        ctx.note_launch("head_few");
+        const auto run = [&](auto kernel, int padded) {
+            const size_t smem = (size_t)padded * a.hidden.cols * sizeof(T);
+            sage_status s = ctx.check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024), "head_few");
+            return s ? s
+                     : ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3(grid), dim3(256), smem, (const T *)a.hidden.ptr, a.hidden.pitch, (const T *)a.weight.ptr, a.weight.pitch, (int)rows, (int)vocab,
+                                                       (int)a.hidden.cols, (const int *)a.ids.ptr, a.ids.stride, a.scale * kLog2E, parts, asked),
+                                      "head_few");
+        };
+        if (!ctx.dry()) st = pass > 4 ? run(head_few_kernel<T, 8>, 8) : pass > 2 ? run(head_few_kernel<T, 4>, 4) : pass > 1 ? run(head_few_kernel<T, 2>, 2) : run(head_few_kernel<T, 1>, 1);
+        if (!st) st = join(ctx, parts, (int)grid, rows, asked, a.ids, vocab, a.scale, Values{(float *)log_probs.ptr, (float *)entropy.ptr, (float *)stats.ptr, log_probs.stride, entropy.stride, stats.pitch});
+        if (st) return st;
+    }
+    return SAGE_OK;
+}
 
 template <class T>
 sage_status forward16(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
@@ -634,8 +645,8 @@ sage_status grad32(Context &ctx, const Head &a, const RowsArg &stats, const Vect
 
 sage_status head_log_probs(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
     if (!a.hidden.rows) return SAGE_OK;
-    if (head::few(a))
-        return with_type(a.hidden.dtype, [&](auto t) { return head::forward_few<decltype(t)>(ctx, a, log_probs, entropy, stats); });
+    if (const long long pass = head::few(a))
+        return with_type(a.hidden.dtype, [&](auto t) { return head::forward_few<decltype(t)>(ctx, a, pass, log_probs, entropy, stats); });
     if (a.hidden.dtype == SAGE_F32) return head::forward32(ctx, a, log_probs, entropy, stats);
     return a.hidden.dtype == SAGE_F16 ? head::forward16<__half>(ctx, a, log_probs, entropy, stats) : head::forward16<__nv_bfloat16>(ctx, a, log_probs, entropy, stats);
 }
