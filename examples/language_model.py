@@ -1,7 +1,10 @@
 """A small language model trained and asked: the embedding with its gradient, the log probabilities of the next tokens with an entropy
 bonus, and AdamW with 8-bit states, as one lazy graph; then single contexts with their likeliest continuations.
 
-    python examples/language_model.py [--steps 60] [--tokens 2000] [--width 64]
+    python examples/language_model.py [--steps 60] [--tokens 2000] [--width 64] [--blocks 0] [--dropout 0.1]
+
+With --blocks the layers are followed by as many residual blocks, their norms, gates and dropout in one operator, and the log probabilities come
+straight from the last hidden states.
 
 The data is a made-up language: a sentence steps through the vocabulary by one of three strides that its first token names.
 """
@@ -20,24 +23,42 @@ CONTEXT = 3
 class Model:
     """Three tokens -> the next: embeddings side by side, two dense layers, and the embedding table again as the last product."""
 
-    def __init__(self, ctx, tokens, width, rng):
-        def param(*extents, std):
+    def __init__(self, ctx, tokens, width, rng, blocks=0, dropout=0.0):
+        def param(*extents, std, mean=0.0):
             v = S.Var.empty(extents)
-            ctx.set(v, (rng.standard_normal(extents) * std).astype(np.float32))
+            ctx.set(v, (mean + rng.standard_normal(extents) * std).astype(np.float32))
             return v
         self.width = width
         self.table = param(tokens, width, std=1.0 / width)  # scaled by the root of the width where it is looked up
         self.w1, self.b1 = param(CONTEXT * width, 4 * width, std=(CONTEXT * width) ** -0.5), param(4 * width, std=0.0)
         self.w2, self.b2 = param(4 * width, width, std=(4 * width) ** -0.5), param(width, std=0.0)
+        self.dropout, self.seed = dropout, ctx.var(np.zeros(2, np.uint32))
+        self.norms = [param(width, std=0.0, mean=1.0) for _ in range(blocks + 1)] if blocks else []
+        self.blocks = [(param(width, 2 * width, std=width ** -0.5), param(2 * width, width, std=(2 * width) ** -0.5), param(width, std=0.0, mean=0.5)) for _ in range(blocks)]
 
     def params(self):
-        return [self.table, self.w1, self.b1, self.w2, self.b2]
+        return [self.table, self.w1, self.b1, self.w2, self.b2] + self.norms + [p for block in self.blocks for p in block]
 
-    def logits(self, ids):  # [rows, CONTEXT]
+    def hidden(self, ids, train):  # [rows, CONTEXT]
         x = S.embedding(self.table, ids, scale=self.width ** 0.5)
         x = x.view([ids.extents[0], CONTEXT * self.width])
         x = S.relu(x.matmul(self.w1) + self.b1)
-        return (x.matmul(self.w2) + self.b2).matmul(self.table.tr())
+        x = x.matmul(self.w2) + self.b2
+        if not self.blocks:
+            return x
+        p = self.dropout if train else 0.0
+        x, h = S.block_norms(S.dropout(x, self.seed, p), before="rms", before_weight=self.norms[0])
+        for i, (up, down, gate) in enumerate(self.blocks):  # the stream goes by, each block reads it through its norm
+            x, h = S.block_norms(x, S.relu(h.matmul(up)).matmul(down), gate=gate, p=p, seed=self.seed, site=i + 1, before="rms", before_weight=self.norms[i + 1])
+        return h
+
+    def logits(self, ids):
+        return self.hidden(ids, False).matmul(self.table.tr())
+
+    def log_probs(self, ids, after):
+        if self.blocks:
+            return S.head_log_probs(self.hidden(ids, True), self.table, after)
+        return S.token_log_probs(self.logits(ids), after)
 
 
 def sentences(rng, rows, tokens):
@@ -52,12 +73,14 @@ def main(argv=None):
     ap.add_argument("--tokens", type=int, default=2000)
     ap.add_argument("--width", type=int, default=64)
     ap.add_argument("--batch", type=int, default=1024)
+    ap.add_argument("--blocks", type=int, default=0)
+    ap.add_argument("--dropout", type=float, default=0.1)
     ap.add_argument("--device", type=int, default=0)
     a = ap.parse_args(argv)
     rng, ctx = np.random.default_rng(0), S.Context(a.device)
-    model = Model(ctx, a.tokens, a.width, rng)
+    model = Model(ctx, a.tokens, a.width, rng, a.blocks, a.dropout)
     ids, after = ctx.var(np.zeros((a.batch, CONTEXT), np.uint32)), ctx.var(np.zeros(a.batch, np.uint32))
-    log_probs, entropy = S.token_log_probs(model.logits(ids), after)
+    log_probs, entropy = model.log_probs(ids, after)
     loss = -(log_probs.mean([0]) + entropy.mean([0]) * 0.01)
     grads = dict(zip(model.params(), S.grad(loss, model.params())))
     opt = S.AdamW(3e-3, state_bits=8)
@@ -67,6 +90,7 @@ def main(argv=None):
         s = sentences(rng, a.batch, a.tokens)
         ctx.set(ids, s[:, :CONTEXT])
         ctx.set(after, np.ascontiguousarray(s[:, CONTEXT]))
+        ctx.set(model.seed, np.array([a.steps, step], np.uint32))  # another mask for every step
         ctx.clear()
         ctx.eval(loss, *grads.values())
         losses.append(float(ctx.read(loss)[0]))

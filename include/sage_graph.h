@@ -129,6 +129,19 @@ sage_status sage_op_layer_norm(const sage_var *x, int32_t naxes, const int64_t *
 sage_status sage_op_embedding(const sage_var *table, const sage_var *ids, float scale, sage_var **out);
 sage_status sage_op_token_log_probs(const sage_var *logits, const sage_var *ids, float scale, sage_var **out);
 sage_status sage_op_top_tokens(const sage_var *logits, int64_t k, sage_var **out);
+/* head_log_probs: token_log_probs of hidden weight^T ([rows, width], [tokens, width]), made in pieces and not kept.  dropout: f32 of any extents, its
+ * elements numbered in row-major order; the seed is a variable of two i32 / u32 that is read when the graph is evaluated.  block_norms: out = residual_scale * x +
+ * gate * dropout(A(y)) and h = B(out) over the last axis (y NULL: out = residual_scale * x; h is NULL where there is no norm before), one launch, and one
+ * and a sum for all gradients.  Operands that are not there are NULL; the gate is [width], or [groups, width] whose row g serves the g-th of as many equal runs of rows. */
+sage_status sage_op_head_log_probs(const sage_var *hidden, const sage_var *weight, const sage_var *ids, float scale, sage_var **out);
+sage_status sage_op_dropout(const sage_var *x, const sage_var *seed, float p, uint64_t site, sage_var **out);
+typedef struct {
+    const sage_var *after_weight, *after_bias, *before_weight, *before_bias, *gate, *seed;
+    int32_t after, before; /* sage_norm */
+    float residual_scale, eps, p;
+    uint64_t site;
+} sage_op_norms;
+sage_status sage_op_block_norms(const sage_var *x, const sage_var *y, const sage_op_norms *norms, sage_var **out, sage_var **h);
 
 /* ---- random tensors, src/ops/rand.rs:21-140.  The reference takes two 32-bit seeds from the thread's generator at
  * every evaluation; here the caller gives them, so results can be reproduced.  uniform: [0, 1]; normal: Box-Muller. */

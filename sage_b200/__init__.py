@@ -669,6 +669,37 @@ def top_tokens(logits, k):
     return _mk(lib.sage_op_top_tokens, logits.h, ctypes.c_int64(k))
 
 
+def head_log_probs(hidden, weight, ids, scale=1.0):
+    """token_log_probs of hidden [rows, width] . weight [tokens, width]^T, whose logits are made in pieces and not kept."""
+    y = _mk(lib.sage_op_head_log_probs, hidden.h, weight.h, ids.h, ctypes.c_float(scale))
+    return squeeze(slice_(y, 1, 0, 1), 1), squeeze(slice_(y, 1, 1, 2), 1)
+
+
+def dropout(x, seed, p, site=0):
+    """x / (1 - p) where an element stays, else 0: drawn from `seed` (a variable of two u32, as it is when the graph is evaluated: set it for every step),
+    `site` and the element's place; no mask is stored (sage_b200.language says how it is drawn)."""
+    return _mk(lib.sage_op_dropout, x.h, seed.h, ctypes.c_float(p), ctypes.c_uint64(site))
+
+
+class _Norms(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("after_weight", "after_bias", "before_weight", "before_bias", "gate", "seed")] + [("after", ctypes.c_int32), ("before", ctypes.c_int32)] + \
+               [(n, ctypes.c_float) for n in ("residual_scale", "eps", "p")] + [("site", ctypes.c_uint64)]
+
+
+def block_norms(x, y=None, after=None, after_weight=None, after_bias=None, before=None, before_weight=None, before_bias=None, gate=None, residual_scale=1.0, eps=1e-5,
+                p=0.0, seed=None, site=0):
+    """(out, h): out = residual_scale * x + gate * dropout(A(y)), h = B(out) over the last axis, with A = `after` and B = `before` one of "rms", "layer" and
+    None (then h is None).  One launch, and one and a sum for all gradients."""
+    kinds = {None: 0, "none": 0, "rms": 1, "layer": 2}
+    if after not in kinds or before not in kinds:
+        raise SageError(1, "block_norms: no norm is called %r" % (after if after not in kinds else before,))
+    h = lambda v: None if v is None else v.h  # noqa: E731
+    n = _Norms(h(after_weight), h(after_bias), h(before_weight), h(before_bias), h(gate), h(seed), kinds[after], kinds[before], residual_scale, eps, p, site)
+    out, normed = _P(), _P()
+    _gck(lib.sage_op_block_norms(x.h, h(y), ctypes.byref(n), ctypes.byref(out), ctypes.byref(normed)))
+    return Var(out), Var(normed) if normed else None
+
+
 def uniform(extents, seed_x, seed_y):
     """ops::rand::uniform (src/ops/rand.rs:21-28, 50-90) with explicit seeds: values in [0, 1]."""
     return _mk(lib.sage_op_uniform, len(extents), _arr64(extents), ctypes.c_uint32(seed_x), ctypes.c_uint32(seed_y))

@@ -313,6 +313,34 @@ sage_status sage_op_layer_norm(const sage_var *x, int32_t naxes, const int64_t *
 sage_status sage_op_embedding(const sage_var *table, const sage_var *ids, float scale, sage_var **out) { OP(ops::embedding(table->v, ids->v, scale)); }
 sage_status sage_op_token_log_probs(const sage_var *logits, const sage_var *ids, float scale, sage_var **out) { OP(ops::token_log_probs(logits->v, ids->v, scale)); }
 sage_status sage_op_top_tokens(const sage_var *logits, int64_t k, sage_var **out) { OP(ops::top_tokens(logits->v, k)); }
+sage_status sage_op_head_log_probs(const sage_var *hidden, const sage_var *weight, const sage_var *ids, float scale, sage_var **out) {
+    OP(ops::head_log_probs(hidden->v, weight->v, ids->v, scale));
+}
+sage_status sage_op_dropout(const sage_var *x, const sage_var *seed, float p, uint64_t site, sage_var **out) { OP(ops::dropout(x->v, seed->v, p, site)); }
+sage_status sage_op_block_norms(const sage_var *x, const sage_var *y, const sage_op_norms *norms, sage_var **out, sage_var **h) {
+    return guarded([&]() -> sage_status {
+        if (!norms || !out || !h) return SAGE_ERR_INVALID;
+        const auto given = [](const sage_var *v) { return v ? v->v : Var(); };
+        ops::BlockNorms n;
+        n.after_weight = given(norms->after_weight);
+        n.after_bias = given(norms->after_bias);
+        n.before_weight = given(norms->before_weight);
+        n.before_bias = given(norms->before_bias);
+        n.gate = given(norms->gate);
+        n.seed = given(norms->seed);
+        n.after = norms->after;
+        n.before = norms->before;
+        n.scale = norms->residual_scale;
+        n.eps = norms->eps;
+        n.p = norms->p;
+        n.site = norms->site;
+        Var results[2];
+        ops::block_norms(x->v, given(y), n, &results[0], &results[1]);
+        *h = nullptr;
+        sage_status st = ret(out, results[0]);
+        return st || !results[1].defined() ? st : ret(h, results[1]);
+    });
+}
 
 sage_status sage_op_uniform(int32_t ndim, const int64_t *extents, uint32_t seed_x, uint32_t seed_y, sage_var **out) {
     OP(ops::uniform(arr(ndim, extents), seed_x, seed_y));

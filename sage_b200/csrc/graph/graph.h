@@ -352,6 +352,16 @@ Var accuracy(const Var &logits, const Var &labels);
 Var embedding(const Var &table, const Var &ids, float scale);
 Var token_log_probs(const Var &logits, const Var &ids, float scale);  // [rows, 4]: log probability, entropy, and what the gradient reads
 Var top_tokens(const Var &logits, long long k);
+Var head_log_probs(const Var &hidden, const Var &weight, const Var &ids, float scale);  // [rows, 4], as token_log_probs gives them
+Var dropout(const Var &x, const Var &seed, float p, unsigned long long site);
+// The norms around a block (kernels/block_norms.cu); what is not there is an undefined Var.  out and h have the extents of x.
+struct BlockNorms {
+    Var after_weight, after_bias, before_weight, before_bias, gate, seed;
+    int after = 0, before = 0;
+    float scale = 1.f, eps = 1e-5f, p = 0.f;
+    unsigned long long site = 0;
+};
+void block_norms(const Var &x, const Var &y, const BlockNorms &n, Var *out, Var *h);
 // rand.rs (the seeds the reference draws per evaluation are arguments here)
 Var uniform(const Array &extents, unsigned seed_x, unsigned seed_y);
 Var normal(const Array &extents, unsigned seed_x, unsigned seed_y);
@@ -380,5 +390,6 @@ struct MapOp;
 std::shared_ptr<Operator> fuse_ops(const Operator &parent, const Operator &child, int idx);  // Operator::fuse, ops.rs:104-161
 std::string map_expr_text(const MapExpr &e);
 const MapExpr *map_expr_of(const Operator &op);
+long long unslice_start(const Operator &op);  // ops_core.cc
 
 }  // namespace sage

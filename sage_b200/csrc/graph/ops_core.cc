@@ -174,6 +174,12 @@ struct UnsliceOp : Operator {
     }
 };
 
+// Where an unslice along the first axis puts its input; -1: another operator.
+long long unslice_start(const Operator &op) {
+    const UnsliceOp *u = dynamic_cast<const UnsliceOp *>(&op);
+    return u && u->axis == 0 ? u->start : -1;
+}
+
 Var ops::unslice(const Var &x, long long axis, long long start, long long end) {
     const int a = to_axis(axis, x.rank());
     if (end < start + x.extent(a)) shape_fail("unslice: range smaller than the input");
