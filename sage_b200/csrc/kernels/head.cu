@@ -43,33 +43,42 @@ struct Values {
     long long log_probs_stride, entropy_stride, stats_pitch;
 };
 
-// 32 rows a block, its warps share the parts.
+// 32 rows a block: its warps share the parts of all of them, a lane to a row, then a warp takes a row, a lane to what each warp found.
 __global__ void __launch_bounds__(1024) head_join_kernel(const float4 *parts, int count, int rows, const float *asked, const int *ids, long long ids_stride, int vocab, float scale, float c2,
                                                          Values y) {
     __shared__ Sums all[32][33];
     grid_dependency_sync();
-    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, warps = (int)blockDim.x >> 5, row = (int)blockIdx.x * 32 + lane;
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
     Sums x{-INFINITY, 0.f, 0.f};
-    if (row < rows) {
+    if ((int)blockIdx.x * 32 + lane < rows) {
 #pragma unroll 4
         for (int i = warp; i < count; i += warps) {
-            const float4 p = __ldg(parts + (long long)i * rows + row);
+            const float4 p = __ldg(parts + (long long)i * rows + (int)blockIdx.x * 32 + lane);
             x = joined(x, Sums{p.x, p.y, p.z}, c2);
         }
     }
     all[warp][lane] = x;
     __syncthreads();
-    if (warp || row >= rows) return;
-    for (int w = 1; w < warps; ++w) x = joined(x, all[w][lane], c2);
-    const bool none = x.m == -INFINITY && x.s == 0.f;  // no token has a chance
-    const float ln_s = logf(x.s);
-    const int id = __ldg(ids + row * ids_stride);
-    const bool scored = id >= 0 && id < vocab;
-    if (y.log_probs) y.log_probs[row * y.log_probs_stride] = !scored ? 0.f : none ? -INFINITY : (asked[row] - x.m) * scale - ln_s;
-    if (y.entropy) y.entropy[row * y.entropy_stride] = none ? 0.f : ln_s - kLn2 * x.a / x.s;
-    if (y.stats) {
-        y.stats[row * y.stats_pitch] = x.m;
-        y.stats[row * y.stats_pitch + 1] = x.s;
+    for (int r = warp; r < 32; r += warps) {
+        const int row = (int)blockIdx.x * 32 + r;
+        if (row >= rows) return;
+        x = lane < warps ? all[lane][r] : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int off = 16; off; off >>= 1) {
+            const Sums o{__shfl_xor_sync(0xffffffffu, x.m, off), __shfl_xor_sync(0xffffffffu, x.s, off), __shfl_xor_sync(0xffffffffu, x.a, off)};
+            x = lane & off ? joined(o, x, c2) : joined(x, o, c2);  // (the same order on both sides: the same bits)
+        }
+        if (lane) continue;
+        const bool none = x.m == -INFINITY && x.s == 0.f;  // no token has a chance
+        const float ln_s = logf(x.s);
+        const int id = __ldg(ids + row * ids_stride);
+        const bool scored = id >= 0 && id < vocab;
+        if (y.log_probs) y.log_probs[row * y.log_probs_stride] = !scored ? 0.f : none ? -INFINITY : (asked[row] - x.m) * scale - ln_s;
+        if (y.entropy) y.entropy[row * y.entropy_stride] = none ? 0.f : ln_s - kLn2 * x.a / x.s;
+        if (y.stats) {
+            y.stats[row * y.stats_pitch] = x.m;
+            y.stats[row * y.stats_pitch + 1] = x.s;
+        }
     }
 }
 
@@ -189,18 +198,31 @@ __global__ void __launch_bounds__(256) head_rows_kernel(const float *stats, long
     }
 }
 
-// Rows into others: the sum of `slices` that lie apart, in another type, with another pitch.
-template <class A, class B>
+// Rows into others: the sum of `slices` that lie apart, in another type, with another pitch.  WIDE: four elements of `x` on 16-byte (f32) or 8-byte boundaries.
+template <class A, class B, bool WIDE>
 __global__ void __launch_bounds__(256) head_rows_copy_kernel(const A *x, long long px, B *y, long long py, long long rows, int cols, int slices, long long slice) {
+    struct alignas(4 * sizeof(A)) Four {
+        A v[4];
+    };
     grid_dependency_sync();
     const int per = (cols + 3) / 4;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * per; i += gridDim.x * 256ll) {
-        const long long r = i / per, c = (i - r * per) * 4;
+        const long long r = rows * per <= 0x7fffffffll ? (int)i / per : i / per, c = (i - r * per) * 4;
+        const A *from = x + r * px + c;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < slices; ++s)
+        if (WIDE) {
+#pragma unroll 4
+            for (int s = 0; s < slices; ++s) {
+                const Four f = *(const Four *)(from + s * slice);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c + e < cols) v[e] += widen(x[s * slice + r * px + c + e]);
+                for (int e = 0; e < 4; ++e) v[e] += widen(f.v[e]);
+            }
+        } else {
+            for (int s = 0; s < slices; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < cols) v[e] += widen(from[s * slice + e]);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (c + e < cols) y[r * py + c + e] = narrowed<B>(v[e]);
@@ -211,7 +233,8 @@ sage_status copy_rows(Context &ctx, const A *x, long long px, B *y, long long py
     ctx.note_launch("head_rows_copy");
     if (ctx.dry()) return SAGE_OK;
     const long long blocks = std::min<long long>((rows * ((cols + 3) / 4) + 255) / 256, ctx.sm_count * 16ll);
-    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_rows_copy_kernel<A, B>, dim3((unsigned)blocks), dim3(256), 0, x, px, y, py, rows, cols, slices, slice), "head_rows_copy");
+    const bool wide = (uintptr_t)x % (4 * sizeof(A)) == 0 && px % 4 == 0 && cols % 4 == 0 && slice % 4 == 0;
+    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? head_rows_copy_kernel<A, B, true> : head_rows_copy_kernel<A, B, false>, dim3((unsigned)blocks), dim3(256), 0, x, px, y, py, rows, cols, slices, slice), "head_rows_copy");
 }
 
 // Three bf16 pieces of each f32 element, eight to a thread.
