@@ -249,3 +249,56 @@ def test_block_norms_of_no_rows_and_strange_rows(ctx, dim):
         # (a row of one value: its mean in 32 bits is off by 53 U of it at most, which a deviation of the root of eps makes as large as this)
         assert np.all(np.abs(out.numpy()[1] - c.host["ab"]) <= np.abs(c.host["aw"]) * 53 * O.U * 3e4 / np.sqrt(1e-5) + 1e-6)
         assert np.isnan(out.numpy()[4]).all() and np.isnan(h.numpy()[4]).all() and not np.isnan(h.numpy()[5]).any()
+
+
+# ------------------------------------------------------------------------------------------ captured
+def test_a_captured_run_follows_its_operands():
+    """Dropout, both directions of the norms and of the head, captured once and replayed on new contents: the same bits as calls, and masks by the seed of the moment."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n = lambda *s, t=torch.bfloat16: torch.randn(s, generator=g, device="cuda").to(t)  # noqa: E731
+    rows, dim, vocab = 300, 264, 1000
+    t = {"x": n(rows, dim), "y": n(rows, dim), "w": n(dim, t=torch.float32), "gate": n(4, dim, t=torch.float32), "table": n(vocab, dim), "gl": n(rows, t=torch.float32)}
+    t["seed"] = torch.tensor([5, 6], dtype=torch.int32, device="cuda")
+    t["ids"] = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    e = lambda *s, d=torch.bfloat16: torch.empty(s, dtype=d, device="cuda")  # noqa: E731
+    f32 = torch.float32
+    r = {"drop": e(rows, dim), "out": e(rows, dim), "h": e(rows, dim), "stats": e(rows, 4, d=f32), "logp": e(rows, d=f32), "ent": e(rows, d=f32), "st": e(rows, 2, d=f32), "dh": e(rows, dim),
+         "dtable": e(vocab, dim), "dx": e(rows, dim), "dy": e(rows, dim), "dw": e(dim, d=f32), "dgate": e(4, dim, d=f32)}
+    ctx, stream = S.Context(0), torch.cuda.Stream()
+    ctx.use_stream(stream.cuda_stream)
+    b = {k: ctx.borrow(v) for k, v in {**t, **r}.items()}
+    norms = L.BlockNorms(ctx, after="rms", before="rms", before_weight=b["w"], gate=b["gate"], p=0.2, seed=b["seed"], site=4)
+
+    def step():
+        L.dropout(b["x"], b["drop"], b["seed"], 0.1, site=1)
+        L.block_norms(norms, b["drop"], b["y"], b["out"], b["h"], b["stats"])
+        L.head_log_probs(b["h"], b["table"], b["ids"], b["logp"], b["ent"], b["st"])
+        L.head_log_probs_grad(b["h"], b["table"], b["ids"], b["st"], b["ent"], b["gl"], b["gl"], b["dh"], b["dtable"])
+        L.block_norms_grad(norms, b["out"], b["y"], b["stats"], None, b["dh"], b["dx"], b["dy"], dgate=b["dgate"], dbefore_weight=b["dw"])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step()  # the pool's memory is there before anything is captured
+        step()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for seed in ((5, 6), (-1, 9)):
+        with torch.cuda.stream(stream):
+            t["seed"].copy_(torch.tensor(seed, dtype=torch.int32))
+            t["y"].mul_(1.5)
+            step()
+            stream.synchronize()
+            want = {k: v.clone() for k, v in r.items()}
+            for v in r.values():
+                v.zero_()
+            graph.replay()
+            stream.synchronize()
+        for k, v in r.items():
+            assert torch.equal(v, want[k]), k
+        kept = torch.from_numpy(B.keep(np.array(seed, np.int32).astype(np.uint32), 1, rows * dim, 0.1).reshape(rows, dim)).cuda()
+        assert torch.equal(r["drop"] != 0, kept & (t["x"] != 0))
+    del graph
+    assert ctx.status_word() == 0
+    ctx.close()
