@@ -13,7 +13,7 @@ namespace {
 constexpr int kRegisters = 80;  // of a thread of the general form
 __host__ __device__ constexpr int wide_registers(int nv) { return nv <= 2 ? 64 : nv == 3 ? 72 : 96; }
 
-// Whole runs of eight columns on 16-byte boundaries: a team takes one row, all of whose columns are asked for before anything waits.  Teams enough for
+// Whole runs of eight columns on 32-byte (16 bits: 16-byte) boundaries: a team takes one row, all of whose columns are asked for before anything waits.  Teams enough for
 // the memory's latency are there at once, and the weights stay in L1 (with rows brought through rings in shared memory by teams that stay,
 // 16384 x 4096 took 232 us: what is left of L1 then does not hold the weights).
 __device__ __forceinline__ void prefetch_row(const char *p, int bytes) { asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory"); }

@@ -202,7 +202,7 @@ __device__ __forceinline__ Place place_of(const NormsArgs &a, float2 *slots) {
 // Which of a thread's eight columns of a row stay.
 __device__ __forceinline__ unsigned kept(const Dropout &d, Key key, int row, int dim, int col) { return keep_from(d, key, (unsigned long long)row * dim + col); }
 
-// ---- rows that come through shared memory: 8 | dim, rows on 16-byte boundaries less than 4 GB apart.  All but a thread's last run of columns are
+// ---- rows that come through shared memory: 8 | dim, rows on 32-byte (16 bits: 16-byte) boundaries, less than 4 GB apart.  All but a thread's last run of columns are
 // there; `last` says whether that one is.  Addresses are made from the kernel's parameters where they are used: held in registers they
 // took more of them than the sums over rows do.
 template <class T>
@@ -229,14 +229,14 @@ template <class T>
 __device__ __forceinline__ void put8(char *to, const float2 (&v)[4]) {
     Eight<T> q;
     q.close(v);
-#pragma unroll
-    for (int i = 0; i < Eight<T>::kPacks; ++i) ((Pack<T> *)to)[i] = q.p[i];
+    q.store(to);
 }
 __device__ __forceinline__ void get8(const float *p, float2 (&v)[4]) {  // weights, biases, gates
     const float4 a = __ldg((const float4 *)p), b = __ldg((const float4 *)p + 1);
     v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
 }
-inline bool boundary(const Rows &r, long long size) { return (uintptr_t)r.p % 16 == 0 && r.pitch * size % 16 == 0 && r.pitch * size < 0x100000000ll; }
+// Eight elements of a row in one access (f32: 32 bytes).
+inline bool boundary(const Rows &r, long long size) { return (uintptr_t)r.p % (8 * size) == 0 && r.pitch % 8 == 0 && r.pitch * size < 0x100000000ll; }
 inline bool boundary(const float *p) { return (uintptr_t)p % 16 == 0; }
 inline Rows of(const RowsArg &r) {
     const long long pitch = r.rows > 1 ? r.pitch : r.cols;

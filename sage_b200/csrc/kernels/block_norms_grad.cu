@@ -45,7 +45,7 @@ __device__ __forceinline__ void join_teams(const NormsArgs &a, const Place &at, 
 __host__ __device__ constexpr int ring_registers(int nv, bool full) { return full ? (nv == 1 ? 96 : 128) : nv == 1 ? 80 : nv == 2 ? 96 : 128; }
 
 // What models call: both gradients arrive, there is a norm before the next block and norms have weights; whole runs of columns on
-// 16-byte boundaries.
+// 32-byte (16 bits: 16-byte) boundaries.
 template <class TX, class T, int NV, bool FULL, bool BIAS>
 __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kernel(const NormsArgs a) {
     extern __shared__ __align__(16) char ring[];

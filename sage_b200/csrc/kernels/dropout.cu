@@ -2,7 +2,7 @@
 // (counter_random.h says which stay).  Its gradient is the same map of the gradient that arrives.
 //
 // Bound by memory: an element is read and written once; a draw of 60 integer instructions serves eight of them.  A thread takes one block of
-// eight elements, whatever the layout: as vectors where rows keep blocks whole and on 16-byte boundaries, element by element elsewhere.
+// eight elements, whatever the layout: as vectors where rows keep blocks whole and on 32-byte (16 bits: 16-byte) boundaries, element by element elsewhere.
 #include <algorithm>
 
 #include "counter_random.h"
@@ -21,7 +21,7 @@ struct DropoutArgs {
     Dropout d;
 };
 
-constexpr int kThreads = 256, kBlocks = 4;  // of a CTA; blocks of eight elements to a thread
+constexpr int kThreads = 256, kBlocks = 2;  // of a CTA; blocks of eight elements to a thread
 
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs a) {
@@ -77,7 +77,7 @@ sage_status dropout(Context &ctx, const RowsArg &x, const RowsArg &y, const Drop
     const long long size = x.dtype == SAGE_F32 ? 4 : 2, blocks = (a.n + 8 * kThreads * kBlocks - 1) / (8 * kThreads * kBlocks);
     if (blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "dropout: more than 2^44 elements");
     const bool one = a.cols == a.n;
-    const bool wide = (uintptr_t)x.ptr % 16 == 0 && (uintptr_t)y.ptr % 16 == 0 && (one || (a.cols % 8 == 0 && x.pitch * size % 16 == 0 && y.pitch * size % 16 == 0));
+    const bool wide = (uintptr_t)x.ptr % (8 * size) == 0 && (uintptr_t)y.ptr % (8 * size) == 0 && (one || (a.cols % 8 == 0 && x.pitch % 8 == 0 && y.pitch % 8 == 0));  // eight elements in one access
     ctx.note_launch("dropout");
     if (ctx.dry()) return SAGE_OK;
     return with_type(x.dtype, [&](auto t) {

@@ -28,9 +28,17 @@ template <class T>
 struct Eight {  // columns, as they are stored
     static constexpr int kPacks = 8 / Pack<T>::N;
     Pack<T> p[kPacks];
+    // f32: 32 bytes at once, from a 32-byte boundary (two halves of a sector asked for one after the other cost twice the requests)
     __device__ __forceinline__ void load(const char *from) {
-#pragma unroll
-        for (int i = 0; i < kPacks; ++i) p[i] = ((const Pack<T> *)from)[i];
+        if constexpr (sizeof(T) == 4) {
+            float *f = (float *)p;
+            asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7])
+                         : "l"(from)
+                         : "memory");
+        } else {
+            p[0] = *(const Pack<T> *)from;
+        }
     }
     // ... what nothing reads again
     __device__ __forceinline__ void load_once(const char *from) {
@@ -46,8 +54,12 @@ struct Eight {  // columns, as they are stored
         for (int i = 0; i < kPacks; ++i) *(uint4 *)&p[i] = make_uint4(0u, 0u, 0u, 0u);
     }
     __device__ __forceinline__ void store(char *to) const {
-#pragma unroll
-        for (int i = 0; i < kPacks; ++i) ((Pack<T> *)to)[i] = p[i];
+        if constexpr (sizeof(T) == 4) {
+            const float *f = (const float *)p;
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]) : "memory");
+        } else {
+            *(Pack<T> *)to = p[0];
+        }
     }
     __device__ __forceinline__ void open(float2 (&v)[4]) const {
 #pragma unroll

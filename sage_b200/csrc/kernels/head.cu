@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(256, 2) head_few_kernel(const T *hidden, long 
     Eight<T> *states = (Eight<T> *)smem;
     for (int i = (int)threadIdx.x; i < RB * runs; i += 256) {
         const int r = i / runs;
-        if (r < rows) states[i].load((const char *)(hidden + r * hidden_pitch + (i - r * runs) * 8));
+        if (r < rows) states[i].load_once((const char *)(hidden + r * hidden_pitch + (i - r * runs) * 8));
         else states[i].clear();
     }
     __syncthreads();
