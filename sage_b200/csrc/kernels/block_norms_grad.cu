@@ -477,7 +477,10 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
     const int tx = n.x_dtype, t = n.dtype, sx = tx == SAGE_F32 ? 4 : 2, st = t == SAGE_F32 ? 4 : 2;
     // Without a norm after the block or a gate its values are not read, and two kinds of sums are kept.
     const bool full = a.y.p && (a.after != SAGE_NORM_NONE || a.gate);
-    const int nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, 1, a.dim > 8 * kMaxThreads ? 2 : 1);
+    // Runs of eight columns to a thread.  Two where rows are long: what a row costs each thread is then shared by twice the columns, though two times five kinds of
+    // sums do not all fit its registers.  33.5 M elements bf16, one run | two, us: all five kinds, 768 columns 131 | 161, 1024 140 | 140, 1536 144 | 141, 2048
+    // 156 | 143, 4096 187 | 157; two kinds, 4096 columns 104 | 82.
+    const int least = a.dim > (full ? 1024 : 2048) ? 2 : 1, nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, least, least);
     const bool wide = a.dim % 8 == 0 && boundary(a.out, sx) && boundary(a.go, sx) && boundary(a.dx, sx) && boundary(a.y, st) && boundary(a.gh, st) && boundary(a.dy, st);
     size_t smem;
     const size_t bytes = (a.gh.p ? sx + st : 0) + (a.go.p ? sx : 0) + (full ? st : 0);

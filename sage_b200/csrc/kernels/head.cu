@@ -237,28 +237,34 @@ sage_status copy_rows(Context &ctx, const A *x, long long px, B *y, long long py
     return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? head_rows_copy_kernel<A, B, true> : head_rows_copy_kernel<A, B, false>, dim3((unsigned)blocks), dim3(256), 0, x, px, y, py, rows, cols, slices, slice), "head_rows_copy");
 }
 
-// Three bf16 pieces of each f32 element, eight to a thread.
-template <bool WIDE>
-__global__ void __launch_bounds__(256) head_pieces_kernel(const float *x, long long px, __nv_bfloat16 *y, long long py, long long plane, long long rows, int cols) {
+// Three bf16 pieces of each f32 element of up to two matrices, eight to a thread.
+struct ToPieces {
+    const float *x;
+    __nv_bfloat16 *y;
+    long long px, py, plane, groups;  // groups: of eight elements, rows of py / 8
+    int cols, wide;                   // wide: whole groups on 16-byte boundaries
+};
+__global__ void __launch_bounds__(256) head_pieces_kernel(const ToPieces a, const ToPieces b) {
     grid_dependency_sync();
-    const long long per = py / 8;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * per; i += gridDim.x * 256ll) {
-        const long long r = i / per, c = (i - r * per) * 8;
-        const float *from = x + r * px + c;
+    for (long long n = blockIdx.x * 256ll + threadIdx.x; n < a.groups + b.groups; n += gridDim.x * 256ll) {
+        const bool second = n >= a.groups;
+        const ToPieces &m = second ? b : a;
+        const long long i = second ? n - a.groups : n, per = m.py / 8, r = m.groups <= 0x7fffffffll ? (int)i / (int)per : i / per, c = (i - r * per) * 8;
+        const float *from = m.x + r * m.px + c;
         float v[8];
-        if (WIDE) {
-            const float4 a = *(const float4 *)from, b = *((const float4 *)from + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        if (m.wide) {
+            const float4 p = *(const float4 *)from, q = *((const float4 *)from + 1);
+            v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w, v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? from[e] : 0.f;
+            for (int e = 0; e < 8; ++e) v[e] = c + e < m.cols ? from[e] : 0.f;
         }
 #pragma unroll
-        for (int n = 0; n < 3; ++n) {
+        for (int k = 0; k < 3; ++k) {
             unsigned w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] = take_piece(v[2 * e], v[2 * e + 1]);
-            *(uint4 *)(y + n * plane + r * py + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            *(uint4 *)(m.y + k * m.plane + r * m.py + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 }
@@ -573,21 +579,24 @@ sage_status grad16(Context &ctx, const Head &a, const RowsArg &stats, const Vect
 // ------------------------------------------------------------------------------------------ f32
 typedef __nv_bfloat16 Piece;
 
-// The operand's pieces, in planes of their own.
-sage_status pieces_of(Context &ctx, Scratch &scratch, const RowsArg &r, Matrix *m) {
-    Piece *to = nullptr;
-    *m = Matrix{nullptr, r.rows, r.cols, (r.cols + 7) / 8 * 8, 0};
-    m->plane = r.rows * m->pitch;
-    sage_status st = scratch.get((size_t)(3 * m->plane) * 2, &to);
+// The pieces of one or two operands, in planes of their own.
+sage_status pieces_of(Context &ctx, Scratch &scratch, const RowsArg &r, Matrix *m, const RowsArg &r2 = RowsArg{}, Matrix *m2 = nullptr) {
+    ToPieces to[2] = {};
+    sage_status st = SAGE_OK;
+    const RowsArg *of[2] = {&r, &r2};
+    Matrix *into[2] = {m, m2};
+    for (int i = 0; i < 2 && into[i] && !st; ++i) {
+        const RowsArg &x = *of[i];
+        const long long pitch = (x.cols + 7) / 8 * 8, px = x.rows > 1 ? x.pitch : x.cols;
+        st = scratch.get((size_t)(3 * x.rows * pitch) * 2, &to[i].y);
+        *into[i] = Matrix{to[i].y, x.rows, x.cols, pitch, x.rows * pitch};
+        to[i] = ToPieces{(const float *)x.ptr, to[i].y, px, pitch, x.rows * pitch, x.rows * (pitch / 8), (int)x.cols, x.cols % 8 == 0 && on_16(x.ptr, px, 4)};
+    }
     if (st) return st;
-    m->p = to;
     ctx.note_launch("head_pieces");
     if (ctx.dry()) return SAGE_OK;
-    const long long pitch = r.rows > 1 ? r.pitch : r.cols, blocks = std::min<long long>((r.rows * (m->pitch / 8) + 255) / 256, ctx.sm_count * 16ll);
-    const bool wide = r.cols % 8 == 0 && on_16(r.ptr, pitch, 4);
-    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), wide ? head_pieces_kernel<true> : head_pieces_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, (const float *)r.ptr, pitch, to, m->pitch, m->plane,
-                                           r.rows, (int)r.cols),
-                          "head_pieces");
+    const long long blocks = std::min<long long>((to[0].groups + to[1].groups + 255) / 256, ctx.sm_count * 16ll);
+    return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), head_pieces_kernel, dim3((unsigned)blocks), dim3(256), 0, to[0], to[1]), "head_pieces");
 }
 
 sage_status forward32(Context &ctx, const Head &a, const VectorArg &log_probs, const VectorArg &entropy, const RowsArg &stats) {
@@ -596,7 +605,7 @@ sage_status forward32(Context &ctx, const Head &a, const VectorArg &log_probs, c
     Product p = shape_of(ctx, rows, vocab, width);
     const long long parts_of_row = 2ll * p.tiles_n, most = std::max<long long>(256, (long long)(kPartBytes / (16 * parts_of_row)) / 256 * 256);  // rows at a time
     Matrix x, w;
-    sage_status st = pieces_of(ctx, scratch, a.weight, &w);
+    sage_status st = rows <= most ? pieces_of(ctx, scratch, a.weight, &w, a.hidden, &x) : pieces_of(ctx, scratch, a.weight, &w);
     if (!st) st = scratch.get((size_t)(std::min(rows, most) * parts_of_row) * 16, &p.parts);
     if (!st) st = scratch.get((size_t)std::min(rows, most) * 4, &p.asked);
     p.c2 = a.scale * kLog2E;
@@ -605,7 +614,7 @@ sage_status forward32(Context &ctx, const Head &a, const VectorArg &log_probs, c
         const long long count = std::min(most, rows - at);
         const VectorArg ids = cut(a.ids, at), lp = cut(log_probs, at), h = cut(entropy, at);
         const RowsArg s = cut(stats, at, count);
-        st = pieces_of(ctx, scratch, cut(a.hidden, at, count), &x);
+        if (rows > most) st = pieces_of(ctx, scratch, cut(a.hidden, at, count), &x);
         p.m = (int)count;
         p.tiles_m = (int)((count + 255) / 256);
         p.band = (int)std::max<long long>(8, ((long long)48 << 20) / (256 * width * 6));
@@ -626,8 +635,7 @@ sage_status grad32(Context &ctx, const Head &a, const RowsArg &stats, const Vect
     unsigned *gmax;
     Piece *probs = nullptr;
     Matrix x, w;
-    sage_status st = pieces_of(ctx, scratch, a.hidden, &x);
-    if (!st) st = pieces_of(ctx, scratch, a.weight, &w);
+    sage_status st = pieces_of(ctx, scratch, a.hidden, &x, a.weight, &w);
     if (!st) st = rows_about(ctx, scratch, a, stats, entropy, gl, ge, false, &about, &gls, &gmax);
     if (!st) st = scratch.get((size_t)(3 * padded * pitch) * 2, &probs);
     Result to_hidden;
