@@ -6,6 +6,8 @@
 // Bound by memory, with as many operations beside it as the instruction slots hold: sums over rows take eight registers for each run of columns and kind, of
 // which programs without a norm after the block and without a gate (FULL false) have two.  They are joined in a fixed order: team by team within a
 // CTA, then CTA by CTA in a second launch.
+#include <type_traits>
+
 #include "block_norms.h"
 
 namespace sage {
@@ -15,12 +17,31 @@ namespace {
 
 constexpr int kRegisters = 112;  // of a thread of the general form
 
+// Which sums over rows a kernel keeps, and where.
+template <bool FULL, int BIASES, bool GATE>  // BIASES: 1 the one before, 2 both
+struct Kinds {
+    __host__ __device__ constexpr int at(int kind) const {
+        const bool there[kSums] = {true, BIASES >= 1, FULL, FULL && BIASES == 2, FULL && GATE};
+        if (!there[kind]) return -1;
+        int n = 0;
+        for (int k = 0; k < kind; ++k) n += there[k] ? 1 : 0;
+        return n;
+    }
+    __host__ __device__ constexpr int count() const {
+        int n = 0;
+        for (int k = 0; k < kSums; ++k) n += at(k) >= 0 ? 1 : 0;
+        return n;
+    }
+};
+
 // The teams' sums of a CTA, team by team, through shared memory (a kind at a time: dim floats).
-template <int KINDS, int NV>
-__device__ __forceinline__ void join_teams(const NormsArgs &a, const Place &at, float2 (&sum)[KINDS][NV][4], const int (&count)[NV], bool wide, float *shared) {
+template <class KINDS, int KEPT, int NV>
+__device__ __forceinline__ void join_teams(const NormsArgs &a, const Place &at, float2 (&sum)[KEPT][NV][4], const int (&count)[NV], bool wide, float *shared) {
 #pragma unroll
-    for (int s = 0; s < KINDS; ++s) {
-        if (!(a.sums >> s & 1)) continue;
+    for (int kind = 0; kind < kSums; ++kind) {
+        constexpr KINDS kept{};
+        if (kept.at(kind) < 0 || !(a.sums >> kind & 1)) continue;
+        const int s = kept.at(kind) < 0 ? 0 : kept.at(kind);
         for (int t = 0; t < a.teams; ++t) {
             if (a.teams > 1) __syncthreads();
             if (t != at.team.index) continue;
@@ -36,7 +57,7 @@ __device__ __forceinline__ void join_teams(const NormsArgs &a, const Place &at, 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = add2(x[i], y[i]);
                 }
-                store8(t + 1 == a.teams ? a.partial + ((long long)blockIdx.x * kSums + s) * a.dim + col : shared + col, count[v], wide, x);
+                store8(t + 1 == a.teams ? a.partial + ((long long)blockIdx.x * kSums + kind) * a.dim + col : shared + col, count[v], wide, x);
             }
         }
     }
@@ -46,7 +67,7 @@ __host__ __device__ constexpr int ring_registers(int nv, bool full) { return ful
 
 // What models call: both gradients arrive, there is a norm before the next block and norms have weights; whole runs of columns on
 // 32-byte (16 bits: 16-byte) boundaries.
-template <class TX, class T, int NV, bool FULL, bool BIAS>
+template <class TX, class T, int NV, bool FULL, int BIASES, bool GATE>
 __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kernel(const NormsArgs a) {
     extern __shared__ __align__(16) char ring[];
     __shared__ __align__(16) float2 slots[kSlots];
@@ -77,7 +98,8 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
     }
     const float per = 1.f / (float)a.dim;
     const float2 zero = make_float2(0.f, 0.f);
-    constexpr int kKept = FULL ? (int)kSums : 2;
+    constexpr Kinds<FULL, BIASES, GATE> kept{};
+    constexpr int kKept = kept.count(), kWb = 0, kBb = BIASES >= 1 ? kept.at(kSumBb) : 0, kWa = FULL ? kept.at(kSumWa) : 0, kBa = FULL && BIASES == 2 ? kept.at(kSumBa) : 0, kGate = FULL && GATE ? kept.at(kSumGate) : 0;
     float2 sum[kKept][NV][4];
 #pragma unroll
     for (int s = 0; s < kKept; ++s)
@@ -130,8 +152,8 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         u[i] = fma2(u[i], both(rstd_b), both(from_b));
-                        sum[kSumWb][v][i] = fma2(q[v][i], u[i], sum[kSumWb][v][i]);
-                        sum[kSumBb][v][i] = add2(sum[kSumBb][v][i], q[v][i]);
+                        sum[kWb][v][i] = fma2(q[v][i], u[i], sum[kWb][v][i]);
+                        if (BIASES >= 1) sum[kBb][v][i] = add2(sum[kBb][v][i], q[v][i]);
                         q[v][i] = mul2(q[v][i], w[i]);
                         along = fma2(q[v][i], u[i], along);
                         all = add2(all, q[v][i]);
@@ -177,7 +199,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
 #pragma unroll
                             for (int i = 0; i < 4; ++i) n[i] = make_float2(G[i].x == 0.f ? 0.f : n[i].x, G[i].y == 0.f ? 0.f : n[i].y);
                     }
-                    if (a.gate) {
+                    if (GATE) {
                         float2 by[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) by[i] = mul2(n[i], w[i]);
@@ -189,14 +211,13 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
                         get8(a.gate + (long long)group * a.gate_pitch + at_col, b);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            sum[kKept - 1][v][i] = fma2(G[i], by[i], sum[kKept - 1][v][i]);
+                            sum[kGate][v][i] = fma2(G[i], by[i], sum[kGate][v][i]);
                             G[i] = mul2(G[i], b[i]);
                         }
                     }
-                    constexpr int kWa = FULL ? (int)kSumWa : 0, kBa = FULL ? (int)kSumBa : 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (BIAS) sum[kBa][v][i] = add2(sum[kBa][v][i], G[i]);
+                        if (BIASES == 2) sum[kBa][v][i] = add2(sum[kBa][v][i], G[i]);
                         sum[kWa][v][i] = fma2(G[i], n[i], sum[kWa][v][i]);
                         q[v][i] = mul2(G[i], w[i]);
                         along_t = fma2(q[v][i], n[i], along_t);
@@ -222,13 +243,13 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
             }
             take = take + stage == ring1 ? ring0 : take + stage;
         }
-        if (FULL && a.gate_partial) {
+        if (FULL && GATE && a.gate_partial) {
             float *to = a.gate_partial + (long long)share * a.dim + col;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                if (v + 1 < NV || last) store8(to + v * run, 8, true, sum[kKept - 1][v]);
+                if (v + 1 < NV || last) store8(to + v * run, 8, true, sum[kGate][v]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[kKept - 1][v][i] = zero;
+                for (int i = 0; i < 4; ++i) sum[kGate][v][i] = zero;
             }
         }
     }
@@ -237,7 +258,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
     int count[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) count[v] = v + 1 < NV || last ? 8 : 0;
-    join_teams(a, at, sum, count, true, (float *)ring);
+    join_teams<Kinds<FULL, BIASES, GATE>>(a, at, sum, count, true, (float *)ring);
 }
 
 // Any layout: rows are read where they are used, as vectors if `wide`.
@@ -393,7 +414,7 @@ __global__ void __maxnreg__(kRegisters) block_norms_grad_kernel(const NormsArgs 
         now.next();
     }
     if (!a.partial) return;
-    join_teams(a, at, sum, count, wide, (float *)ring);
+    join_teams<Kinds<FULL, FULL ? 2 : 1, true>>(a, at, sum, count, wide, (float *)ring);
 }
 
 // The sums that CTAs, and shares of a group's rows, left: y[j] = the sum over i of x[i * pitch + j], in a fixed order: warp by warp every 32nd, then
@@ -477,10 +498,11 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
     const int tx = n.x_dtype, t = n.dtype, sx = tx == SAGE_F32 ? 4 : 2, st = t == SAGE_F32 ? 4 : 2;
     // Without a norm after the block or a gate its values are not read, and two kinds of sums are kept.
     const bool full = a.y.p && (a.after != SAGE_NORM_NONE || a.gate);
-    // Runs of eight columns to a thread.  Two where rows are long: what a row costs each thread is then shared by twice the columns, though two times five kinds of
-    // sums do not all fit its registers.  33.5 M elements bf16, one run | two, us: all five kinds, 768 columns 131 | 161, 1024 140 | 140, 1536 144 | 141, 2048
-    // 156 | 143, 4096 187 | 157; two kinds, 4096 columns 104 | 82.
-    const int least = a.dim > (full ? 1024 : 2048) ? 2 : 1, nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, least, least);
+    // Runs of eight columns to a thread.  Two where rows are long: what a row costs each thread is then shared by twice the columns; four kinds of sums of
+    // two runs fit its registers, five do not.  33.5 M elements bf16, one run | two, us: five kinds, 768 columns 131 | 161, 1024 140 | 140, 1536 144 | 147, 2048
+    // 156 | 152, 4096 187 | 166; two norms alone, 2048 columns 127 | 95, 4096 151 | 101; a norm before alone, 4096 columns 104 | 89.
+    const bool many = full && a.gate && to[kSumBb];
+    const int least = a.dim > (many ? 1536 : full ? 1024 : 2048) ? 2 : 1, most = least == 2 || (full && !many) ? 2 : 1, nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, least, most);
     const bool wide = a.dim % 8 == 0 && boundary(a.out, sx) && boundary(a.go, sx) && boundary(a.dx, sx) && boundary(a.y, st) && boundary(a.gh, st) && boundary(a.dy, st);
     size_t smem;
     const size_t bytes = (a.gh.p ? sx + st : 0) + (a.go.p ? sx : 0) + (full ? st : 0);
@@ -534,9 +556,16 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
             };
             const auto any = [&](auto kernel) { return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3((unsigned)grid), dim3((unsigned)threads), smem, a, wide, weights_wide(a)), "block_norms_grad"); };
             if (ring) {
-                if (full && to[kSumBa]) return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, true, true>) : by_ring(block_norms_grad_ring_kernel<TX, T, 2, true, true>);
-                if (full) return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, true, false>) : by_ring(block_norms_grad_ring_kernel<TX, T, 2, true, false>);
-                return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, false, false>) : nv == 2 ? by_ring(block_norms_grad_ring_kernel<TX, T, 2, false, false>) : by_ring(block_norms_grad_ring_kernel<TX, T, 4, false, false>);
+                const auto of_full = [&](auto biases, auto gate) {
+                    constexpr int B = decltype(biases)::value;
+                    constexpr bool G = decltype(gate)::value;
+                    return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, true, B, G>) : by_ring(block_norms_grad_ring_kernel<TX, T, 2, true, B, G>);
+                };
+                const auto of_biases = [&](auto gate) {
+                    return to[kSumBa] ? of_full(std::integral_constant<int, 2>(), gate) : to[kSumBb] ? of_full(std::integral_constant<int, 1>(), gate) : of_full(std::integral_constant<int, 0>(), gate);
+                };
+                if (full) return a.gate ? of_biases(std::true_type()) : of_biases(std::false_type());
+                return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, false, 1, false>) : nv == 2 ? by_ring(block_norms_grad_ring_kernel<TX, T, 2, false, 1, false>) : by_ring(block_norms_grad_ring_kernel<TX, T, 4, false, 1, false>);
             }
             if (full) return nv == 1 ? any(block_norms_grad_kernel<TX, T, 1, true>) : nv == 2 ? any(block_norms_grad_kernel<TX, T, 2, true>) : any(block_norms_grad_kernel<TX, T, 4, true>);
             return nv == 1   ? any(block_norms_grad_kernel<TX, T, 1, false>)
