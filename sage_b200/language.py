@@ -1,10 +1,11 @@
-"""Operators at the two ends of a language model and of its training step, on device tensors (include/sage_cuda.h, "language
-models"): token embedding and its gradient, log probabilities of given tokens with entropy, alternatives and gradient, AdamW
-over many tensors.
+"""Operators of a language model's training step beside its products and attention, on device tensors (include/sage_cuda.h, "language
+models"): token embedding and its gradient, log probabilities of given tokens with entropy, alternatives and gradient, the same from
+hidden states, dropout, the norms around a block with gate and residual scale and their gradient, AdamW over many tensors.
 
 Every operand is a DeviceTensor of one context: `Context.tensor` / `Context.empty`, or `Context.borrow` of another package's
 memory.  Results go into tensors that the caller gives; calls enqueue work on the context's stream and return.  The lazy-graph
-forms of the same operators are `sage_b200.embedding`, `token_log_probs`, `top_tokens` and `AdamW`.
+forms of the same operators are `sage_b200.embedding`, `token_log_probs`, `top_tokens`, `head_log_probs`, `dropout`, `block_norms`
+and `AdamW`.
 """
 import ctypes
 
