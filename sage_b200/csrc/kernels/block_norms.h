@@ -1,9 +1,10 @@
 // What the norms around a block (block_norms.cu) and their gradient (block_norms_grad.cu) have in common: teams of threads that go through rows.
 //
 // A thread owns NV runs of eight neighbouring columns and a team of threads a row, so that the sums over rows stay in registers, a sum over a row is
-// one shuffle tree and, in teams of several warps, one exchange in shared memory, and a block of dropout's mask is one draw.  Teams go through rows in
-// steps of their number; what a thread reads of its team's next rows is copied into places of its own in shared memory while the present row
-// is worked on (no barrier: only the thread that asked reads them).  Arithmetic is on pairs of columns, two f32 operations an instruction.
+// one shuffle tree and, in teams of several warps, one exchange in shared memory, and a block of dropout's mask is one draw.  Forward, a team takes one
+// row; in the gradient teams go through rows in steps of their number, and what a thread reads of its team's next rows is copied into places of its own in
+// shared memory while the present row is worked on (no barrier: only the thread that asked reads them).  Arithmetic is on pairs of columns, two f32
+// operations an instruction.
 #pragma once
 #include <algorithm>
 

@@ -37,7 +37,7 @@ __device__ __forceinline__ uint4 philox(Key k, unsigned long long count, unsigne
 }
 
 // ... with the rounds' keys made once (a block of threads keeps them in shared memory: five loads instead of twenty additions).
-struct RoundKeys {
+struct alignas(16) RoundKeys {  // (two rounds' are read at a time)
     uint2 k[10];
 };
 __device__ __forceinline__ void round_keys(RoundKeys *to, Key k, int thread) {
