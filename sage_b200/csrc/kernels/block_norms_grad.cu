@@ -146,85 +146,85 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
             float2 q[NV][4], along = zero, all = zero;  // what arrives through the norm
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                    float2 u[4], w[4];
-                    ring_get<TX>(take, v, piece, u);
-                    ring_get<T>(take + kGh * piece, v, piece, q[v]);
-                    get8(a.wb + (v + 1 < NV ? col + v * run : wcol), w);
+                float2 u[4], w[4];
+                ring_get<TX>(take, v, piece, u);
+                ring_get<T>(take + kGh * piece, v, piece, q[v]);
+                get8(a.wb + (v + 1 < NV ? col + v * run : wcol), w);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        u[i] = fma2(u[i], both(rstd_b), both(from_b));
-                        sum[kWb][v][i] = fma2(q[v][i], u[i], sum[kWb][v][i]);
-                        if (BIASES >= 1) sum[kBb][v][i] = add2(sum[kBb][v][i], q[v][i]);
-                        q[v][i] = mul2(q[v][i], w[i]);
-                        along = fma2(q[v][i], u[i], along);
-                        all = add2(all, q[v][i]);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    u[i] = fma2(u[i], both(rstd_b), both(from_b));
+                    sum[kWb][v][i] = fma2(q[v][i], u[i], sum[kWb][v][i]);
+                    if (BIASES >= 1) sum[kBb][v][i] = add2(sum[kBb][v][i], q[v][i]);
+                    q[v][i] = mul2(q[v][i], w[i]);
+                    along = fma2(q[v][i], u[i], along);
+                    all = add2(all, q[v][i]);
                 }
+            }
             const float2 s1 = team.sum(make_float2(along.x + along.y, all.x + all.y));
             const float along_u = s1.x * per, mean_q = a.before == SAGE_NORM_LAYER ? s1.y * per : 0.f;
             float2 along_t = zero, all_t = zero;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                    const bool there = v + 1 < NV || last;
-                    const int at_col = v + 1 < NV ? col + v * run : wcol;
-                    const float through = there ? rstd_b : 0.f;
-                    float2 G[4], u[4];
-                    ring_get<TX>(take + kGo * piece, v, piece, G);
-                    ring_get<TX>(take, v, piece, u);
+                const bool there = v + 1 < NV || last;
+                const int at_col = v + 1 < NV ? col + v * run : wcol;
+                const float through = there ? rstd_b : 0.f;
+                float2 G[4], u[4];
+                ring_get<TX>(take + kGo * piece, v, piece, G);
+                ring_get<TX>(take, v, piece, u);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    u[i] = fma2(u[i], both(rstd_b), both(from_b));
+                    G[i] = fma2(fma2(u[i], both(-along_u), add2(q[v][i], both(-mean_q))), both(through), G[i]);
+                    u[i] = mul2(G[i], both(a.scale));
+                }
+                if (a.dx.p && there) put8<TX>((char *)a.dx.p + x_at + (unsigned)(v * run * (int)sizeof(TX)), u);
+                if (a.d.bar) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) G[i] = mul2(G[i], both(a.d.factor));
+                    drop8(G, philox(keys, ((unsigned long long)(unsigned)row * (unsigned)a.dim + at_col) >> 3, a.d.site), a.d.bar);
+                }
+                if (!FULL) {
+                    if (a.dy.p && there) put8<T>((char *)a.dy.p + t_at + (unsigned)(v * run * (int)sizeof(T)), G);
+                    continue;
+                }
+                float2 n[4], w[4], b[4];
+                ring_get<T>(take + kY * piece, v, piece, n);
+                if (a.after != SAGE_NORM_NONE) {
+                    get8(a.wa + at_col, w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) n[i] = fma2(n[i], both(rstd_a), both(from_a));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = both(1.f);
+                    if (a.d.bar)  // a value that is dropped may be anything (a norm would have spread it)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) n[i] = make_float2(G[i].x == 0.f ? 0.f : n[i].x, G[i].y == 0.f ? 0.f : n[i].y);
+                }
+                if (GATE) {
+                    float2 by[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) by[i] = mul2(n[i], w[i]);
+                    if (a.ba) {
+                        get8(a.ba + at_col, b);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) by[i] = add2(by[i], b[i]);
+                    }
+                    get8(a.gate + (long long)group * a.gate_pitch + at_col, b);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        u[i] = fma2(u[i], both(rstd_b), both(from_b));
-                        G[i] = fma2(fma2(u[i], both(-along_u), add2(q[v][i], both(-mean_q))), both(through), G[i]);
-                        u[i] = mul2(G[i], both(a.scale));
-                    }
-                    if (a.dx.p && there) put8<TX>((char *)a.dx.p + x_at + (unsigned)(v * run * (int)sizeof(TX)), u);
-                    if (a.d.bar) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) G[i] = mul2(G[i], both(a.d.factor));
-                        drop8(G, philox(keys, ((unsigned long long)(unsigned)row * (unsigned)a.dim + at_col) >> 3, a.d.site), a.d.bar);
-                    }
-                    if (!FULL) {
-                        if (a.dy.p && there) put8<T>((char *)a.dy.p + t_at + (unsigned)(v * run * (int)sizeof(T)), G);
-                        continue;
-                    }
-                    float2 n[4], w[4], b[4];
-                    ring_get<T>(take + kY * piece, v, piece, n);
-                    if (a.after != SAGE_NORM_NONE) {
-                        get8(a.wa + at_col, w);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) n[i] = fma2(n[i], both(rstd_a), both(from_a));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = both(1.f);
-                        if (a.d.bar)  // a value that is dropped may be anything (a norm would have spread it)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) n[i] = make_float2(G[i].x == 0.f ? 0.f : n[i].x, G[i].y == 0.f ? 0.f : n[i].y);
-                    }
-                    if (GATE) {
-                        float2 by[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) by[i] = mul2(n[i], w[i]);
-                        if (a.ba) {
-                            get8(a.ba + at_col, b);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) by[i] = add2(by[i], b[i]);
-                        }
-                        get8(a.gate + (long long)group * a.gate_pitch + at_col, b);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            sum[kGate][v][i] = fma2(G[i], by[i], sum[kGate][v][i]);
-                            G[i] = mul2(G[i], b[i]);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (BIASES == 2) sum[kBa][v][i] = add2(sum[kBa][v][i], G[i]);
-                        sum[kWa][v][i] = fma2(G[i], n[i], sum[kWa][v][i]);
-                        q[v][i] = mul2(G[i], w[i]);
-                        along_t = fma2(q[v][i], n[i], along_t);
-                        all_t = add2(all_t, q[v][i]);
+                        sum[kGate][v][i] = fma2(G[i], by[i], sum[kGate][v][i]);
+                        G[i] = mul2(G[i], b[i]);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (BIASES == 2) sum[kBa][v][i] = add2(sum[kBa][v][i], G[i]);
+                    sum[kWa][v][i] = fma2(G[i], n[i], sum[kWa][v][i]);
+                    q[v][i] = mul2(G[i], w[i]);
+                    along_t = fma2(q[v][i], n[i], along_t);
+                    all_t = add2(all_t, q[v][i]);
+                }
+            }
             if (FULL && a.dy.p) {
                 float2 s2 = zero;
                 if (a.after != SAGE_NORM_NONE) s2 = team.sum(make_float2(along_t.x + along_t.y, all_t.x + all_t.y));

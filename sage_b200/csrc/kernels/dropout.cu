@@ -76,7 +76,7 @@ sage_status dropout(Context &ctx, const RowsArg &x, const RowsArg &y, const Drop
     DropoutArgs a{x.ptr, y.ptr, x.rows * x.cols, x.cols, x.pitch, y.pitch, d};
     if (x.rows == 1 || (x.pitch == x.cols && y.pitch == x.cols)) a.cols = a.n;
     const long long size = x.dtype == SAGE_F32 ? 4 : 2, blocks = (a.n + 8 * kThreads * kBlocks - 1) / (8 * kThreads * kBlocks);
-    if (blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "dropout: more than 2^44 elements");
+    if (blocks > 0x7fffffffll) return ctx.fail(SAGE_ERR_INVALID, "dropout: more than 2^43 elements");
     const bool one = a.cols == a.n;
     const bool wide = (uintptr_t)x.ptr % (8 * size) == 0 && (uintptr_t)y.ptr % (8 * size) == 0 && (one || (a.cols % 8 == 0 && x.pitch % 8 == 0 && y.pitch % 8 == 0));  // eight elements in one access
     ctx.note_launch("dropout");

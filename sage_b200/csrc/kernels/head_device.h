@@ -384,8 +384,8 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 }
                 if (!live) break;
                 if constexpr (END == kStats) {
-                const float4 found = stats_of(p, acc, half / 32, col0, id, row);
-                if (there) p.parts[(long long)(tile.n0 / half + side) * p.m + row] = found;
+                    const float4 found = stats_of(p, acc, half / 32, col0, id, row);
+                    if (there) p.parts[(long long)(tile.n0 / half + side) * p.m + row] = found;
                 } else {
                     float4 about = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (END == kProbs && there) {
