@@ -18,11 +18,14 @@ namespace {
 
 constexpr int kRegisters = 112;  // of a thread of the general form
 
+// Gates: none; one row of them for all rows that a team goes through, which then multiplies sums instead of rows (with P = sum of K v, Q = sum of K the gate's sum
+// is wa P + ba Q, the weight's gate P, the bias's gate Q); rows of their own for each group of rows.
+enum { kUngated, kGateOnce, kGateEach };
 // Which sums over rows a kernel keeps, and where.
-template <bool FULL, int BIASES, bool GATE>  // BIASES: 1 the one before, 2 both
+template <bool FULL, int BIASES, int GATE>  // BIASES: 1 the one before, 2 both
 struct Kinds {
     __host__ __device__ constexpr int at(int kind) const {
-        const bool there[kSums] = {true, BIASES >= 1, FULL, FULL && BIASES == 2, FULL && GATE};
+        const bool there[kSums] = {true, BIASES >= 1, FULL, FULL && BIASES == 2, FULL && GATE != kUngated};
         if (!there[kind]) return -1;
         int n = 0;
         for (int k = 0; k < kind; ++k) n += there[k] ? 1 : 0;
@@ -68,7 +71,7 @@ __host__ __device__ constexpr int ring_registers(int nv, bool full) { return ful
 
 // What models call: both gradients arrive, there is a norm before the next block and norms have weights; whole runs of columns on
 // 32-byte (16 bits: 16-byte) boundaries.
-template <class TX, class T, int NV, bool FULL, int BIASES, bool GATE>
+template <class TX, class T, int NV, bool FULL, int BIASES, int GATE>
 __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kernel(const NormsArgs a) {
     extern __shared__ __align__(16) char ring[];
     __shared__ __align__(16) float2 slots[kSlots];
@@ -100,7 +103,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
     const float per = 1.f / (float)a.dim;
     const float2 zero = make_float2(0.f, 0.f);
     constexpr Kinds<FULL, BIASES, GATE> kept{};
-    constexpr int kKept = kept.count(), kWb = 0, kBb = BIASES >= 1 ? kept.at(kSumBb) : 0, kWa = FULL ? kept.at(kSumWa) : 0, kBa = FULL && BIASES == 2 ? kept.at(kSumBa) : 0, kGate = FULL && GATE ? kept.at(kSumGate) : 0;
+    constexpr int kKept = kept.count(), kWb = 0, kBb = BIASES >= 1 ? kept.at(kSumBb) : 0, kWa = FULL ? kept.at(kSumWa) : 0, kBa = FULL && BIASES == 2 ? kept.at(kSumBa) : 0, kGate = FULL && GATE != kUngated ? kept.at(kSumGate) : 0;
     float2 sum[kKept][NV][4];
 #pragma unroll
     for (int s = 0; s < kKept; ++s)
@@ -200,7 +203,7 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
 #pragma unroll
                         for (int i = 0; i < 4; ++i) n[i] = make_float2(G[i].x == 0.f ? 0.f : n[i].x, G[i].y == 0.f ? 0.f : n[i].y);
                 }
-                if (GATE) {
+                if (GATE == kGateEach) {
                     float2 by[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) by[i] = mul2(n[i], w[i]);
@@ -216,10 +219,12 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
                         G[i] = mul2(G[i], b[i]);
                     }
                 }
+                if (GATE == kGateOnce) get8(a.gate + (long long)group * a.gate_pitch + at_col, b);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (BIASES == 2) sum[kBa][v][i] = add2(sum[kBa][v][i], G[i]);
                     sum[kWa][v][i] = fma2(G[i], n[i], sum[kWa][v][i]);
+                    if (GATE == kGateOnce) G[i] = mul2(G[i], b[i]);
                     q[v][i] = mul2(G[i], w[i]);
                     along_t = fma2(q[v][i], n[i], along_t);
                     all_t = add2(all_t, q[v][i]);
@@ -244,7 +249,30 @@ __global__ void __maxnreg__(ring_registers(NV, FULL)) block_norms_grad_ring_kern
             }
             take = take + stage == ring1 ? ring0 : take + stage;
         }
-        if (FULL && GATE && a.gate_partial) {
+        if (FULL && GATE == kGateOnce) {  // the team's only share
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int at_col = v + 1 < NV ? col + v * run : wcol;
+                float2 f[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = both(1.f);
+                if (a.after != SAGE_NORM_NONE) get8(a.wa + at_col, f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[kGate][v][i] = mul2(sum[kWa][v][i], f[i]);
+                if (BIASES == 2 && a.ba) {
+                    get8(a.ba + at_col, f);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[kGate][v][i] = fma2(sum[kBa][v][i], f[i], sum[kGate][v][i]);
+                }
+                get8(a.gate + (long long)group * a.gate_pitch + at_col, f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sum[kWa][v][i] = mul2(sum[kWa][v][i], f[i]);
+                    if (BIASES == 2) sum[kBa][v][i] = mul2(sum[kBa][v][i], f[i]);
+                }
+            }
+        }
+        if (FULL && GATE != kUngated && a.gate_partial) {
             float *to = a.gate_partial + (long long)share * a.dim + col;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
@@ -415,7 +443,7 @@ __global__ void __maxnreg__(kRegisters) block_norms_grad_kernel(const NormsArgs 
         now.next();
     }
     if (!a.partial) return;
-    join_teams<Kinds<FULL, FULL ? 2 : 1, true>>(a, at, sum, count, wide, (float *)ring);
+    join_teams<Kinds<FULL, FULL ? 2 : 1, kGateEach>>(a, at, sum, count, wide, (float *)ring);
 }
 
 // The sums that CTAs, and shares of a group's rows, left: y[j] = the sum over i of x[i * pitch + j], in a fixed order: warp by warp every 32nd, then
@@ -558,15 +586,16 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
             const auto any = [&](auto kernel) { return ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3((unsigned)grid), dim3((unsigned)threads), smem, a, wide, weights_wide(a)), "block_norms_grad"); };
             if (ring) {
                 const auto of_full = [&](auto biases, auto gate) {
-                    constexpr int B = decltype(biases)::value;
-                    constexpr bool G = decltype(gate)::value;
+                    constexpr int B = decltype(biases)::value, G = decltype(gate)::value;
                     return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, true, B, G>) : by_ring(block_norms_grad_ring_kernel<TX, T, 2, true, B, G>);
                 };
                 const auto of_biases = [&](auto gate) {
-                    return to[kSumBa] ? of_full(std::integral_constant<int, 2>(), gate) : to[kSumBb] ? of_full(std::integral_constant<int, 1>(), gate) : of_full(std::integral_constant<int, 0>(), gate);
+                    const bool both = to[kSumBa] || (a.ba && decltype(gate)::value == kGateOnce);
+                    return both ? of_full(std::integral_constant<int, 2>(), gate) : to[kSumBb] ? of_full(std::integral_constant<int, 1>(), gate) : of_full(std::integral_constant<int, 0>(), gate);
                 };
-                if (full) return a.gate ? of_biases(std::true_type()) : of_biases(std::false_type());
-                return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, false, 1, false>) : nv == 2 ? by_ring(block_norms_grad_ring_kernel<TX, T, 2, false, 1, false>) : by_ring(block_norms_grad_ring_kernel<TX, T, 4, false, 1, false>);
+                if (full && !a.gate) return of_biases(std::integral_constant<int, kUngated>());
+                if (full) return groups * a.splits <= (long long)grid * a.teams ? of_biases(std::integral_constant<int, kGateOnce>()) : of_biases(std::integral_constant<int, kGateEach>());
+                return nv == 1 ? by_ring(block_norms_grad_ring_kernel<TX, T, 1, false, 1, kUngated>) : nv == 2 ? by_ring(block_norms_grad_ring_kernel<TX, T, 2, false, 1, kUngated>) : by_ring(block_norms_grad_ring_kernel<TX, T, 4, false, 1, kUngated>);
             }
             if (full) return nv == 1 ? any(block_norms_grad_kernel<TX, T, 1, true>) : nv == 2 ? any(block_norms_grad_kernel<TX, T, 2, true>) : any(block_norms_grad_kernel<TX, T, 4, true>);
             return nv == 1   ? any(block_norms_grad_kernel<TX, T, 1, false>)
