@@ -530,7 +530,7 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
     // Runs of eight columns to a thread.  Two where rows are long: what a row costs each thread is then shared by twice the columns; four kinds of sums of
     // two runs fit its registers, five do not.  33.5 M elements bf16, one run | two, us: five kinds, 768 columns 131 | 161, 1024 140 | 140, 1536 144 | 147, 2048
     // 156 | 152, 4096 187 | 166; two norms alone, 2048 columns 127 | 95, 4096 151 | 101; a norm before alone, 4096 columns 104 | 89.
-    const bool many = full && a.gate && to[kSumBb];
+    const bool many = full && a.gate && to[kSumBb] && groups > ctx.sm_count;
     const int least = a.dim > (many ? 1536 : full ? 1024 : 2048) ? 2 : 1, most = least == 2 || (full && !many) ? 2 : 1, nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, least, most);
     const bool wide = a.dim % 8 == 0 && boundary(a.out, sx) && boundary(a.go, sx) && boundary(a.dx, sx) && boundary(a.y, st) && boundary(a.gh, st) && boundary(a.dy, st);
     size_t smem;
