@@ -5,7 +5,8 @@
 //
 // Bound by memory, with as many operations beside it as the instruction slots hold: sums over rows take eight registers for each run of columns and kind, of
 // which programs without a norm after the block and without a gate (FULL false) have two.  They are joined in a fixed order: team by team within a
-// CTA, then CTA by CTA in a second launch.  16376 x 2056 bf16 with everything 165 us (2.4 TB/s, 43 % of the issue slots); 33.5 M elements in rows of 2048, two rms
+// CTA, then CTA by CTA in a second launch.  16376 x 2056 bf16 with everything 132 us (3.0 TB/s, 49 % of the issue slots; with a gate's
+// and a bias's sums made row by row 165); 33.5 M elements in rows of 2048, two rms
 // norms 92 us, a norm before alone 83 (0.67 and 0.75 of the memory's rate); 4096 x 768 f32 24 us.
 #include <type_traits>
 
@@ -528,8 +529,9 @@ sage_status block_norms_grad(Context &ctx, const BlockNorms &n, const RowsArg &o
     // Without a norm after the block or a gate its values are not read, and two kinds of sums are kept.
     const bool full = a.y.p && (a.after != SAGE_NORM_NONE || a.gate);
     // Runs of eight columns to a thread.  Two where rows are long: what a row costs each thread is then shared by twice the columns; four kinds of sums of
-    // two runs fit its registers, five do not.  33.5 M elements bf16, one run | two, us: five kinds, 768 columns 131 | 161, 1024 140 | 140, 1536 144 | 147, 2048
-    // 156 | 152, 4096 187 | 166; two norms alone, 2048 columns 127 | 95, 4096 151 | 101; a norm before alone, 4096 columns 104 | 89.
+    // two runs fit its registers, five (gates that change on a team's way) do not.  33.5 M elements bf16, one run | two, us: five kinds, 768 columns 131 | 161, 1024 140 | 140,
+    // 1536 144 | 147, 2048 156 | 152, 4096 187 | 166; four kinds 1024 128 | 120, 1536 135 | 118; two norms alone, 2048 columns 127 | 95, 4096 151 | 101; a norm before
+    // alone, 4096 columns 104 | 89.
     const bool many = full && a.gate && to[kSumBb] && groups > ctx.sm_count;
     const int least = a.dim > (many ? 1536 : full ? 1024 : 2048) ? 2 : 1, most = least == 2 || (full && !many) ? 2 : 1, nv = a.dim > 8 * kMaxThreads * 2 ? shape_of(&a, 4, 4) : shape_of(&a, least, most);
     const bool wide = a.dim % 8 == 0 && boundary(a.out, sx) && boundary(a.go, sx) && boundary(a.dx, sx) && boundary(a.y, st) && boundary(a.gh, st) && boundary(a.dy, st);

@@ -206,6 +206,23 @@ def test_block_norms_many_rows(ctx, rows, dim, gate):
             assert np.array_equal(t.numpy(), first[n].numpy()), n
 
 
+@pytest.mark.parametrize("rows,dim,gate", [(9000, 136, 9000), (6000, 1160, 3000), (5000, 1032, 1), (1200, 2056, 600)])
+@pytest.mark.parametrize("after,before", [("layer", "rms"), ("rms", "rms"), ("none", "layer")])
+def test_block_norms_gates_of_one_group_and_of_many(ctx, rows, dim, gate, after, before):
+    """Gates whose row serves all of a team's rows, and gates that change on the way; and each sum when it is asked for alone."""
+    rng = np.random.default_rng(rows + dim)
+    with Held(ctx) as d:
+        c = Case(d, rng, rows, dim, "bf16", "bf16", after, before, gate=gate, p=0.1)
+        c.forward()
+        all_of, go, gh = c.backward(rng)
+        want = c.oracle.grad(c.ov, c.yv, c.sv, values(go, "bf16"), values(gh, "bf16"))
+        for name in [n for n in all_of if n not in ("dx", "dy") and n in want]:
+            alone = d.empty(all_of[name].extents)
+            L.block_norms_grad(c.norms, c.out, c.y, c.stats, go, gh, **{name: alone})
+            value, tol = want[name]
+            close(alone.numpy(), value, B.stored_tol(value, tol, "f32"), name)
+
+
 def test_block_norms_without_a_branch(ctx):
     rng = np.random.default_rng(5)
     with Held(ctx) as d:
