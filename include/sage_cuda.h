@@ -142,7 +142,7 @@ typedef struct {
     uint64_t num_device_allocs; /* cudaMalloc calls so far (new: shows the cache working) */
 } sage_mem_stats_t;
 sage_status sage_mem_stats(sage_ctx *ctx, sage_mem_stats_t *stats);
-/* Pool::release_cached_blocks — memory.rs:454-474: return every fully-free segment to the device. */
+/* Pool::release_cached_blocks — memory.rs:454-474: return every fully-free segment to the device (none while the context's stream is capturing). */
 sage_status sage_release_cached(sage_ctx *ctx);
 /* Pool::garbage_collect — memory.rs:410-452: when 80 % of the capacity is in use, whole cached segments go
  * back to the device, oldest first (age = searches of the pool a block sat through), until 20 % of the
@@ -274,7 +274,13 @@ sage_status sage_conv2d_nhwc(sage_ctx *ctx, const sage_tensor *x, const sage_ten
  * contiguous along the last axis with any distance between rows that keeps them apart (inputs: any that is not negative), vectors
  * may have any stride (inputs: also 0, a broadcast value).  No more than 2^31 - 2^16 rows or columns.  Outputs may not share memory with an operand unless it says so.
  * Calls with no rows return at once.  All sums are held in 32 bits in a fixed order: the same inputs, as far from 16-byte boundaries,
- * give the same bits. */
+ * give the same bits.
+ *
+ * The calls may be captured into a CUDA graph from the context's stream (sage_ctx_use_stream).  sage_embedding_grad, sage_token_log_probs_grad, sage_block_norms_grad,
+ * sage_head_log_probs and its gradient work in memory of the context's pool.  What a capture takes from the pool, or gives back to it, stays with
+ * the graph: calls of the same capture share it, nothing else gets it (another graph has its own), sage_release_cached leaves it, and the pool has it again at the first call
+ * after the graph and all that was instantiated from it are gone.  A graph is not replayed once its context is destroyed, and for the first time behind the calls that
+ * were made before its capture. */
 
 /* y[t, :] = scale * table[ids[t], :].  table [V, D] f32 / f16 / bf16, ids [T] i32 / u32, y [T, D] f32 or the table's type.  An id
  * outside [0, V) stands for no token: its row is zeros. */

@@ -191,8 +191,8 @@ sage_status sage_release_cached(sage_ctx *ctx) {
     return SAGE_OK;
 }
 sage_status sage_garbage_collect(sage_ctx *ctx, uint64_t *reclaimed, uint64_t *runs_total, uint64_t *reclaimed_total) {
-    if (!ctx || !ctx->impl) return SAGE_ERR_INVALID;
-    Allocator &a = ctx->impl->allocator();
+    CTX_OR_FAIL(ctx);
+    Allocator &a = C.allocator();
     const uint64_t r = a.garbage_collect();
     if (reclaimed) *reclaimed = r;
     if (runs_total) *runs_total = a.gc_runs;

@@ -11,6 +11,8 @@ Allocator::Allocator(std::unique_ptr<DeviceMem> mem, uint64_t capacity, bool use
     : mem_(std::move(mem)), capacity_(capacity), use_cache_(use_cache) {}
 
 Allocator::~Allocator() {
+    capture_ = 0;
+    while (!held_.empty()) return_held(held_.begin()->first);  // graphs are not replayed behind their context's end
     // Walk every segment from its head block and hand it back.
     std::vector<Block *> heads;
     auto collect = [&](FreeSet &s) {
@@ -111,8 +113,68 @@ bool Allocator::grow(size_t size, bool small) {
     return true;
 }
 
-// Pool::alloc — memory.rs:336-363.
+void Allocator::look() {
+    if (gone_->any.load(std::memory_order_acquire)) {
+        std::vector<uint64_t> captures;
+        {
+            std::lock_guard<std::mutex> lock(gone_->m);
+            captures.swap(gone_->captures);
+            gone_->any.store(false, std::memory_order_relaxed);
+        }
+        capture_ = 0;
+        for (uint64_t c : captures) return_held(c);
+    }
+    capture_ = mem_->capture();
+}
+
+Allocator::FreeSet &Allocator::held_by(uint64_t capture) {
+    const auto it = held_.find(capture);
+    if (it != held_.end()) return it->second;
+    mem_->tell(capture, gone_);
+    return held_[capture];
+}
+
+// The graph of this capture is gone.  (A block that a capture was given back may be another, living graph's.)
+void Allocator::return_held(uint64_t capture) {
+    const auto it = held_.find(capture);
+    if (it == held_.end()) return;
+    const FreeSet blocks = std::move(it->second);
+    held_.erase(it);
+    for (Block *b : blocks) free(b);
+}
+
 Block *Allocator::alloc(size_t bytes) {
+    if (!capture_) return take(bytes);
+    FreeSet &held = held_by(capture_);
+    const size_t size = round_size(bytes);
+    Block key;
+    key.size = size;
+    for (auto it = held.lower_bound(&key); it != held.end() && (*it)->size - size <= std::max(size, kSmallSize); ++it)
+        if (!(*it)->capture || (*it)->capture == capture_) {
+            Block *b = *it;
+            held.erase(it);
+            b->capture = capture_;
+            return b;
+        }
+    Block *b = take(bytes);
+    if (b) b->capture = capture_;
+    return b;
+}
+
+void Allocator::free(Block *b) {
+    if (!b) return;
+    if (capture_) look();  // (tensors are dropped between calls, too)
+    const uint64_t c = capture_ ? capture_ : b->capture;
+    if (c && (capture_ || held_.count(c))) {
+        held_by(c).insert(b);
+        return;
+    }
+    b->capture = 0;
+    give(b);
+}
+
+// Pool::alloc — memory.rs:336-363.
+Block *Allocator::take(size_t bytes) {
     size_t size = round_size(bytes);
     if (!use_cache_) {
         // The reference's shipped configuration (context.rs:49): one device buffer per tensor.
@@ -144,6 +206,7 @@ Block *Allocator::alloc(size_t bytes) {
     if (!b) {
         garbage_collect();  // memory.rs:339: old cached segments go first, when the pool is nearly full
         if (!grow(size, small)) {
+            if (capture_) return nullptr;  // (nothing can be given back now)
             release_largest(size);  // memory.rs:344-349: give cached segments back, largest first, then retry
             if (!grow(size, small)) {
                 release_cached();  // (not in the reference) everything that is cached, small pool included
@@ -158,8 +221,7 @@ Block *Allocator::alloc(size_t bytes) {
 }
 
 // Pool::free — memory.rs:365-408: merge with free neighbours of the same segment.
-void Allocator::free(Block *b) {
-    if (!b) return;
+void Allocator::give(Block *b) {
     if (!use_cache_) {
         used_ -= b->size;
         total_ -= b->size;
@@ -195,7 +257,7 @@ void Allocator::free(Block *b) {
 // the capacity has been given back or nothing old enough remains.
 size_t Allocator::garbage_collect() {
     const uint64_t threshold = (uint64_t)((double)capacity_ * 0.8);  // GC_THRESHOLD
-    if (used_ < threshold) return 0;
+    if (used_ < threshold || capture_) return 0;
     const uint64_t target = capacity_ - threshold;
     const uint64_t now = searches_[0];
     uint64_t total_age = 0, freeable = 0;
@@ -256,6 +318,7 @@ size_t Allocator::release_largest(size_t size) {
 
 // Every unsplit free segment of both pools (sage_release_cached, and the last resort of alloc).
 void Allocator::release_cached() {
+    if (capture_) return;
     for (FreeSet *pool : {&small_free_, &large_free_}) {
         for (auto it = pool->begin(); it != pool->end();) {
             Block *b = *it;

@@ -71,15 +71,56 @@ static std::string cu_err(int e) {
 
 // ---- device memory sources
 struct CudaMem : DeviceMem {
+    cudaStream_t stream = nullptr;
+    bool follows = false;  // there is a stream
     void *alloc(size_t bytes) override {
+        // While any stream is capturing, memory is to be had only by a thread that says it knows what it does: nothing here waits for the device.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
         void *p = nullptr;
-        if (cudaMalloc(&p, bytes) != cudaSuccess) {
-            cudaGetLastError();
-            return nullptr;
-        }
-        return p;
+        const bool ok = cudaMalloc(&p, bytes) == cudaSuccess;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (ok) return p;
+        cudaGetLastError();
+        return nullptr;
     }
     void release(void *p) override { cudaFree(p); }
+    uint64_t capture() override {
+        if (!follows) return 0;
+        cudaStreamCaptureStatus status;
+        if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) {  // (the legacy stream, while another one is)
+            cudaGetLastError();
+            return 0;
+        }
+        unsigned long long id = 0;
+        if (status != cudaStreamCaptureStatusActive || cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess || status != cudaStreamCaptureStatusActive) return 0;
+        return id + 1;
+    }
+    struct Ending {
+        uint64_t capture;
+        std::shared_ptr<GoneGraphs> gone;
+    };
+    static void CUDART_CB ended(void *p) {  // (no CUDA call may be made here)
+        std::unique_ptr<Ending> e((Ending *)p);
+        std::lock_guard<std::mutex> lock(e->gone->m);
+        e->gone->captures.push_back(e->capture);
+        e->gone->any.store(true, std::memory_order_release);
+    }
+    void tell(uint64_t capture, std::shared_ptr<GoneGraphs> gone) override {
+        cudaStreamCaptureStatus status;
+        unsigned long long id = 0;
+        cudaGraph_t graph = nullptr;
+        if (!follows || cudaStreamGetCaptureInfo(stream, &status, &id, &graph) != cudaSuccess || status != cudaStreamCaptureStatusActive || id + 1 != capture) return;
+        Ending *e = new Ending{capture, std::move(gone)};
+        cudaUserObject_t object;
+        if (cudaUserObjectCreate(&object, e, ended, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
+            delete e;
+            cudaGetLastError();
+            return;
+        }
+        // The graph has the reference, as has each executable made of it, until its last launch has run.
+        if (cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) cudaGetLastError();  // (the object stays, and with it the memory)
+    }
 };
 
 // Planning contexts hand out addresses from a counter; they are never dereferenced.
@@ -130,7 +171,10 @@ sage_status Context::create(int device, const sage_ctx_opts &opts, Context **out
         cudaMemGetInfo(&free_b, &total_b);
         cap = (uint64_t)(free_b * 0.9);
     }
-    c->alloc_.reset(new Allocator(std::unique_ptr<DeviceMem>(new CudaMem()), cap, opts.use_cache != 0));
+    c->cuda_mem_ = new CudaMem();
+    c->alloc_.reset(new Allocator(std::unique_ptr<DeviceMem>(c->cuda_mem_), cap, opts.use_cache != 0));
+    c->cuda_mem_->stream = c->stream_;
+    c->cuda_mem_->follows = true;
     if (cudaMalloc(&c->status_word_dev, 4096) != cudaSuccess) return SAGE_ERR_DEVICE;
     cudaMemsetAsync(c->status_word_dev, 0, 4096, c->stream_);
     *out = c.release();
@@ -153,7 +197,8 @@ sage_status Context::use_stream(cudaStream_t s, bool own) {
     if (st) return st;
     st = check_cuda(cudaStreamWaitEvent(s, ev, 0), "use_stream: wait");
     if (st) return st;
-    stream_ = s;
+    stream_ = cuda_mem_->stream = s;
+    alloc_->look();
     return SAGE_OK;
 }
 
@@ -161,12 +206,15 @@ void Context::make_current() const {
     if (dry()) return;
     int cur = -1;
     if (cudaGetDevice(&cur) != cudaSuccess || cur != device_) cudaSetDevice(device_);
+    alloc_->look();
 }
 
 Context::~Context() {
     if (!dry()) {
         cudaSetDevice(device_);
         cudaStreamSynchronize(stream_);
+        cuda_mem_->follows = false;
+        alloc_->look();
         for (auto &kv : modules_)
             if (kv.second->cu_module && driver().ModuleUnload) driver().ModuleUnload(kv.second->cu_module);
         if (streamk_block) alloc_->free(streamk_block);

@@ -3,10 +3,12 @@
 // src/session/device.rs, src/session/memory.rs and the cache half of
 // src/session/context.rs.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <list>
 #include <map>
 #include <memory>
+#include <mutex>
 #include <set>
 #include <string>
 #include <unordered_map>
@@ -22,6 +24,7 @@ namespace sage {
 namespace k {
 struct LeafBatch;  // kernels/kernels.h
 }
+struct CudaMem;  // context.cc
 
 // ------------------------------------------------------------------------------------------
 // Allocator: restates the pool policy of src/session/memory.rs (size classes :23-43, best fit
@@ -29,11 +32,24 @@ struct LeafBatch;  // kernels/kernels.h
 // elements, with the merge defect fixed (merged size is the sum), and reuse ordered by the
 // context's single stream: a block freed after kernel k was enqueued may be handed to kernel
 // k+1 without a synchronisation because both run in stream order.
+//
+// A stream capture breaks that order: what it records runs again at every replay, behind work that nobody knew of then.  So a block
+// that is taken or given back while the stream is capturing belongs to that capture's graph.  Later calls of the same capture may have
+// it, and the pool gets it back when the graph, and all that was instantiated from it, is gone.
 // ------------------------------------------------------------------------------------------
+struct GoneGraphs {  // captures whose graphs were destroyed; the driver says so from a thread of its own
+    std::mutex m;
+    std::vector<uint64_t> captures;
+    std::atomic<bool> any{false};
+};
 struct DeviceMem {  // where segments come from: cudaMalloc, or fake addresses on a planning context
     virtual ~DeviceMem() {}
     virtual void *alloc(size_t bytes) = 0;  // nullptr on failure
     virtual void release(void *p) = 0;
+    // The capture that the pool's stream is in now; 0: none.
+    virtual uint64_t capture() { return 0; }
+    // `gone` will hear of the end of the graph that the capture under way becomes (where the driver refuses, it never does).
+    virtual void tell(uint64_t, std::shared_ptr<GoneGraphs>) {}
 };
 
 struct Block {
@@ -44,6 +60,7 @@ struct Block {
     Block *prev = nullptr, *next = nullptr;  // neighbours inside the same segment
     void *segment = nullptr;
     uint64_t entered = 0;  // the pool's search count when the block last entered its free list (Age, memory.rs:756-786)
+    uint64_t capture = 0;  // the stream capture that took it; 0: none
 };
 
 class Allocator {
@@ -62,6 +79,10 @@ public:
     // Returns nullptr on out-of-memory and fills needed/total like MemoryError::OutOfMemory.
     Block *alloc(size_t bytes);
     void free(Block *b);
+    // Looks whether the stream is capturing, and takes back what graphs that are gone had.  Every entry point does this once: a
+    // capture begins and ends between calls.
+    void look();
+    // (these two give nothing back while the stream is capturing: cudaFree is refused then)
     void release_cached();
     // Pool::garbage_collect — memory.rs:410-452; returns the bytes given back to the device.
     size_t garbage_collect();
@@ -87,11 +108,18 @@ private:
     void enter(FreeSet &pool, Block *b);
     uint64_t searches_[2] = {0, 0};  // get_free_block calls per pool (large, small): the clock block ages are read against
     static size_t round_size(size_t bytes);
+    Block *take(size_t bytes);
+    void give(Block *b);
+    FreeSet &held_by(uint64_t capture);
+    void return_held(uint64_t capture);
 
     std::unique_ptr<DeviceMem> mem_;
     uint64_t capacity_, total_ = 0, used_ = 0, peak_ = 0, device_allocs_ = 0;
     bool use_cache_;
     FreeSet small_free_, large_free_;
+    uint64_t capture_ = 0;             // the capture under way
+    std::map<uint64_t, FreeSet> held_; // by capture: blocks that its graph writes and no tensor has
+    std::shared_ptr<GoneGraphs> gone_ = std::make_shared<GoneGraphs>();
 };
 
 // ------------------------------------------------------------------------------------------
@@ -208,6 +236,7 @@ private:
     void *handover_event_ = nullptr;  // cudaEvent_t of use_stream
     sage_ctx_opts opts_{};
     std::shared_ptr<Allocator> alloc_;
+    CudaMem *cuda_mem_ = nullptr;  // the allocator's, which follows the stream
     std::string last_error_;
     std::unordered_map<std::string, std::unique_ptr<Module>> modules_;
     std::unordered_map<std::string, Module *> module_keys_;  // short keys of modules_ entries (which own them)
