@@ -340,6 +340,12 @@ Product shape_of(Context &ctx, long long m, long long n, long long k) {
     return p;
 }
 
+// K-blocks that the tensor cores add up where logits are made, by the values and by the gradient alike: chains of equal length, 512 k at most.
+int logits_chain(const Product &p) {
+    const int chains = (p.slice_blocks + 7) / 8;
+    return (p.slice_blocks + chains - 1) / chains;
+}
+
 template <class T, bool A_MN, bool B_MN, End END, bool F32 = false>
 sage_status launch(Context &ctx, const char *name, Product p, int dtype, const Matrix &a, const Matrix &b, int out_type, const Matrix &c) {
     ctx.note_launch(name);
@@ -492,7 +498,7 @@ sage_status forward16(Context &ctx, const Head &a, const VectorArg &log_probs, c
         p.ids = (const int *)ids.ptr;
         p.ids_stride = ids.stride;
         p.c2 = a.scale * kLog2E;
-        p.chain = (p.slice_blocks + (p.slice_blocks + 7) / 8 - 1) / ((p.slice_blocks + 7) / 8);  // of equal length
+        p.chain = logits_chain(p);
         p.parts = parts;
         p.asked = asked;
         st = launch<T, false, false, kStats>(ctx, "head_log_probs", p, a.hidden.dtype, x, w, 0, Matrix{});
@@ -554,6 +560,7 @@ sage_status grad16(Context &ctx, const Head &a, const RowsArg &stats, const Vect
         p.rows = about;
         p.gl = gls;
         p.gmax = gmax;
+        p.chain = logits_chain(p);
         p.band = (int)std::max<long long>(8, ((long long)48 << 20) / (256 * width * 2));
         st = launch<T, false, false, kProbs>(ctx, "head_probs", p, dtype, x, here, dtype, q);
         if (!st && dhidden.ptr) {

@@ -329,7 +329,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         const int quarter = warp & 3, side = (warp - 2) >> 2;  // a warp reaches the 32 rows of tensor memory that its number gives
         char *out = smem + kStages * kStageSize + (warp - 2) * kOutBytes;
         float factor = 1.f;
-        if (END == kProbs && p.gmax) factor = power_of_two(stored_exponent(p.gmax));
+        if (END == kProbs) factor = F32 ? p.alpha : p.gmax ? power_of_two(stored_exponent(p.gmax)) : 1.f;  // (the products of f32 operands have no scale: q has it)
         if (END == kNarrow || END == kWide) factor = p.gmax ? p.alpha * power_of_two(-stored_exponent(p.gmax)) : p.alpha;
         int chains = 0;
         bool live = true;
@@ -361,9 +361,10 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 id = __ldg(p.ids + row * p.ids_stride);
                 id = id < p.first ? -1 : id - p.first;
             }
-            if constexpr (END == kStats || F32) {
+            if constexpr (END == kStats || END == kProbs || F32) {
                 // The tensor cores cut what lies below a sum's last place at every addition: log probabilities of 4096 k in one chain were 4e-6 off.
-                // Chains of 512 k at most are added up here, to nearest.
+                // Chains of 512 k at most are added up here, to nearest; the gradient's in the same chains as the values', so that its logits are theirs
+                // to the bit and a row's probabilities come from the logits that its sum was made of.
                 float acc[4][32];
 #pragma unroll
                 for (int e = 0; e < 128; ++e) acc[e / 32][e % 32] = 0.f;
@@ -390,7 +391,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     float4 about = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (END == kProbs && there) {
                         about = __ldg(p.rows + row);
-                        about.z *= p.alpha, about.w *= p.alpha;  // q with its scale: the products of f32 operands have none
+                        about.z *= factor, about.w *= factor;
                     }
                     // 32 columns at a time: the sums as they are, or q in three planes
                     const auto open = [&]() {  // the warp's last store has been read
@@ -411,8 +412,16 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     for (int j = 0; j < 4; ++j)
                         if (j * 32 < half) {
                             const int col = col0 + j * 32;
-                            if constexpr (END == kProbs) {
-                                probs_of(p, acc[j], about, id - col, row, there, p.alpha);
+                            if constexpr (END == kProbs && !F32) {  // 64 columns to a store of 128 bytes
+                                probs_of(p, acc[j], about, id - col, row, there, factor);
+                                if (j % 2 == 0) open();
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    put_chunk(out, lane, 4 * (j % 2) + c, make_uint4(pair16<T>(acc[j][8 * c], acc[j][8 * c + 1]), pair16<T>(acc[j][8 * c + 2], acc[j][8 * c + 3]),
+                                                                                     pair16<T>(acc[j][8 * c + 4], acc[j][8 * c + 5]), pair16<T>(acc[j][8 * c + 6], acc[j][8 * c + 7])));
+                                if (j % 2) close(col - 32, row0);
+                            } else if constexpr (END == kProbs) {
+                                probs_of(p, acc[j], about, id - col, row, there, factor);
 #pragma unroll 1
                                 for (int n = 0; n < 3; ++n) {
                                     open();
@@ -432,35 +441,28 @@ head_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         }
                 }
             } else {
-                float4 about = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (END == kProbs && there) {
-                    about = __ldg(p.rows + row);
-                    about.z *= factor, about.w *= factor;
-                }
                 const unsigned at = arrived();
                 if (!live) break;
                 for (int j = 0; j < half; j += 32) {
                     float v[32];
                     tmem_ld32(at + j, v);
                     const int col = col0 + j;
-                    if (END == kProbs) probs_of(p, v, about, id - col, row, there, factor);
                     constexpr int kPer = END == kWide ? 1 : 2;  // loads of 32 columns to a store of 128 bytes
                     const int part = (j / 32) % kPer;
                     if (part == 0) {  // the warp's last store has been read
                         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         __syncwarp();
                     }
-                    const float f = END == kProbs ? 1.f : factor;
                     if (END == kWide) {
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
-                            put_chunk(out, lane, c, make_uint4(__float_as_uint(v[4 * c] * f), __float_as_uint(v[4 * c + 1] * f), __float_as_uint(v[4 * c + 2] * f), __float_as_uint(v[4 * c + 3] * f)));
+                            put_chunk(out, lane, c, make_uint4(__float_as_uint(v[4 * c] * factor), __float_as_uint(v[4 * c + 1] * factor), __float_as_uint(v[4 * c + 2] * factor), __float_as_uint(v[4 * c + 3] * factor)));
                     } else {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
                             put_chunk(out, lane, 4 * part + c,
-                                      make_uint4(pair16<T>(v[8 * c] * f, v[8 * c + 1] * f), pair16<T>(v[8 * c + 2] * f, v[8 * c + 3] * f), pair16<T>(v[8 * c + 4] * f, v[8 * c + 5] * f),
-                                                 pair16<T>(v[8 * c + 6] * f, v[8 * c + 7] * f)));
+                                      make_uint4(pair16<T>(v[8 * c] * factor, v[8 * c + 1] * factor), pair16<T>(v[8 * c + 2] * factor, v[8 * c + 3] * factor), pair16<T>(v[8 * c + 4] * factor, v[8 * c + 5] * factor),
+                                                 pair16<T>(v[8 * c + 6] * factor, v[8 * c + 7] * factor)));
                     }
                     if (part == kPer - 1) {
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
