@@ -84,10 +84,20 @@ __global__ void __launch_bounds__(1024) head_join_kernel(const float4 *parts, in
 
 // Few rows (one token of each of a few sequences): a warp takes four rows of the weights at a time, straight from memory in order, with the hidden states in
 // shared memory.  Bound by the weights' bytes.  A lane sums its columns in f32; of the 4 x RB sums of a warp every lane ends up with one (half of
-// what it has goes to another lane at each step), and keeps the sums of exponentials for those of its place.
-template <class T, int RB>
+// what it has goes to another lane at each step), and keeps the sums of exponentials for those of its place, or (Q) makes of its logit its part of the gradient: from
+// logits of the tensor cores, which differ in their last places, p = exp(x - m) / S of a likely token would be off by as much.
+struct FewProbs {
+    const float4 *about;  // head_rows_kernel's
+    const float *gl;
+    const unsigned *gmax;
+    float alpha;          // f32
+    unsigned short *q;    // 16 bits; f32: three planes of pieces
+    long long pitch, plane;
+    int first;            // token that the weights' first row stands for
+};
+template <class T, int RB, bool Q>
 __global__ void __launch_bounds__(256, 2) head_few_kernel(const T *hidden, long long hidden_pitch, const T *weight, long long weight_pitch, int rows, int vocab, int width, const int *ids,
-                                                          long long ids_stride, float c2, float4 *parts, float *asked) {
+                                                          long long ids_stride, float c2, float4 *parts, float *asked, const FewProbs to) {
     extern __shared__ __align__(16) char smem[];
     __shared__ Sums all[8][RB];
     grid_dependency_sync();
@@ -102,6 +112,14 @@ __global__ void __launch_bounds__(256, 2) head_few_kernel(const T *hidden, long 
     constexpr int N = 4 * RB, kLanes = 32 / N;  // sums; lanes that end up with the same one
     const int index = lane / kLanes, mine = index % RB, which = index / RB;
     const int id = mine < rows ? __ldg(ids + mine * ids_stride) : -1;
+    float4 about = make_float4(0.f, 0.f, 0.f, 0.f);
+    float gl = 0.f;
+    if (Q && mine < rows) {
+        const float by = sizeof(T) == 4 ? to.alpha : to.gmax ? power_of_two(stored_exponent(to.gmax)) : 1.f;
+        about = __ldg(to.about + mine);
+        about.z *= by, about.w *= by;
+        gl = __ldg(to.gl + mine) * by;
+    }
     Sums kept{-INFINITY, 0.f, 0.f};
     for (long long first = 4ll * ((long long)blockIdx.x * 8 + warp); first < vocab; first += 32ll * gridDim.x) {
         const char *row[4];
@@ -148,7 +166,20 @@ __global__ void __launch_bounds__(256, 2) head_few_kernel(const T *hidden, long 
             }
         }
         const long long token = first + which;
-        if (token < vocab) {
+        if (Q) {
+            if (token < vocab && mine < rows && lane % kLanes == 0) {
+                const float d = fmaf(v[0] - about.x, c2, about.y);
+                float q = exp2_of(d) * fmaf(about.w, fmaxf(d, kFar), about.z), none = 0.f;
+                if (token + to.first == id) q += gl;
+                unsigned short *at = to.q + mine * to.pitch + token;
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) at[k * to.plane] = (unsigned short)take_piece(q, none);
+                } else {
+                    *(T *)at = narrowed<T>(q);
+                }
+            }
+        } else if (token < vocab) {
             const float x = v[0];
             if (x > kept.m) {
                 const float by = kept.m == -INFINITY ? 0.f : (kept.m - x) * c2, f = kept.m == -INFINITY ? 0.f : exp2_of(by);
@@ -162,15 +193,17 @@ __global__ void __launch_bounds__(256, 2) head_few_kernel(const T *hidden, long 
             if (token == id) asked[mine] = x;
         }
     }
+    if constexpr (!Q) {
 #pragma unroll
-    for (int off = 16; off >= 8; off >>= 1)  // the four weights' rows of a hidden state
-        kept = joined(kept, Sums{__shfl_xor_sync(0xffffffffu, kept.m, off), __shfl_xor_sync(0xffffffffu, kept.s, off), __shfl_xor_sync(0xffffffffu, kept.a, off)}, c2);
-    if (lane < 8 && lane % kLanes == 0) all[warp][mine] = kept;
-    __syncthreads();
-    if ((int)threadIdx.x < rows) {
-        Sums t = all[0][threadIdx.x];
-        for (int w = 1; w < 8; ++w) t = joined(t, all[w][threadIdx.x], c2);
-        parts[(long long)blockIdx.x * rows + threadIdx.x] = make_float4(t.m, t.s, t.a, 0.f);
+        for (int off = 16; off >= 8; off >>= 1)  // the four weights' rows of a hidden state
+            kept = joined(kept, Sums{__shfl_xor_sync(0xffffffffu, kept.m, off), __shfl_xor_sync(0xffffffffu, kept.s, off), __shfl_xor_sync(0xffffffffu, kept.a, off)}, c2);
+        if (lane < 8 && lane % kLanes == 0) all[warp][mine] = kept;
+        __syncthreads();
+        if ((int)threadIdx.x < rows) {
+            Sums t = all[0][threadIdx.x];
+            for (int w = 1; w < 8; ++w) t = joined(t, all[w][threadIdx.x], c2);
+            parts[(long long)blockIdx.x * rows + threadIdx.x] = make_float4(t.m, t.s, t.a, 0.f);
+        }
     }
 }
 
@@ -440,6 +473,25 @@ RowsArg cut(const RowsArg &r, long long at, long long count) {
 }
 VectorArg cut(const VectorArg &v, long long at) { return v.ptr ? VectorArg{(char *)v.ptr + at * v.stride * 4, v.stride} : v; }
 
+// One pass over the weights for `pass` rows at most.
+template <class T, bool Q>
+sage_status launch_few(Context &ctx, const Head &a, long long pass, unsigned grid, float4 *parts, float *asked, const FewProbs &to) {
+    ctx.note_launch(Q ? "head_few_probs" : "head_few");
+    if (ctx.dry()) return SAGE_OK;
+    const auto run = [&](auto kernel, int padded) {
+        const size_t smem = (size_t)padded * a.hidden.cols * sizeof(T);
+        sage_status s = ctx.check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024), "head_few");
+        return s ? s
+                 : ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3(grid), dim3(256), smem, (const T *)a.hidden.ptr, a.hidden.pitch, (const T *)a.weight.ptr, a.weight.pitch, (int)a.hidden.rows,
+                                                   (int)a.weight.rows, (int)a.hidden.cols, (const int *)a.ids.ptr, a.ids.stride, a.scale * kLog2E, parts, asked, to),
+                                  "head_few");
+    };
+    if constexpr (sizeof(T) == 4)
+        if (pass > 4) return run(head_few_kernel<T, 8, Q>, 8);
+    return pass > 2 ? run(head_few_kernel<T, 4, Q>, 4) : pass > 1 ? run(head_few_kernel<T, 2, Q>, 2) : run(head_few_kernel<T, 1, Q>, 1);
+}
+unsigned few_grid(Context &ctx, long long vocab) { return (unsigned)std::min<long long>((vocab + 31) / 32, 2ll * ctx.sm_count); }
+
 template <class T>
 sage_status forward_few(Context &ctx, const Head &all, long long pass, const VectorArg &all_log_probs, const VectorArg &all_entropy, const RowsArg &all_stats) {
     for (long long at = 0; at < all.hidden.rows; at += pass) {
@@ -450,24 +502,31 @@ sage_status forward_few(Context &ctx, const Head &all, long long pass, const Vec
         const VectorArg log_probs = cut(all_log_probs, at), entropy = cut(all_entropy, at);
         const RowsArg stats = cut(all_stats, at, a.hidden.rows);
         const long long rows = a.hidden.rows, vocab = a.weight.rows;
-        const unsigned grid = (unsigned)std::min<long long>((vocab + 31) / 32, 2ll * ctx.sm_count);
+        const unsigned grid = few_grid(ctx, vocab);
         float4 *parts = nullptr;
         float *asked = nullptr;
         sage_status st = scratch.get((size_t)(grid * rows) * 16, &parts);
         if (!st) st = scratch.get((size_t)rows * 4, &asked);
-        if (st) return st;
-        ctx.note_launch("head_few");
-        const auto run = [&](auto kernel, int padded) {
-            const size_t smem = (size_t)padded * a.hidden.cols * sizeof(T);
-            sage_status s = ctx.check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024), "head_few");
-            return s ? s
-                     : ctx.check_cuda(launch_dependent(ctx.pdl, ctx.stream(), kernel, dim3(grid), dim3(256), smem, (const T *)a.hidden.ptr, a.hidden.pitch, (const T *)a.weight.ptr, a.weight.pitch, (int)rows, (int)vocab,
-                                                       (int)a.hidden.cols, (const int *)a.ids.ptr, a.ids.stride, a.scale * kLog2E, parts, asked),
-                                      "head_few");
-        };
-        if (!ctx.dry()) st = pass > 4 ? run(head_few_kernel<T, 8>, 8) : pass > 2 ? run(head_few_kernel<T, 4>, 4) : pass > 1 ? run(head_few_kernel<T, 2>, 2) : run(head_few_kernel<T, 1>, 1);
+        if (!st) st = launch_few<T, false>(ctx, a, pass, grid, parts, asked, FewProbs{});
         if (!st) st = join(ctx, parts, (int)grid, rows, asked, a.ids, vocab, a.scale, Values{(float *)log_probs.ptr, (float *)entropy.ptr, (float *)stats.ptr, log_probs.stride, entropy.stride, stats.pitch});
         if (st) return st;
+    }
+    return SAGE_OK;
+}
+// q of tokens [first, first + count) for few rows, from the values' own dot products.
+template <class T>
+sage_status probs_few(Context &ctx, const Head &all, long long pass, long long first, long long count, FewProbs to) {
+    Head a = all;
+    a.weight = cut(all.weight, first, count);
+    to.first = (int)first;
+    for (long long at = 0; at < all.hidden.rows; at += pass) {
+        a.hidden = cut(all.hidden, at, std::min(pass, all.hidden.rows - at));
+        a.ids = cut(all.ids, at);
+        sage_status st = launch_few<T, true>(ctx, a, pass, few_grid(ctx, count), nullptr, nullptr, to);
+        if (st) return st;
+        to.about += pass;
+        to.gl += pass;
+        to.q += pass * to.pitch;
     }
     return SAGE_OK;
 }
@@ -546,6 +605,7 @@ sage_status grad16(Context &ctx, const Head &a, const RowsArg &stats, const Vect
     if (!st) st = aligned<T>(ctx, scratch, a.weight, &w);
     if (!st) st = rows_about(ctx, scratch, a, stats, entropy, gl, ge, dtype == SAGE_F16, &about, &gls, &gmax);
     if (!st) st = scratch.get((size_t)(rows * pitch) * 2, &probs);
+    const long long pass = few(a);  // rows whose values came from dot products
     Result to_hidden;
     to_hidden.out = dhidden;
     for (long long at = 0; at < vocab && !st; at += piece) {
@@ -562,7 +622,8 @@ sage_status grad16(Context &ctx, const Head &a, const RowsArg &stats, const Vect
         p.gmax = gmax;
         p.chain = logits_chain(p);
         p.band = (int)std::max<long long>(8, ((long long)48 << 20) / (256 * width * 2));
-        st = launch<T, false, false, kProbs>(ctx, "head_probs", p, dtype, x, here, dtype, q);
+        if (pass) st = probs_few<T>(ctx, a, pass, at, n, FewProbs{about, gls, gmax, 1.f, (unsigned short *)probs, pitch, 0, 0});
+        else st = launch<T, false, false, kProbs>(ctx, "head_probs", p, dtype, x, here, dtype, q);
         if (!st && dhidden.ptr) {
             p = shape_of(ctx, rows, width, n);
             p.gmax = gmax;
@@ -645,6 +706,7 @@ sage_status grad32(Context &ctx, const Head &a, const RowsArg &stats, const Vect
     sage_status st = pieces_of(ctx, scratch, a.hidden, &x, a.weight, &w);
     if (!st) st = rows_about(ctx, scratch, a, stats, entropy, gl, ge, false, &about, &gls, &gmax);
     if (!st) st = scratch.get((size_t)(3 * padded * pitch) * 2, &probs);
+    const long long pass = few(a);  // rows whose values came from dot products
     Result to_hidden;
     to_hidden.out = dhidden;
     for (long long at = 0; at < vocab && !st; at += piece) {
@@ -661,7 +723,8 @@ sage_status grad32(Context &ctx, const Head &a, const RowsArg &stats, const Vect
         p.band = (int)std::max<long long>(8, ((long long)48 << 20) / (256 * width * 6));
         p.slice_rows = (int)padded;  // of a plane
         p.alpha = a.scale;
-        st = launch<Piece, false, false, kProbs, true>(ctx, "head_probs", p, SAGE_BF16, x, here, SAGE_BF16, Matrix{probs, 3 * padded, n, pitch});
+        if (pass) st = probs_few<float>(ctx, a, pass, at, n, FewProbs{about, gls, nullptr, a.scale, (unsigned short *)probs, pitch, padded * pitch, 0});
+        else st = launch<Piece, false, false, kProbs, true>(ctx, "head_probs", p, SAGE_BF16, x, here, SAGE_BF16, Matrix{probs, 3 * padded, n, pitch});
         if (!st && dhidden.ptr) {
             p = shape_of(ctx, rows, width, n);
             if (first) plan(ctx, p, n, !last, &to_hidden);

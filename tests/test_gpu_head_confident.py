@@ -70,3 +70,9 @@ def confident(ctx, kind, rows, vocab, dim, logit):
 @pytest.mark.parametrize("rows,vocab,dim,logit", [(300, 20000, 4096, 24.0), (64, 8192, 1000, 23.0)])
 def test_gradients_of_confident_tokens(ctx, kind, rows, vocab, dim, logit):
     confident(ctx, kind, rows, vocab, dim, logit)
+
+
+@pytest.mark.parametrize("kind,rows", [("bf16", 1), ("bf16", 3), ("f16", 4), ("f32", 2), ("f32", 20)])
+def test_gradients_of_confident_tokens_in_few_rows(ctx, kind, rows):
+    """Their values come from dot products."""
+    confident(ctx, kind, rows, 20000, 4096, 24.0)
