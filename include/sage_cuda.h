@@ -317,8 +317,10 @@ sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logi
  * the logits again; with q = d / d logits, dhidden = q weight and dweight = q^T hidden are of the operands' type or f32 (NULL: not wanted).  Between 16-bit operands q is
  * rounded to their type (f16: by a power of two that brings its largest near 2^14), an operand like the others of both products.  The order of all sums is fixed.
  * Sums over pieces of the vocabulary are added as the memory's unit adds (results below 2^-126 in size become zero).  Infinite f32 operands give NaN where there are more
- * than a few rows.  Memory for a call comes from the context's pool: up to 512 MB for the values, 256 MB for a piece of q and f32 sums of [R, D] for the gradient, and
- * 6 bytes for each element of f32 operands. */
+ * than a few rows.  Memory for a call comes from the context's pool, and goes back to it with the call.  Values: up to 512 MB (vocabularies
+ * above 2^24: 32 bytes a token).  Gradient: a piece of q, up to 256 MB or 512 bytes for each row (f32 operands: 1536) where that is more; f32 sums of [R, D] where q comes in several pieces, and of a
+ * piece of the weight, where a result's rows do not lie on 16-byte boundaries; up to 20 MB where few tiles share out their sums.  Both: 6 bytes for each element of f32 operands, a copy of 16-bit ones whose rows do
+ * not lie on 16-byte boundaries. */
 sage_status sage_head_log_probs(sage_ctx *ctx, const sage_tensor *hidden, const sage_tensor *weight, const sage_tensor *ids, float scale, const sage_tensor *log_probs,
                                 const sage_tensor *entropy, const sage_tensor *stats);
 sage_status sage_head_log_probs_grad(sage_ctx *ctx, const sage_tensor *hidden, const sage_tensor *weight, const sage_tensor *ids, float scale, const sage_tensor *stats,

@@ -635,10 +635,11 @@ sage_status grad16(Context &ctx, const Head &a, const RowsArg &stats, const Vect
             p = shape_of(ctx, n, width, rows);
             p.gmax = gmax;
             p.alpha = a.scale;
+            Scratch sums(ctx);  // of this piece alone
             Result r;
             r.out = cut(dweight, at, n);
             plan(ctx, p, rows, false, &r);
-            st = multiply<T, true, true>(ctx, scratch, "head_dweight", p, dtype, q, x, true, true, &r);
+            st = multiply<T, true, true>(ctx, sums, "head_dweight", p, dtype, q, x, true, true, &r);
         }
     }
     return st;
@@ -732,10 +733,11 @@ sage_status grad32(Context &ctx, const Head &a, const RowsArg &stats, const Vect
         }
         if (!st && dweight.ptr) {
             p = shape_of(ctx, n, width, rows);
+            Scratch sums(ctx);  // of this piece alone
             Result r;
             r.out = cut(dweight, at, n);
             plan(ctx, p, rows, false, &r);
-            st = multiply<Piece, true, true, true>(ctx, scratch, "head_dweight", p, SAGE_BF16, q, x, true, true, &r);
+            st = multiply<Piece, true, true, true>(ctx, sums, "head_dweight", p, SAGE_BF16, q, x, true, true, &r);
         }
     }
     return st;
