@@ -213,8 +213,10 @@ Context::~Context() {
     if (!dry()) {
         cudaSetDevice(device_);
         cudaStreamSynchronize(stream_);
-        cuda_mem_->follows = false;
-        alloc_->look();
+        if (cuda_mem_) {  // (a context that could not be made has none)
+            cuda_mem_->follows = false;
+            alloc_->look();
+        }
         for (auto &kv : modules_)
             if (kv.second->cu_module && driver().ModuleUnload) driver().ModuleUnload(kv.second->cu_module);
         if (streamk_block) alloc_->free(streamk_block);
