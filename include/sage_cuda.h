@@ -316,8 +316,8 @@ sage_status sage_token_log_probs_and_grad(sage_ctx *ctx, const sage_tensor *logi
  * head is `weight`).  Products are summed in f32 (f32 operands: with f32's accuracy).  The gradient reads the stats and the entropy that the values left and makes
  * the logits again; with q = d / d logits, dhidden = q weight and dweight = q^T hidden are of the operands' type or f32 (NULL: not wanted).  Between 16-bit operands q is
  * rounded to their type (f16: by a power of two that brings its largest near 2^14), an operand like the others of both products.  The order of all sums is fixed.
- * Sums over pieces of the vocabulary are added as the memory's unit adds (results below 2^-126 in size become zero).  Infinite f32 operands give NaN where there are more
- * than a few rows.  Memory for a call comes from the context's pool, and goes back to it with the call.  Values: up to 512 MB (vocabularies
+ * Sums over pieces of the vocabulary are added as the memory's unit adds (results below 2^-126 in size become zero).  Infinite f32 operands, and finite ones above bf16's largest (3.39e38), give NaN where there are
+ * more than a few rows.  Logits and their differences lie in f32's range before they are scaled.  Memory for a call comes from the context's pool, and goes back to it with the call.  Values: up to 512 MB (vocabularies
  * above 2^24: 32 bytes a token).  Gradient: a piece of q, up to 256 MB or 512 bytes for each row (f32 operands: 1536) where that is more; f32 sums of [R, D] where q comes in several pieces, and of a
  * piece of the weight, where a result's rows do not lie on 16-byte boundaries; up to 20 MB where few tiles share out their sums.  Both: 6 bytes for each element of f32 operands, a copy of 16-bit ones whose rows do
  * not lie on 16-byte boundaries. */
@@ -352,7 +352,7 @@ typedef struct { /* buf NULL: absent */
 sage_status sage_block_norms(sage_ctx *ctx, const sage_block_norms_opts *opts, const sage_tensor *x, const sage_tensor *y, const sage_tensor *out, const sage_tensor *h, const sage_tensor *stats);
 /* Its gradient, from `out` (x where that was NULL), y and stats as they are behind the call, and the gradients g_out and g_h of both results (either may be NULL: zero):
  * dx and dy (of the types of x and y; NULL: not wanted), and the sums over rows that `sums` asks for (buf NULL: not wanted; f32, of the operand's shape),
- * in a fixed order.  Without y: dy, the gate's and the norm after's sums are NULL. */
+ * in a fixed order.  Without y: dy, the gate's and the norm after's sums are NULL.  (Fastest where y, g_out, g_h and the weights of the norms are given, in whole runs of eight columns on 32-byte boundaries, 16 bits: 16-byte.) */
 typedef struct {
     sage_tensor after_weight, after_bias, before_weight, before_bias, gate;
 } sage_block_norms_sums;

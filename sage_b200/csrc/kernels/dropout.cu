@@ -1,8 +1,8 @@
 // Dropout whose mask is drawn from each element's position and never stored: y_i = x_i 65536 / (65536 - bar) where element i stays, else 0
 // (counter_random.h says which stay).  Its gradient is the same map of the gradient that arrives.
 //
-// Bound by memory, nearly as much by instructions: an element is read and written once, a draw of 60 integer instructions serves eight of them (16384 x 4096 bf16
-// 49 us, 5.5 TB/s, 69 % of the issue slots; one block to a thread 63).  A thread takes blocks of
+// Bound by memory, nearly as much by instructions: an element is read and written once, a draw of 40 instructions (two products and two exclusive ors a round; the keys' sums are made
+// once for a warp) serves eight of them (16384 x 4096 bf16 46-49 us, 5.5-5.8 TB/s, 69 % of the issue slots; one block to a thread 63).  A thread takes blocks of
 // eight elements, whatever the layout: as vectors where rows keep blocks whole and on 32-byte (16 bits: 16-byte) boundaries, element by element elsewhere.
 #include <algorithm>
 

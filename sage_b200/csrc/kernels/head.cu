@@ -455,7 +455,8 @@ sage_status join(Context &ctx, const float4 *parts, int count, long long rows, c
 
 // Rows that are few enough for dot products, and how many of them a pass over the weights takes: eight, or what 96 KB of shared memory hold.  16-bit operands
 // up to four rows (one, four, eight rows of 131072 x 4096 164, 208, 290 us, the tensor cores 203; 30522 x 768 20, 22, 27 and 23); f32 operands up
-// to four passes (16 rows of 131072 x 4096 in four 1250 us, the tensor cores, which need the weights in pieces first, 1820; 32 of 50021 x 2048 460 and 475).
+// to four passes (16 rows of 131072 x 4096 in four 1250 us, the tensor cores, which need the weights in pieces first, 1820; 32 of 50021 x 2048 460 and 475).  The gradient goes the values'
+// way (one row of 131072 x 4096 bf16 557 us, by the tensor cores 662; four f32 rows 2850 and 3800, sixteen 4000 and 3790).
 long long few(const Head &a) {
     const int size = a.hidden.dtype == SAGE_F32 ? 4 : 2;
     if (a.hidden.cols % 8 || !on_16(a.hidden.ptr, a.hidden.rows > 1 ? a.hidden.pitch : 0, size) || !on_16(a.weight.ptr, a.weight.rows > 1 ? a.weight.pitch : 0, size)) return 0;

@@ -3,11 +3,11 @@
 //
 // Two CTAs work on one tile of 256 rows and BN columns (cta_group::2): each loads its 128 rows of A and its half of B's rows, 64 k at a time,
 // through a ring of TMA stages; the first of them issues the MMAs, whose sums lie 128 rows to a CTA in tensor memory, two tiles' worth, so that
-// eight warps finish a tile while the next one's sums are made: the tensor pipe is 88 % busy (8192 x 50021 x 2048 bf16, values 1190 us, 1410 TFLOP/s, where a plain
-// product of the library reaches 1376 for seconds on end).  Either operand may be stored with K or with its rows contiguous.
+// eight warps finish a tile while the next one's sums are made: the tensor pipe is 88-94 % busy (8192 x 50021 x 2048 bf16, values 1163-1210 us, 1390-1440 TFLOP/s, where a
+// plain product of the library reaches 1376 for seconds on end).  Either operand may be stored with K or with its rows contiguous.
 //
-// f32 operands (F32), with f32's accuracy: every element is the sum of three bf16 numbers, x = x0 + x1 + x2 (8 bits each, to nearest, 24 in all, in f32's
-// whole range), which lie in three planes, and of the nine products of pieces the six that reach 2^-24 of the result are made,
+// f32 operands (F32), with f32's accuracy: every element is the sum of three bf16 numbers, x = x0 + x1 + x2 (8 bits each, to nearest, 24 in all; what
+// rounds to a finite bf16, 3.39e38 at most), which lie in three planes, and of the nine products of pieces the six that reach 2^-24 of the result are made,
 //   x2 y0 + x0 y2 + x1 y1 + x1 y0 + x0 y1 + x0 y0,
 // in this order for each 64 k, so that the tensor cores, which cut what lies below the last place of a sum, add the small ones to small sums; the sum of
 // each 64 k is then added to registers, to nearest.  (Two f16 pieces would need three products, but a scale for each row, and what is far below a row's
