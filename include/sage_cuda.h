@@ -280,7 +280,7 @@ sage_status sage_conv2d_nhwc(sage_ctx *ctx, const sage_tensor *x, const sage_ten
  * sage_head_log_probs and its gradient work in memory of the context's pool.  What a capture takes from the pool, or gives back to it, stays with
  * the graph: calls of the same capture share it, nothing else gets it (another graph has its own), sage_release_cached leaves it, and the pool has it again at the first call
  * after the graph and all that was instantiated from it are gone.  A graph is not replayed once its context is destroyed, and for the first time behind the calls that
- * were made before its capture. */
+ * were made before its capture; one whose nodes were taken over into another executable (cudaGraphExecUpdate) lives as long as that. */
 
 /* y[t, :] = scale * table[ids[t], :].  table [V, D] f32 / f16 / bf16, ids [T] i32 / u32, y [T, D] f32 or the table's type.  An id
  * outside [0, V) stands for no token: its row is zeros. */

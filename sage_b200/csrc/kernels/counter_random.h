@@ -70,10 +70,10 @@ __device__ __forceinline__ unsigned keep8(const Dropout &d, Key k, unsigned long
     return keep;
 }
 // Eight elements, those that are dropped zero: of a word's halves the upper one is compared in place, the lower one shifted there.
-__device__ __forceinline__ void drop8(float2 (&v)[4], const uint4 &w, unsigned bar) {
+__device__ __forceinline__ void drop8(float2 (&v)[4], const uint4 &w, unsigned bar, float zero = 0.f) {
     const unsigned words[4] = {w.x, w.y, w.z, w.w}, high = bar << 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = make_float2((words[i] << 16) >= high ? v[i].x : 0.f, words[i] >= high ? v[i].y : 0.f);
+    for (int i = 0; i < 4; ++i) v[i] = make_float2((words[i] << 16) >= high ? v[i].x : zero, words[i] >= high ? v[i].y : zero);
 }
 // ... of eight elements from `first` on, wherever that lies in a block.
 __device__ __forceinline__ unsigned keep_from(const Dropout &d, Key k, unsigned long long first) {
